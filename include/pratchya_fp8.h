@@ -661,6 +661,74 @@ int pratchya_debug_bf16_to_e4m3(const uint16_t* in, uint8_t* out, int64_t n, int
 int pratchya_debug_f32_to_bf16(const float* in, uint16_t* out, int64_t n, int mode,
                                hipStream_t stream);
 
+/* ---- row operators around the quantized linears ------------------------ */
+
+/* Layer norm over segments of a row: `rows` rows of `width` elements (dtype f32
+ * or bf16, `ldx` elements apart) hold `groups` segments of D = width / groups
+ * each; per segment y = (x - mean) / sqrt(var + eps) * w + b, with w and b
+ * [width] vectors (f32 or bf16; null: 1 and 0).  y is contiguous and of x's
+ * dtype.  stats, if not null, receives (mean, 1 / sqrt(var + eps)) per segment
+ * (f32 [rows * groups][2]), which the backward pass reads.  x8 / sc8 / sc32, if
+ * x8 is not null, receive x quantized with tgrid (1, blk) as
+ * pratchya_quantize(x [rows, width]) in the same pass, for the layouts
+ * pratchya_layer_norm_stores takes (PRATCHYA_EUNSUPPORTED for others). */
+int pratchya_layer_norm(const void* x, int64_t ldx, int dtype, const void* w, int w_dtype, const void* b, int b_dtype,
+                        int64_t rows, int64_t width, int64_t groups, float eps, void* y, float* stats, uint8_t* x8,
+                        uint8_t* sc8, float* sc32, int64_t blk, hipStream_t stream);
+
+/* 1 if pratchya_layer_norm quantizes rows of this layout in the same pass, else 0. */
+int pratchya_layer_norm_stores(int64_t width, int64_t groups, int64_t blk);
+
+/* Gradients of pratchya_layer_norm.  x as the forward pass read it (x_dtype =
+ * dtype, ldx), or its quantized form (x_dtype PRATCHYA_DT_E4M3, payload
+ * contiguous, with sc8 / sc32 and blk; ldx unused); dy of dtype, rows ldy
+ * elements apart; stats of the forward pass.  Writes dx (contiguous, dtype), dw
+ * and db ([width], f32 or bf16); each may be null.  dw and db need a workspace
+ * of pratchya_layer_norm_bwd_workspace_bytes, 4-byte aligned; they are sums of a
+ * fixed order, the same bits for the same inputs. */
+int64_t pratchya_layer_norm_bwd_workspace_bytes(int64_t rows, int64_t width, int64_t groups);
+int pratchya_layer_norm_bwd(const void* x, int64_t ldx, int x_dtype, const uint8_t* sc8, const float* sc32,
+                            int64_t blk, const void* dy, int64_t ldy, int dtype, const void* w, int w_dtype,
+                            const float* stats, int64_t rows, int64_t width, int64_t groups, void* dx, void* dw,
+                            int dw_dtype, void* db, int db_dtype, void* workspace, int64_t workspace_bytes,
+                            hipStream_t stream);
+
+/* Activations: max(x, 0)^2, x / (1 + e^-x), and x times the normal distribution
+ * function of x. */
+#define PRATCHYA_ACT_RELU2 0
+#define PRATCHYA_ACT_SILU 1
+#define PRATCHYA_ACT_GELU 2
+
+/* y = f(x) of [rows, width] elements (f32 or bf16, rows ldx elements apart; y
+ * contiguous, of x's dtype).  x8 / sc8 / sc32, if x8 is not null, receive x
+ * quantized with tgrid (1, blk), blk 16, 32, 64 or 128, as pratchya_quantize(x)
+ * in the same pass. */
+int pratchya_activation(const void* x, int64_t ldx, int dtype, int kind, int64_t rows, int64_t width, void* y,
+                        uint8_t* x8, uint8_t* sc8, float* sc32, int64_t blk, hipStream_t stream);
+
+/* dx = f'(x) dy, with x as in pratchya_layer_norm_bwd; dx is contiguous, of dy's dtype. */
+int pratchya_activation_bwd(const void* x, int64_t ldx, int x_dtype, const uint8_t* sc8, const float* sc32,
+                            int64_t blk, const void* dy, int64_t ldy, int dtype, int kind, int64_t rows,
+                            int64_t width, void* dx, hipStream_t stream);
+
+/* Log probabilities of one token per row of logits (f32 or bf16 [rows, vocab],
+ * rows ld elements apart; vocab below 2^31): logprobs [rows] f32; entropy [rows]
+ * f32 if not null; stats [rows][3] f32 if not null, for the backward pass; and
+ * the `top` (0 to 64, at most vocab) largest logits' log probabilities and
+ * indices [rows, top], in falling order, equal logits by index, NaN above all
+ * numbers.  A token below 0 stands for none (log probability 0); one of vocab or
+ * more gives NaN.  Logits of -inf are masked; a row of nothing else has log
+ * probabilities of -inf and entropy 0. */
+int pratchya_token_logprobs(const void* logits, int64_t ld, int dtype, const int64_t* tokens, int64_t rows,
+                            int64_t vocab, int top, float* logprobs, float* entropy, float* stats,
+                            float* top_logprobs, int64_t* top_tokens, hipStream_t stream);
+
+/* The logits' gradient from the cotangents of logprobs and entropy ([rows] f32,
+ * either may be null): d_logits contiguous [rows, vocab], of the logits' dtype. */
+int pratchya_token_logprobs_bwd(const void* logits, int64_t ld, int dtype, const int64_t* tokens, const float* stats,
+                                const float* g_logprobs, const float* g_entropy, int64_t rows, int64_t vocab,
+                                void* d_logits, hipStream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

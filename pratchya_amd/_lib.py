@@ -126,6 +126,21 @@ SIGNATURES = {
     "pratchya_planes": (_c_int, [_c_int, _c_p, _c_p, _c_p, _c_i64, _c_i64, _c_i64, _c_i64, _c_i64, _c_p, _c_p, _c_p]),
     "pratchya_gemm_span": (_c_i64, [_c_i64, _c_i64, _c_i64, _c_i64, _c_i64, _c_i64]),
     "pratchya_transpose_u8": (_c_int, [_c_p, _c_i64, _c_i64, _c_p, _c_p]),
+    "pratchya_layer_norm": (_c_int, [_c_p, _c_i64, _c_int, _c_p, _c_int, _c_p, _c_int, _c_i64, _c_i64, _c_i64,
+                                     ctypes.c_float, _c_p, _c_p, _c_p, _c_p, _c_p, _c_i64, _c_p]),
+    "pratchya_layer_norm_stores": (_c_int, [_c_i64, _c_i64, _c_i64]),
+    "pratchya_layer_norm_bwd_workspace_bytes": (_c_i64, [_c_i64, _c_i64, _c_i64]),
+    "pratchya_layer_norm_bwd": (_c_int, [_c_p, _c_i64, _c_int, _c_p, _c_p, _c_i64, _c_p, _c_i64, _c_int, _c_p, _c_int,
+                                         _c_p, _c_i64, _c_i64, _c_i64, _c_p, _c_p, _c_int, _c_p, _c_int, _c_p,
+                                         _c_i64, _c_p]),
+    "pratchya_activation": (_c_int, [_c_p, _c_i64, _c_int, _c_int, _c_i64, _c_i64, _c_p, _c_p, _c_p, _c_p, _c_i64,
+                                     _c_p]),
+    "pratchya_activation_bwd": (_c_int, [_c_p, _c_i64, _c_int, _c_p, _c_p, _c_i64, _c_p, _c_i64, _c_int, _c_int,
+                                         _c_i64, _c_i64, _c_p, _c_p]),
+    "pratchya_token_logprobs": (_c_int, [_c_p, _c_i64, _c_int, _c_p, _c_i64, _c_i64, _c_int, _c_p, _c_p, _c_p, _c_p,
+                                         _c_p, _c_p]),
+    "pratchya_token_logprobs_bwd": (_c_int, [_c_p, _c_i64, _c_int, _c_p, _c_p, _c_p, _c_p, _c_i64, _c_i64, _c_p,
+                                             _c_p]),
     "pratchya_mfma_ceiling": (_c_int, [_c_p, _c_p, _c_i64, _c_int, _c_i64, _c_p, ctypes.POINTER(_c_i64), _c_p]),
     "pratchya_debug_bf16_to_e4m3": (_c_int, [_c_p, _c_p, _c_i64, _c_int, _c_p]),
     "pratchya_debug_f32_to_bf16": (_c_int, [_c_p, _c_p, _c_i64, _c_int, _c_p]),
