@@ -718,10 +718,14 @@ int pratchya_activation_bwd(const void* x, int64_t ldx, int x_dtype, const uint8
  * indices [rows, top], in falling order, equal logits by index, NaN above all
  * numbers.  A token below 0 stands for none (log probability 0); one of vocab or
  * more gives NaN.  Logits of -inf are masked; a row of nothing else has log
- * probabilities of -inf and entropy 0. */
+ * probabilities of -inf and entropy 0.  Alternatives may need a workspace of
+ * pratchya_token_logprobs_workspace_bytes, 8-byte aligned.  stats hold the
+ * entropy only if entropy is not null. */
+int64_t pratchya_token_logprobs_workspace_bytes(int64_t rows, int64_t vocab, int top);
 int pratchya_token_logprobs(const void* logits, int64_t ld, int dtype, const int64_t* tokens, int64_t rows,
                             int64_t vocab, int top, float* logprobs, float* entropy, float* stats,
-                            float* top_logprobs, int64_t* top_tokens, hipStream_t stream);
+                            float* top_logprobs, int64_t* top_tokens, void* workspace, int64_t workspace_bytes,
+                            hipStream_t stream);
 
 /* The logits' gradient from the cotangents of logprobs and entropy ([rows] f32,
  * either may be null): d_logits contiguous [rows, vocab], of the logits' dtype. */

@@ -1718,11 +1718,15 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, entropy: bool = F
     st = torch.empty((rows, 3), dtype=torch.float32, device=dev) if stats else None
     top_lp = torch.empty(lead + (top,), dtype=torch.float32, device=dev) if top else None
     top_tok = torch.empty(lead + (top,), dtype=torch.int64, device=dev) if top else None
+    ws, ws_bytes = None, 0
+    if top:
+        ws_bytes = _ws_bytes("pratchya_token_logprobs_workspace_bytes", rows, vocab, top)
+        ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev) if ws_bytes else None
     _lib.check(_lib.load().pratchya_token_logprobs(
         logits.data_ptr(), ld, code, tokens.data_ptr(), rows, vocab, top, out.data_ptr(),
         None if ent is None else ent.data_ptr(), None if st is None else st.data_ptr(),
         None if top_lp is None else top_lp.data_ptr(), None if top_tok is None else top_tok.data_ptr(),
-        _stream(logits)), "token_logprobs")
+        None if ws is None else ws.data_ptr(), ws_bytes, _stream(logits)), "token_logprobs")
     return out, ent, top_lp, top_tok, st
 
 

@@ -137,8 +137,9 @@ SIGNATURES = {
                                      _c_p]),
     "pratchya_activation_bwd": (_c_int, [_c_p, _c_i64, _c_int, _c_p, _c_p, _c_i64, _c_p, _c_i64, _c_int, _c_int,
                                          _c_i64, _c_i64, _c_p, _c_p]),
+    "pratchya_token_logprobs_workspace_bytes": (_c_i64, [_c_i64, _c_i64, _c_int]),
     "pratchya_token_logprobs": (_c_int, [_c_p, _c_i64, _c_int, _c_p, _c_i64, _c_i64, _c_int, _c_p, _c_p, _c_p, _c_p,
-                                         _c_p, _c_p]),
+                                         _c_p, _c_p, _c_i64, _c_p]),
     "pratchya_token_logprobs_bwd": (_c_int, [_c_p, _c_i64, _c_int, _c_p, _c_p, _c_p, _c_p, _c_i64, _c_i64, _c_p,
                                              _c_p]),
     "pratchya_mfma_ceiling": (_c_int, [_c_p, _c_p, _c_i64, _c_int, _c_i64, _c_p, ctypes.POINTER(_c_i64), _c_p]),

@@ -21,6 +21,8 @@ int pratchya_set_error(int code, const char* fmt, ...);
 namespace {
 
 constexpr int kMaxTop = 64;
+constexpr float kLowest = -3.4028234663852886e38f;
+constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.69314718055994531f;
 
 int check_launch(const char* what) {
   const hipError_t e = hipGetLastError();
@@ -40,95 +42,360 @@ __device__ __forceinline__ uint32_t rank_bits(float x) {
 __device__ __forceinline__ uint64_t rank_key(float x, int64_t i) {
   return ((uint64_t)rank_bits(x) << 32) | (uint32_t)(0xFFFFFFFFu - (uint32_t)i);
 }
-
-template <int N>
-__device__ __forceinline__ float block_max(float v, float* lds) {
-#pragma unroll
-  for (int m = 32; m >= 1; m >>= 1) v = fmaxf(v, __shfl_xor(v, m, 64));
-  __syncthreads();
-  if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = v;
-  __syncthreads();
-  float s = lds[0];
-#pragma unroll
-  for (int i = 1; i < N; ++i) s = fmaxf(s, lds[i]);
-  return s;
-}
+__device__ __forceinline__ int64_t key_index(uint64_t key) { return 0xFFFFFFFFu - (uint32_t)key; }
 
 __device__ __forceinline__ uint64_t umax64(uint64_t a, uint64_t b) { return a > b ? a : b; }
+__device__ __forceinline__ uint64_t shfl_xor_u64(uint64_t v, int m) {
+  return (uint64_t)__shfl_xor((unsigned long long)v, m, 64);
+}
 
-template <typename T>
-__global__ __launch_bounds__(256) void k_logprobs(const T* __restrict__ x, int64_t ld,
-                                                  const int64_t* __restrict__ tokens, int64_t vocab, int top,
-                                                  float* __restrict__ logprobs, float* __restrict__ entropy,
-                                                  float* __restrict__ stats, float* __restrict__ top_logprobs,
-                                                  int64_t* __restrict__ top_tokens) {
-  __shared__ float lds[4];
-  __shared__ uint64_t best[4];
-  const int64_t row = blockIdx.x;
-  const T* xr = x + row * ld;
-  float m = -__builtin_inff();
-  for (int64_t i = threadIdx.x; i < vocab; i += 256) m = fmaxf(m, load_elem(xr + i));
-  m = block_max<4>(m, lds);
-  if (m == -__builtin_inff()) m = 0.0f;
-  float s = 0.0f, t = 0.0f;
-  for (int64_t i = threadIdx.x; i < vocab; i += 256) {
-    const float d = load_elem(xr + i) - m, e = __expf(d);
-    s += e;
-    t += e > 0.0f ? e * d : 0.0f;
+// A thread's running sums over the logits it has seen, relative to m: s = sum
+// 2^((x - m) log2 e), t = sum of the same times (x - m) log2 e.  m follows the
+// largest logit within kSlack only: a larger step of the sums is rare, and
+// e^kSlack times a row's length is far from f32's range.
+constexpr float kSlack = 8.0f;
+template <bool ENTROPY>
+struct Running {
+  float m = kLowest, s = 0.0f, t = 0.0f;
+
+  __device__ __forceinline__ void move(float to) {
+    // differences of infinities and lowest values count as lowest: their power is 0
+    const float d = fmaxf((m - to) * kLog2e, kLowest), f = __builtin_amdgcn_exp2f(d);
+    if constexpr (ENTROPY) t = f * (t + (f > 0.0f ? s * d : 0.0f));
+    s *= f;
+    m = to;
   }
-  s = block_add<4>(s, lds);
-  t = block_add<4>(t, lds);
-  const float logs = s == 0.0f ? 0.0f : logf(s), h = s == 0.0f ? 0.0f : logs - t / s;
-  if (threadIdx.x == 0) {
-    const int64_t tok = tokens[row];
-    float lp = 0.0f;
-    if (tok >= vocab) lp = __builtin_nanf("");
-    else if (tok >= 0) lp = (load_elem(xr + tok) - m) - logs;
-    logprobs[row] = lp;
-    if (entropy) entropy[row] = s != s ? s : h;
-    if (stats) {
-      stats[3 * row] = m;
-      stats[3 * row + 1] = logs;
-      stats[3 * row + 2] = h;
-    }
-  }
-  // one alternative after the other: the largest key below the last one found
-  uint64_t last = ~0ull;
-  for (int k = 0; k < top; ++k) {
-    uint64_t b = 0;
-    for (int64_t i = threadIdx.x; i < vocab; i += 256) {
-      const uint64_t key = rank_key(load_elem(xr + i), i);
-      if (key < last) b = umax64(b, key);
+  __device__ __forceinline__ void add(const float (&v)[kVec]) {
+    const float c = fmaxf(fmaxf(fmaxf(v[0], v[1]), fmaxf(v[2], v[3])), fmaxf(fmaxf(v[4], v[5]), fmaxf(v[6], v[7])));
+    if (__any(c > m + kSlack)) {
+      if (c > m) move(c);
     }
 #pragma unroll
-    for (int w = 32; w >= 1; w >>= 1) b = umax64(b, __shfl_xor((unsigned long long)b, w, 64));
-    __syncthreads();
-    if ((threadIdx.x & 63) == 0) best[threadIdx.x >> 6] = b;
-    __syncthreads();
-    last = umax64(umax64(best[0], best[1]), umax64(best[2], best[3]));
-    if (threadIdx.x == 0) {
-      const int64_t i = 0xFFFFFFFFu - (uint32_t)last;
-      top_tokens[row * top + k] = i;
-      top_logprobs[row * top + k] = (load_elem(xr + i) - m) - logs;
+    for (int i = 0; i < kVec; ++i) {
+      const float d = (v[i] - m) * kLog2e, e = __builtin_amdgcn_exp2f(d);
+      s += e;
+      if constexpr (ENTROPY) t += e * fmaxf(d, kLowest);   // 0, not NaN, for a masked logit
     }
+  }
+};
+
+// Maximum and sums over the WPR waves of a row, for every thread (lds: 3 * WPR floats).
+template <int WPR, bool ENTROPY>
+__device__ __forceinline__ void join_running(Running<ENTROPY>& r, float* lds) {
+  float m = r.m;
+#pragma unroll
+  for (int w = 32; w >= 1; w >>= 1) m = fmaxf(m, __shfl_xor(m, w, 64));
+  if constexpr (WPR > 1) {
+    if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = m;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < WPR; ++w) m = fmaxf(m, lds[w]);
+  }
+  r.move(m);
+  r.s = wave_add(r.s);
+  if constexpr (ENTROPY) r.t = wave_add(r.t);
+  if constexpr (WPR > 1) {
+    if ((threadIdx.x & 63) == 0) {
+      lds[WPR + (threadIdx.x >> 6)] = r.s;
+      if constexpr (ENTROPY) lds[2 * WPR + (threadIdx.x >> 6)] = r.t;
+    }
+    __syncthreads();
+    float s = 0.0f, t = 0.0f;
+#pragma unroll
+    for (int w = 0; w < WPR; ++w) {
+      s += lds[WPR + w];
+      if constexpr (ENTROPY) t += lds[2 * WPR + w];
+    }
+    r.s = s;
+    r.t = t;
   }
 }
 
-template <typename T>
+// log s and H of joined sums; a row without any unmasked logit has s = 0.
+template <bool ENTROPY>
+__device__ __forceinline__ void finish(Running<ENTROPY>& r, float& logs, float& h) {
+  logs = r.s == 0.0f ? 0.0f : logf(r.s);
+  h = r.s == 0.0f ? 0.0f : logs - (r.t / r.s) * kLn2;
+  if (r.s == 0.0f) r.m = 0.0f;
+}
+
+__device__ __forceinline__ float token_logprob(float x, float m, float logs) { return (x - m) - logs; }
+
+// Row results from joined sums: for one thread.
+__device__ __forceinline__ void store_row(float x_token, int64_t tok, int64_t vocab, int64_t row, float m, float logs,
+                                          float h, float* logprobs, float* entropy, float* stats) {
+  logprobs[row] = tok < 0 ? 0.0f : tok < vocab ? token_logprob(x_token, m, logs) : __builtin_nanf("");
+  if (entropy) entropy[row] = h;
+  if (stats) {
+    stats[3 * row] = m;
+    stats[3 * row + 1] = logs;
+    stats[3 * row + 2] = h;
+  }
+}
+
+constexpr int kUnroll = 4;        // vectors of one thread in flight
+
+// One row per WPR waves, 4 / WPR rows (at least one) per workgroup.
+template <typename T, int WPR, bool ENTROPY>
+__global__ __launch_bounds__(WPR < 4 ? 256 : WPR * 64) void k_logprobs(
+    const T* __restrict__ x, int64_t ld, const int64_t* __restrict__ tokens, int64_t rows, int64_t vocab,
+    float* __restrict__ logprobs, float* __restrict__ entropy, float* __restrict__ stats) {
+  constexpr int THREADS = WPR * 64, ROWS = WPR < 4 ? 4 / WPR : 1;
+  __shared__ float lds[3 * WPR];
+  const int tid = threadIdx.x % THREADS;
+  const int64_t row = (int64_t)blockIdx.x * ROWS + threadIdx.x / THREADS;
+  if (ROWS > 1 && row >= rows) return;      // whole waves; a row of one wave meets no barrier
+  const T* xr = x + row * ld;
+  const int64_t vecs = vocab / kVec;
+  Running<ENTROPY> r;
+  int64_t i = tid;
+  for (; i + (kUnroll - 1) * THREADS < vecs; i += kUnroll * THREADS) {
+    typename RawOf<T>::type raw[kUnroll];
+#pragma unroll
+    for (int u = 0; u < kUnroll; ++u) raw[u] = load_raw(xr + (i + u * THREADS) * kVec);
+#pragma unroll
+    for (int u = 0; u < kUnroll; ++u) {
+      float v[kVec];
+      widen(raw[u], v);
+      r.add(v);
+    }
+  }
+  for (; i < vecs; i += THREADS) {
+    float v[kVec];
+    widen(load_raw(xr + i * kVec), v);
+    r.add(v);
+  }
+  if (i == vecs && vocab % kVec) {
+    float v[kVec];
+    load_some(xr + vecs * kVec, vocab - vecs * kVec, -__builtin_inff(), v);
+    r.add(v);
+  }
+  join_running<WPR>(r, lds);
+  float logs, h;
+  finish(r, logs, h);
+  if (tid == 0) {
+    const int64_t tok = tokens[row];
+    store_row(tok >= 0 && tok < vocab ? load_elem(xr + tok) : 0.0f, tok, vocab, row, r.m, logs, h, logprobs, entropy,
+              stats);
+  }
+}
+
+// Alternatives.  A row is cut into parts of up to kBlock logits (longer ones where
+// that would be more than kParts), a workgroup each, because one compute unit
+// alone would take longer over a row than all parts and the join together; a part
+// stays in registers, so its logits are read once for the sums and the selection.
+constexpr int kPartThreads = 256, kPartVecs = 2, kBlock = kPartThreads * kPartVecs * kVec, kParts = 64;
+constexpr int kKeys = kPartVecs * kVec + 1;             // keys of a thread: a block's logits and one kept key
+
+// LDS of a selection among up to kKeys keys per thread.
+struct Selection {
+  uint64_t cand[kPartThreads * kKeys];
+  uint64_t seen[kPartThreads];
+  uint64_t bound;
+  int found;
+};
+
+// The `top` largest of all threads' keys (0: no key) in falling order into
+// out[0 .. top), padded with 0, for the whole workgroup.  The top-th largest of
+// the maxima of 64 groups (threads of equal lane) is a bound that `top` keys
+// reach, if there are so many; keys that reach it are collected and ranked by
+// counting.  A lane's keys lie 8 logits apart from its neighbours', so rows of
+// equal logits leave some 8 top candidates, as rising or falling ones do.
+// out may be written before all threads have read it (barriers below).
+__device__ __forceinline__ void select_top(const uint64_t (&keys)[kKeys], int top, Selection& sel, uint64_t* out) {
+  const int tid = threadIdx.x, lane = tid & 63;
+  uint64_t best = 0;
+#pragma unroll
+  for (int i = 0; i < kKeys; ++i) best = umax64(best, keys[i]);
+  sel.seen[tid] = best;
+  if (tid == 0) sel.found = 0;
+  __syncthreads();
+  if (tid < 64) {
+    const uint64_t own = umax64(umax64(sel.seen[lane], sel.seen[64 + lane]),
+                                umax64(sel.seen[128 + lane], sel.seen[192 + lane]));
+    int above = 0;
+#pragma unroll 8
+    for (int g = 0; g < 64; ++g) above += __shfl((unsigned long long)own, g, 64) > own;
+    // groups without a key are equal (0); where fewer than `top` have one, every key is collected
+    if (own ? above == top - 1 : above < top) sel.bound = own;
+  }
+  __syncthreads();
+  const uint64_t bound = sel.bound;
+  if (best != 0 && best >= bound) {
+#pragma unroll
+    for (int i = 0; i < kKeys; ++i)
+      if (keys[i] != 0 && keys[i] >= bound) sel.cand[atomicAdd(&sel.found, 1)] = keys[i];
+  }
+  __syncthreads();
+  const int n = sel.found;
+  if (tid >= n && tid < top) out[tid] = 0;
+  for (int c = tid; c < n; c += kPartThreads) {
+    const uint64_t own = sel.cand[c];
+    int above = 0;
+    for (int o = 0; o < n; ++o) above += sel.cand[o] > own;
+    if (above < top) out[above] = own;
+  }
+  __syncthreads();
+}
+
+struct Out {
+  float* logprobs;
+  float* entropy;
+  float* stats;
+  float* top_logprobs;
+  int64_t* top_tokens;
+};
+
+// One part of a row: its sums and its `top` largest keys, into sums
+// [rows][parts][3] and kept [rows][parts][top], or for a row of one part the
+// results themselves.
+template <typename T, bool ENTROPY>
+__global__ __launch_bounds__(kPartThreads) void k_logprobs_part(const T* __restrict__ x, int64_t ld,
+                                                                const int64_t* __restrict__ tokens, int64_t vocab,
+                                                                int top, int parts, int64_t part_len,
+                                                                float* __restrict__ sums, uint64_t* __restrict__ kept,
+                                                                Out o) {
+  __shared__ float lds[3 * 4];
+  __shared__ Selection sel;
+  __shared__ uint64_t list[kMaxTop];
+  const int tid = threadIdx.x;
+  const int64_t row = blockIdx.x / (unsigned)parts;
+  const int part = (int)(blockIdx.x - (unsigned)row * (unsigned)parts);
+  const T* xr = x + row * ld;
+  const int64_t from = part * part_len, to = from + part_len < vocab ? from + part_len : vocab;
+  Running<ENTROPY> r;
+  if (tid < kMaxTop) list[tid] = 0;
+  __syncthreads();
+  for (int64_t base = from; base < to; base += kBlock) {
+    float v[kPartVecs][kVec];
+#pragma unroll
+    for (int u = 0; u < kPartVecs; ++u) {
+      const int64_t at = base + (u * kPartThreads + tid) * kVec;
+      if (at + kVec <= to) widen(load_raw(xr + at), v[u]);
+      else load_some(xr + at, to - at, -__builtin_inff(), v[u]);
+    }
+    uint64_t keys[kKeys];
+#pragma unroll
+    for (int u = 0; u < kPartVecs; ++u) {
+      const int64_t at = base + (u * kPartThreads + tid) * kVec;
+      if (at < to) r.add(v[u]);
+#pragma unroll
+      for (int j = 0; j < kVec; ++j) keys[u * kVec + j] = at + j < to ? rank_key(v[u][j], at + j) : 0;
+    }
+    keys[kKeys - 1] = tid < top ? list[tid] : 0;
+    select_top(keys, top, sel, list);
+  }
+  join_running<4>(r, lds);
+  if (parts > 1) {
+    const int64_t at = row * parts + part;
+    if (tid < top) kept[at * top + tid] = list[tid];
+    if (tid < 3) sums[at * 3 + tid] = tid == 0 ? r.m : tid == 1 ? r.s : r.t;
+    return;
+  }
+  float logs, h;
+  finish(r, logs, h);
+  if (tid == 0) {
+    const int64_t tok = tokens[row];
+    store_row(tok >= 0 && tok < vocab ? load_elem(xr + tok) : 0.0f, tok, vocab, row, r.m, logs, h, o.logprobs,
+              o.entropy, o.stats);
+  }
+  if (tid < top) {
+    const int64_t i = key_index(list[tid]);
+    o.top_tokens[row * top + tid] = i;
+    o.top_logprobs[row * top + tid] = token_logprob(load_elem(xr + i), r.m, logs);
+  }
+}
+
+// The parts of a row (at most kParts) together.
+template <typename T, bool ENTROPY>
+__global__ __launch_bounds__(kPartThreads) void k_logprobs_join(const T* __restrict__ x, int64_t ld,
+                                                                const int64_t* __restrict__ tokens, int64_t vocab,
+                                                                int top, int parts, const float* __restrict__ sums,
+                                                                const uint64_t* __restrict__ kept, Out o) {
+  __shared__ Selection sel;
+  __shared__ uint64_t list[kMaxTop];
+  static_assert(kParts * kMaxTop <= kPartThreads * kKeys, "a thread's keys hold every part's");
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int64_t row = blockIdx.x;
+  const T* xr = x + row * ld;
+  uint64_t keys[kKeys];
+#pragma unroll
+  for (int i = 0; i < kKeys; ++i) {
+    const int at = i * kPartThreads + tid;
+    keys[i] = at < parts * top ? kept[row * parts * top + at] : 0;
+  }
+  // every wave joins the sums: a part per lane
+  Running<ENTROPY> r;
+  if (lane < parts) {
+    const float* p = sums + (row * parts + lane) * 3;
+    r.m = p[0];
+    r.s = p[1];
+    r.t = p[2];
+  }
+  join_running<1>(r, nullptr);
+  float logs, h;
+  finish(r, logs, h);
+  if (tid == 0) {
+    const int64_t tok = tokens[row];
+    store_row(tok >= 0 && tok < vocab ? load_elem(xr + tok) : 0.0f, tok, vocab, row, r.m, logs, h, o.logprobs,
+              o.entropy, o.stats);
+  }
+  select_top(keys, top, sel, list);
+  if (tid < top) {
+    const int64_t i = key_index(list[tid]);
+    o.top_tokens[row * top + tid] = i;
+    o.top_logprobs[row * top + tid] = token_logprob(load_elem(xr + i), r.m, logs);
+  }
+}
+
+// dx of kVec * kUnroll * TPR logits of a row per TPR threads: elementwise, one
+// read and one write of each logit.
+template <typename T, int TPR>
 __global__ __launch_bounds__(256) void k_logprobs_bwd(const T* __restrict__ x, int64_t ld,
                                                       const int64_t* __restrict__ tokens,
                                                       const float* __restrict__ stats, const float* __restrict__ g,
-                                                      const float* __restrict__ gh, int64_t vocab,
-                                                      T* __restrict__ dx) {
-  const int64_t row = blockIdx.x;
+                                                      const float* __restrict__ gh, int64_t rows, int64_t vocab,
+                                                      unsigned pieces, T* __restrict__ dx) {
+  const int tid = threadIdx.x % TPR;
+  // several rows per workgroup are rows of one piece
+  const int64_t row = TPR < 256 ? (int64_t)blockIdx.x * (256 / TPR) + threadIdx.x / TPR : blockIdx.x / pieces;
+  const int64_t first = TPR < 256 ? tid : (int64_t)(blockIdx.x - (unsigned)row * pieces) * (TPR * kUnroll) + tid;
+  if (row >= rows) return;
   const int64_t tok = tokens[row];
-  const float m = stats[3 * row], logs = stats[3 * row + 1], H = stats[3 * row + 2];
-  const float c = g && tok >= 0 ? g[row] : 0.0f, ch = gh ? gh[row] : 0.0f;
-  for (int64_t i = threadIdx.x; i < vocab; i += 256) {
-    const float lp = (load_elem(x + row * ld + i) - m) - logs, p = __expf(lp);
-    float v = p == 0.0f ? 0.0f : -p * (c + ch * (lp + H));
-    if (i == tok) v += c;
-    store_elem(dx + row * vocab + i, v);
+  const float m = stats[3 * row], logs = stats[3 * row + 1];
+  const float c = g && tok >= 0 ? g[row] : 0.0f, ch = gh ? gh[row] : 0.0f, H = stats[3 * row + 2];
+  const T* xr = x + row * ld;
+  T* dr = dx + row * vocab;
+  auto grad = [&](float (&v)[kVec], int64_t at) {
+#pragma unroll
+    for (int i = 0; i < kVec; ++i) {
+      const float lp = (v[i] - m) - logs, p = __builtin_amdgcn_exp2f(lp * kLog2e);
+      v[i] = -p * (c + ch * (fmaxf(lp, -1000.0f) + H));   // a masked logit: p = 0 times a finite number
+    }
+    if ((uint64_t)(tok - at) < (uint64_t)kVec) {
+#pragma unroll
+      for (int i = 0; i < kVec; ++i)
+        if (at + i == tok) v[i] += c;
+    }
+  };
+  typename RawOf<T>::type raw[kUnroll];
+  const int64_t vecs = vocab / kVec;
+#pragma unroll
+  for (int u = 0; u < kUnroll; ++u)
+    if (first + u * TPR < vecs) raw[u] = load_raw(xr + (first + u * TPR) * kVec);
+#pragma unroll
+  for (int u = 0; u < kUnroll; ++u) {
+    const int64_t i = first + u * TPR;
+    float v[kVec];
+    if (i < vecs) {
+      widen(raw[u], v);
+      grad(v, i * kVec);
+      store_vec(dr + i * kVec, v);
+    } else if (i == vecs && vocab % kVec) {
+      load_some(xr + i * kVec, vocab - i * kVec, 0.0f, v);
+      grad(v, i * kVec);
+      store_some(dr + i * kVec, vocab - i * kVec, v);
+    }
   }
 }
 
@@ -141,11 +408,78 @@ int check_args(const char* what, int dtype, int64_t rows, int64_t vocab) {
   return PRATCHYA_OK;
 }
 
+// How a row with alternatives is cut.
+struct Cut {
+  int parts;
+  int64_t len;
+};
+Cut cut_row(int64_t vocab) {
+  const int64_t blocks = (vocab + kBlock - 1) / kBlock, per = (blocks + kParts - 1) / kParts;
+  return {(int)((blocks + per - 1) / per), per * kBlock};
+}
+// The keys of all rows' parts, then their sums.
+int64_t keys_bytes(int64_t rows, int parts, int top) { return rows * parts * top * (int64_t)sizeof(uint64_t); }
+
+template <typename T, bool ENTROPY>
+int launch(const void* logits, int64_t ld, const int64_t* tokens, int64_t rows, int64_t vocab, int top, Out o,
+           void* workspace, hipStream_t stream) {
+  const T* x = static_cast<const T*>(logits);
+  if (top) {
+    const Cut cut = cut_row(vocab);
+    if (rows * cut.parts > 0x7FFFFFFF)
+      return pratchya_set_error(PRATCHYA_EUNSUPPORTED, "token_logprobs: more than 2^31 parts of rows");
+    uint64_t* kept = static_cast<uint64_t*>(workspace);
+    float* sums = reinterpret_cast<float*>(static_cast<char*>(workspace) + keys_bytes(rows, cut.parts, top));
+    hipLaunchKernelGGL((k_logprobs_part<T, ENTROPY>), dim3((unsigned)(rows * cut.parts)), dim3(kPartThreads), 0, stream,
+                       x, ld, tokens, vocab, top, cut.parts, cut.len, sums, kept, o);
+    if (cut.parts > 1)
+      hipLaunchKernelGGL((k_logprobs_join<T, ENTROPY>), dim3((unsigned)rows), dim3(kPartThreads), 0, stream, x, ld,
+                         tokens, vocab, top, cut.parts, sums, kept, o);
+    return check_launch("token_logprobs");
+  }
+#define PRATCHYA_LP(WPR)                                                                                            \
+  hipLaunchKernelGGL((k_logprobs<T, WPR, ENTROPY>), dim3((unsigned)((rows + (WPR < 4 ? 4 / WPR : 1) - 1) /          \
+                                                                     (WPR < 4 ? 4 / WPR : 1))),                     \
+                     dim3(WPR < 4 ? 256 : WPR * 64), 0, stream, x, ld, tokens, rows, vocab, o.logprobs, o.entropy,  \
+                     o.stats)
+  if (vocab <= 2048) PRATCHYA_LP(1);
+  else if (rows < 512) PRATCHYA_LP(16);
+  else PRATCHYA_LP(4);
+#undef PRATCHYA_LP
+  return check_launch("token_logprobs");
+}
+
+template <typename T>
+int launch_bwd(const void* logits, int64_t ld, const int64_t* tokens, const float* stats, const float* g,
+               const float* gh, int64_t rows, int64_t vocab, void* dx, hipStream_t stream) {
+  const int tpr = vocab <= 64 * kVec * kUnroll ? 64 : 256;
+  const int64_t pieces = (vocab + (int64_t)tpr * kVec * kUnroll - 1) / ((int64_t)tpr * kVec * kUnroll);
+  const int64_t blocks = (rows * pieces + 256 / tpr - 1) / (256 / tpr);
+  if (blocks > 0x7FFFFFFF)
+    return pratchya_set_error(PRATCHYA_EUNSUPPORTED, "token_logprobs_bwd: more than 2^31 workgroups");
+  if (tpr == 64)
+    hipLaunchKernelGGL((k_logprobs_bwd<T, 64>), dim3((unsigned)blocks), dim3(256), 0, stream,
+                       static_cast<const T*>(logits), ld, tokens, stats, g, gh, rows, vocab,
+                       (unsigned)pieces, static_cast<T*>(dx));
+  else
+    hipLaunchKernelGGL((k_logprobs_bwd<T, 256>), dim3((unsigned)blocks), dim3(256), 0, stream,
+                       static_cast<const T*>(logits), ld, tokens, stats, g, gh, rows, vocab,
+                       (unsigned)pieces, static_cast<T*>(dx));
+  return check_launch("token_logprobs_bwd");
+}
+
 }  // namespace
+
+extern "C" int64_t pratchya_token_logprobs_workspace_bytes(int64_t rows, int64_t vocab, int top) {
+  if (rows < 1 || vocab < 1 || vocab > 0x7FFFFFFF || top < 1) return 0;
+  const Cut cut = cut_row(vocab);
+  return cut.parts > 1 ? keys_bytes(rows, cut.parts, top) + rows * cut.parts * 3 * (int64_t)sizeof(float) : 0;
+}
 
 extern "C" int pratchya_token_logprobs(const void* logits, int64_t ld, int dtype, const int64_t* tokens, int64_t rows,
                                        int64_t vocab, int top, float* logprobs, float* entropy, float* stats,
-                                       float* top_logprobs, int64_t* top_tokens, hipStream_t stream) {
+                                       float* top_logprobs, int64_t* top_tokens, void* workspace,
+                                       int64_t workspace_bytes, hipStream_t stream) {
   const int rc = check_args("token_logprobs", dtype, rows, vocab);
   if (rc) return rc;
   if (top < 0 || top > kMaxTop || top > vocab)
@@ -154,15 +488,15 @@ extern "C" int pratchya_token_logprobs(const void* logits, int64_t ld, int dtype
   if (rows == 0) return pratchya_set_error(PRATCHYA_OK, "");
   if (!logits || !tokens || !logprobs || (top && (!top_logprobs || !top_tokens)))
     return pratchya_set_error(PRATCHYA_EINVAL, "token_logprobs: null buffer");
-  if (dtype == PRATCHYA_DT_BF16)
-    hipLaunchKernelGGL((k_logprobs<uint16_t>), dim3((unsigned)rows), dim3(256), 0, stream,
-                       static_cast<const uint16_t*>(logits), ld, tokens, vocab, top, logprobs, entropy, stats,
-                       top_logprobs, top_tokens);
-  else
-    hipLaunchKernelGGL((k_logprobs<float>), dim3((unsigned)rows), dim3(256), 0, stream,
-                       static_cast<const float*>(logits), ld, tokens, vocab, top, logprobs, entropy, stats,
-                       top_logprobs, top_tokens);
-  return check_launch("token_logprobs");
+  const int64_t need = pratchya_token_logprobs_workspace_bytes(rows, vocab, top);
+  if (need && (!workspace || workspace_bytes < need || reinterpret_cast<uintptr_t>(workspace) % 8))
+    return pratchya_set_error(PRATCHYA_EINVAL, "token_logprobs: workspace of %lld bytes needed, 8-byte aligned",
+                              (long long)need);
+  const Out o = {logprobs, entropy, stats, top_logprobs, top_tokens};
+#define PRATCHYA_LPT(T, E) launch<T, E>(logits, ld, tokens, rows, vocab, top, o, workspace, stream)
+  if (dtype == PRATCHYA_DT_BF16) return entropy ? PRATCHYA_LPT(uint16_t, true) : PRATCHYA_LPT(uint16_t, false);
+  return entropy ? PRATCHYA_LPT(float, true) : PRATCHYA_LPT(float, false);
+#undef PRATCHYA_LPT
 }
 
 extern "C" int pratchya_token_logprobs_bwd(const void* logits, int64_t ld, int dtype, const int64_t* tokens,
@@ -173,13 +507,7 @@ extern "C" int pratchya_token_logprobs_bwd(const void* logits, int64_t ld, int d
   if (rows == 0) return pratchya_set_error(PRATCHYA_OK, "");
   if (!logits || !tokens || !stats || !d_logits)
     return pratchya_set_error(PRATCHYA_EINVAL, "token_logprobs_bwd: null buffer");
-  if (dtype == PRATCHYA_DT_BF16)
-    hipLaunchKernelGGL((k_logprobs_bwd<uint16_t>), dim3((unsigned)rows), dim3(256), 0, stream,
-                       static_cast<const uint16_t*>(logits), ld, tokens, stats, g_logprobs, g_entropy, vocab,
-                       static_cast<uint16_t*>(d_logits));
-  else
-    hipLaunchKernelGGL((k_logprobs_bwd<float>), dim3((unsigned)rows), dim3(256), 0, stream,
-                       static_cast<const float*>(logits), ld, tokens, stats, g_logprobs, g_entropy, vocab,
-                       static_cast<float*>(d_logits));
-  return check_launch("token_logprobs_bwd");
+  return dtype == PRATCHYA_DT_BF16
+             ? launch_bwd<uint16_t>(logits, ld, tokens, stats, g_logprobs, g_entropy, rows, vocab, d_logits, stream)
+             : launch_bwd<float>(logits, ld, tokens, stats, g_logprobs, g_entropy, rows, vocab, d_logits, stream);
 }

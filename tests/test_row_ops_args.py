@@ -74,13 +74,16 @@ def test_token_logprobs():
     lib = L.load()
 
     def fwd(x=FAKE, dtype=1, tokens=FAKE, rows=4, vocab=96, top=0, out=FAKE, best=None):
-        return lib.pratchya_token_logprobs(x, vocab, dtype, tokens, rows, vocab, top, out, None, None, best, best, None)
+        return lib.pratchya_token_logprobs(x, vocab, dtype, tokens, rows, vocab, top, out, None, None, best, best, None,
+                                           0, None)
     assert fwd(rows=0) == L.OK
     for bad in (dict(dtype=2), dict(rows=-1), dict(vocab=0), dict(vocab=1 << 31), dict(top=-1), dict(top=65),
                 dict(top=97, vocab=96), dict(top=3), dict(x=None), dict(tokens=None), dict(out=None)):
         assert fwd(**bad) == L.EINVAL, bad
         assert b"token_logprobs" in lib.pratchya_last_error()
     assert fwd(rows=1 << 31) == L.EUNSUPPORTED
+    assert lib.pratchya_token_logprobs_workspace_bytes(4, 96, 20) == 0 and fwd(vocab=1 << 20, top=3, best=FAKE) == L.EINVAL
+    assert b"workspace" in lib.pratchya_last_error()
 
     def bwd(x=FAKE, dtype=1, stats=FAKE, rows=4, vocab=96, dx=FAKE):
         return lib.pratchya_token_logprobs_bwd(x, vocab, dtype, FAKE, stats, None, None, rows, vocab, dx, None)
