@@ -43,10 +43,209 @@ struct Affine {
   bool w16, b16;
 };
 
+// A segment that fits P threads of NV vectors of eight elements each stays in
+// registers.  A workgroup of TB threads holds TB / P such teams; a team keeps one
+// segment position of the row (its slice of w and b, and of dw and db) and walks
+// over rows: `gt` neighbouring segments side by side, the other teams on
+// further rows.  Thread t of a team holds vectors (t / 64 * NV + j) * 64 + t % 64
+// (P >= 64), so a wave reads runs of 512 elements and groups of stored blocks lie
+// in one wave.
+template <int P_, int NV_, int TB_>
+struct Shape {
+  static constexpr int P = P_, NV = NV_, TB = TB_, TEAMS = TB_ / P_, WAVES = P_ > 64 ? P_ / 64 : 1;
+};
+
+template <typename G>
+struct Place {
+  int t, team;         // thread in its team, team in the workgroup
+  int rl, rt;          // the team's row lane, row lanes
+  int64_t g;           // its segment of the row
+  bool live;
+  __device__ __forceinline__ Place(int64_t groups) {
+    t = threadIdx.x % G::P;
+    team = threadIdx.x / G::P;
+    const int gt = groups < G::TEAMS ? (int)groups : G::TEAMS;
+    rt = G::TEAMS / gt;
+    rl = team / gt;
+    g = (int64_t)blockIdx.y * gt + team % gt;
+    live = rl < rt && g < groups;
+  }
+  // first element of this thread's vector j in its segment
+  __device__ __forceinline__ int64_t at(int j) const {
+    if constexpr (G::P < 64) return t * kVec;
+    else return (int64_t)(((t >> 6) * G::NV + j) * 64 + (t & 63)) * kVec;
+  }
+};
+
+__device__ __forceinline__ int clamp8(int64_t n) { return n < 0 ? 0 : n < kVec ? (int)n : kVec; }
+
 template <typename T>
-__global__ __launch_bounds__(256) void k_layer_norm(const T* __restrict__ x, int64_t ldx, Affine p, int64_t width,
-                                                    int64_t groups, float eps, T* __restrict__ y,
-                                                    float* __restrict__ stats) {
+__device__ __forceinline__ void load_vec_or_some(const T* p, int left, float (&v)[kVec]) {
+  if (left == kVec) widen(load_raw(p), v);
+  else load_some(p, left, 0.0f, v);
+}
+
+// A vector of a row in registers, in its type.
+template <typename T>
+struct Held {
+  typename RawOf<T>::type raw;
+  __device__ __forceinline__ void load(const T* p, int left) {
+    if (left == kVec) {
+      raw = load_raw(p);
+    } else {
+      float v[kVec];
+      load_some(p, left, 0.0f, v);
+      if constexpr (sizeof(T) == 2)
+        raw.v = u32x4_t{pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]), pack_bf16x2(v[4], v[5]),
+                        pack_bf16x2(v[6], v[7])};
+      else {
+        raw.lo = u32x4_t{f2u(v[0]), f2u(v[1]), f2u(v[2]), f2u(v[3])};
+        raw.hi = u32x4_t{f2u(v[4]), f2u(v[5]), f2u(v[6]), f2u(v[7])};
+      }
+    }
+  }
+  __device__ __forceinline__ void get(float (&v)[kVec]) const { widen(raw, v); }
+};
+
+__device__ __forceinline__ void load_params(const void* p, bool bf16, int64_t at, int left, float none,
+                                            float (&v)[kVec]) {
+  if (!p) {
+#pragma unroll
+    for (int i = 0; i < kVec; ++i) v[i] = none;
+  } else if (bf16) {
+    load_vec_or_some(static_cast<const uint16_t*>(p) + at, left, v);
+  } else {
+    load_vec_or_some(static_cast<const float*>(p) + at, left, v);
+  }
+}
+
+// y and the statistics of whole segments; with BLK, x's stored form beside them
+// (groups = 1).  Mean and squared deviations are taken within each wave, from
+// registers, and joined by counts, so a mean far from zero costs no digits.
+template <typename T, typename G, int BLK>
+__global__ __launch_bounds__(G::TB) void k_layer_norm(const T* __restrict__ x, int64_t ldx, Affine p, int64_t rows,
+                                                      int64_t width, int64_t groups, float eps, T* __restrict__ y,
+                                                      float* __restrict__ stats, uint8_t* __restrict__ x8,
+                                                      uint8_t* __restrict__ sc8, float* __restrict__ sc32) {
+  constexpr int NV = G::NV, LANES = G::P < 64 ? G::P : 64;
+  __shared__ float red[2][G::TEAMS * G::WAVES][2];
+  const Place<G> me(groups);
+  const int64_t D = width / groups, c0 = me.g * D;
+  int left[NV];
+  float w[NV][kVec], b[NV][kVec];
+#pragma unroll
+  for (int j = 0; j < NV; ++j) {
+    left[j] = me.live ? clamp8(D - me.at(j)) : 0;
+    load_params(p.w, p.w16, c0 + me.at(j), left[j], 1.0f, w[j]);
+    load_params(p.b, p.b16, c0 + me.at(j), left[j], 0.0f, b[j]);
+  }
+  // elements of the segment that this wave holds
+  const int64_t first = (int64_t)(me.t >> 6) * NV * 512;
+  const float mine = G::P < 64 ? (float)D : (float)(D - first < 0 ? 0 : D - first < NV * 512 ? D - first : NV * 512);
+  const int64_t step = (int64_t)gridDim.x * me.rt;
+  int64_t row = (int64_t)blockIdx.x * me.rt + me.rl;
+  Held<T> cur[NV], next[NV];
+#pragma unroll
+  for (int j = 0; j < NV; ++j) next[j].load(x + row * ldx + c0 + me.at(j), row < rows ? left[j] : 0);
+  // the workgroup's first team has the first row: all teams make as many rounds
+  int buf = 0;
+  for (int64_t lead = (int64_t)blockIdx.x * me.rt; lead < rows; lead += step, row += step, buf ^= 1) {
+    const bool on = me.live && row < rows;
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+      cur[j] = next[j];
+      next[j].load(x + (row + step) * ldx + c0 + me.at(j), row + step < rows ? left[j] : 0);
+    }
+    float v[kVec], s = 0.0f, q = 0.0f;
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+      cur[j].get(v);
+#pragma unroll
+      for (int i = 0; i < kVec; ++i) s += v[i];
+    }
+    s = lane_group_add<LANES>(s);
+    float mean = mine > 0.0f ? s / mine : 0.0f;
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+      cur[j].get(v);
+#pragma unroll
+      for (int i = 0; i < kVec; ++i) {
+        const float d = v[i] - mean;
+        q += i < left[j] ? d * d : 0.0f;
+      }
+    }
+    q = lane_group_add<LANES>(q);
+    if constexpr (G::WAVES > 1) {
+      float (*r)[2] = &red[buf][me.team * G::WAVES];
+      if ((me.t & 63) == 0) {
+        r[me.t >> 6][0] = s;
+        r[me.t >> 6][1] = q;
+      }
+      __syncthreads();
+      float sum = 0.0f;
+#pragma unroll
+      for (int k = 0; k < G::WAVES; ++k) sum += r[k][0];
+      mean = sum / (float)D;
+      q = 0.0f;
+#pragma unroll
+      for (int k = 0; k < G::WAVES; ++k) {
+        const int64_t from = (int64_t)k * NV * 512;
+        if (from < D) {
+          const float n = (float)(D - from < NV * 512 ? D - from : NV * 512), d = r[k][0] / n - mean;
+          q += r[k][1] + n * d * d;
+        }
+      }
+    }
+    const float rstd = 1.0f / sqrtf(q / (float)D + eps);
+    if (!on) continue;
+    if (stats && me.t == 0) {
+      stats[2 * (row * groups + me.g)] = mean;
+      stats[2 * (row * groups + me.g) + 1] = rstd;
+    }
+    T* yr = y + row * width + c0;
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+      cur[j].get(v);
+#pragma unroll
+      for (int i = 0; i < kVec; ++i) v[i] = (v[i] - mean) * rstd * w[j][i] + b[j][i];
+      if (left[j] == kVec) store_vec(yr + me.at(j), v);
+      else if (left[j]) store_some(yr + me.at(j), left[j], v);
+    }
+    if constexpr (BLK != 0) {
+      constexpr int LB = BLK / kVec, LG = BLK <= 16 ? LB : BLK == 32 ? 8 : BLK == 64 ? 32 : 64;
+      uint32_t mb[NV], Gb[NV];
+#pragma unroll
+      for (int j = 0; j < NV; ++j) {
+        cur[j].get(v);
+        mb[j] = lane_group_max<LB>(absmax8(v));
+        Gb[j] = lane_group_max<LG>(mb[j]);
+      }
+      if constexpr (BLK == 128) {
+#pragma unroll
+        for (int j = 0; j + 1 < NV; j += 2) Gb[j] = Gb[j + 1] = umax(Gb[j], Gb[j + 1]);
+      }
+#pragma unroll
+      for (int j = 0; j < NV; ++j) {
+        if (left[j] == 0) continue;
+        cur[j].get(v);
+        uint32_t e;
+        const int64_t at = row * width + me.at(j);
+        const u32x2_t q8 = store_form(v, mb[j], Gb[j], e);
+        *reinterpret_cast<u32x2_t*>(x8 + at) = q8;
+        constexpr int K = BLK <= 16 ? 1 : BLK / 16;
+        if (at % BLK == 0) sc8[at / BLK] = (uint8_t)e;
+        if (at % (BLK * K) == 0) sc32[at / (BLK * K)] = u2f(Gb[j]);
+      }
+    }
+  }
+}
+
+// Segments longer than a workgroup's registers: three passes over the row, the
+// later ones from the caches.
+template <typename T>
+__global__ __launch_bounds__(256) void k_layer_norm_long(const T* __restrict__ x, int64_t ldx, Affine p, int64_t width,
+                                                         int64_t groups, float eps, T* __restrict__ y,
+                                                         float* __restrict__ stats) {
   __shared__ float lds[4];
   const int64_t D = width / groups, row = blockIdx.x / groups, c0 = (blockIdx.x - row * groups) * D;
   const T* xs = x + row * ldx + c0;
@@ -72,7 +271,7 @@ __global__ __launch_bounds__(256) void k_layer_norm(const T* __restrict__ x, int
   }
 }
 
-// x as the backward pass reads it: element i of row `row`.
+// x as the backward pass reads it: as it is, or its stored form.
 template <typename X>
 struct Source {
   const X* x;
@@ -83,15 +282,197 @@ struct Stored {
   const uint8_t* x8;
   const uint8_t* sc8;
   const float* sc32;
-  int64_t width, blk, K;
+  int64_t width;
+  int blk_log2, K_log2;      // elements per block and blocks per group are powers of two
   __device__ __forceinline__ float at(int64_t row, int64_t i) const {
-    const int64_t e = row * width + i, n = e / blk;
-    return (e4m3fn_to_f32(x8[e]) * (e8m0_decode(sc8[n]) * sc32[n / K])) * 0.0078125f;
+    const int64_t e = row * width + i, n = e >> blk_log2;
+    return (e4m3fn_to_f32(x8[e]) * (e8m0_decode(sc8[n]) * sc32[n >> K_log2])) * 0.0078125f;
   }
 };
+template <typename T, bool STORED> struct SourceOf { typedef Source<T> type; };
+template <typename T> struct SourceOf<T, true> { typedef Stored type; };
+
+// The backward pass's x of one vector: as it is, or its stored form.
+template <typename T, bool STORED> struct HeldSource;
+template <typename T> struct HeldSource<T, false> {
+  Held<T> x;
+  __device__ __forceinline__ void load(const Source<T>& s, int64_t row, int64_t c, int left) {
+    x.load(s.x + row * s.ldx + c, left);
+  }
+  __device__ __forceinline__ void get(float (&v)[kVec]) const { x.get(v); }
+};
+template <typename T> struct HeldSource<T, true> {
+  u32x2_t w;
+  uint32_t e;
+  float G;
+  __device__ __forceinline__ void load(const Stored& s, int64_t row, int64_t c, int left) {
+    w = u32x2_t{0, 0};
+    e = 0;
+    G = 0.0f;
+    if (left) {     // blocks are a multiple of eight elements: a vector lies in one
+      const int64_t at = row * s.width + c, n = at >> s.blk_log2;
+      w = *reinterpret_cast<const u32x2_t*>(s.x8 + at);
+      e = s.sc8[n];
+      G = s.sc32[n >> s.K_log2];
+    }
+  }
+  __device__ __forceinline__ void get(float (&v)[kVec]) const { stored_values(w, e8m0_decode(e) * G, v); }
+};
+
+// dx of whole segments, and the sums of dy h and dy over the rows that a team
+// has walked: joined over the workgroup's row lanes and written to
+// part[blockIdx.x][0 / 1][width], or as the results where there is one workgroup
+// per column.
+template <typename T, typename G, bool STORED, bool AHEAD>
+__global__ __launch_bounds__(G::TB) void k_layer_norm_bwd(typename SourceOf<T, STORED>::type src,
+                                                          const T* __restrict__ dy, int64_t ldy, Affine p,
+                                                          int64_t rows, int64_t width, int64_t groups,
+                                                          const float* __restrict__ stats, T* __restrict__ dx,
+                                                          float* __restrict__ part, void* dw, bool dw16, void* db,
+                                                          bool db16) {
+  constexpr int NV = G::NV, LANES = G::P < 64 ? G::P : 64, SUMS = 2 * NV * kVec;
+  __shared__ float red[2][G::TEAMS * G::WAVES][2];
+  __shared__ float sums[G::TEAMS > 1 ? SUMS * (G::TB / 2) : 1];
+  const Place<G> me(groups);
+  const int64_t D = width / groups, c0 = me.g * D;
+  int left[NV];
+  float w[NV][kVec], aw[NV][kVec], ab[NV][kVec];
+#pragma unroll
+  for (int j = 0; j < NV; ++j) {
+    left[j] = me.live ? clamp8(D - me.at(j)) : 0;
+    load_params(p.w, p.w16, c0 + me.at(j), left[j], 1.0f, w[j]);
+#pragma unroll
+    for (int i = 0; i < kVec; ++i) aw[j][i] = ab[j][i] = 0.0f;
+  }
+  const int64_t step = (int64_t)gridDim.x * me.rt;
+  int64_t row = (int64_t)blockIdx.x * me.rt + me.rl;
+  HeldSource<T, STORED> cx[NV], nx[NV];
+  Held<T> cg[NV], ng[NV];
+  float nm = 0.0f, nr = 0.0f;
+  auto fetch = [&](int64_t r) {
+    const bool on = me.live && r < rows;
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+      nx[j].load(src, r, c0 + me.at(j), on ? left[j] : 0);
+      ng[j].load(dy + r * ldy + c0 + me.at(j), on ? left[j] : 0);
+    }
+    nm = on ? stats[2 * (r * groups + me.g)] : 0.0f;
+    nr = on ? stats[2 * (r * groups + me.g) + 1] : 0.0f;
+  };
+  if constexpr (AHEAD) fetch(row);
+  int buf = 0;
+  for (int64_t lead = (int64_t)blockIdx.x * me.rt; lead < rows; lead += step, row += step, buf ^= 1) {
+    if constexpr (!AHEAD) fetch(row);
+    const float mean = nm, rstd = nr;
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+      cx[j] = nx[j];
+      cg[j] = ng[j];
+    }
+    if constexpr (AHEAD) fetch(row + step);
+    float s1 = 0.0f, s2 = 0.0f, h[kVec], g[kVec];
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+      cx[j].get(h);
+      cg[j].get(g);
+#pragma unroll
+      for (int i = 0; i < kVec; ++i) {
+        h[i] = (h[i] - mean) * rstd;
+        aw[j][i] += g[i] * h[i];
+        ab[j][i] += g[i];
+        const float a = g[i] * w[j][i];
+        s1 += a;
+        s2 += a * h[i];
+      }
+    }
+    if (dx) {
+      s1 = lane_group_add<LANES>(s1);
+      s2 = lane_group_add<LANES>(s2);
+      if constexpr (G::WAVES > 1) {
+        float (*r)[2] = &red[buf][me.team * G::WAVES];
+        if ((me.t & 63) == 0) {
+          r[me.t >> 6][0] = s1;
+          r[me.t >> 6][1] = s2;
+        }
+        __syncthreads();
+        s1 = s2 = 0.0f;
+#pragma unroll
+        for (int k = 0; k < G::WAVES; ++k) {
+          s1 += r[k][0];
+          s2 += r[k][1];
+        }
+      }
+      const float m1 = s1 / (float)D, m2 = s2 / (float)D;
+      if (me.live && row < rows) {
+        T* out = dx + row * width + c0;
+#pragma unroll
+        for (int j = 0; j < NV; ++j) {
+          cx[j].get(h);
+          cg[j].get(g);
+#pragma unroll
+          for (int i = 0; i < kVec; ++i) g[i] = rstd * (g[i] * w[j][i] - m1 - (h[i] - mean) * rstd * m2);
+          if (left[j] == kVec) store_vec(out + me.at(j), g);
+          else if (left[j]) store_some(out + me.at(j), left[j], g);
+        }
+      }
+    }
+  }
+  if (!dw && !db) return;
+  // the row lanes' sums, halves onto halves
+  if constexpr (G::TEAMS > 1) {
+    const int cols = G::TEAMS / me.rt * G::P;      // threads of one row lane at most
+    const int col = (int)threadIdx.x - me.rl * (groups < G::TEAMS ? (int)groups * G::P : G::TB);
+    for (int n = me.rt; n > 1;) {
+      const int half = (n + 1) / 2;
+      if (me.rl >= half && me.rl < n) {
+#pragma unroll
+        for (int j = 0; j < NV; ++j)
+#pragma unroll
+          for (int i = 0; i < kVec; ++i) {
+            sums[(j * kVec + i) * (G::TB / 2) + (me.rl - half) * cols + col] = aw[j][i];
+            sums[((NV + j) * kVec + i) * (G::TB / 2) + (me.rl - half) * cols + col] = ab[j][i];
+          }
+      }
+      __syncthreads();
+      if (me.rl < n - half) {
+#pragma unroll
+        for (int j = 0; j < NV; ++j)
+#pragma unroll
+          for (int i = 0; i < kVec; ++i) {
+            aw[j][i] += sums[(j * kVec + i) * (G::TB / 2) + me.rl * cols + col];
+            ab[j][i] += sums[((NV + j) * kVec + i) * (G::TB / 2) + me.rl * cols + col];
+          }
+      }
+      __syncthreads();
+      n = half;
+    }
+  }
+  if (!me.live || me.rl) return;
+#pragma unroll
+  for (int j = 0; j < NV; ++j) {
+    const int64_t c = c0 + me.at(j);
+    if (gridDim.x > 1) {
+      float* to = part + 2 * (int64_t)blockIdx.x * width + c;
+      if (left[j] == kVec) {
+        store_vec(to, aw[j]);
+        store_vec(to + width, ab[j]);
+      } else {
+        store_some(to, left[j], aw[j]);
+        store_some(to + width, left[j], ab[j]);
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < kVec; ++i)
+        if (i < left[j]) {
+          if (dw) store_param(dw, dw16, c + i, aw[j][i]);
+          if (db) store_param(db, db16, c + i, ab[j][i]);
+        }
+    }
+  }
+}
 
 template <typename T, typename S>
-__global__ __launch_bounds__(256) void k_layer_norm_dx(S src, const T* __restrict__ dy, int64_t ldy, Affine p,
+__global__ __launch_bounds__(256) void k_layer_norm_long_dx(S src, const T* __restrict__ dy, int64_t ldy, Affine p,
                                                        int64_t width, int64_t groups, const float* __restrict__ stats,
                                                        T* __restrict__ dx) {
   __shared__ float lds[4];
@@ -116,7 +497,7 @@ __global__ __launch_bounds__(256) void k_layer_norm_dx(S src, const T* __restric
 
 // Column sums over the rows of one of gridDim.y slices: part[slice][0 / 1][width].
 template <typename T, typename S>
-__global__ __launch_bounds__(256) void k_layer_norm_dp(S src, const T* __restrict__ dy, int64_t ldy, int64_t rows,
+__global__ __launch_bounds__(256) void k_layer_norm_long_dp(S src, const T* __restrict__ dy, int64_t ldy, int64_t rows,
                                                        int64_t width, int64_t groups,
                                                        const float* __restrict__ stats, float* __restrict__ part) {
   const int64_t c = (int64_t)blockIdx.x * 256 + threadIdx.x;
@@ -133,57 +514,160 @@ __global__ __launch_bounds__(256) void k_layer_norm_dp(S src, const T* __restric
   part[(2 * (int64_t)blockIdx.y + 1) * width + c] = db;
 }
 
-__global__ __launch_bounds__(256) void k_layer_norm_join(const float* __restrict__ part, int slices, int64_t width,
-                                                         void* dw, bool dw16, void* db, bool db16) {
-  const int64_t c = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  if (c >= width) return;
+// dw and db from the slices' sums: kJoinCols columns per workgroup, its waves on
+// different slices.
+constexpr int kJoinCols = 64, kJoinWaves = 16, kJoinThreads = kJoinWaves * 64;
+__global__ __launch_bounds__(kJoinThreads) void k_layer_norm_join(const float* __restrict__ part, int slices,
+                                                                  int64_t width, void* dw, bool dw16, void* db,
+                                                                  bool db16) {
+  __shared__ float lds[2][kJoinWaves][64];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int64_t c = (int64_t)blockIdx.x * kJoinCols + lane;
   float s = 0.0f, t = 0.0f;
-  for (int i = 0; i < slices; ++i) {
-    s += part[2 * i * width + c];
-    t += part[(2 * i + 1) * width + c];
+  if (c < width) {
+#pragma unroll 4
+    for (int i = wave; i < slices; i += kJoinWaves) {
+      s += part[2 * i * width + c];
+      t += part[(2 * i + 1) * width + c];
+    }
   }
-  if (dw) store_param(dw, dw16, c, s);
-  if (db) store_param(db, db16, c, t);
+  lds[0][wave][lane] = s;
+  lds[1][wave][lane] = t;
+  __syncthreads();
+  if (wave > 1 || c >= width) return;
+  void* to = wave ? db : dw;
+  if (!to) return;
+  s = 0.0f;
+#pragma unroll
+  for (int k = 0; k < kJoinWaves; ++k) s += lds[wave][k][lane];
+  store_param(to, wave ? db16 : dw16, c, s);
 }
 
-constexpr int kSlices = 64;
+constexpr int64_t kLongest = 16384;     // elements of a segment held in registers
+constexpr int kSlices = 64;             // row slices of the long segments' column sums
+
+bool power_of_two(int64_t v) { return v > 0 && (v & (v - 1)) == 0; }
+int log2_of(int64_t v) {
+  int n = 0;
+  while (v > 1) {
+    v >>= 1;
+    ++n;
+  }
+  return n;
+}
 
 int check_shape(const char* what, int64_t rows, int64_t width, int64_t groups) {
   if (rows < 0 || width < 0 || groups < 1 || width % groups)
     return pratchya_set_error(PRATCHYA_EINVAL, "%s: %lld groups do not divide rows of %lld (%lld rows)", what,
                               (long long)groups, (long long)width, (long long)rows);
-  if (rows > 0 && (rows * groups > 0x7FFFFFFF || width / 256 > 0x7FFFFFFF))
-    return pratchya_set_error(PRATCHYA_EUNSUPPORTED, "%s: more than 2^31 segments", what);
+  if (rows > 0x7FFFFFFF || groups > (1 << 20) || rows * groups > 0x7FFFFFFF || width > ((int64_t)1 << 38))
+    return pratchya_set_error(PRATCHYA_EUNSUPPORTED, "%s: more than 2^31 segments, or 2^20 in a row", what);
   return PRATCHYA_OK;
 }
 
-template <typename T, typename S>
-int launch_bwd(S src, const void* dy, int64_t ldy, const void* w, int w_dtype, const float* stats, int64_t rows,
-               int64_t width, int64_t groups, void* dx, void* dw, int dw_dtype, void* db, int db_dtype, float* part,
-               hipStream_t stream) {
+// Calls f(Shape) with the smallest team that holds a segment of D elements.
+// Forward teams share workgroups of 256 threads, backward teams of `TB`.
+template <int TB, typename F>
+auto with_shape(int64_t D, F f) {
+  if (D <= 64) return f(Shape<8, 1, TB>());
+  if (D <= 128) return f(Shape<16, 1, TB>());
+  if (D <= 256) return f(Shape<32, 1, TB>());
+  if (D <= 512) return f(Shape<64, 1, TB>());
+  if (D <= 1024) return f(Shape<64, 2, TB>());
+  if (D <= 2048) return f(Shape<128, 2, TB>());
+  if (D <= 4096) return f(Shape<256, 2, TB>());
+  if (D <= 8192) return f(Shape<512, 2, 512>());
+  return f(Shape<1024, 2, 1024>());
+}
+
+// Workgroups along the rows and along the segments of a row.
+template <typename G>
+dim3 grid_of(int64_t rows, int64_t groups, int64_t most) {
+  const int64_t gt = groups < G::TEAMS ? groups : G::TEAMS, rt = G::TEAMS / gt;
+  const int64_t gy = (groups + gt - 1) / gt, gx = (rows + rt - 1) / rt, cap = most / gy > 1 ? most / gy : 1;
+  return dim3((unsigned)(gx < cap ? gx : cap), (unsigned)gy);
+}
+
+constexpr int kFwdThreads = 256, kBwdThreads = 512;
+constexpr int64_t kFwdBlocks = 2048, kBwdBlocks = 512;
+
+dim3 bwd_grid(int64_t rows, int64_t width, int64_t groups) {
+  return with_shape<kBwdThreads>(width / groups, [&](auto shape) {
+    return grid_of<decltype(shape)>(rows, groups, kBwdBlocks * kBwdThreads / decltype(shape)::TB);
+  });
+}
+
+template <typename T, typename G>
+void launch_fwd(G, const T* x, int64_t ldx, const Affine& p, int64_t rows, int64_t width, int64_t groups, float eps,
+                T* y, float* stats, uint8_t* x8, uint8_t* sc8, float* sc32, int64_t blk, hipStream_t stream) {
+  const dim3 grid = grid_of<G>(rows, groups, kFwdBlocks * kFwdThreads / G::TB);
+#define PRATCHYA_LN(B)                                                                                              \
+  hipLaunchKernelGGL((k_layer_norm<T, G, B>), grid, dim3(G::TB), 0, stream, x, ldx, p, rows, width, groups, eps, y, \
+                     stats, x8, sc8, sc32)
+  if (!x8) PRATCHYA_LN(0);
+  else if (blk == 16) PRATCHYA_LN(16);
+  else if (blk == 32) PRATCHYA_LN(32);
+  else if (blk == 64) { if constexpr (G::P >= 32) PRATCHYA_LN(64); }
+  else { if constexpr (G::P >= 64 && G::NV >= 2) PRATCHYA_LN(128); }
+#undef PRATCHYA_LN
+}
+
+template <typename T>
+int layer_norm(const void* x, int64_t ldx, const Affine& p, int64_t rows, int64_t width, int64_t groups, float eps,
+               void* y, float* stats, uint8_t* x8, uint8_t* sc8, float* sc32, int64_t blk, hipStream_t stream) {
+  const T* xt = static_cast<const T*>(x);
+  T* yt = static_cast<T*>(y);
+  if (width / groups > kLongest)
+    hipLaunchKernelGGL((k_layer_norm_long<T>), dim3((unsigned)(rows * groups)), dim3(256), 0, stream, xt, ldx, p, width,
+                       groups, eps, yt, stats);
+  else
+    with_shape<kFwdThreads>(width / groups, [&](auto shape) {
+      launch_fwd<T>(shape, xt, ldx, p, rows, width, groups, eps, yt, stats, x8, sc8, sc32, blk, stream);
+    });
+  return check_launch("layer_norm");
+}
+
+template <typename T, bool STORED>
+int layer_norm_bwd(typename SourceOf<T, STORED>::type src, const void* dy, int64_t ldy, const void* w, int w_dtype,
+                   const float* stats, int64_t rows, int64_t width, int64_t groups, void* dx, void* dw, int dw_dtype,
+                   void* db, int db_dtype, float* part, hipStream_t stream) {
+  typedef typename SourceOf<T, STORED>::type S;
   const T* g = static_cast<const T*>(dy);
   const Affine p = {w, nullptr, w_dtype == PRATCHYA_DT_BF16, false};
-  if (dx)
-    hipLaunchKernelGGL((k_layer_norm_dx<T, S>), dim3((unsigned)(rows * groups)), dim3(256), 0, stream, src, g, ldy, p,
-                       width, groups, stats, static_cast<T*>(dx));
-  if (dw || db) {
-    const int slices = rows < kSlices ? (int)rows : kSlices;
-    const dim3 grid((unsigned)((width + 255) / 256), (unsigned)slices);
-    hipLaunchKernelGGL((k_layer_norm_dp<T, S>), grid, dim3(256), 0, stream, src, g, ldy, rows, width, groups, stats,
-                       part);
-    hipLaunchKernelGGL(k_layer_norm_join, dim3(grid.x), dim3(256), 0, stream, part, slices, width, dw,
-                       dw_dtype == PRATCHYA_DT_BF16, db, db_dtype == PRATCHYA_DT_BF16);
+  const bool dw16 = dw_dtype == PRATCHYA_DT_BF16, db16 = db_dtype == PRATCHYA_DT_BF16;
+  int slices = 1;
+  if (width / groups > kLongest) {
+    if (dx)
+      hipLaunchKernelGGL((k_layer_norm_long_dx<T, S>), dim3((unsigned)(rows * groups)), dim3(256), 0, stream, src, g,
+                         ldy, p, width, groups, stats, static_cast<T*>(dx));
+    if (dw || db) {
+      slices = rows < kSlices ? (int)rows : kSlices;
+      hipLaunchKernelGGL((k_layer_norm_long_dp<T, S>), dim3((unsigned)((width + 255) / 256), (unsigned)slices),
+                         dim3(256), 0, stream, src, g, ldy, rows, width, groups, stats, part);
+    }
+  } else {
+    with_shape<kBwdThreads>(width / groups, [&](auto shape) {
+      typedef decltype(shape) G;
+      // a workgroup of 1024 threads has 128 registers a thread, none for a row ahead
+      constexpr bool AHEAD = G::TB <= 512;
+      const dim3 grid = grid_of<G>(rows, groups, kBwdBlocks * kBwdThreads / G::TB);
+      slices = (int)grid.x;
+      hipLaunchKernelGGL((k_layer_norm_bwd<T, G, STORED, AHEAD>), grid, dim3(G::TB), 0, stream, src, g, ldy, p, rows,
+                         width, groups, stats, static_cast<T*>(dx), part, dw, dw16, db, db16);
+    });
+    if (slices == 1) return check_launch("layer_norm_bwd");
   }
+  if (dw || db)
+    hipLaunchKernelGGL(k_layer_norm_join, dim3((unsigned)((width + kJoinCols - 1) / kJoinCols)), dim3(kJoinThreads), 0,
+                       stream, part, slices, width, dw, dw16, db, db16);
   return check_launch("layer_norm_bwd");
 }
 
 }  // namespace
 
 extern "C" int pratchya_layer_norm_stores(int64_t width, int64_t groups, int64_t blk) {
-  (void)width;
-  (void)groups;
-  (void)blk;
-  return 0;
+  if (groups != 1 || width < 1 || width > kLongest || (blk != 16 && blk != 32 && blk != 64 && blk != 128)) return 0;
+  return width % (blk * (blk / 16)) == 0;      // whole groups of blk / 16 blocks in a row
 }
 
 extern "C" int pratchya_layer_norm(const void* x, int64_t ldx, int dtype, const void* w, int w_dtype, const void* b,
@@ -192,8 +676,6 @@ extern "C" int pratchya_layer_norm(const void* x, int64_t ldx, int dtype, const 
                                    hipStream_t stream) {
   const int rc = check_shape("layer_norm", rows, width, groups);
   if (rc) return rc;
-  (void)sc8;
-  (void)sc32;
   if (x8 && !pratchya_layer_norm_stores(width, groups, blk))
     return pratchya_set_error(PRATCHYA_EUNSUPPORTED, "layer_norm: blocks of %lld are not stored in the same pass",
                               (long long)blk);
@@ -201,21 +683,17 @@ extern "C" int pratchya_layer_norm(const void* x, int64_t ldx, int dtype, const 
     return pratchya_set_error(PRATCHYA_EINVAL, "layer_norm: unsupported dtypes (x %d, weight %d, bias %d)", dtype,
                               w_dtype, b_dtype);
   if (rows == 0 || width == 0) return pratchya_set_error(PRATCHYA_OK, "");
-  if (!x || !y) return pratchya_set_error(PRATCHYA_EINVAL, "layer_norm: null buffer");
+  if (!x || !y || (x8 && (!sc8 || !sc32))) return pratchya_set_error(PRATCHYA_EINVAL, "layer_norm: null buffer");
   const Affine p = {w, b, w_dtype == PRATCHYA_DT_BF16, b_dtype == PRATCHYA_DT_BF16};
-  const dim3 grid((unsigned)(rows * groups));
-  if (dtype == PRATCHYA_DT_BF16)
-    hipLaunchKernelGGL((k_layer_norm<uint16_t>), grid, dim3(256), 0, stream, static_cast<const uint16_t*>(x), ldx, p,
-                       width, groups, eps, static_cast<uint16_t*>(y), stats);
-  else
-    hipLaunchKernelGGL((k_layer_norm<float>), grid, dim3(256), 0, stream, static_cast<const float*>(x), ldx, p, width,
-                       groups, eps, static_cast<float*>(y), stats);
-  return check_launch("layer_norm");
+  return dtype == PRATCHYA_DT_BF16
+             ? layer_norm<uint16_t>(x, ldx, p, rows, width, groups, eps, y, stats, x8, sc8, sc32, blk, stream)
+             : layer_norm<float>(x, ldx, p, rows, width, groups, eps, y, stats, x8, sc8, sc32, blk, stream);
 }
 
 extern "C" int64_t pratchya_layer_norm_bwd_workspace_bytes(int64_t rows, int64_t width, int64_t groups) {
-  (void)groups;
-  return (rows < kSlices ? rows : kSlices) * 2 * width * (int64_t)sizeof(float);
+  if (rows < 1 || width < 1 || groups < 1 || width % groups) return 0;
+  const int64_t slices = width / groups > kLongest ? (rows < kSlices ? rows : kSlices) : bwd_grid(rows, width, groups).x;
+  return slices * 2 * width * (int64_t)sizeof(float);
 }
 
 extern "C" int pratchya_layer_norm_bwd(const void* x, int64_t ldx, int x_dtype, const uint8_t* sc8, const float* sc32,
@@ -229,9 +707,11 @@ extern "C" int pratchya_layer_norm_bwd(const void* x, int64_t ldx, int x_dtype, 
   if (!is_float_dtype(dtype) || (!stored && x_dtype != dtype) || (w && !is_float_dtype(w_dtype)) ||
       (dw && !is_float_dtype(dw_dtype)) || (db && !is_float_dtype(db_dtype)))
     return pratchya_set_error(PRATCHYA_EINVAL, "layer_norm_bwd: unsupported dtypes (x %d, dy %d)", x_dtype, dtype);
-  if (stored && (blk < 1 || width % blk))
-    return pratchya_set_error(PRATCHYA_EINVAL, "layer_norm_bwd: blocks of %lld do not divide rows of %lld",
-                              (long long)blk, (long long)width);
+  if (stored && (blk < kVec || !power_of_two(blk) || width % blk))
+    return pratchya_set_error(PRATCHYA_EINVAL, "layer_norm_bwd: blocks of %lld for rows of %lld", (long long)blk,
+                              (long long)width);
+  if (stored && reinterpret_cast<uintptr_t>(x) % 8)
+    return pratchya_set_error(PRATCHYA_EINVAL, "layer_norm_bwd: the payload must be 8-byte aligned");
   if (rows == 0 || width == 0) return pratchya_set_error(PRATCHYA_OK, "");
   if (!x || !dy || !stats || (stored && (!sc8 || !sc32)))
     return pratchya_set_error(PRATCHYA_EINVAL, "layer_norm_bwd: null buffer");
@@ -240,15 +720,16 @@ extern "C" int pratchya_layer_norm_bwd(const void* x, int64_t ldx, int x_dtype, 
     return pratchya_set_error(PRATCHYA_EINVAL, "layer_norm_bwd: workspace of %lld bytes needed, 4-byte aligned",
                               (long long)need);
   float* part = static_cast<float*>(workspace);
-#define PRATCHYA_LNB(T, SRC)                                                                                     \
-  launch_bwd<T>(SRC, dy, ldy, w, w_dtype, stats, rows, width, groups, dx, dw, dw_dtype, db, db_dtype, part, stream)
+#define PRATCHYA_LNB(T, ST, SRC)                                                                                   \
+  layer_norm_bwd<T, ST>(SRC, dy, ldy, w, w_dtype, stats, rows, width, groups, dx, dw, dw_dtype, db, db_dtype, part, \
+                        stream)
   if (stored) {
-    const int64_t n_blk = rows * (width / blk);
-    const Stored s = {static_cast<const uint8_t*>(x), sc8, sc32, width, blk, gcd64(blk / 16 > 1 ? blk / 16 : 1, n_blk)};
-    return dtype == PRATCHYA_DT_BF16 ? PRATCHYA_LNB(uint16_t, s) : PRATCHYA_LNB(float, s);
+    const int64_t K = gcd64(blk / 16 > 1 ? blk / 16 : 1, rows * (width / blk));
+    const Stored s = {static_cast<const uint8_t*>(x), sc8, sc32, width, log2_of(blk), log2_of(K)};
+    return dtype == PRATCHYA_DT_BF16 ? PRATCHYA_LNB(uint16_t, true, s) : PRATCHYA_LNB(float, true, s);
   }
   if (dtype == PRATCHYA_DT_BF16)
-    return PRATCHYA_LNB(uint16_t, (Source<uint16_t>{static_cast<const uint16_t*>(x), ldx}));
-  return PRATCHYA_LNB(float, (Source<float>{static_cast<const float*>(x), ldx}));
+    return PRATCHYA_LNB(uint16_t, false, (Source<uint16_t>{static_cast<const uint16_t*>(x), ldx}));
+  return PRATCHYA_LNB(float, false, (Source<float>{static_cast<const float*>(x), ldx}));
 #undef PRATCHYA_LNB
 }

@@ -214,17 +214,24 @@ __device__ __forceinline__ void select_top(const uint64_t (&keys)[kKeys], int to
     const uint64_t own = umax64(umax64(sel.seen[lane], sel.seen[64 + lane]),
                                 umax64(sel.seen[128 + lane], sel.seen[192 + lane]));
     int above = 0;
-#pragma unroll 8
-    for (int g = 0; g < 64; ++g) above += __shfl((unsigned long long)own, g, 64) > own;
+#pragma unroll
+    for (int g = 0; g < 64; ++g) {
+      const uint64_t other = (uint64_t)readlane_u32((uint32_t)(own >> 32), g) << 32 | readlane_u32((uint32_t)own, g);
+      above += other > own;
+    }
     // groups without a key are equal (0); where fewer than `top` have one, every key is collected
     if (own ? above == top - 1 : above < top) sel.bound = own;
   }
   __syncthreads();
   const uint64_t bound = sel.bound;
   if (best != 0 && best >= bound) {
+    int mine = 0;
+#pragma unroll
+    for (int i = 0; i < kKeys; ++i) mine += keys[i] != 0 && keys[i] >= bound;
+    int at = atomicAdd(&sel.found, mine);
 #pragma unroll
     for (int i = 0; i < kKeys; ++i)
-      if (keys[i] != 0 && keys[i] >= bound) sel.cand[atomicAdd(&sel.found, 1)] = keys[i];
+      if (keys[i] != 0 && keys[i] >= bound) sel.cand[at++] = keys[i];
   }
   __syncthreads();
   const int n = sel.found;
@@ -232,6 +239,7 @@ __device__ __forceinline__ void select_top(const uint64_t (&keys)[kKeys], int to
   for (int c = tid; c < n; c += kPartThreads) {
     const uint64_t own = sel.cand[c];
     int above = 0;
+#pragma unroll 8
     for (int o = 0; o < n; ++o) above += sel.cand[o] > own;
     if (above < top) out[above] = own;
   }

@@ -97,12 +97,31 @@ __device__ __forceinline__ void store_some(T* p, int64_t n, const float (&v)[kVe
     if (i < n) store_elem(p + i, v[i]);
 }
 
-// Sum over the lanes of a wave, for every lane.
-__device__ __forceinline__ float wave_add(float v) {
-#pragma unroll
-  for (int m = 32; m >= 1; m >>= 1) v += __shfl_xor(v, m, 64);
+// Sum over aligned groups of BL lanes, for every lane of the group (the
+// exchanges of lane_group_max; every lane adds the same pairs, so all get the
+// same bits).
+template <int CTRL>
+__device__ __forceinline__ float dpp_add_f32(float v) {
+  return v + u2f((uint32_t)__builtin_amdgcn_update_dpp(0, (int)f2u(v), CTRL, 0xF, 0xF, true));
+}
+template <int BL>
+__device__ __forceinline__ float lane_group_add(float v) {
+  if constexpr (BL >= 2) v = dpp_add_f32<0xB1>(v);   // quad_perm [1,0,3,2]
+  if constexpr (BL >= 4) v = dpp_add_f32<0x4E>(v);   // quad_perm [2,3,0,1]
+  if constexpr (BL >= 8) v = dpp_add_f32<0x141>(v);  // row_half_mirror
+  if constexpr (BL >= 16) v = dpp_add_f32<0x140>(v); // row_mirror
+  if constexpr (BL >= 32) {
+    const auto p = __builtin_amdgcn_permlane16_swap(f2u(v), f2u(v), false, false);
+    v = u2f(p[0]) + u2f(p[1]);
+  }
+  if constexpr (BL >= 64) {
+    const auto p = __builtin_amdgcn_permlane32_swap(f2u(v), f2u(v), false, false);
+    v = u2f(p[0]) + u2f(p[1]);
+  }
   return v;
 }
+// Sum over the lanes of a wave, for every lane.
+__device__ __forceinline__ float wave_add(float v) { return lane_group_add<64>(v); }
 
 // Sum over a workgroup of N waves, for every thread.  lds: N floats that
 // nothing else uses between the call's barriers.
@@ -116,4 +135,50 @@ __device__ __forceinline__ float block_add(float v, float* lds) {
 #pragma unroll
   for (int i = 1; i < N; ++i) s += lds[i];
   return s;
+}
+
+// --------------------------------------------------------------------------
+// The 8-bit form of a row's values, eight consecutive ones per lane: blocks of
+// BLK elements are BLK / 8 neighbouring lanes, groups of BLK / 16 blocks (one
+// for 16) up to 32 lanes, or for BLK 128 the wave's 64 lanes of two vectors.
+// --------------------------------------------------------------------------
+__device__ __forceinline__ uint32_t absmax8(const float (&v)[kVec]) {
+  uint32_t m = 0;
+#pragma unroll
+  for (int i = 0; i < kVec; ++i) m = umax(m, abs_bits(v[i]));
+  return m;
+}
+
+// The payload of eight values of a block with maximum mb in a group with
+// maximum Gb (f32 bits), and the block's e8m0 byte: quantize_impl's (fp8_math.h),
+// by the division-free cast of block_scale; values near a bf16 rounding
+// midpoint, and clamped blocks and groups that are not finite, by the exact
+// composition.
+__device__ __forceinline__ u32x2_t store_form(const float (&v)[kVec], uint32_t mb, uint32_t Gb, uint32_t& e) {
+  const float G = u2f(Gb);
+  const BlockScale b = block_scale(mb, Gb, __builtin_amdgcn_rcpf(G * 0.0078125f));
+  e = b.e;
+  bool fast = is_finite_f(G) && !b.clamped;
+  u32x2_t w = {0, 0};
+  if (fast) {
+    float t[kVec];
+#pragma unroll
+    for (int i = 0; i < kVec; ++i) t[i] = v[i] * b.y;
+    w = {cvt4_hw(t[0], t[1], t[2], t[3]), cvt4_hw(t[4], t[5], t[6], t[7])};
+    fast = umin(mid_key4(t[0], t[1], t[2], t[3]), mid_key4(t[4], t[5], t[6], t[7])) > kMidKey;
+  }
+  if (!fast) {
+    e = b.clamped || !is_finite_f(G) ? e8m0_of(u2f(mb), G) : b.e;
+    const float S = quant_scale(e, G);
+    w = {cvt4_exact(v[0], v[1], v[2], v[3], S), cvt4_exact(v[4], v[5], v[6], v[7], S)};
+  }
+  return w;
+}
+
+// What eight payload bytes of a block stand for.
+__device__ __forceinline__ void stored_values(u32x2_t w, float scale, float (&v)[kVec]) {
+  fp8_word(w.x, v[0], v[1], v[2], v[3]);
+  fp8_word(w.y, v[4], v[5], v[6], v[7]);
+#pragma unroll
+  for (int i = 0; i < kVec; ++i) v[i] = (v[i] * scale) * 0.0078125f;
 }
