@@ -1671,9 +1671,10 @@ def activation(x: torch.Tensor, kind: str, tgrid=None):
     x, ldx = _strided_rows(x)
     rows = x.numel() // width if width else 0
     y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    stored = quantize(x.reshape(rows, width), (1, blk)) if blk else None
-    _lib.check(_lib.load().pratchya_activation(x.data_ptr(), ldx, code, k, rows, width, y.data_ptr(), None, None,
-                                               None, 0, _stream(x)), "activation")
+    stored = _stored_buffers(rows, width, blk, x.device) if blk else None
+    q = [t.data_ptr() for t in stored] if blk else (None, None, None)
+    _lib.check(_lib.load().pratchya_activation(x.data_ptr(), ldx, code, k, rows, width, y.data_ptr(), q[0], q[1], q[2],
+                                               blk, _stream(x)), "activation")
     return y, stored
 
 

@@ -33,48 +33,196 @@ int check_launch(const char* what) {
 
 bool is_float_dtype(int d) { return d == PRATCHYA_DT_F32 || d == PRATCHYA_DT_BF16; }
 
-__device__ __forceinline__ float act(float x, int kind) {
+constexpr float kLog2e = 1.4426950408889634f;
+
+// P(x) and p(x) of the normal distribution: with z = |x| / sqrt 2 and t = 1 / (1 +
+// 0.3275911 z), erfc(z) = (a1 t + ... + a5 t^5) e^(-z^2) to 1.5e-7 (Abramowitz and
+// Stegun, Handbook of Mathematical Functions, 7.1.26); p shares the exponential.
+__device__ __forceinline__ void normal(float x, float& P, float& p) {
+  const float z = fabsf(x) * 0.70710678118654752f;
+  const float t = __builtin_amdgcn_rcpf(__builtin_fmaf(0.3275911f, z, 1.0f));
+  const float e = __builtin_amdgcn_exp2f(-z * z * kLog2e);
+  float c = __builtin_fmaf(1.061405429f, t, -1.453152027f);
+  c = __builtin_fmaf(c, t, 1.421413741f);
+  c = __builtin_fmaf(c, t, -0.284496736f);
+  c = __builtin_fmaf(c, t, 0.254829592f);
+  const float tail = 0.5f * c * t * e;       // P(-|x|)
+  P = x < 0.0f ? tail : 1.0f - tail;
+  p = 0.39894228040143268f * e;
+}
+__device__ __forceinline__ float sigmoid(float x) {
+  return __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(-x * kLog2e));
+}
+
+// f of eight values; the kind is the same for the whole launch.
+__device__ __forceinline__ void act(float (&v)[kVec], int kind) {
   if (kind == PRATCHYA_ACT_RELU2) {
-    const float r = x < 0.0f ? 0.0f : x;
-    return r * r;
-  }
-  if (kind == PRATCHYA_ACT_SILU) return x / (1.0f + __expf(-x));
-  return 0.5f * x * (1.0f + erff(x * 0.70710678118654752f));
-}
-
-__device__ __forceinline__ float act_grad(float x, int kind) {
-  if (kind == PRATCHYA_ACT_RELU2) return x < 0.0f ? 0.0f : 2.0f * x;
-  if (kind == PRATCHYA_ACT_SILU) {
-    const float s = 1.0f / (1.0f + __expf(-x));
-    return s * (1.0f + x * (1.0f - s));
-  }
-  return 0.5f * (1.0f + erff(x * 0.70710678118654752f)) + x * 0.39894228040143268f * __expf(-0.5f * x * x);
-}
-
-template <typename T>
-__global__ __launch_bounds__(256) void k_act(const T* __restrict__ x, int64_t ldx, int64_t width, int64_t n, int kind,
-                                             T* __restrict__ y) {
-  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) {
-    const int64_t row = i / width;
-    store_elem(y + i, act(load_elem(x + row * ldx + (i - row * width)), kind));
-  }
-}
-
-template <typename T>
-__global__ __launch_bounds__(256) void k_act_bwd(const T* __restrict__ x, int64_t ldx, const uint8_t* __restrict__ x8,
-                                                 const uint8_t* __restrict__ sc8, const float* __restrict__ sc32,
-                                                 int64_t blk, int64_t K, const T* __restrict__ dy, int64_t ldy,
-                                                 int64_t width, int64_t n, int kind, T* __restrict__ dx) {
-  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) {
-    const int64_t row = i / width, c = i - row * width;
-    float v;
-    if (x8) {
-      const int64_t k = i / blk;
-      v = (e4m3fn_to_f32(x8[i]) * (e8m0_decode(sc8[k]) * sc32[k / K])) * 0.0078125f;
-    } else {
-      v = load_elem(x + row * ldx + c);
+#pragma unroll
+    for (int i = 0; i < kVec; ++i) {
+      const float r = v[i] < 0.0f ? 0.0f : v[i];
+      v[i] = r * r;
     }
-    store_elem(dx + i, act_grad(v, kind) * load_elem(dy + row * ldy + c));
+  } else if (kind == PRATCHYA_ACT_SILU) {
+#pragma unroll
+    for (int i = 0; i < kVec; ++i) v[i] *= sigmoid(v[i]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < kVec; ++i) {
+      float P, p;
+      normal(v[i], P, p);
+      v[i] *= P;
+    }
+  }
+}
+
+// g *= f'(v).
+__device__ __forceinline__ void act_grad(const float (&v)[kVec], float (&g)[kVec], int kind) {
+  if (kind == PRATCHYA_ACT_RELU2) {
+#pragma unroll
+    for (int i = 0; i < kVec; ++i) g[i] *= v[i] < 0.0f ? 0.0f : 2.0f * v[i];
+  } else if (kind == PRATCHYA_ACT_SILU) {
+#pragma unroll
+    for (int i = 0; i < kVec; ++i) {
+      const float s = sigmoid(v[i]);
+      g[i] *= s * (1.0f + v[i] * (1.0f - s));
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < kVec; ++i) {
+      float P, p;
+      normal(v[i], P, p);
+      g[i] *= P + v[i] * p;
+    }
+  }
+}
+
+// Vectors of eight elements, numbered through all rows; a wave takes 128
+// neighbouring ones, two per lane, so a group of stored blocks (at most 1024
+// elements) lies in one wave.  ONE: the array is one row (contiguous rows).
+constexpr int kThreads = 256, kPer = 2, kWaveVecs = 64 * kPer;
+
+struct Rows {
+  int64_t ldx, width, vecs_per_row, vecs;
+};
+struct At {
+  int64_t row, c;
+  int left;        // elements of the vector, 0 beyond the array
+};
+template <bool ONE>
+__device__ __forceinline__ At place(const Rows& r, int64_t vec) {
+  if (vec >= r.vecs) return {0, 0, 0};
+  const int64_t row = ONE ? 0 : vec / r.vecs_per_row, c = (ONE ? vec : vec - row * r.vecs_per_row) * kVec;
+  return {row, c, r.width - c < kVec ? (int)(r.width - c) : kVec};
+}
+__device__ __forceinline__ int64_t first_vec() {
+  return ((int64_t)blockIdx.x * (kThreads / 64) + (threadIdx.x >> 6)) * kWaveVecs + (threadIdx.x & 63);
+}
+
+// Maximum over groups of K blocks of BLK elements, from the blocks' maxima of
+// this lane's two vectors (64 lanes apart).
+template <int BLK>
+__device__ __forceinline__ void group_max(uint32_t m0, uint32_t m1, int K, uint32_t& G0, uint32_t& G1) {
+  constexpr int LB = BLK / kVec;
+  G0 = m0;
+  G1 = m1;
+  if constexpr (BLK >= 32)
+    if (K == 2) {
+      G0 = lane_group_max<2 * LB>(m0);
+      G1 = lane_group_max<2 * LB>(m1);
+    }
+  if constexpr (BLK >= 64)
+    if (K == 4) {
+      G0 = lane_group_max<4 * LB>(m0);
+      G1 = lane_group_max<4 * LB>(m1);
+    }
+  if constexpr (BLK >= 128)
+    if (K == 8) G0 = G1 = lane_group_max<64>(umax(m0, m1));
+}
+
+template <typename T, int BLK, bool ONE>
+__global__ __launch_bounds__(kThreads) void k_act(const T* __restrict__ x, Rows r, int kind, T* __restrict__ y,
+                                                  uint8_t* __restrict__ x8, uint8_t* __restrict__ sc8,
+                                                  float* __restrict__ sc32, int K) {
+  const int64_t vec = first_vec();
+  At at[kPer];
+  float v[kPer][kVec];
+#pragma unroll
+  for (int u = 0; u < kPer; ++u) {
+    at[u] = place<ONE>(r, vec + u * 64);
+    const T* p = x + at[u].row * r.ldx + at[u].c;
+    if (at[u].left == kVec) widen(load_raw<true>(p), v[u]);
+    else load_some(p, at[u].left, 0.0f, v[u]);
+  }
+  if constexpr (BLK != 0) {
+    uint32_t m[kPer], G[kPer];
+#pragma unroll
+    for (int u = 0; u < kPer; ++u) m[u] = lane_group_max<BLK / kVec>(absmax8(v[u]));
+    group_max<BLK>(m[0], m[1], K, G[0], G[1]);
+#pragma unroll
+    for (int u = 0; u < kPer; ++u) {
+      if (at[u].left == 0) continue;          // blocks divide rows: a vector is whole
+      const int64_t e0 = (vec + u * 64) * kVec;
+      uint32_t e;
+      const u32x2_t q = store_form(v[u], m[u], G[u], e);
+      __builtin_nontemporal_store(q, reinterpret_cast<u32x2_t*>(x8 + e0));
+      const int64_t n = e0 / BLK;
+      if (e0 % BLK == 0) {
+        sc8[n] = (uint8_t)e;
+        if ((n & (K - 1)) == 0) sc32[n / K] = u2f(G[u]);
+      }
+    }
+  }
+#pragma unroll
+  for (int u = 0; u < kPer; ++u) {
+    act(v[u], kind);
+    T* p = y + at[u].row * r.width + at[u].c;
+    if (at[u].left == kVec) store_vec<true>(p, v[u]);
+    else store_some(p, at[u].left, v[u]);
+  }
+}
+
+struct StoredX {
+  const uint8_t* x8;
+  const uint8_t* sc8;
+  const float* sc32;
+  int blk_log2, K_log2;
+};
+
+template <typename T, bool STORED, bool ONE>
+__global__ __launch_bounds__(kThreads) void k_act_bwd(const T* __restrict__ x, Rows r, StoredX s,
+                                                      const T* __restrict__ dy, int64_t ldy, int kind,
+                                                      T* __restrict__ dx) {
+  const int64_t vec = first_vec();
+  At at[kPer];
+  float v[kPer][kVec], g[kPer][kVec];
+  u32x2_t q[kPer];
+  float scale[kPer];
+#pragma unroll
+  for (int u = 0; u < kPer; ++u) {
+    at[u] = place<ONE>(r, vec + u * 64);
+    const T* p = dy + at[u].row * ldy + at[u].c;
+    if constexpr (STORED) {
+      if (at[u].left) {
+        const int64_t e0 = (vec + u * 64) * kVec, n = e0 >> s.blk_log2;
+        q[u] = __builtin_nontemporal_load(reinterpret_cast<const u32x2_t*>(s.x8 + e0));
+        scale[u] = e8m0_decode(s.sc8[n]) * s.sc32[n >> s.K_log2];
+      }
+    } else {
+      const T* px = x + at[u].row * r.ldx + at[u].c;
+      if (at[u].left == kVec) widen(load_raw<true>(px), v[u]);
+      else load_some(px, at[u].left, 0.0f, v[u]);
+    }
+    if (at[u].left == kVec) widen(load_raw<true>(p), g[u]);
+    else load_some(p, at[u].left, 0.0f, g[u]);
+  }
+#pragma unroll
+  for (int u = 0; u < kPer; ++u) {
+    if (at[u].left == 0) continue;
+    if constexpr (STORED) stored_values(q[u], scale[u], v[u]);
+    act_grad(v[u], g[u], kind);
+    T* p = dx + at[u].row * r.width + at[u].c;
+    if (at[u].left == kVec) store_vec<true>(p, g[u]);
+    else store_some(p, at[u].left, g[u]);
   }
 }
 
@@ -88,9 +236,64 @@ int check_args(const char* what, int kind, int dtype, int64_t rows, int64_t widt
   return PRATCHYA_OK;
 }
 
-unsigned flat_grid(int64_t n) {
-  const int64_t g = (n + 255) / 256;
-  return (unsigned)(g < 65536 ? g : 65536);
+// Rows as one where nothing lies between them.
+Rows make_rows(int64_t ldx, int64_t ldy, int64_t rows, int64_t width, bool& one) {
+  one = rows == 1 || (ldx == width && ldy == width);
+  const int64_t w = one ? rows * width : width, per = (w + kVec - 1) / kVec;
+  return {ldx, w, per, one ? per : rows * per};
+}
+
+int log2_of(int64_t v) {
+  int n = 0;
+  while (v > 1) {
+    v >>= 1;
+    ++n;
+  }
+  return n;
+}
+
+int64_t workgroups(const Rows& r) { return (r.vecs + kThreads * kPer - 1) / (kThreads * kPer); }
+
+template <typename T>
+int launch(const void* x, int64_t ldx, int kind, int64_t rows, int64_t width, void* y, uint8_t* x8, uint8_t* sc8,
+           float* sc32, int64_t blk, hipStream_t stream) {
+  bool one;
+  const Rows r = make_rows(ldx, width, rows, width, one);
+  const int K = x8 ? (int)gcd64(blk / 16, rows * width / blk) : 1;
+  if (workgroups(r) > 0x7FFFFFFF)
+    return pratchya_set_error(PRATCHYA_EUNSUPPORTED, "activation: more than 2^31 workgroups");
+#define PRATCHYA_ACT(B)                                                                                              \
+  if (one)                                                                                                           \
+    hipLaunchKernelGGL((k_act<T, B, true>), dim3((unsigned)workgroups(r)), dim3(kThreads), 0, stream,                \
+                       static_cast<const T*>(x), r, kind, static_cast<T*>(y), x8, sc8, sc32, K);                     \
+  else                                                                                                               \
+    hipLaunchKernelGGL((k_act<T, B, false>), dim3((unsigned)workgroups(r)), dim3(kThreads), 0, stream,               \
+                       static_cast<const T*>(x), r, kind, static_cast<T*>(y), x8, sc8, sc32, K)
+  if (!x8) { PRATCHYA_ACT(0); }
+  else if (blk == 16) { PRATCHYA_ACT(16); }
+  else if (blk == 32) { PRATCHYA_ACT(32); }
+  else if (blk == 64) { PRATCHYA_ACT(64); }
+  else { PRATCHYA_ACT(128); }
+#undef PRATCHYA_ACT
+  return check_launch("activation");
+}
+
+template <typename T, bool STORED>
+int launch_bwd(const void* x, int64_t ldx, const StoredX& s, const void* dy, int64_t ldy, int kind, int64_t rows,
+               int64_t width, void* dx, hipStream_t stream) {
+  bool one;
+  const Rows r = make_rows(STORED ? width : ldx, ldy, rows, width, one);
+  if (workgroups(r) > 0x7FFFFFFF)
+    return pratchya_set_error(PRATCHYA_EUNSUPPORTED, "activation_bwd: more than 2^31 workgroups");
+  const dim3 grid((unsigned)workgroups(r));
+  const T* xt = STORED ? nullptr : static_cast<const T*>(x);
+  if (one)
+    hipLaunchKernelGGL((k_act_bwd<T, STORED, true>), grid, dim3(kThreads), 0, stream, xt, r, s,
+                       static_cast<const T*>(dy), ldy, kind, static_cast<T*>(dx));
+  else
+    hipLaunchKernelGGL((k_act_bwd<T, STORED, false>), grid, dim3(kThreads), 0, stream, xt, r, s,
+                       static_cast<const T*>(dy), ldy, kind, static_cast<T*>(dx));
+  return check_launch("activation_bwd");
 }
 
 }  // namespace
@@ -99,20 +302,16 @@ extern "C" int pratchya_activation(const void* x, int64_t ldx, int dtype, int ki
                                    void* y, uint8_t* x8, uint8_t* sc8, float* sc32, int64_t blk, hipStream_t stream) {
   const int rc = check_args("activation", kind, dtype, rows, width);
   if (rc) return rc;
-  (void)sc8;
-  (void)sc32;
-  (void)blk;
-  if (x8) return pratchya_set_error(PRATCHYA_EUNSUPPORTED, "activation: x is not stored in the same pass");
-  const int64_t n = rows * width;
-  if (n == 0) return pratchya_set_error(PRATCHYA_OK, "");
-  if (!x || !y) return pratchya_set_error(PRATCHYA_EINVAL, "activation: null buffer");
-  if (dtype == PRATCHYA_DT_BF16)
-    hipLaunchKernelGGL((k_act<uint16_t>), dim3(flat_grid(n)), dim3(256), 0, stream, static_cast<const uint16_t*>(x),
-                       ldx, width, n, kind, static_cast<uint16_t*>(y));
-  else
-    hipLaunchKernelGGL((k_act<float>), dim3(flat_grid(n)), dim3(256), 0, stream, static_cast<const float*>(x), ldx,
-                       width, n, kind, static_cast<float*>(y));
-  return check_launch("activation");
+  if (x8 && ((blk != 16 && blk != 32 && blk != 64 && blk != 128) || width % blk))
+    return pratchya_set_error(PRATCHYA_EINVAL, "activation: blocks of %lld for rows of %lld", (long long)blk,
+                              (long long)width);
+  if (rows * width == 0) return pratchya_set_error(PRATCHYA_OK, "");
+  if (!x || !y || (x8 && (!sc8 || !sc32))) return pratchya_set_error(PRATCHYA_EINVAL, "activation: null buffer");
+  if (reinterpret_cast<uintptr_t>(x8) % 8)
+    return pratchya_set_error(PRATCHYA_EINVAL, "activation: the payload must be 8-byte aligned");
+  return dtype == PRATCHYA_DT_BF16
+             ? launch<uint16_t>(x, ldx, kind, rows, width, y, x8, sc8, sc32, blk, stream)
+             : launch<float>(x, ldx, kind, rows, width, y, x8, sc8, sc32, blk, stream);
 }
 
 extern "C" int pratchya_activation_bwd(const void* x, int64_t ldx, int x_dtype, const uint8_t* sc8, const float* sc32,
@@ -123,22 +322,23 @@ extern "C" int pratchya_activation_bwd(const void* x, int64_t ldx, int x_dtype, 
   const bool stored = x_dtype == PRATCHYA_DT_E4M3;
   if (!stored && x_dtype != dtype)
     return pratchya_set_error(PRATCHYA_EINVAL, "activation_bwd: unsupported dtypes (x %d, dy %d)", x_dtype, dtype);
-  if (stored && (blk < 1 || width % blk))
-    return pratchya_set_error(PRATCHYA_EINVAL, "activation_bwd: blocks of %lld do not divide rows of %lld",
-                              (long long)blk, (long long)width);
+  if (stored && (blk < kVec || (blk & (blk - 1)) || width % blk))
+    return pratchya_set_error(PRATCHYA_EINVAL, "activation_bwd: blocks of %lld for rows of %lld", (long long)blk,
+                              (long long)width);
   const int64_t n = rows * width;
   if (n == 0) return pratchya_set_error(PRATCHYA_OK, "");
   if (!x || !dy || !dx || (stored && (!sc8 || !sc32)))
     return pratchya_set_error(PRATCHYA_EINVAL, "activation_bwd: null buffer");
-  const int64_t K = stored ? gcd64(blk / 16 > 1 ? blk / 16 : 1, n / blk) : 1;
-  const uint8_t* x8 = stored ? static_cast<const uint8_t*>(x) : nullptr;
-  if (dtype == PRATCHYA_DT_BF16)
-    hipLaunchKernelGGL((k_act_bwd<uint16_t>), dim3(flat_grid(n)), dim3(256), 0, stream,
-                       static_cast<const uint16_t*>(x), ldx, x8, sc8, sc32, blk, K, static_cast<const uint16_t*>(dy),
-                       ldy, width, n, kind, static_cast<uint16_t*>(dx));
-  else
-    hipLaunchKernelGGL((k_act_bwd<float>), dim3(flat_grid(n)), dim3(256), 0, stream, static_cast<const float*>(x), ldx,
-                       x8, sc8, sc32, blk, K, static_cast<const float*>(dy), ldy, width, n, kind,
-                       static_cast<float*>(dx));
-  return check_launch("activation_bwd");
+  if (stored && reinterpret_cast<uintptr_t>(x) % 8)
+    return pratchya_set_error(PRATCHYA_EINVAL, "activation_bwd: the payload must be 8-byte aligned");
+  StoredX s = {nullptr, sc8, sc32, 0, 0};
+  if (stored) {
+    s.x8 = static_cast<const uint8_t*>(x);
+    s.blk_log2 = log2_of(blk);
+    s.K_log2 = log2_of(gcd64(blk / 16 > 1 ? blk / 16 : 1, n / blk));
+    return dtype == PRATCHYA_DT_BF16 ? launch_bwd<uint16_t, true>(x, ldx, s, dy, ldy, kind, rows, width, dx, stream)
+                                     : launch_bwd<float, true>(x, ldx, s, dy, ldy, kind, rows, width, dx, stream);
+  }
+  return dtype == PRATCHYA_DT_BF16 ? launch_bwd<uint16_t, false>(x, ldx, s, dy, ldy, kind, rows, width, dx, stream)
+                                   : launch_bwd<float, false>(x, ldx, s, dy, ldy, kind, rows, width, dx, stream);
 }
