@@ -1494,72 +1494,17 @@ def apply_update(u: torch.Tensor, use_sign: bool, scale: float, p, tgrid, arith:
 
 # --------------------------------------------------------------------------
 # Row operators around the quantized Linears: layer norm, activations, token
-# log probabilities.
+# log probabilities.  The binding of these is compiled (csrc/row_ops.cpp); the
+# functions here are its parts without autograd.
 # --------------------------------------------------------------------------
-_STORED_BLOCKS = (16, 32, 64, 128)
 _ACTIVATIONS = {"relu2": 0, "silu": 1, "gelu": 2}
-MAX_TOP = 64
-_FLOATS = {torch.float32: _lib.DT_F32, torch.bfloat16: _lib.DT_BF16}
 
 
-def _strided_rows(x: torch.Tensor):
-    """``(x, elements between rows)`` of an array read as rows of its last axis:
-    x itself where its rows are one stride apart (slices of a wider array, broadcast
-    rows), else a contiguous copy."""
-    width = x.shape[-1]
-    if x.is_contiguous():
-        return x, width
-    if x.stride(-1) == 1:
-        step = span = None
-        for n, s in zip(reversed(x.shape[:-1]), reversed(x.stride()[:-1])):
-            if n == 1:
-                continue
-            if step is None:
-                step = s
-            elif s != span:
-                break
-            span = s * n
-        else:
-            return x, width if step is None else step
-    return x.contiguous(), width
-
-
-def _float_code(t: torch.Tensor, what: str) -> int:
-    code = _FLOATS.get(t.dtype)
+def _activation_code(kind: str) -> int:
+    code = _ACTIVATIONS.get(kind)
     if code is None:
-        raise TypeError(f"{what}: unsupported dtype {t.dtype}; expected float32 or bfloat16")
+        raise ValueError(f"unknown activation {kind!r}; expected one of {tuple(_ACTIVATIONS)}")
     return code
-
-
-def _param(p, width: int, x: torch.Tensor, what: str):
-    """(address, dtype code) of a [width] parameter vector, or (None, f32)."""
-    if p is None:
-        return None, _lib.DT_F32
-    if p.dim() != 1 or p.shape[0] != width or p.device != x.device:
-        raise ValueError(f"{what} of shape {tuple(p.shape)} on {p.device} for rows of {width} on {x.device}")
-    if not p.is_contiguous():
-        raise ValueError(f"{what} must be contiguous")
-    return p.data_ptr(), _float_code(p, what)
-
-
-def _stored_block(tgrid, width: int, what: str) -> int:
-    a, b = tgrid
-    if a != 1 or b not in _STORED_BLOCKS or width % b:
-        raise ValueError(f"{what}: block grid {tuple(tgrid)} for rows of {width}; expected (1, b) with b of "
-                         f"{_STORED_BLOCKS} dividing them")
-    return int(b)
-
-
-def _stored_buffers(rows: int, width: int, blk: int, device):
-    """(payload, e8m0 scales, group maxima) of a [rows, width] array quantized (1, blk)."""
-    _, K, M = _group_layout(rows, width, 1, blk)
-    return (torch.empty((rows, width), dtype=E4M3, device=device), torch.empty((M, K), dtype=E8M0, device=device),
-            torch.empty((M, 1, 1), dtype=torch.float32, device=device))
-
-
-@functools.lru_cache(maxsize=4096)
-def _layer_norm_stores(width: int, groups: int, blk: int) -> bool:
-    return bool(_lib.load().pratchya_layer_norm_stores(width, groups, blk))
 
 
 def layer_norm(x: torch.Tensor, weight=None, bias=None, eps: float = 1e-5, groups: int = 1, stats: bool = False,
@@ -1571,50 +1516,7 @@ def layer_norm(x: torch.Tensor, weight=None, bias=None, eps: float = 1e-5, group
     deviations [rows * groups, 2] that ``layer_norm_bwd`` reads, else None; with
     ``tgrid`` (1, b), x's quantized form ``quantize(x.reshape(-1, C), tgrid)``,
     else None."""
-    if not x.is_cuda:
-        _require_gpu(x)
-    code = _float_code(x, "layer_norm")
-    if x.dim() < 1:
-        raise ValueError("layer_norm needs an array of rows")
-    width = x.shape[-1]
-    groups = int(groups)
-    if groups < 1 or width % groups:
-        raise ValueError(f"layer_norm: {groups} groups do not divide rows of {width}")
-    w, w_code = _param(weight, width, x, "layer_norm: weight")
-    b, b_code = _param(bias, width, x, "layer_norm: bias")
-    blk = 0 if tgrid is None else _stored_block(tgrid, width, "layer_norm")
-    x, ldx = _strided_rows(x)
-    rows = x.numel() // width if width else 0
-    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    st = torch.empty((rows * groups, 2), dtype=torch.float32, device=x.device) if stats else None
-    stored, fused = None, False
-    if blk and rows:
-        fused = _layer_norm_stores(width, groups, blk)
-        stored = _stored_buffers(rows, width, blk, x.device) if fused else quantize(x.reshape(rows, width), (1, blk))
-    elif blk:
-        stored = _stored_buffers(rows, width, blk, x.device)
-    q = [t.data_ptr() for t in stored] if fused else (None, None, None)
-    _lib.check(_lib.load().pratchya_layer_norm(
-        x.data_ptr(), ldx, code, w, w_code, b, b_code, rows, width, groups, eps, y.data_ptr(),
-        st.data_ptr() if stats else None, q[0], q[1], q[2], blk, _stream(x)), "layer_norm")
-    return y, st, stored
-
-
-def _source(x, rows: int, width: int, dtype: torch.dtype, tgrid, what: str):
-    """A backward pass's input as its kernel takes it: the array itself, or its stored form (payload, e8m0
-    scales, group maxima) with the block grid ``tgrid``.  Returns the tensor to keep alive and (address, row
-    stride, dtype code, e8m0 address, group maxima's address, block)."""
-    if tgrid is None:
-        if x.numel() != rows * width or x.dtype != dtype:
-            raise ValueError(f"{what}: an input of {tuple(x.shape)} {x.dtype} for a cotangent of [{rows}, {width}] "
-                             f"{dtype}")
-        x, ldx = _strided_rows(x)
-        return x, (x.data_ptr(), ldx, _FLOATS[dtype], None, None, 0)
-    x8, sc8, sc32 = x
-    blk = _stored_block(tgrid, width, what)
-    if tuple(x8.shape) != (rows, width) or not (x8.is_contiguous() and sc8.is_contiguous() and sc32.is_contiguous()):
-        raise ValueError(f"{what}: a stored input of {tuple(x8.shape)} for a cotangent of [{rows}, {width}]")
-    return x8, (x8.data_ptr(), width, _lib.DT_E4M3, sc8.data_ptr(), sc32.data_ptr(), blk)
+    return _lib.row_ops().layer_norm_fwd(x, weight, bias, eps, groups, stats, tgrid)
 
 
 def layer_norm_bwd(x, dy: torch.Tensor, weight, stats: torch.Tensor, groups: int = 1, tgrid=None,
@@ -1623,138 +1525,31 @@ def layer_norm_bwd(x, dy: torch.Tensor, weight, stats: torch.Tensor, groups: int
     and the forward pass's ``stats``; ``need`` says which are wanted (None for
     the others).  ``x``: the forward pass's input, or with ``tgrid`` its stored
     form.  dweight has weight's dtype (f32 without a weight), dbias ``bias_dtype``."""
-    if not dy.is_cuda:
-        _require_gpu(dy)
-    code = _float_code(dy, "layer_norm_bwd")
-    dy, ldy = _strided_rows(dy)
-    width = dy.shape[-1]
-    rows = dy.numel() // width if width else 0
-    if stats.numel() != 2 * rows * groups or not stats.is_contiguous():
-        raise ValueError(f"layer_norm_bwd: statistics of {tuple(stats.shape)} for {rows} rows of {groups} segments")
-    keep, src = _source(x, rows, width, dy.dtype, tgrid, "layer_norm_bwd")
-    w, w_code = _param(weight, width, dy, "layer_norm_bwd: weight")
-    w_dtype = torch.float32 if weight is None else weight.dtype
-    new = torch.empty if rows and width else torch.zeros
-    dx = torch.empty(dy.shape, dtype=dy.dtype, device=dy.device) if need[0] else None
-    dw = new((width,), dtype=w_dtype, device=dy.device) if need[1] else None
-    db = new((width,), dtype=bias_dtype, device=dy.device) if need[2] else None
-    ws, ws_bytes = None, 0
-    if need[1] or need[2]:
-        ws_bytes = _ws_bytes("pratchya_layer_norm_bwd_workspace_bytes", rows, width, groups)
-        ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dy.device)
-    _lib.check(_lib.load().pratchya_layer_norm_bwd(
-        *src, dy.data_ptr(), ldy, code, w, w_code, stats.data_ptr(), rows, width, groups,
-        None if dx is None else dx.data_ptr(), None if dw is None else dw.data_ptr(), _FLOATS[w_dtype],
-        None if db is None else db.data_ptr(), _FLOATS[bias_dtype], None if ws is None else ws.data_ptr(), ws_bytes,
-        _stream(dy)), "layer_norm_bwd")
-    return dx, dw, db
-
-
-def _activation_code(kind: str) -> int:
-    code = _ACTIVATIONS.get(kind)
-    if code is None:
-        raise ValueError(f"unknown activation {kind!r}; expected one of {tuple(_ACTIVATIONS)}")
-    return code
+    return _lib.row_ops().layer_norm_bwd(x, dy, weight, stats, groups, tgrid, *need, bias_dtype)
 
 
 def activation(x: torch.Tensor, kind: str, tgrid=None):
     """``(y, stored)``: y = f(x) for f "relu2", "silu" or "gelu" (bf16 or f32
     [..., C], f32 arithmetic) and, with ``tgrid`` (1, b), x's quantized form
     ``quantize(x.reshape(-1, C), tgrid)``, else None."""
-    if not x.is_cuda:
-        _require_gpu(x)
-    k, code = _activation_code(kind), _float_code(x, "activation")
-    if x.dim() < 1:
-        raise ValueError("activation needs an array of rows")
-    width = x.shape[-1]
-    blk = 0 if tgrid is None else _stored_block(tgrid, width, "activation")
-    x, ldx = _strided_rows(x)
-    rows = x.numel() // width if width else 0
-    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    stored = _stored_buffers(rows, width, blk, x.device) if blk else None
-    q = [t.data_ptr() for t in stored] if blk else (None, None, None)
-    _lib.check(_lib.load().pratchya_activation(x.data_ptr(), ldx, code, k, rows, width, y.data_ptr(), q[0], q[1], q[2],
-                                               blk, _stream(x)), "activation")
-    return y, stored
+    return _lib.row_ops().activation_fwd(x, _activation_code(kind), tgrid)
 
 
 def activation_bwd(x, dy: torch.Tensor, kind: str, tgrid=None) -> torch.Tensor:
     """dx = f'(x) dy, with ``x`` the forward pass's input or, with ``tgrid``, its stored form."""
-    if not dy.is_cuda:
-        _require_gpu(dy)
-    k, code = _activation_code(kind), _float_code(dy, "activation_bwd")
-    dy, ldy = _strided_rows(dy)
-    width = dy.shape[-1]
-    rows = dy.numel() // width if width else 0
-    keep, src = _source(x, rows, width, dy.dtype, tgrid, "activation_bwd")
-    dx = torch.empty(dy.shape, dtype=dy.dtype, device=dy.device)
-    _lib.check(_lib.load().pratchya_activation_bwd(*src, dy.data_ptr(), ldy, code, k, rows, width, dx.data_ptr(),
-                                                   _stream(dy)), "activation_bwd")
-    return dx
+    return _lib.row_ops().activation_bwd(x, dy, _activation_code(kind), tgrid)
 
 
 def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, entropy: bool = False, top: int = 0,
                    stats: bool = False):
     """``(logprobs, entropy, top_logprobs, top_tokens, stats)`` of logits [..., V]
-    (bf16 or f32) and one token per row (int64, or int32); what is not asked for is None."""
-    if not logits.is_cuda or not tokens.is_cuda:
-        _require_gpu(logits, tokens)
-    code = _float_code(logits, "token_logprobs")
-    if logits.dim() < 1 or tokens.shape != logits.shape[:-1] or tokens.device != logits.device:
-        raise ValueError(f"token_logprobs: tokens of {tuple(tokens.shape)} on {tokens.device} for logits of "
-                         f"{tuple(logits.shape)} on {logits.device}")
-    if tokens.dtype != torch.int64:
-        if tokens.dtype != torch.int32:
-            raise TypeError(f"token_logprobs: tokens of {tokens.dtype}; expected int64 or int32")
-        tokens = tokens.long()
-    vocab = logits.shape[-1]
-    if vocab < 1 or not 0 <= top <= min(vocab, MAX_TOP):
-        raise ValueError(f"token_logprobs: {top} alternatives of {vocab} (0 to {MAX_TOP}, at most the vocabulary)")
-    lead, dev = tokens.shape, logits.device
-    tokens = tokens.contiguous()
-    logits, ld = _strided_rows(logits)
-    rows = tokens.numel()
-    out = torch.empty(lead, dtype=torch.float32, device=dev)
-    ent = torch.empty(lead, dtype=torch.float32, device=dev) if entropy else None
-    st = torch.empty((rows, 3), dtype=torch.float32, device=dev) if stats else None
-    top_lp = torch.empty(lead + (top,), dtype=torch.float32, device=dev) if top else None
-    top_tok = torch.empty(lead + (top,), dtype=torch.int64, device=dev) if top else None
-    ws, ws_bytes = None, 0
-    if top:
-        ws_bytes = _ws_bytes("pratchya_token_logprobs_workspace_bytes", rows, vocab, top)
-        ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev) if ws_bytes else None
-    _lib.check(_lib.load().pratchya_token_logprobs(
-        logits.data_ptr(), ld, code, tokens.data_ptr(), rows, vocab, top, out.data_ptr(),
-        None if ent is None else ent.data_ptr(), None if st is None else st.data_ptr(),
-        None if top_lp is None else top_lp.data_ptr(), None if top_tok is None else top_tok.data_ptr(),
-        None if ws is None else ws.data_ptr(), ws_bytes, _stream(logits)), "token_logprobs")
-    return out, ent, top_lp, top_tok, st
+    (bf16 or f32) and one token per row (int64, or int32); what is not asked for is
+    None.  ``stats`` hold the entropy only if it is asked for."""
+    return _lib.row_ops().token_logprobs_fwd(logits, tokens, entropy, top, stats)
 
 
 def token_logprobs_bwd(logits: torch.Tensor, tokens: torch.Tensor, stats: torch.Tensor, g_logprobs=None,
                        g_entropy=None) -> torch.Tensor:
     """The logits' gradient of ``token_logprobs`` from the cotangents of the log
     probabilities and the entropies (f32 [...], either may be None)."""
-    if not logits.is_cuda:
-        _require_gpu(logits)
-    code = _float_code(logits, "token_logprobs_bwd")
-    vocab = logits.shape[-1]
-    tokens = tokens.long().contiguous()
-    rows = tokens.numel()
-    if logits.numel() != rows * vocab or tuple(stats.shape) != (rows, 3) or not stats.is_contiguous():
-        raise ValueError(f"token_logprobs_bwd: statistics of {tuple(stats.shape)} and {rows} tokens for logits of "
-                         f"{tuple(logits.shape)}")
-    gs = []
-    for g in (g_logprobs, g_entropy):
-        if g is not None:
-            if g.numel() != rows or g.dtype != torch.float32:
-                raise ValueError(f"token_logprobs_bwd: a cotangent of {tuple(g.shape)} {g.dtype} for {rows} rows")
-            g = g.contiguous()
-        gs.append(g)
-    logits, ld = _strided_rows(logits)
-    dx = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
-    _lib.check(_lib.load().pratchya_token_logprobs_bwd(
-        logits.data_ptr(), ld, code, tokens.data_ptr(), stats.data_ptr(),
-        *(None if g is None else g.data_ptr() for g in gs), rows, vocab, dx.data_ptr(), _stream(logits)),
-        "token_logprobs_bwd")
-    return dx
+    return _lib.row_ops().token_logprobs_bwd(logits, tokens, stats, g_logprobs, g_entropy)

@@ -7,6 +7,7 @@ an ImportError-style failure at first use, never a silent slow path.
 from __future__ import annotations
 
 import ctypes
+import functools
 import threading
 from pathlib import Path
 
@@ -189,6 +190,18 @@ def load() -> ctypes.CDLL:
             raise ImportError(f"{LIB_PATH} has ABI {ver}, expected {ABI_VERSION}; rebuild it")
         _lib = lib
     return _lib
+
+
+@functools.lru_cache(maxsize=None)
+def row_ops():
+    """The compiled binding of the row operators (csrc/row_ops.cpp)."""
+    load()
+    try:
+        from . import _row_ops
+    except ImportError as e:
+        raise ImportError(f"{LIB_PATH.parent / '_row_ops.so'} is not built or does not fit this torch; run "
+                          f"`python -m pratchya_amd.build` ({e})") from e
+    return _row_ops
 
 
 def check(rc: int, what: str) -> None:

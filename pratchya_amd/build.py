@@ -1,7 +1,9 @@
-"""Build the gfx950 shared library ``pratchya_amd/libpratchya_fp8.so``.
+"""Build the gfx950 shared library ``pratchya_amd/libpratchya_fp8.so`` and the
+compiled binding of the row operators, ``pratchya_amd/_row_ops.so``.
 
 The library is built in-tree with ``hipcc --offload-arch=gfx950`` so that it
-travels with the source tree to the GPU machine.  Usage::
+travels with the source tree to the GPU machine; the binding holds no GPU code and
+is built with the host compiler against torch's headers.  Usage::
 
     python -m pratchya_amd.build          # or pratchya_amd.build.build()
 """
@@ -10,6 +12,7 @@ from __future__ import annotations
 import os
 import subprocess
 import sys
+import sysconfig
 from pathlib import Path
 
 PKG = Path(__file__).resolve().parent
@@ -17,10 +20,12 @@ ROOT = PKG.parent
 CSRC = PKG / "csrc"
 INCLUDE = ROOT / "include"
 LIB = PKG / "libpratchya_fp8.so"
+ROW_OPS = PKG / "_row_ops.so"
 SOURCES = ["quantize.hip", "quantize_t.hip", "gemm.hip", "gemm_t128.hip", "optim.hip", "elementwise.hip",
            "layer_norm.hip", "activation.hip", "logprobs.hip"]
 
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
+CXX = os.environ.get("CXX", "g++")
 
 # -packed-fp32-ops: keep the compiler from emitting v_pk_{add,mul,fma}_f32.
 DEVICE_FLAGS = [
@@ -57,7 +62,25 @@ def build(verbose: bool = False) -> Path:
     tmp = LIB.with_suffix(".so.tmp")
     _run([HIPCC, "--offload-arch=gfx950", "-shared", "-fPIC", *objs, "-o", str(tmp)])
     os.replace(tmp, LIB)
+    build_row_ops()
     return LIB
+
+
+def build_row_ops() -> Path:
+    """Compile the row operators' binding against this interpreter and its torch."""
+    import torch
+    torch_dir = Path(torch.__file__).resolve().parent
+    include = torch_dir / "include"
+    rocm = Path(HIPCC).resolve().parent.parent if "/" in HIPCC else Path("/opt/rocm")
+    tmp = ROW_OPS.with_suffix(".so.tmp")
+    _run([CXX, "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden", "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM",
+          f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", f"-I{INCLUDE}", f"-I{include}",
+          f"-I{include / 'torch' / 'csrc' / 'api' / 'include'}", f"-I{rocm / 'include'}",
+          f"-I{sysconfig.get_paths()['include']}", str(CSRC / "row_ops.cpp"), "-o", str(tmp), f"-L{PKG}",
+          f"-l:{LIB.name}", f"-L{torch_dir / 'lib'}", "-lc10", "-ltorch_cpu", "-ltorch_python", "-lc10_hip",
+          "-ltorch_hip", "-Wl,-rpath,$ORIGIN"])
+    os.replace(tmp, ROW_OPS)
+    return ROW_OPS
 
 
 if __name__ == "__main__":

@@ -22,28 +22,11 @@ from __future__ import annotations
 from typing import NamedTuple, Optional, Tuple
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from . import _kernels as K
+from . import _lib
 
-
-class _LayerNorm(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, x, weight, bias, eps, groups, tgrid):
-        need = ctx.needs_input_grad
-        y, stats, stored = K.layer_norm(x, weight, bias, eps, groups, True, tgrid if need[0] or need[1] else None)
-        ctx.groups, ctx.tgrid = groups, None if stored is None else tgrid
-        ctx.bias_dtype = torch.float32 if bias is None else bias.dtype
-        ctx.save_for_backward(weight, stats, *((x,) if stored is None else stored))
-        return y
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, dy):
-        weight, stats, *x = ctx.saved_tensors
-        grads = K.layer_norm_bwd(x[0] if ctx.tgrid is None else x, dy, weight, stats, ctx.groups, ctx.tgrid,
-                                 ctx.needs_input_grad[:3], ctx.bias_dtype)
-        return grads + (None, None, None)
+_ops = _lib.row_ops()
 
 
 def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, bias: Optional[torch.Tensor] = None,
@@ -52,36 +35,18 @@ def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, bias: Opt
     [..., C], or over each of ``groups`` equal segments of it (the heads of a norm
     over heads); weight and bias [C] or None.  With ``tgrid=(1, b)``, b 16, 32, 64 or
     128 dividing C, x is kept for the backward pass in 8 bits with that block
-    grid (its mean and deviation in f32, of x itself)."""
-    if torch.is_grad_enabled() and (x.requires_grad or (weight is not None and weight.requires_grad)
-                                    or (bias is not None and bias.requires_grad)):
-        return _LayerNorm.apply(x, weight, bias, eps, groups, tgrid)
-    return K.layer_norm(x, weight, bias, eps, groups)[0]
-
-
-class _Activation(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, x, kind, tgrid):
-        y, stored = K.activation(x, kind, tgrid)
-        ctx.kind, ctx.tgrid = kind, tgrid
-        ctx.save_for_backward(*((x,) if stored is None else stored))
-        return y
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, dy):
-        x = ctx.saved_tensors
-        return K.activation_bwd(x[0] if ctx.tgrid is None else x, dy, ctx.kind, ctx.tgrid), None, None
+    grid (its mean and deviation in f32, of x itself).  Without a gradient to
+    compute nothing is kept, and ``tgrid`` has no effect."""
+    return _ops.layer_norm(x, weight, bias, eps, groups, tgrid)
 
 
 def activation(x: torch.Tensor, kind: str = "relu2", tgrid: Optional[Tuple[int, int]] = None) -> torch.Tensor:
     """``max(x, 0)^2`` ("relu2"), ``x / (1 + exp(-x))`` ("silu") or x times the
     normal distribution function of x ("gelu"), for x [..., C].  With
     ``tgrid=(1, b)``, b 16, 32, 64 or 128 dividing C, x is kept for the backward
-    pass in 8 bits with that block grid."""
-    if torch.is_grad_enabled() and x.requires_grad:
-        return _Activation.apply(x, kind, tgrid)
-    return K.activation(x, kind)[0]
+    pass in 8 bits with that block grid; without a gradient to compute it has no
+    effect."""
+    return _ops.activation(x, K._activation_code(kind), tgrid)
 
 
 class TokenLogprobs(NamedTuple):
@@ -92,23 +57,6 @@ class TokenLogprobs(NamedTuple):
     top_tokens: Optional[torch.Tensor]          # int64 [..., top]
 
 
-class _TokenLogprobs(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, logits, tokens, entropy, top):
-        logprobs, ent, top_lp, top_tok, stats = K.token_logprobs(logits, tokens, entropy, top, True)
-        ctx.save_for_backward(logits, tokens, stats)
-        ctx.set_materialize_grads(False)
-        ctx.mark_non_differentiable(*(t for t in (top_lp, top_tok) if t is not None))
-        return logprobs, ent, top_lp, top_tok
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, g, g_entropy, *_):
-        if g is None and g_entropy is None:
-            return None, None, None, None
-        return K.token_logprobs_bwd(*ctx.saved_tensors, g, g_entropy), None, None, None
-
-
 def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, entropy: bool = False, top: int = 0) -> TokenLogprobs:
     """Log probability of ``tokens`` [...] (int64 or int32) under softmax of
     ``logits`` [..., V], with ``entropy`` the distributions' entropy, and with
@@ -117,8 +65,6 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, entropy: bool = F
     differentiable in the logits, the alternatives are not.
 
     A negative token stands for none: its log probability is 0 and has no
-    gradient.  A token of V or more gives NaN.  Logits of -inf are masked; a row of nothing
-    else has log probabilities of -inf, entropy 0 and no gradient."""
-    if torch.is_grad_enabled() and logits.requires_grad:
-        return TokenLogprobs(*_TokenLogprobs.apply(logits, tokens, entropy, top))
-    return TokenLogprobs(*K.token_logprobs(logits, tokens, entropy, top)[:4])
+    gradient.  A token of V or more gives NaN.  Logits of -inf are masked; a row of
+    nothing else has log probabilities of -inf, entropy 0 and no gradient."""
+    return TokenLogprobs(*_ops.token_logprobs(logits, tokens, entropy, top))
