@@ -49,7 +49,10 @@ struct Affine {
 // over rows: `gt` neighbouring segments side by side, the other teams on
 // further rows.  Thread t of a team holds vectors (t / 64 * NV + j) * 64 + t % 64
 // (P >= 64), so a wave reads runs of 512 elements and groups of stored blocks lie
-// in one wave.
+// in one wave.  Streaming accesses where they measured faster, [16384, 4096] bf16:
+// the forward pass's stores (55.2 -> 52.3 us; its loads 55.2 -> 50.8, but 25.2 ->
+// 25.7 us and 11.0 -> 12.0 us where the caches hold x), the backward pass's
+// loads (84.3 -> 79.8 us; its stores 84.3 -> 83.4, with the loads 82.7 us).
 template <int P_, int NV_, int TB_>
 struct Shape {
   static constexpr int P = P_, NV = NV_, TB = TB_, TEAMS = TB_ / P_, WAVES = P_ > 64 ? P_ / 64 : 1;
@@ -86,12 +89,12 @@ __device__ __forceinline__ void load_vec_or_some(const T* p, int left, float (&v
 }
 
 // A vector of a row in registers, in its type.
-template <typename T>
+template <typename T, bool NT = false>
 struct Held {
   typename RawOf<T>::type raw;
   __device__ __forceinline__ void load(const T* p, int left) {
     if (left == kVec) {
-      raw = load_raw(p);
+      raw = load_raw<NT>(p);
     } else {
       float v[kVec];
       load_some(p, left, 0.0f, v);
@@ -122,7 +125,7 @@ __device__ __forceinline__ void load_params(const void* p, bool bf16, int64_t at
 // y and the statistics of whole segments; with BLK, x's stored form beside them
 // (groups = 1).  Mean and squared deviations are taken within each wave, from
 // registers, and joined by counts, so a mean far from zero costs no digits.
-template <typename T, typename G, int BLK>
+template <typename T, typename G, int BLK, int AHEAD>
 __global__ __launch_bounds__(G::TB) void k_layer_norm(const T* __restrict__ x, int64_t ldx, Affine p, int64_t rows,
                                                       int64_t width, int64_t groups, float eps, T* __restrict__ y,
                                                       float* __restrict__ stats, uint8_t* __restrict__ x8,
@@ -144,18 +147,25 @@ __global__ __launch_bounds__(G::TB) void k_layer_norm(const T* __restrict__ x, i
   const float mine = G::P < 64 ? (float)D : (float)(D - first < 0 ? 0 : D - first < NV * 512 ? D - first : NV * 512);
   const int64_t step = (int64_t)gridDim.x * me.rt;
   int64_t row = (int64_t)blockIdx.x * me.rt + me.rl;
-  Held<T> cur[NV], next[NV];
+  // the next AHEAD rows are on their way while one is computed
+  Held<T> cur[NV], next[AHEAD][NV];
+  auto fetch = [&](int64_t r, Held<T> (&to)[NV]) {
 #pragma unroll
-  for (int j = 0; j < NV; ++j) next[j].load(x + row * ldx + c0 + me.at(j), row < rows ? left[j] : 0);
+    for (int j = 0; j < NV; ++j) to[j].load(x + r * ldx + c0 + me.at(j), r < rows ? left[j] : 0);
+  };
+#pragma unroll
+  for (int d = 0; d < AHEAD; ++d) fetch(row + d * step, next[d]);
   // the workgroup's first team has the first row: all teams make as many rounds
   int buf = 0;
   for (int64_t lead = (int64_t)blockIdx.x * me.rt; lead < rows; lead += step, row += step, buf ^= 1) {
     const bool on = me.live && row < rows;
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
-      cur[j] = next[j];
-      next[j].load(x + (row + step) * ldx + c0 + me.at(j), row + step < rows ? left[j] : 0);
+      cur[j] = next[0][j];
+#pragma unroll
+      for (int d = 1; d < AHEAD; ++d) next[d - 1][j] = next[d][j];
     }
+    fetch(row + AHEAD * step, next[AHEAD - 1]);
     float v[kVec], s = 0.0f, q = 0.0f;
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
@@ -208,7 +218,7 @@ __global__ __launch_bounds__(G::TB) void k_layer_norm(const T* __restrict__ x, i
       cur[j].get(v);
 #pragma unroll
       for (int i = 0; i < kVec; ++i) v[i] = (v[i] - mean) * rstd * w[j][i] + b[j][i];
-      if (left[j] == kVec) store_vec(yr + me.at(j), v);
+      if (left[j] == kVec) store_vec<true>(yr + me.at(j), v);
       else if (left[j]) store_some(yr + me.at(j), left[j], v);
     }
     if constexpr (BLK != 0) {
@@ -231,7 +241,7 @@ __global__ __launch_bounds__(G::TB) void k_layer_norm(const T* __restrict__ x, i
         uint32_t e;
         const int64_t at = row * width + me.at(j);
         const u32x2_t q8 = store_form(v, mb[j], Gb[j], e);
-        *reinterpret_cast<u32x2_t*>(x8 + at) = q8;
+        __builtin_nontemporal_store(q8, reinterpret_cast<u32x2_t*>(x8 + at));
         constexpr int K = BLK <= 16 ? 1 : BLK / 16;
         if (at % BLK == 0) sc8[at / BLK] = (uint8_t)e;
         if (at % (BLK * K) == 0) sc32[at / (BLK * K)] = u2f(Gb[j]);
@@ -295,7 +305,7 @@ template <typename T> struct SourceOf<T, true> { typedef Stored type; };
 // The backward pass's x of one vector: as it is, or its stored form.
 template <typename T, bool STORED> struct HeldSource;
 template <typename T> struct HeldSource<T, false> {
-  Held<T> x;
+  Held<T, true> x;
   __device__ __forceinline__ void load(const Source<T>& s, int64_t row, int64_t c, int left) {
     x.load(s.x + row * s.ldx + c, left);
   }
@@ -311,7 +321,7 @@ template <typename T> struct HeldSource<T, true> {
     G = 0.0f;
     if (left) {     // blocks are a multiple of eight elements: a vector lies in one
       const int64_t at = row * s.width + c, n = at >> s.blk_log2;
-      w = *reinterpret_cast<const u32x2_t*>(s.x8 + at);
+      w = __builtin_nontemporal_load(reinterpret_cast<const u32x2_t*>(s.x8 + at));
       e = s.sc8[n];
       G = s.sc32[n >> s.K_log2];
     }
@@ -323,7 +333,7 @@ template <typename T> struct HeldSource<T, true> {
 // has walked: joined over the workgroup's row lanes and written to
 // part[blockIdx.x][0 / 1][width], or as the results where there is one workgroup
 // per column.
-template <typename T, typename G, bool STORED, bool AHEAD>
+template <typename T, typename G, bool STORED, int AHEAD>
 __global__ __launch_bounds__(G::TB) void k_layer_norm_bwd(typename SourceOf<T, STORED>::type src,
                                                           const T* __restrict__ dy, int64_t ldy, Affine p,
                                                           int64_t rows, int64_t width, int64_t groups,
@@ -346,35 +356,41 @@ __global__ __launch_bounds__(G::TB) void k_layer_norm_bwd(typename SourceOf<T, S
   }
   const int64_t step = (int64_t)gridDim.x * me.rt;
   int64_t row = (int64_t)blockIdx.x * me.rt + me.rl;
-  HeldSource<T, STORED> cx[NV], nx[NV];
-  Held<T> cg[NV], ng[NV];
-  float nm = 0.0f, nr = 0.0f;
-  auto fetch = [&](int64_t r) {
+  // a row's data; the next AHEAD rows are on their way while one is computed
+  struct Row {
+    HeldSource<T, STORED> x[NV];
+    Held<T, true> g[NV];
+    float mean, rstd;
+  };
+  Row cur, next[AHEAD ? AHEAD : 1];
+  auto fetch = [&](int64_t r, Row& to) {
     const bool on = me.live && r < rows;
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
-      nx[j].load(src, r, c0 + me.at(j), on ? left[j] : 0);
-      ng[j].load(dy + r * ldy + c0 + me.at(j), on ? left[j] : 0);
+      to.x[j].load(src, r, c0 + me.at(j), on ? left[j] : 0);
+      to.g[j].load(dy + r * ldy + c0 + me.at(j), on ? left[j] : 0);
     }
-    nm = on ? stats[2 * (r * groups + me.g)] : 0.0f;
-    nr = on ? stats[2 * (r * groups + me.g) + 1] : 0.0f;
+    to.mean = on ? stats[2 * (r * groups + me.g)] : 0.0f;
+    to.rstd = on ? stats[2 * (r * groups + me.g) + 1] : 0.0f;
   };
-  if constexpr (AHEAD) fetch(row);
+#pragma unroll
+  for (int d = 0; d < AHEAD; ++d) fetch(row + d * step, next[d]);
   int buf = 0;
   for (int64_t lead = (int64_t)blockIdx.x * me.rt; lead < rows; lead += step, row += step, buf ^= 1) {
-    if constexpr (!AHEAD) fetch(row);
-    const float mean = nm, rstd = nr;
+    if constexpr (AHEAD > 0) {
+      cur = next[0];
 #pragma unroll
-    for (int j = 0; j < NV; ++j) {
-      cx[j] = nx[j];
-      cg[j] = ng[j];
+      for (int d = 1; d < AHEAD; ++d) next[d - 1] = next[d];
+      fetch(row + AHEAD * step, next[AHEAD - 1]);
+    } else {
+      fetch(row, cur);
     }
-    if constexpr (AHEAD) fetch(row + step);
+    const float mean = cur.mean, rstd = cur.rstd;
     float s1 = 0.0f, s2 = 0.0f, h[kVec], g[kVec];
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
-      cx[j].get(h);
-      cg[j].get(g);
+      cur.x[j].get(h);
+      cur.g[j].get(g);
 #pragma unroll
       for (int i = 0; i < kVec; ++i) {
         h[i] = (h[i] - mean) * rstd;
@@ -407,8 +423,8 @@ __global__ __launch_bounds__(G::TB) void k_layer_norm_bwd(typename SourceOf<T, S
         T* out = dx + row * width + c0;
 #pragma unroll
         for (int j = 0; j < NV; ++j) {
-          cx[j].get(h);
-          cg[j].get(g);
+          cur.x[j].get(h);
+          cur.g[j].get(g);
 #pragma unroll
           for (int i = 0; i < kVec; ++i) g[i] = rstd * (g[i] * w[j][i] - m1 - (h[i] - mean) * rstd * m2);
           if (left[j] == kVec) store_vec(out + me.at(j), g);
@@ -565,10 +581,17 @@ int check_shape(const char* what, int64_t rows, int64_t width, int64_t groups) {
   return PRATCHYA_OK;
 }
 
-// Calls f(Shape) with the smallest team that holds a segment of D elements.
-// Forward teams share workgroups of 256 threads, backward teams of `TB`.
-template <int TB, typename F>
-auto with_shape(int64_t D, F f) {
+// Threads of a workgroup (more where a team is larger), workgroups of a launch,
+// rows on their way.
+constexpr int kFwdThreads = 256, kFwdAhead = 1, kBwdThreads = 1024, kBwdAhead = 1;
+constexpr int64_t kFwdBlocks = 2048, kBwdBlocks = 256;
+
+// Call f(Shape) with the smallest team that holds a segment of D elements: in the
+// forward pass with two vectors a thread where a wave is full, in the backward
+// pass, where a vector takes 40 registers more for its sums, with one.
+template <typename F>
+auto with_fwd_shape(int64_t D, F f) {
+  constexpr int TB = kFwdThreads;
   if (D <= 64) return f(Shape<8, 1, TB>());
   if (D <= 128) return f(Shape<16, 1, TB>());
   if (D <= 256) return f(Shape<32, 1, TB>());
@@ -579,6 +602,19 @@ auto with_shape(int64_t D, F f) {
   if (D <= 8192) return f(Shape<512, 2, 512>());
   return f(Shape<1024, 2, 1024>());
 }
+template <typename F>
+auto with_bwd_shape(int64_t D, F f) {
+  constexpr int TB = kBwdThreads;
+  if (D <= 64) return f(Shape<8, 1, TB>());
+  if (D <= 128) return f(Shape<16, 1, TB>());
+  if (D <= 256) return f(Shape<32, 1, TB>());
+  if (D <= 512) return f(Shape<64, 1, TB>());
+  if (D <= 1024) return f(Shape<128, 1, TB>());
+  if (D <= 2048) return f(Shape<256, 1, TB>());
+  if (D <= 4096) return f(Shape<512, 1, TB>());
+  if (D <= 8192) return f(Shape<1024, 1, TB>());
+  return f(Shape<1024, 2, TB>());
+}
 
 // Workgroups along the rows and along the segments of a row.
 template <typename G>
@@ -588,12 +624,9 @@ dim3 grid_of(int64_t rows, int64_t groups, int64_t most) {
   return dim3((unsigned)(gx < cap ? gx : cap), (unsigned)gy);
 }
 
-constexpr int kFwdThreads = 256, kBwdThreads = 512;
-constexpr int64_t kFwdBlocks = 2048, kBwdBlocks = 512;
-
 dim3 bwd_grid(int64_t rows, int64_t width, int64_t groups) {
-  return with_shape<kBwdThreads>(width / groups, [&](auto shape) {
-    return grid_of<decltype(shape)>(rows, groups, kBwdBlocks * kBwdThreads / decltype(shape)::TB);
+  return with_bwd_shape(width / groups, [&](auto shape) {
+    return grid_of<decltype(shape)>(rows, groups, kBwdBlocks);
   });
 }
 
@@ -602,7 +635,7 @@ void launch_fwd(G, const T* x, int64_t ldx, const Affine& p, int64_t rows, int64
                 T* y, float* stats, uint8_t* x8, uint8_t* sc8, float* sc32, int64_t blk, hipStream_t stream) {
   const dim3 grid = grid_of<G>(rows, groups, kFwdBlocks * kFwdThreads / G::TB);
 #define PRATCHYA_LN(B)                                                                                              \
-  hipLaunchKernelGGL((k_layer_norm<T, G, B>), grid, dim3(G::TB), 0, stream, x, ldx, p, rows, width, groups, eps, y, \
+  hipLaunchKernelGGL((k_layer_norm<T, G, B, kFwdAhead>), grid, dim3(G::TB), 0, stream, x, ldx, p, rows, width, groups, eps, y, \
                      stats, x8, sc8, sc32)
   if (!x8) PRATCHYA_LN(0);
   else if (blk == 16) PRATCHYA_LN(16);
@@ -621,7 +654,7 @@ int layer_norm(const void* x, int64_t ldx, const Affine& p, int64_t rows, int64_
     hipLaunchKernelGGL((k_layer_norm_long<T>), dim3((unsigned)(rows * groups)), dim3(256), 0, stream, xt, ldx, p, width,
                        groups, eps, yt, stats);
   else
-    with_shape<kFwdThreads>(width / groups, [&](auto shape) {
+    with_fwd_shape(width / groups, [&](auto shape) {
       launch_fwd<T>(shape, xt, ldx, p, rows, width, groups, eps, yt, stats, x8, sc8, sc32, blk, stream);
     });
   return check_launch("layer_norm");
@@ -646,11 +679,11 @@ int layer_norm_bwd(typename SourceOf<T, STORED>::type src, const void* dy, int64
                          dim3(256), 0, stream, src, g, ldy, rows, width, groups, stats, part);
     }
   } else {
-    with_shape<kBwdThreads>(width / groups, [&](auto shape) {
+    with_bwd_shape(width / groups, [&](auto shape) {
       typedef decltype(shape) G;
-      // a workgroup of 1024 threads has 128 registers a thread, none for a row ahead
-      constexpr bool AHEAD = G::TB <= 512;
-      const dim3 grid = grid_of<G>(rows, groups, kBwdBlocks * kBwdThreads / G::TB);
+      // two vectors a thread leave none of the 128 registers for a row ahead
+      constexpr int AHEAD = G::NV == 1 ? kBwdAhead : 0;
+      const dim3 grid = grid_of<G>(rows, groups, kBwdBlocks);
       slices = (int)grid.x;
       hipLaunchKernelGGL((k_layer_norm_bwd<T, G, STORED, AHEAD>), grid, dim3(G::TB), 0, stream, src, g, ldy, p, rows,
                          width, groups, stats, static_cast<T*>(dx), part, dw, dw16, db, db16);
