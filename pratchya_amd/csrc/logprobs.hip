@@ -82,9 +82,7 @@ struct Running {
 // Maximum and sums over the WPR waves of a row, for every thread (lds: 3 * WPR floats).
 template <int WPR, bool ENTROPY>
 __device__ __forceinline__ void join_running(Running<ENTROPY>& r, float* lds) {
-  float m = r.m;
-#pragma unroll
-  for (int w = 32; w >= 1; w >>= 1) m = fmaxf(m, __shfl_xor(m, w, 64));
+  float m = wave_max(r.m);
   if constexpr (WPR > 1) {
     if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = m;
     __syncthreads();
@@ -187,40 +185,67 @@ __global__ __launch_bounds__(WPR < 4 ? 256 : WPR * 64) void k_logprobs(
 constexpr int kPartThreads = 256, kPartVecs = 2, kBlock = kPartThreads * kPartVecs * kVec, kParts = 64;
 constexpr int kKeys = kPartVecs * kVec + 1;             // keys of a thread: a block's logits and one kept key
 
-// LDS of a selection among up to kKeys keys per thread.
+// LDS of a selection among up to kKeys keys per thread.  kCandidates is what
+// leaves room for eight workgroups in a compute unit (with room for every key, four
+// fit, and 1280 rows' parts of 4096 logits took twice the time).
+constexpr int kCandidates = 1024;
 struct Selection {
-  uint64_t cand[kPartThreads * kKeys];
+  uint64_t cand[kCandidates];
   uint64_t seen[kPartThreads];
+  uint32_t above[kPartThreads / 64][64];
   uint64_t bound;
   int found;
 };
 
 // The `top` largest of all threads' keys (0: no key) in falling order into
 // out[0 .. top), padded with 0, for the whole workgroup.  The top-th largest of
-// the maxima of 64 groups (threads of equal lane) is a bound that `top` keys
-// reach, if there are so many; keys that reach it are collected and ranked by
-// counting.  A lane's keys lie 8 logits apart from its neighbours', so rows of
-// equal logits leave some 8 top candidates, as rising or falling ones do.
-// out may be written before all threads have read it (barriers below).
+// the maxima of 64 or 128 groups (threads of equal lane, and parity of the wave)
+// is a bound that `top` keys reach, if there are so many; the keys that do are
+// ranked by counting: some 24 for 20 alternatives, 90 for 64.  A lane's keys lie 8
+// logits apart from its neighbours', so rows of equal logits leave some 8 top
+// candidates, as rising or falling ones do.  Where there are more than
+// kCandidates, the largest key is taken `top` times.  out may hold keys of this
+// selection: they are in registers.
+constexpr int kFewTop = 32;     // alternatives up to which 64 groups do
 __device__ __forceinline__ void select_top(const uint64_t (&keys)[kKeys], int top, Selection& sel, uint64_t* out) {
-  const int tid = threadIdx.x, lane = tid & 63;
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   uint64_t best = 0;
 #pragma unroll
   for (int i = 0; i < kKeys; ++i) best = umax64(best, keys[i]);
   sel.seen[tid] = best;
-  if (tid == 0) sel.found = 0;
+  if (tid == 0) {
+    sel.found = 0;
+    sel.bound = 0;       // where fewer than `top` groups have a key, every key is collected
+  }
+  __syncthreads();
+  // every wave holds all groups, two per lane, and counts how many of a quarter of
+  // the groups are larger than each
+  const bool few = top <= kFewTop;
+  uint64_t k0 = umax64(sel.seen[lane], sel.seen[128 + lane]), k1 = umax64(sel.seen[64 + lane], sel.seen[192 + lane]);
+  if (few) k0 = umax64(k0, k1);
+  uint32_t above0 = 0, above1 = 0;
+#pragma unroll
+  for (int g = 0; g < 16; ++g) {
+    const int from = wave * 16 + g;
+    const uint64_t key = (uint64_t)readlane_u32((uint32_t)(k0 >> 32), from) << 32 | readlane_u32((uint32_t)k0, from);
+    above0 += key > k0;
+    if (!few) above1 += key > k1;
+  }
+  if (!few) {
+#pragma unroll
+    for (int g = 0; g < 16; ++g) {
+      const int from = wave * 16 + g;
+      const uint64_t key = (uint64_t)readlane_u32((uint32_t)(k1 >> 32), from) << 32 | readlane_u32((uint32_t)k1, from);
+      above0 += key > k0;
+      above1 += key > k1;
+    }
+  }
+  sel.above[wave][lane] = above0 | above1 << 16;
   __syncthreads();
   if (tid < 64) {
-    const uint64_t own = umax64(umax64(sel.seen[lane], sel.seen[64 + lane]),
-                                umax64(sel.seen[128 + lane], sel.seen[192 + lane]));
-    int above = 0;
-#pragma unroll
-    for (int g = 0; g < 64; ++g) {
-      const uint64_t other = (uint64_t)readlane_u32((uint32_t)(own >> 32), g) << 32 | readlane_u32((uint32_t)own, g);
-      above += other > own;
-    }
-    // groups without a key are equal (0); where fewer than `top` have one, every key is collected
-    if (own ? above == top - 1 : above < top) sel.bound = own;
+    const uint32_t n = sel.above[0][lane] + sel.above[1][lane] + sel.above[2][lane] + sel.above[3][lane];
+    if (k0 != 0 && (int)(n & 0xFFFFu) == top - 1) sel.bound = k0;
+    if (!few && k1 != 0 && (int)(n >> 16) == top - 1) sel.bound = k1;
   }
   __syncthreads();
   const uint64_t bound = sel.bound;
@@ -231,17 +256,37 @@ __device__ __forceinline__ void select_top(const uint64_t (&keys)[kKeys], int to
     int at = atomicAdd(&sel.found, mine);
 #pragma unroll
     for (int i = 0; i < kKeys; ++i)
-      if (keys[i] != 0 && keys[i] >= bound) sel.cand[at++] = keys[i];
+      if (keys[i] != 0 && keys[i] >= bound) {
+        if (at < kCandidates) sel.cand[at] = keys[i];
+        ++at;
+      }
   }
   __syncthreads();
   const int n = sel.found;
-  if (tid >= n && tid < top) out[tid] = 0;
-  for (int c = tid; c < n; c += kPartThreads) {
-    const uint64_t own = sel.cand[c];
-    int above = 0;
+  if (n <= kCandidates) {
+    if (tid >= n && tid < top) out[tid] = 0;
+    for (int c = tid; c < n; c += kPartThreads) {
+      const uint64_t own = sel.cand[c];
+      int above = 0;
 #pragma unroll 8
-    for (int o = 0; o < n; ++o) above += sel.cand[o] > own;
-    if (above < top) out[above] = own;
+      for (int o = 0; o < n; ++o) above += sel.cand[o] > own;
+      if (above < top) out[above] = own;
+    }
+  } else {
+    uint64_t last = ~0ull;
+    for (int k = 0; k < top; ++k) {
+      uint64_t b = 0;
+#pragma unroll
+      for (int i = 0; i < kKeys; ++i)
+        if (keys[i] < last) b = umax64(b, keys[i]);
+#pragma unroll
+      for (int w = 32; w >= 1; w >>= 1) b = umax64(b, shfl_xor_u64(b, w));
+      if (lane == 0) sel.seen[wave] = b;
+      __syncthreads();
+      last = umax64(umax64(sel.seen[0], sel.seen[1]), umax64(sel.seen[2], sel.seen[3]));
+      if (tid == 0) out[k] = last;
+      __syncthreads();
+    }
   }
   __syncthreads();
 }
@@ -282,14 +327,17 @@ __global__ __launch_bounds__(kPartThreads) void k_logprobs_part(const T* __restr
       if (at + kVec <= to) widen(load_raw(xr + at), v[u]);
       else load_some(xr + at, to - at, -__builtin_inff(), v[u]);
     }
+#pragma unroll
+    for (int u = 0; u < kPartVecs; ++u)
+      if (base + (u * kPartThreads + tid) * kVec < to) r.add(v[u]);
     uint64_t keys[kKeys];
 #pragma unroll
-    for (int u = 0; u < kPartVecs; ++u) {
-      const int64_t at = base + (u * kPartThreads + tid) * kVec;
-      if (at < to) r.add(v[u]);
+    for (int u = 0; u < kPartVecs; ++u)
 #pragma unroll
-      for (int j = 0; j < kVec; ++j) keys[u * kVec + j] = at + j < to ? rank_key(v[u][j], at + j) : 0;
-    }
+      for (int j = 0; j < kVec; ++j) {
+        const int64_t i = base + (u * kPartThreads + tid) * kVec + j;
+        keys[u * kVec + j] = i < to ? rank_key(v[u][j], i) : 0;
+      }
     keys[kKeys - 1] = tid < top ? list[tid] : 0;
     select_top(keys, top, sel, list);
   }

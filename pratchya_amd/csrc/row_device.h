@@ -120,6 +120,21 @@ __device__ __forceinline__ float lane_group_add(float v) {
   }
   return v;
 }
+// The largest of the wave's values, for every lane; NaN is passed over.
+template <int CTRL>
+__device__ __forceinline__ float dpp_max_f32(float v) {
+  return fmaxf(v, u2f((uint32_t)__builtin_amdgcn_update_dpp((int)f2u(v), (int)f2u(v), CTRL, 0xF, 0xF, false)));
+}
+__device__ __forceinline__ float wave_max(float v) {
+  v = dpp_max_f32<0xB1>(v);
+  v = dpp_max_f32<0x4E>(v);
+  v = dpp_max_f32<0x141>(v);
+  v = dpp_max_f32<0x140>(v);
+  const auto p = __builtin_amdgcn_permlane16_swap(f2u(v), f2u(v), false, false);
+  v = fmaxf(u2f(p[0]), u2f(p[1]));
+  const auto q = __builtin_amdgcn_permlane32_swap(f2u(v), f2u(v), false, false);
+  return fmaxf(u2f(q[0]), u2f(q[1]));
+}
 // Sum over the lanes of a wave, for every lane.
 __device__ __forceinline__ float wave_add(float v) { return lane_group_add<64>(v); }
 
