@@ -54,20 +54,21 @@ __device__ __forceinline__ float sigmoid(float x) {
   return __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(-x * kLog2e));
 }
 
-// f of eight values; the kind is the same for the whole launch.
-__device__ __forceinline__ void act(float (&v)[kVec], int kind) {
+// f of a vector; the kind is the same for the whole launch.
+template <int N>
+__device__ __forceinline__ void act(float (&v)[N], int kind) {
   if (kind == PRATCHYA_ACT_RELU2) {
 #pragma unroll
-    for (int i = 0; i < kVec; ++i) {
+    for (int i = 0; i < N; ++i) {
       const float r = v[i] < 0.0f ? 0.0f : v[i];
       v[i] = r * r;
     }
   } else if (kind == PRATCHYA_ACT_SILU) {
 #pragma unroll
-    for (int i = 0; i < kVec; ++i) v[i] *= sigmoid(v[i]);
+    for (int i = 0; i < N; ++i) v[i] *= sigmoid(v[i]);
   } else {
 #pragma unroll
-    for (int i = 0; i < kVec; ++i) {
+    for (int i = 0; i < N; ++i) {
       float P, p;
       normal(v[i], P, p);
       v[i] *= P;
@@ -76,19 +77,20 @@ __device__ __forceinline__ void act(float (&v)[kVec], int kind) {
 }
 
 // g *= f'(v).
-__device__ __forceinline__ void act_grad(const float (&v)[kVec], float (&g)[kVec], int kind) {
+template <int N>
+__device__ __forceinline__ void act_grad(const float (&v)[N], float (&g)[N], int kind) {
   if (kind == PRATCHYA_ACT_RELU2) {
 #pragma unroll
-    for (int i = 0; i < kVec; ++i) g[i] *= v[i] < 0.0f ? 0.0f : 2.0f * v[i];
+    for (int i = 0; i < N; ++i) g[i] *= v[i] < 0.0f ? 0.0f : 2.0f * v[i];
   } else if (kind == PRATCHYA_ACT_SILU) {
 #pragma unroll
-    for (int i = 0; i < kVec; ++i) {
+    for (int i = 0; i < N; ++i) {
       const float s = sigmoid(v[i]);
       g[i] *= s * (1.0f + v[i] * (1.0f - s));
     }
   } else {
 #pragma unroll
-    for (int i = 0; i < kVec; ++i) {
+    for (int i = 0; i < N; ++i) {
       float P, p;
       normal(v[i], P, p);
       g[i] *= P + v[i] * p;
@@ -96,10 +98,12 @@ __device__ __forceinline__ void act_grad(const float (&v)[kVec], float (&g)[kVec
   }
 }
 
-// Vectors of eight elements, numbered through all rows; a wave takes 128
-// neighbouring ones, two per lane, so a group of stored blocks (at most 1024
-// elements) lies in one wave.  ONE: the array is one row (contiguous rows).
-constexpr int kThreads = 256, kPer = 2, kWaveVecs = 64 * kPer;
+// Vectors, numbered through all rows; a wave takes 1024 neighbouring elements, a
+// vector per lane and step, so a group of stored blocks (at most 1024 elements)
+// lies in one wave.  ONE: the array is one row (contiguous rows).
+constexpr int kThreads = 256;
+template <typename T>
+constexpr int kPer = 16 / kN<T>;         // vectors of a thread
 
 struct Rows {
   int64_t ldx, width, vecs_per_row, vecs;
@@ -108,63 +112,72 @@ struct At {
   int64_t row, c;
   int left;        // elements of the vector, 0 beyond the array
 };
-template <bool ONE>
+template <int N, bool ONE>
 __device__ __forceinline__ At place(const Rows& r, int64_t vec) {
   if (vec >= r.vecs) return {0, 0, 0};
-  const int64_t row = ONE ? 0 : vec / r.vecs_per_row, c = (ONE ? vec : vec - row * r.vecs_per_row) * kVec;
-  return {row, c, r.width - c < kVec ? (int)(r.width - c) : kVec};
+  const int64_t row = ONE ? 0 : vec / r.vecs_per_row, c = (ONE ? vec : vec - row * r.vecs_per_row) * N;
+  return {row, c, r.width - c < N ? (int)(r.width - c) : N};
 }
+template <typename T>
 __device__ __forceinline__ int64_t first_vec() {
-  return ((int64_t)blockIdx.x * (kThreads / 64) + (threadIdx.x >> 6)) * kWaveVecs + (threadIdx.x & 63);
+  return ((int64_t)blockIdx.x * (kThreads / 64) + (threadIdx.x >> 6)) * (64 * kPer<T>) + (threadIdx.x & 63);
 }
 
-// Maximum over groups of K blocks of BLK elements, from the blocks' maxima of
-// this lane's two vectors (64 lanes apart).
-template <int BLK>
-__device__ __forceinline__ void group_max(uint32_t m0, uint32_t m1, int K, uint32_t& G0, uint32_t& G1) {
-  constexpr int LB = BLK / kVec;
-  G0 = m0;
-  G1 = m1;
+// Maxima over groups of K blocks of LB lanes, from the blocks' maxima m of a
+// lane's PER vectors (64 lanes apart), for a K of 1, 2, 4 or 8.
+template <int LB, int PER, int K>
+__device__ __forceinline__ void group_max_of(const uint32_t (&m)[PER], uint32_t (&G)[PER]) {
+  constexpr int LG = LB * K, LR = LG < 64 ? LG : 64, GV = LG / LR;
+  static_assert(GV <= PER, "a group lies in one wave");
+#pragma unroll
+  for (int u = 0; u < PER; u += GV) {
+    uint32_t g = m[u];
+#pragma unroll
+    for (int k = 1; k < GV; ++k) g = umax(g, m[u + k]);
+    g = lane_group_max<LR>(g);
+#pragma unroll
+    for (int k = 0; k < GV; ++k) G[u + k] = g;
+  }
+}
+template <int BLK, int N, int PER>
+__device__ __forceinline__ void group_max(const uint32_t (&m)[PER], int K, uint32_t (&G)[PER]) {
+  constexpr int LB = BLK / N;
+  if (K == 1) group_max_of<LB, PER, 1>(m, G);
   if constexpr (BLK >= 32)
-    if (K == 2) {
-      G0 = lane_group_max<2 * LB>(m0);
-      G1 = lane_group_max<2 * LB>(m1);
-    }
+    if (K == 2) group_max_of<LB, PER, 2>(m, G);
   if constexpr (BLK >= 64)
-    if (K == 4) {
-      G0 = lane_group_max<4 * LB>(m0);
-      G1 = lane_group_max<4 * LB>(m1);
-    }
+    if (K == 4) group_max_of<LB, PER, 4>(m, G);
   if constexpr (BLK >= 128)
-    if (K == 8) G0 = G1 = lane_group_max<64>(umax(m0, m1));
+    if (K == 8) group_max_of<LB, PER, 8>(m, G);
 }
 
 template <typename T, int BLK, bool ONE>
 __global__ __launch_bounds__(kThreads) void k_act(const T* __restrict__ x, Rows r, int kind, T* __restrict__ y,
                                                   uint8_t* __restrict__ x8, uint8_t* __restrict__ sc8,
                                                   float* __restrict__ sc32, int K) {
-  const int64_t vec = first_vec();
-  At at[kPer];
-  float v[kPer][kVec];
+  constexpr int N = kN<T>, PER = kPer<T>;
+  const int64_t vec = first_vec<T>();
+  At at[PER];
+  float v[PER][N];
 #pragma unroll
-  for (int u = 0; u < kPer; ++u) {
-    at[u] = place<ONE>(r, vec + u * 64);
+  for (int u = 0; u < PER; ++u) {
+    at[u] = place<N, ONE>(r, vec + u * 64);
     const T* p = x + at[u].row * r.ldx + at[u].c;
-    if (at[u].left == kVec) widen(load_raw<true>(p), v[u]);
+    if (at[u].left == N) widen(load_raw<true>(p), v[u]);
     else load_some(p, at[u].left, 0.0f, v[u]);
   }
   if constexpr (BLK != 0) {
-    uint32_t m[kPer], G[kPer];
+    uint32_t m[PER], G[PER] = {};
 #pragma unroll
-    for (int u = 0; u < kPer; ++u) m[u] = lane_group_max<BLK / kVec>(absmax8(v[u]));
-    group_max<BLK>(m[0], m[1], K, G[0], G[1]);
+    for (int u = 0; u < PER; ++u) m[u] = lane_group_max<BLK / N>(absmax(v[u]));
+    group_max<BLK, N>(m, K, G);
 #pragma unroll
-    for (int u = 0; u < kPer; ++u) {
+    for (int u = 0; u < PER; ++u) {
       if (at[u].left == 0) continue;          // blocks divide rows: a vector is whole
-      const int64_t e0 = (vec + u * 64) * kVec;
+      const int64_t e0 = (vec + u * 64) * N;
       uint32_t e;
-      const u32x2_t q = store_form(v[u], m[u], G[u], e);
-      __builtin_nontemporal_store(q, reinterpret_cast<u32x2_t*>(x8 + e0));
+      const auto q = store_form(v[u], m[u], G[u], e);
+      __builtin_nontemporal_store(q, reinterpret_cast<typename Payload<N>::type*>(x8 + e0));
       const int64_t n = e0 / BLK;
       if (e0 % BLK == 0) {
         sc8[n] = (uint8_t)e;
@@ -173,10 +186,10 @@ __global__ __launch_bounds__(kThreads) void k_act(const T* __restrict__ x, Rows 
     }
   }
 #pragma unroll
-  for (int u = 0; u < kPer; ++u) {
+  for (int u = 0; u < PER; ++u) {
     act(v[u], kind);
     T* p = y + at[u].row * r.width + at[u].c;
-    if (at[u].left == kVec) store_vec<true>(p, v[u]);
+    if (at[u].left == N) store_vec<true>(p, v[u]);
     else store_some(p, at[u].left, v[u]);
   }
 }
@@ -192,36 +205,38 @@ template <typename T, bool STORED, bool ONE>
 __global__ __launch_bounds__(kThreads) void k_act_bwd(const T* __restrict__ x, Rows r, StoredX s,
                                                       const T* __restrict__ dy, int64_t ldy, int kind,
                                                       T* __restrict__ dx) {
-  const int64_t vec = first_vec();
-  At at[kPer];
-  float v[kPer][kVec], g[kPer][kVec];
-  u32x2_t q[kPer];
-  float scale[kPer];
+  constexpr int N = kN<T>, PER = kPer<T>;
+  typedef typename Payload<N>::type W;
+  const int64_t vec = first_vec<T>();
+  At at[PER];
+  float v[PER][N], g[PER][N];
+  W q[PER];
+  float scale[PER];
 #pragma unroll
-  for (int u = 0; u < kPer; ++u) {
-    at[u] = place<ONE>(r, vec + u * 64);
+  for (int u = 0; u < PER; ++u) {
+    at[u] = place<N, ONE>(r, vec + u * 64);
     const T* p = dy + at[u].row * ldy + at[u].c;
     if constexpr (STORED) {
       if (at[u].left) {
-        const int64_t e0 = (vec + u * 64) * kVec, n = e0 >> s.blk_log2;
-        q[u] = __builtin_nontemporal_load(reinterpret_cast<const u32x2_t*>(s.x8 + e0));
+        const int64_t e0 = (vec + u * 64) * N, n = e0 >> s.blk_log2;
+        q[u] = __builtin_nontemporal_load(reinterpret_cast<const W*>(s.x8 + e0));
         scale[u] = e8m0_decode(s.sc8[n]) * s.sc32[n >> s.K_log2];
       }
     } else {
       const T* px = x + at[u].row * r.ldx + at[u].c;
-      if (at[u].left == kVec) widen(load_raw<true>(px), v[u]);
+      if (at[u].left == N) widen(load_raw<true>(px), v[u]);
       else load_some(px, at[u].left, 0.0f, v[u]);
     }
-    if (at[u].left == kVec) widen(load_raw<true>(p), g[u]);
+    if (at[u].left == N) widen(load_raw<true>(p), g[u]);
     else load_some(p, at[u].left, 0.0f, g[u]);
   }
 #pragma unroll
-  for (int u = 0; u < kPer; ++u) {
+  for (int u = 0; u < PER; ++u) {
     if (at[u].left == 0) continue;
     if constexpr (STORED) stored_values(q[u], scale[u], v[u]);
     act_grad(v[u], g[u], kind);
     T* p = dx + at[u].row * r.width + at[u].c;
-    if (at[u].left == kVec) store_vec<true>(p, g[u]);
+    if (at[u].left == N) store_vec<true>(p, g[u]);
     else store_some(p, at[u].left, g[u]);
   }
 }
@@ -237,9 +252,10 @@ int check_args(const char* what, int kind, int dtype, int64_t rows, int64_t widt
 }
 
 // Rows as one where nothing lies between them.
+template <typename T>
 Rows make_rows(int64_t ldx, int64_t ldy, int64_t rows, int64_t width, bool& one) {
   one = rows == 1 || (ldx == width && ldy == width);
-  const int64_t w = one ? rows * width : width, per = (w + kVec - 1) / kVec;
+  const int64_t w = one ? rows * width : width, per = (w + kN<T> - 1) / kN<T>;
   return {ldx, w, per, one ? per : rows * per};
 }
 
@@ -252,22 +268,25 @@ int log2_of(int64_t v) {
   return n;
 }
 
-int64_t workgroups(const Rows& r) { return (r.vecs + kThreads * kPer - 1) / (kThreads * kPer); }
+template <typename T>
+int64_t workgroups(const Rows& r) {
+  return (r.vecs + kThreads * kPer<T> - 1) / (kThreads * kPer<T>);
+}
 
 template <typename T>
 int launch(const void* x, int64_t ldx, int kind, int64_t rows, int64_t width, void* y, uint8_t* x8, uint8_t* sc8,
            float* sc32, int64_t blk, hipStream_t stream) {
   bool one;
-  const Rows r = make_rows(ldx, width, rows, width, one);
+  const Rows r = make_rows<T>(ldx, width, rows, width, one);
   const int K = x8 ? (int)gcd64(blk / 16, rows * width / blk) : 1;
-  if (workgroups(r) > 0x7FFFFFFF)
+  if (workgroups<T>(r) > 0x7FFFFFFF)
     return pratchya_set_error(PRATCHYA_EUNSUPPORTED, "activation: more than 2^31 workgroups");
 #define PRATCHYA_ACT(B)                                                                                              \
   if (one)                                                                                                           \
-    hipLaunchKernelGGL((k_act<T, B, true>), dim3((unsigned)workgroups(r)), dim3(kThreads), 0, stream,                \
+    hipLaunchKernelGGL((k_act<T, B, true>), dim3((unsigned)workgroups<T>(r)), dim3(kThreads), 0, stream,                \
                        static_cast<const T*>(x), r, kind, static_cast<T*>(y), x8, sc8, sc32, K);                     \
   else                                                                                                               \
-    hipLaunchKernelGGL((k_act<T, B, false>), dim3((unsigned)workgroups(r)), dim3(kThreads), 0, stream,               \
+    hipLaunchKernelGGL((k_act<T, B, false>), dim3((unsigned)workgroups<T>(r)), dim3(kThreads), 0, stream,               \
                        static_cast<const T*>(x), r, kind, static_cast<T*>(y), x8, sc8, sc32, K)
   if (!x8) { PRATCHYA_ACT(0); }
   else if (blk == 16) { PRATCHYA_ACT(16); }
@@ -282,10 +301,10 @@ template <typename T, bool STORED>
 int launch_bwd(const void* x, int64_t ldx, const StoredX& s, const void* dy, int64_t ldy, int kind, int64_t rows,
                int64_t width, void* dx, hipStream_t stream) {
   bool one;
-  const Rows r = make_rows(STORED ? width : ldx, ldy, rows, width, one);
-  if (workgroups(r) > 0x7FFFFFFF)
+  const Rows r = make_rows<T>(STORED ? width : ldx, ldy, rows, width, one);
+  if (workgroups<T>(r) > 0x7FFFFFFF)
     return pratchya_set_error(PRATCHYA_EUNSUPPORTED, "activation_bwd: more than 2^31 workgroups");
-  const dim3 grid((unsigned)workgroups(r));
+  const dim3 grid((unsigned)workgroups<T>(r));
   const T* xt = STORED ? nullptr : static_cast<const T*>(x);
   if (one)
     hipLaunchKernelGGL((k_act_bwd<T, STORED, true>), grid, dim3(kThreads), 0, stream, xt, r, s,
@@ -322,7 +341,7 @@ extern "C" int pratchya_activation_bwd(const void* x, int64_t ldx, int x_dtype, 
   const bool stored = x_dtype == PRATCHYA_DT_E4M3;
   if (!stored && x_dtype != dtype)
     return pratchya_set_error(PRATCHYA_EINVAL, "activation_bwd: unsupported dtypes (x %d, dy %d)", x_dtype, dtype);
-  if (stored && (blk < kVec || (blk & (blk - 1)) || width % blk))
+  if (stored && (blk < 8 || (blk & (blk - 1)) || width % blk))
     return pratchya_set_error(PRATCHYA_EINVAL, "activation_bwd: blocks of %lld for rows of %lld", (long long)blk,
                               (long long)width);
   const int64_t n = rows * width;

@@ -43,19 +43,19 @@ struct Affine {
   bool w16, b16;
 };
 
-// A segment that fits P threads of NV vectors of eight elements each stays in
+// A segment that fits P threads of NV vectors of N = kN<T> elements each stays in
 // registers.  A workgroup of TB threads holds TB / P such teams; a team keeps one
 // segment position of the row (its slice of w and b, and of dw and db) and walks
 // over rows: `gt` neighbouring segments side by side, the other teams on
-// further rows.  Thread t of a team holds vectors (t / 64 * NV + j) * 64 + t % 64
-// (P >= 64), so a wave reads runs of 512 elements and groups of stored blocks lie
-// in one wave.  Streaming accesses where they measured faster, [16384, 4096] bf16:
+// further rows.  Thread t of a team holds vectors (t / L * NV + j) * L + t % L, L =
+// min(P, 64), j < NV: groups of stored blocks lie in one wave.  Streaming accesses where they measured faster, [16384, 4096] bf16:
 // the forward pass's stores (55.2 -> 52.3 us; its loads 55.2 -> 50.8, but 25.2 ->
 // 25.7 us and 11.0 -> 12.0 us where the caches hold x), the backward pass's
 // loads (84.3 -> 79.8 us; its stores 84.3 -> 83.4, with the loads 82.7 us).
 template <int P_, int NV_, int TB_>
 struct Shape {
   static constexpr int P = P_, NV = NV_, TB = TB_, TEAMS = TB_ / P_, WAVES = P_ > 64 ? P_ / 64 : 1;
+  static constexpr int LANES = P_ < 64 ? P_ : 64;
 };
 
 template <typename G>
@@ -73,52 +73,52 @@ struct Place {
     g = (int64_t)blockIdx.y * gt + team % gt;
     live = rl < rt && g < groups;
   }
-  // first element of this thread's vector j in its segment
+  // first element of this thread's vector j, of N elements, in its segment
+  template <int N>
   __device__ __forceinline__ int64_t at(int j) const {
-    if constexpr (G::P < 64) return t * kVec;
-    else return (int64_t)(((t >> 6) * G::NV + j) * 64 + (t & 63)) * kVec;
+    return (int64_t)((t / G::LANES * G::NV + j) * G::LANES + t % G::LANES) * N;
   }
 };
 
-__device__ __forceinline__ int clamp8(int64_t n) { return n < 0 ? 0 : n < kVec ? (int)n : kVec; }
-
-template <typename T>
-__device__ __forceinline__ void load_vec_or_some(const T* p, int left, float (&v)[kVec]) {
-  if (left == kVec) widen(load_raw(p), v);
-  else load_some(p, left, 0.0f, v);
-}
+// Elements of a vector that lie in the segment.
+template <int N>
+__device__ __forceinline__ int part_of(int64_t n) { return n < 0 ? 0 : n < N ? (int)n : N; }
 
 // A vector of a row in registers, in its type.
 template <typename T, bool NT = false>
 struct Held {
-  typename RawOf<T>::type raw;
+  u32x4_t raw;
   __device__ __forceinline__ void load(const T* p, int left) {
-    if (left == kVec) {
+    if (left == kN<T>) {
       raw = load_raw<NT>(p);
     } else {
-      float v[kVec];
+      float v[kN<T>];
       load_some(p, left, 0.0f, v);
-      if constexpr (sizeof(T) == 2)
-        raw.v = u32x4_t{pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]), pack_bf16x2(v[4], v[5]),
-                        pack_bf16x2(v[6], v[7])};
-      else {
-        raw.lo = u32x4_t{f2u(v[0]), f2u(v[1]), f2u(v[2]), f2u(v[3])};
-        raw.hi = u32x4_t{f2u(v[4]), f2u(v[5]), f2u(v[6]), f2u(v[7])};
-      }
+      raw = narrow(v);
     }
   }
-  __device__ __forceinline__ void get(float (&v)[kVec]) const { widen(raw, v); }
+  __device__ __forceinline__ void get(float (&v)[kN<T>]) const { widen(raw, v); }
 };
 
+template <int N>
 __device__ __forceinline__ void load_params(const void* p, bool bf16, int64_t at, int left, float none,
-                                            float (&v)[kVec]) {
-  if (!p) {
+                                            float (&v)[N]) {
 #pragma unroll
-    for (int i = 0; i < kVec; ++i) v[i] = none;
+  for (int i = 0; i < N; ++i) v[i] = none;
+  if (!p) return;
+  if (left == N && !bf16) {
+#pragma unroll
+    for (int i = 0; i < N; i += 4) {
+      const u32x4_t r = load_raw(static_cast<const float*>(p) + at + i);
+      v[i] = u2f(r[0]);
+      v[i + 1] = u2f(r[1]);
+      v[i + 2] = u2f(r[2]);
+      v[i + 3] = u2f(r[3]);
+    }
   } else if (bf16) {
-    load_vec_or_some(static_cast<const uint16_t*>(p) + at, left, v);
+    load_some(static_cast<const uint16_t*>(p) + at, left, none, v);
   } else {
-    load_vec_or_some(static_cast<const float*>(p) + at, left, v);
+    load_some(static_cast<const float*>(p) + at, left, none, v);
   }
 }
 
@@ -130,28 +130,28 @@ __global__ __launch_bounds__(G::TB) void k_layer_norm(const T* __restrict__ x, i
                                                       int64_t width, int64_t groups, float eps, T* __restrict__ y,
                                                       float* __restrict__ stats, uint8_t* __restrict__ x8,
                                                       uint8_t* __restrict__ sc8, float* __restrict__ sc32) {
-  constexpr int NV = G::NV, LANES = G::P < 64 ? G::P : 64;
+  constexpr int N = kN<T>, NV = G::NV, LANES = G::LANES, SPAN = NV * LANES * N;   // SPAN: elements of a wave
   __shared__ float red[2][G::TEAMS * G::WAVES][2];
   const Place<G> me(groups);
   const int64_t D = width / groups, c0 = me.g * D;
   int left[NV];
-  float w[NV][kVec], b[NV][kVec];
+  float w[NV][N], b[NV][N];
 #pragma unroll
   for (int j = 0; j < NV; ++j) {
-    left[j] = me.live ? clamp8(D - me.at(j)) : 0;
-    load_params(p.w, p.w16, c0 + me.at(j), left[j], 1.0f, w[j]);
-    load_params(p.b, p.b16, c0 + me.at(j), left[j], 0.0f, b[j]);
+    left[j] = me.live ? part_of<N>(D - me.template at<N>(j)) : 0;
+    load_params(p.w, p.w16, c0 + me.template at<N>(j), left[j], 1.0f, w[j]);
+    load_params(p.b, p.b16, c0 + me.template at<N>(j), left[j], 0.0f, b[j]);
   }
   // elements of the segment that this wave holds
-  const int64_t first = (int64_t)(me.t >> 6) * NV * 512;
-  const float mine = G::P < 64 ? (float)D : (float)(D - first < 0 ? 0 : D - first < NV * 512 ? D - first : NV * 512);
+  const int64_t first = (int64_t)(me.t / LANES) * SPAN;
+  const float mine = (float)(D - first < 0 ? 0 : D - first < SPAN ? D - first : SPAN);
   const int64_t step = (int64_t)gridDim.x * me.rt;
   int64_t row = (int64_t)blockIdx.x * me.rt + me.rl;
   // the next AHEAD rows are on their way while one is computed
   Held<T> cur[NV], next[AHEAD][NV];
   auto fetch = [&](int64_t r, Held<T> (&to)[NV]) {
 #pragma unroll
-    for (int j = 0; j < NV; ++j) to[j].load(x + r * ldx + c0 + me.at(j), r < rows ? left[j] : 0);
+    for (int j = 0; j < NV; ++j) to[j].load(x + r * ldx + c0 + me.template at<N>(j), r < rows ? left[j] : 0);
   };
 #pragma unroll
   for (int d = 0; d < AHEAD; ++d) fetch(row + d * step, next[d]);
@@ -166,12 +166,12 @@ __global__ __launch_bounds__(G::TB) void k_layer_norm(const T* __restrict__ x, i
       for (int d = 1; d < AHEAD; ++d) next[d - 1][j] = next[d][j];
     }
     fetch(row + AHEAD * step, next[AHEAD - 1]);
-    float v[kVec], s = 0.0f, q = 0.0f;
+    float v[N], s = 0.0f, q = 0.0f;
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
       cur[j].get(v);
 #pragma unroll
-      for (int i = 0; i < kVec; ++i) s += v[i];
+      for (int i = 0; i < N; ++i) s += v[i];
     }
     s = lane_group_add<LANES>(s);
     float mean = mine > 0.0f ? s / mine : 0.0f;
@@ -179,7 +179,7 @@ __global__ __launch_bounds__(G::TB) void k_layer_norm(const T* __restrict__ x, i
     for (int j = 0; j < NV; ++j) {
       cur[j].get(v);
 #pragma unroll
-      for (int i = 0; i < kVec; ++i) {
+      for (int i = 0; i < N; ++i) {
         const float d = v[i] - mean;
         q += i < left[j] ? d * d : 0.0f;
       }
@@ -199,9 +199,9 @@ __global__ __launch_bounds__(G::TB) void k_layer_norm(const T* __restrict__ x, i
       q = 0.0f;
 #pragma unroll
       for (int k = 0; k < G::WAVES; ++k) {
-        const int64_t from = (int64_t)k * NV * 512;
+        const int64_t from = (int64_t)k * SPAN;
         if (from < D) {
-          const float n = (float)(D - from < NV * 512 ? D - from : NV * 512), d = r[k][0] / n - mean;
+          const float n = (float)(D - from < SPAN ? D - from : SPAN), d = r[k][0] / n - mean;
           q += r[k][1] + n * d * d;
         }
       }
@@ -217,32 +217,35 @@ __global__ __launch_bounds__(G::TB) void k_layer_norm(const T* __restrict__ x, i
     for (int j = 0; j < NV; ++j) {
       cur[j].get(v);
 #pragma unroll
-      for (int i = 0; i < kVec; ++i) v[i] = (v[i] - mean) * rstd * w[j][i] + b[j][i];
-      if (left[j] == kVec) store_vec<true>(yr + me.at(j), v);
-      else if (left[j]) store_some(yr + me.at(j), left[j], v);
+      for (int i = 0; i < N; ++i) v[i] = (v[i] - mean) * rstd * w[j][i] + b[j][i];
+      if (left[j] == N) store_vec<true>(yr + me.template at<N>(j), v);
+      else if (left[j]) store_some(yr + me.template at<N>(j), left[j], v);
     }
     if constexpr (BLK != 0) {
-      constexpr int LB = BLK / kVec, LG = BLK <= 16 ? LB : BLK == 32 ? 8 : BLK == 64 ? 32 : 64;
+      // lanes of a block, of a group, and vectors that a group spans
+      constexpr int K = BLK / 16, LB = BLK / N, LG = LB * K, LR = LG < LANES ? LG : LANES, GV = LG / LR;
       uint32_t mb[NV], Gb[NV];
 #pragma unroll
       for (int j = 0; j < NV; ++j) {
         cur[j].get(v);
-        mb[j] = lane_group_max<LB>(absmax8(v));
-        Gb[j] = lane_group_max<LG>(mb[j]);
+        mb[j] = lane_group_max<LB>(absmax(v));
+        Gb[j] = lane_group_max<LR>(mb[j]);
       }
-      if constexpr (BLK == 128) {
 #pragma unroll
-        for (int j = 0; j + 1 < NV; j += 2) Gb[j] = Gb[j + 1] = umax(Gb[j], Gb[j + 1]);
+      for (int j = 0; j < NV; j += GV) {
+#pragma unroll
+        for (int k = 1; k < GV; ++k) Gb[j] = umax(Gb[j], Gb[j + k]);
+#pragma unroll
+        for (int k = 1; k < GV; ++k) Gb[j + k] = Gb[j];
       }
 #pragma unroll
       for (int j = 0; j < NV; ++j) {
         if (left[j] == 0) continue;
         cur[j].get(v);
         uint32_t e;
-        const int64_t at = row * width + me.at(j);
-        const u32x2_t q8 = store_form(v, mb[j], Gb[j], e);
-        __builtin_nontemporal_store(q8, reinterpret_cast<u32x2_t*>(x8 + at));
-        constexpr int K = BLK <= 16 ? 1 : BLK / 16;
+        const int64_t at = row * width + me.template at<N>(j);
+        const auto q8 = store_form(v, mb[j], Gb[j], e);
+        __builtin_nontemporal_store(q8, reinterpret_cast<typename Payload<N>::type*>(x8 + at));
         if (at % BLK == 0) sc8[at / BLK] = (uint8_t)e;
         if (at % (BLK * K) == 0) sc32[at / (BLK * K)] = u2f(Gb[j]);
       }
@@ -309,24 +312,25 @@ template <typename T> struct HeldSource<T, false> {
   __device__ __forceinline__ void load(const Source<T>& s, int64_t row, int64_t c, int left) {
     x.load(s.x + row * s.ldx + c, left);
   }
-  __device__ __forceinline__ void get(float (&v)[kVec]) const { x.get(v); }
+  __device__ __forceinline__ void get(float (&v)[kN<T>]) const { x.get(v); }
 };
 template <typename T> struct HeldSource<T, true> {
-  u32x2_t w;
+  typedef typename Payload<kN<T>>::type W;
+  W w;
   uint32_t e;
   float G;
   __device__ __forceinline__ void load(const Stored& s, int64_t row, int64_t c, int left) {
-    w = u32x2_t{0, 0};
+    w = W{};
     e = 0;
     G = 0.0f;
-    if (left) {     // blocks are a multiple of eight elements: a vector lies in one
+    if (left) {     // blocks are a multiple of a vector: it lies in one
       const int64_t at = row * s.width + c, n = at >> s.blk_log2;
-      w = __builtin_nontemporal_load(reinterpret_cast<const u32x2_t*>(s.x8 + at));
+      w = __builtin_nontemporal_load(reinterpret_cast<const W*>(s.x8 + at));
       e = s.sc8[n];
       G = s.sc32[n >> s.K_log2];
     }
   }
-  __device__ __forceinline__ void get(float (&v)[kVec]) const { stored_values(w, e8m0_decode(e) * G, v); }
+  __device__ __forceinline__ void get(float (&v)[kN<T>]) const { stored_values(w, e8m0_decode(e) * G, v); }
 };
 
 // dx of whole segments, and the sums of dy h and dy over the rows that a team
@@ -340,19 +344,19 @@ __global__ __launch_bounds__(G::TB) void k_layer_norm_bwd(typename SourceOf<T, S
                                                           const float* __restrict__ stats, T* __restrict__ dx,
                                                           float* __restrict__ part, void* dw, bool dw16, void* db,
                                                           bool db16) {
-  constexpr int NV = G::NV, LANES = G::P < 64 ? G::P : 64, SUMS = 2 * NV * kVec;
+  constexpr int N = kN<T>, NV = G::NV, LANES = G::LANES, SUMS = 2 * NV * N;
   __shared__ float red[2][G::TEAMS * G::WAVES][2];
   __shared__ float sums[G::TEAMS > 1 ? SUMS * (G::TB / 2) : 1];
   const Place<G> me(groups);
   const int64_t D = width / groups, c0 = me.g * D;
   int left[NV];
-  float w[NV][kVec], aw[NV][kVec], ab[NV][kVec];
+  float w[NV][N], aw[NV][N], ab[NV][N];
 #pragma unroll
   for (int j = 0; j < NV; ++j) {
-    left[j] = me.live ? clamp8(D - me.at(j)) : 0;
-    load_params(p.w, p.w16, c0 + me.at(j), left[j], 1.0f, w[j]);
+    left[j] = me.live ? part_of<N>(D - me.template at<N>(j)) : 0;
+    load_params(p.w, p.w16, c0 + me.template at<N>(j), left[j], 1.0f, w[j]);
 #pragma unroll
-    for (int i = 0; i < kVec; ++i) aw[j][i] = ab[j][i] = 0.0f;
+    for (int i = 0; i < N; ++i) aw[j][i] = ab[j][i] = 0.0f;
   }
   const int64_t step = (int64_t)gridDim.x * me.rt;
   int64_t row = (int64_t)blockIdx.x * me.rt + me.rl;
@@ -367,8 +371,8 @@ __global__ __launch_bounds__(G::TB) void k_layer_norm_bwd(typename SourceOf<T, S
     const bool on = me.live && r < rows;
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
-      to.x[j].load(src, r, c0 + me.at(j), on ? left[j] : 0);
-      to.g[j].load(dy + r * ldy + c0 + me.at(j), on ? left[j] : 0);
+      to.x[j].load(src, r, c0 + me.template at<N>(j), on ? left[j] : 0);
+      to.g[j].load(dy + r * ldy + c0 + me.template at<N>(j), on ? left[j] : 0);
     }
     to.mean = on ? stats[2 * (r * groups + me.g)] : 0.0f;
     to.rstd = on ? stats[2 * (r * groups + me.g) + 1] : 0.0f;
@@ -386,13 +390,13 @@ __global__ __launch_bounds__(G::TB) void k_layer_norm_bwd(typename SourceOf<T, S
       fetch(row, cur);
     }
     const float mean = cur.mean, rstd = cur.rstd;
-    float s1 = 0.0f, s2 = 0.0f, h[kVec], g[kVec];
+    float s1 = 0.0f, s2 = 0.0f, h[N], g[N];
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
       cur.x[j].get(h);
       cur.g[j].get(g);
 #pragma unroll
-      for (int i = 0; i < kVec; ++i) {
+      for (int i = 0; i < N; ++i) {
         h[i] = (h[i] - mean) * rstd;
         aw[j][i] += g[i] * h[i];
         ab[j][i] += g[i];
@@ -426,9 +430,9 @@ __global__ __launch_bounds__(G::TB) void k_layer_norm_bwd(typename SourceOf<T, S
           cur.x[j].get(h);
           cur.g[j].get(g);
 #pragma unroll
-          for (int i = 0; i < kVec; ++i) g[i] = rstd * (g[i] * w[j][i] - m1 - (h[i] - mean) * rstd * m2);
-          if (left[j] == kVec) store_vec(out + me.at(j), g);
-          else if (left[j]) store_some(out + me.at(j), left[j], g);
+          for (int i = 0; i < N; ++i) g[i] = rstd * (g[i] * w[j][i] - m1 - (h[i] - mean) * rstd * m2);
+          if (left[j] == N) store_vec(out + me.template at<N>(j), g);
+          else if (left[j]) store_some(out + me.template at<N>(j), left[j], g);
         }
       }
     }
@@ -444,9 +448,9 @@ __global__ __launch_bounds__(G::TB) void k_layer_norm_bwd(typename SourceOf<T, S
 #pragma unroll
         for (int j = 0; j < NV; ++j)
 #pragma unroll
-          for (int i = 0; i < kVec; ++i) {
-            sums[(j * kVec + i) * (G::TB / 2) + (me.rl - half) * cols + col] = aw[j][i];
-            sums[((NV + j) * kVec + i) * (G::TB / 2) + (me.rl - half) * cols + col] = ab[j][i];
+          for (int i = 0; i < N; ++i) {
+            sums[(j * N + i) * (G::TB / 2) + (me.rl - half) * cols + col] = aw[j][i];
+            sums[((NV + j) * N + i) * (G::TB / 2) + (me.rl - half) * cols + col] = ab[j][i];
           }
       }
       __syncthreads();
@@ -454,9 +458,9 @@ __global__ __launch_bounds__(G::TB) void k_layer_norm_bwd(typename SourceOf<T, S
 #pragma unroll
         for (int j = 0; j < NV; ++j)
 #pragma unroll
-          for (int i = 0; i < kVec; ++i) {
-            aw[j][i] += sums[(j * kVec + i) * (G::TB / 2) + me.rl * cols + col];
-            ab[j][i] += sums[((NV + j) * kVec + i) * (G::TB / 2) + me.rl * cols + col];
+          for (int i = 0; i < N; ++i) {
+            aw[j][i] += sums[(j * N + i) * (G::TB / 2) + me.rl * cols + col];
+            ab[j][i] += sums[((NV + j) * N + i) * (G::TB / 2) + me.rl * cols + col];
           }
       }
       __syncthreads();
@@ -466,19 +470,24 @@ __global__ __launch_bounds__(G::TB) void k_layer_norm_bwd(typename SourceOf<T, S
   if (!me.live || me.rl) return;
 #pragma unroll
   for (int j = 0; j < NV; ++j) {
-    const int64_t c = c0 + me.at(j);
+    const int64_t c = c0 + me.template at<N>(j);
     if (gridDim.x > 1) {
       float* to = part + 2 * (int64_t)blockIdx.x * width + c;
-      if (left[j] == kVec) {
-        store_vec(to, aw[j]);
-        store_vec(to + width, ab[j]);
+      if (left[j] == N) {
+#pragma unroll
+        for (int i = 0; i < N; i += 4) {
+          *reinterpret_cast<u32x4_a4*>(to + i) =
+              u32x4_t{f2u(aw[j][i]), f2u(aw[j][i + 1]), f2u(aw[j][i + 2]), f2u(aw[j][i + 3])};
+          *reinterpret_cast<u32x4_a4*>(to + width + i) =
+              u32x4_t{f2u(ab[j][i]), f2u(ab[j][i + 1]), f2u(ab[j][i + 2]), f2u(ab[j][i + 3])};
+        }
       } else {
         store_some(to, left[j], aw[j]);
         store_some(to + width, left[j], ab[j]);
       }
     } else {
 #pragma unroll
-      for (int i = 0; i < kVec; ++i)
+      for (int i = 0; i < N; ++i)
         if (i < left[j]) {
           if (dw) store_param(dw, dw16, c + i, aw[j][i]);
           if (db) store_param(db, db16, c + i, ab[j][i]);
@@ -587,33 +596,33 @@ constexpr int kFwdThreads = 256, kFwdAhead = 1, kBwdThreads = 1024, kBwdAhead = 
 constexpr int64_t kFwdBlocks = 2048, kBwdBlocks = 256;
 
 // Call f(Shape) with the smallest team that holds a segment of D elements: in the
-// forward pass with two vectors a thread where a wave is full, in the backward
-// pass, where a vector takes 40 registers more for its sums, with one.
-template <typename F>
+// forward pass of 16 elements a thread where a wave is full, in the backward pass,
+// where an element takes five registers more for its sums and weight, of 8.
+template <typename T, typename F>
 auto with_fwd_shape(int64_t D, F f) {
-  constexpr int TB = kFwdThreads;
-  if (D <= 64) return f(Shape<8, 1, TB>());
-  if (D <= 128) return f(Shape<16, 1, TB>());
-  if (D <= 256) return f(Shape<32, 1, TB>());
-  if (D <= 512) return f(Shape<64, 1, TB>());
-  if (D <= 1024) return f(Shape<64, 2, TB>());
-  if (D <= 2048) return f(Shape<128, 2, TB>());
-  if (D <= 4096) return f(Shape<256, 2, TB>());
-  if (D <= 8192) return f(Shape<512, 2, 512>());
-  return f(Shape<1024, 2, 1024>());
+  constexpr int TB = kFwdThreads, V = 8 / kN<T>;      // vectors of 8 elements
+  if (D <= 64) return f(Shape<8, V, TB>());
+  if (D <= 128) return f(Shape<16, V, TB>());
+  if (D <= 256) return f(Shape<32, V, TB>());
+  if (D <= 512) return f(Shape<64, V, TB>());
+  if (D <= 1024) return f(Shape<64, 2 * V, TB>());
+  if (D <= 2048) return f(Shape<128, 2 * V, TB>());
+  if (D <= 4096) return f(Shape<256, 2 * V, TB>());
+  if (D <= 8192) return f(Shape<512, 2 * V, 512>());
+  return f(Shape<1024, 2 * V, 1024>());
 }
-template <typename F>
+template <typename T, typename F>
 auto with_bwd_shape(int64_t D, F f) {
-  constexpr int TB = kBwdThreads;
-  if (D <= 64) return f(Shape<8, 1, TB>());
-  if (D <= 128) return f(Shape<16, 1, TB>());
-  if (D <= 256) return f(Shape<32, 1, TB>());
-  if (D <= 512) return f(Shape<64, 1, TB>());
-  if (D <= 1024) return f(Shape<128, 1, TB>());
-  if (D <= 2048) return f(Shape<256, 1, TB>());
-  if (D <= 4096) return f(Shape<512, 1, TB>());
-  if (D <= 8192) return f(Shape<1024, 1, TB>());
-  return f(Shape<1024, 2, TB>());
+  constexpr int TB = kBwdThreads, V = 8 / kN<T>;
+  if (D <= 64) return f(Shape<8, V, TB>());
+  if (D <= 128) return f(Shape<16, V, TB>());
+  if (D <= 256) return f(Shape<32, V, TB>());
+  if (D <= 512) return f(Shape<64, V, TB>());
+  if (D <= 1024) return f(Shape<128, V, TB>());
+  if (D <= 2048) return f(Shape<256, V, TB>());
+  if (D <= 4096) return f(Shape<512, V, TB>());
+  if (D <= 8192) return f(Shape<1024, V, TB>());
+  return f(Shape<1024, 2 * V, TB>());
 }
 
 // Workgroups along the rows and along the segments of a row.
@@ -625,7 +634,7 @@ dim3 grid_of(int64_t rows, int64_t groups, int64_t most) {
 }
 
 dim3 bwd_grid(int64_t rows, int64_t width, int64_t groups) {
-  return with_bwd_shape(width / groups, [&](auto shape) {
+  return with_bwd_shape<float>(width / groups, [&](auto shape) {      // the teams are the same for both types
     return grid_of<decltype(shape)>(rows, groups, kBwdBlocks);
   });
 }
@@ -641,7 +650,7 @@ void launch_fwd(G, const T* x, int64_t ldx, const Affine& p, int64_t rows, int64
   else if (blk == 16) PRATCHYA_LN(16);
   else if (blk == 32) PRATCHYA_LN(32);
   else if (blk == 64) { if constexpr (G::P >= 32) PRATCHYA_LN(64); }
-  else { if constexpr (G::P >= 64 && G::NV >= 2) PRATCHYA_LN(128); }
+  else { if constexpr (G::P >= 64 && G::NV * kN<T> >= 16) PRATCHYA_LN(128); }
 #undef PRATCHYA_LN
 }
 
@@ -654,7 +663,7 @@ int layer_norm(const void* x, int64_t ldx, const Affine& p, int64_t rows, int64_
     hipLaunchKernelGGL((k_layer_norm_long<T>), dim3((unsigned)(rows * groups)), dim3(256), 0, stream, xt, ldx, p, width,
                        groups, eps, yt, stats);
   else
-    with_fwd_shape(width / groups, [&](auto shape) {
+    with_fwd_shape<T>(width / groups, [&](auto shape) {
       launch_fwd<T>(shape, xt, ldx, p, rows, width, groups, eps, yt, stats, x8, sc8, sc32, blk, stream);
     });
   return check_launch("layer_norm");
@@ -679,10 +688,10 @@ int layer_norm_bwd(typename SourceOf<T, STORED>::type src, const void* dy, int64
                          dim3(256), 0, stream, src, g, ldy, rows, width, groups, stats, part);
     }
   } else {
-    with_bwd_shape(width / groups, [&](auto shape) {
+    with_bwd_shape<T>(width / groups, [&](auto shape) {
       typedef decltype(shape) G;
-      // two vectors a thread leave none of the 128 registers for a row ahead
-      constexpr int AHEAD = G::NV == 1 ? kBwdAhead : 0;
+      // 16 elements a thread leave none of the 128 registers for a row ahead
+      constexpr int AHEAD = G::NV * kN<T> == 8 ? kBwdAhead : 0;
       const dim3 grid = grid_of<G>(rows, groups, kBwdBlocks);
       slices = (int)grid.x;
       hipLaunchKernelGGL((k_layer_norm_bwd<T, G, STORED, AHEAD>), grid, dim3(G::TB), 0, stream, src, g, ldy, p, rows,
@@ -740,7 +749,7 @@ extern "C" int pratchya_layer_norm_bwd(const void* x, int64_t ldx, int x_dtype, 
   if (!is_float_dtype(dtype) || (!stored && x_dtype != dtype) || (w && !is_float_dtype(w_dtype)) ||
       (dw && !is_float_dtype(dw_dtype)) || (db && !is_float_dtype(db_dtype)))
     return pratchya_set_error(PRATCHYA_EINVAL, "layer_norm_bwd: unsupported dtypes (x %d, dy %d)", x_dtype, dtype);
-  if (stored && (blk < kVec || !power_of_two(blk) || width % blk))
+  if (stored && (blk < 8 || !power_of_two(blk) || width % blk))
     return pratchya_set_error(PRATCHYA_EINVAL, "layer_norm_bwd: blocks of %lld for rows of %lld", (long long)blk,
                               (long long)width);
   if (stored && reinterpret_cast<uintptr_t>(x) % 8)

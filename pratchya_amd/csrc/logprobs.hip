@@ -65,13 +65,16 @@ struct Running {
     s *= f;
     m = to;
   }
-  __device__ __forceinline__ void add(const float (&v)[kVec]) {
-    const float c = fmaxf(fmaxf(fmaxf(v[0], v[1]), fmaxf(v[2], v[3])), fmaxf(fmaxf(v[4], v[5]), fmaxf(v[6], v[7])));
+  template <int N>
+  __device__ __forceinline__ void add(const float (&v)[N]) {
+    float c = v[0];
+#pragma unroll
+    for (int i = 1; i < N; ++i) c = fmaxf(c, v[i]);
     if (__any(c > m + kSlack)) {
       if (c > m) move(c);
     }
 #pragma unroll
-    for (int i = 0; i < kVec; ++i) {
+    for (int i = 0; i < N; ++i) {
       const float d = (v[i] - m) * kLog2e, e = __builtin_amdgcn_exp2f(d);
       s += e;
       if constexpr (ENTROPY) t += e * fmaxf(d, kLowest);   // 0, not NaN, for a masked logit
@@ -131,7 +134,12 @@ __device__ __forceinline__ void store_row(float x_token, int64_t tok, int64_t vo
   }
 }
 
-constexpr int kUnroll = 4;        // vectors of one thread in flight
+// Vectors of one thread in flight: 32 elements, in the backward pass 16 (1000 x
+// 8193 f32 15.5 -> 11.3 us, 8192 x 65536 bf16 356 -> 347 us against 32).
+template <typename T>
+constexpr int kUnroll = 32 / kN<T>;
+template <typename T>
+constexpr int kBwdUnroll = 16 / kN<T>;
 
 // One row per WPR waves, 4 / WPR rows (at least one) per workgroup.
 template <typename T, int WPR, bool ENTROPY, bool NT>
@@ -144,28 +152,29 @@ __global__ __launch_bounds__(WPR < 4 ? 256 : WPR * 64) void k_logprobs(
   const int64_t row = (int64_t)blockIdx.x * ROWS + threadIdx.x / THREADS;
   if (ROWS > 1 && row >= rows) return;      // whole waves; a row of one wave meets no barrier
   const T* xr = x + row * ld;
-  const int64_t vecs = vocab / kVec;
+  constexpr int N = kN<T>, U = kUnroll<T>;
+  const int64_t vecs = vocab / N;
   Running<ENTROPY> r;
   int64_t i = tid;
-  for (; i + (kUnroll - 1) * THREADS < vecs; i += kUnroll * THREADS) {
-    typename RawOf<T>::type raw[kUnroll];
+  for (; i + (U - 1) * THREADS < vecs; i += U * THREADS) {
+    u32x4_t raw[U];
 #pragma unroll
-    for (int u = 0; u < kUnroll; ++u) raw[u] = load_raw<NT>(xr + (i + u * THREADS) * kVec);
+    for (int u = 0; u < U; ++u) raw[u] = load_raw<NT>(xr + (i + u * THREADS) * N);
 #pragma unroll
-    for (int u = 0; u < kUnroll; ++u) {
-      float v[kVec];
+    for (int u = 0; u < U; ++u) {
+      float v[N];
       widen(raw[u], v);
       r.add(v);
     }
   }
   for (; i < vecs; i += THREADS) {
-    float v[kVec];
-    widen(load_raw(xr + i * kVec), v);
+    float v[N];
+    widen(load_raw(xr + i * N), v);
     r.add(v);
   }
-  if (i == vecs && vocab % kVec) {
-    float v[kVec];
-    load_some(xr + vecs * kVec, vocab - vecs * kVec, -__builtin_inff(), v);
+  if (i == vecs && vocab % N) {
+    float v[N];
+    load_some(xr + vecs * N, vocab - vecs * N, -__builtin_inff(), v);
     r.add(v);
   }
   join_running<WPR>(r, lds);
@@ -182,8 +191,8 @@ __global__ __launch_bounds__(WPR < 4 ? 256 : WPR * 64) void k_logprobs(
 // that would be more than kParts), a workgroup each, because one compute unit
 // alone would take longer over a row than all parts and the join together; a part
 // stays in registers, so its logits are read once for the sums and the selection.
-constexpr int kPartThreads = 256, kPartVecs = 2, kBlock = kPartThreads * kPartVecs * kVec, kParts = 64;
-constexpr int kKeys = kPartVecs * kVec + 1;             // keys of a thread: a block's logits and one kept key
+constexpr int kPartThreads = 256, kPartElems = 16, kBlock = kPartThreads * kPartElems, kParts = 64;
+constexpr int kKeys = kPartElems + 1;                   // keys of a thread: a block's logits and one kept key
 
 // LDS of a selection among up to kKeys keys per thread.  kCandidates is what
 // leaves room for eight workgroups in a compute unit (with room for every key, four
@@ -201,8 +210,8 @@ struct Selection {
 // out[0 .. top), padded with 0, for the whole workgroup.  The top-th largest of
 // the maxima of 64 or 128 groups (threads of equal lane, and parity of the wave)
 // is a bound that `top` keys reach, if there are so many; the keys that do are
-// ranked by counting: some 24 for 20 alternatives, 90 for 64.  A lane's keys lie 8
-// logits apart from its neighbours', so rows of equal logits leave some 8 top
+// ranked by counting: some 24 for 20 alternatives, 90 for 64.  A lane's keys lie a
+// vector apart from its neighbours', so rows of equal logits leave up to 8 top
 // candidates, as rising or falling ones do.  Where there are more than
 // kCandidates, the largest key is taken `top` times.  out may hold keys of this
 // selection: they are in registers.
@@ -319,24 +328,25 @@ __global__ __launch_bounds__(kPartThreads) void k_logprobs_part(const T* __restr
   Running<ENTROPY> r;
   if (tid < kMaxTop) list[tid] = 0;
   __syncthreads();
+  constexpr int N = kN<T>, VECS = kPartElems / N;
   for (int64_t base = from; base < to; base += kBlock) {
-    float v[kPartVecs][kVec];
+    float v[VECS][N];
 #pragma unroll
-    for (int u = 0; u < kPartVecs; ++u) {
-      const int64_t at = base + (u * kPartThreads + tid) * kVec;
-      if (at + kVec <= to) widen(load_raw(xr + at), v[u]);
+    for (int u = 0; u < VECS; ++u) {
+      const int64_t at = base + (u * kPartThreads + tid) * N;
+      if (at + N <= to) widen(load_raw(xr + at), v[u]);
       else load_some(xr + at, to - at, -__builtin_inff(), v[u]);
     }
 #pragma unroll
-    for (int u = 0; u < kPartVecs; ++u)
-      if (base + (u * kPartThreads + tid) * kVec < to) r.add(v[u]);
+    for (int u = 0; u < VECS; ++u)
+      if (base + (u * kPartThreads + tid) * N < to) r.add(v[u]);
     uint64_t keys[kKeys];
 #pragma unroll
-    for (int u = 0; u < kPartVecs; ++u)
+    for (int u = 0; u < VECS; ++u)
 #pragma unroll
-      for (int j = 0; j < kVec; ++j) {
-        const int64_t i = base + (u * kPartThreads + tid) * kVec + j;
-        keys[u * kVec + j] = i < to ? rank_key(v[u][j], i) : 0;
+      for (int j = 0; j < N; ++j) {
+        const int64_t i = base + (u * kPartThreads + tid) * N + j;
+        keys[u * N + j] = i < to ? rank_key(v[u][j], i) : 0;
       }
     keys[kKeys - 1] = tid < top ? list[tid] : 0;
     select_top(keys, top, sel, list);
@@ -404,7 +414,7 @@ __global__ __launch_bounds__(kPartThreads) void k_logprobs_join(const T* __restr
   }
 }
 
-// dx of kVec * kUnroll * TPR logits of a row per TPR threads: elementwise, one
+// dx of 16 TPR logits of a row per TPR threads: elementwise, one
 // read and one write of each logit.
 template <typename T, int TPR, bool NT>
 __global__ __launch_bounds__(256) void k_logprobs_bwd(const T* __restrict__ x, int64_t ld,
@@ -412,46 +422,53 @@ __global__ __launch_bounds__(256) void k_logprobs_bwd(const T* __restrict__ x, i
                                                       const float* __restrict__ stats, const float* __restrict__ g,
                                                       const float* __restrict__ gh, int64_t rows, int64_t vocab,
                                                       unsigned pieces, T* __restrict__ dx) {
+  constexpr int N = kN<T>, U = kBwdUnroll<T>;
   const int tid = threadIdx.x % TPR;
   // several rows per workgroup are rows of one piece
   const int64_t row = TPR < 256 ? (int64_t)blockIdx.x * (256 / TPR) + threadIdx.x / TPR : blockIdx.x / pieces;
-  const int64_t first = TPR < 256 ? tid : (int64_t)(blockIdx.x - (unsigned)row * pieces) * (TPR * kUnroll) + tid;
+  const int64_t first = TPR < 256 ? tid : (int64_t)(blockIdx.x - (unsigned)row * pieces) * (TPR * U) + tid;
   if (row >= rows) return;
   const int64_t tok = tokens[row];
   const float m = stats[3 * row], logs = stats[3 * row + 1];
   const float c = g && tok >= 0 ? g[row] : 0.0f, ch = gh ? gh[row] : 0.0f, H = stats[3 * row + 2];
   const T* xr = x + row * ld;
   T* dr = dx + row * vocab;
-  auto grad = [&](float (&v)[kVec], int64_t at) {
+  auto grad = [&](float (&v)[N], int64_t at) {
 #pragma unroll
-    for (int i = 0; i < kVec; ++i) {
+    for (int i = 0; i < N; ++i) {
       const float lp = (v[i] - m) - logs, p = __builtin_amdgcn_exp2f(lp * kLog2e);
       v[i] = -p * (c + ch * (fmaxf(lp, -1000.0f) + H));   // a masked logit: p = 0 times a finite number
     }
-    if ((uint64_t)(tok - at) < (uint64_t)kVec) {
+    if ((uint64_t)(tok - at) < (uint64_t)N) {
 #pragma unroll
-      for (int i = 0; i < kVec; ++i)
+      for (int i = 0; i < N; ++i)
         if (at + i == tok) v[i] += c;
     }
   };
-  typename RawOf<T>::type raw[kUnroll];
-  const int64_t vecs = vocab / kVec;
+  // whole pieces without a test per vector: its branches between the loads took
+  // 1000 x 50021 f32 from 82 to 122 us
+  if ((first - tid + TPR * U) * N <= vocab) {
+    u32x4_t raw[U];
 #pragma unroll
-  for (int u = 0; u < kUnroll; ++u)
-    if (first + u * TPR < vecs) raw[u] = load_raw<NT>(xr + (first + u * TPR) * kVec);
+    for (int u = 0; u < U; ++u) raw[u] = load_raw<NT>(xr + (first + u * TPR) * N);
 #pragma unroll
-  for (int u = 0; u < kUnroll; ++u) {
-    const int64_t i = first + u * TPR;
-    float v[kVec];
-    if (i < vecs) {
+    for (int u = 0; u < U; ++u) {
+      float v[N];
       widen(raw[u], v);
-      grad(v, i * kVec);
-      store_vec<NT>(dr + i * kVec, v);
-    } else if (i == vecs && vocab % kVec) {
-      load_some(xr + i * kVec, vocab - i * kVec, 0.0f, v);
-      grad(v, i * kVec);
-      store_some(dr + i * kVec, vocab - i * kVec, v);
+      grad(v, (first + u * TPR) * N);
+      store_vec<NT>(dr + (first + u * TPR) * N, v);
     }
+    return;
+  }
+  for (int u = 0; u < U; ++u) {
+    const int64_t at = (first + u * TPR) * N, left = vocab - at;
+    if (left <= 0) break;
+    float v[N];
+    if (left >= N) widen(load_raw(xr + at), v);
+    else load_some(xr + at, left, 0.0f, v);
+    grad(v, at);
+    if (left >= N) store_vec(dr + at, v);
+    else store_some(dr + at, left, v);
   }
 }
 
@@ -515,8 +532,9 @@ int launch(const void* logits, int64_t ld, const int64_t* tokens, int64_t rows, 
 template <typename T>
 int launch_bwd(const void* logits, int64_t ld, const int64_t* tokens, const float* stats, const float* g,
                const float* gh, int64_t rows, int64_t vocab, void* dx, hipStream_t stream) {
-  const int tpr = vocab <= 64 * kVec * kUnroll ? 64 : 256;
-  const int64_t pieces = (vocab + (int64_t)tpr * kVec * kUnroll - 1) / ((int64_t)tpr * kVec * kUnroll);
+  constexpr int64_t per = kN<T> * kBwdUnroll<T>;          // logits of a thread
+  const int tpr = vocab <= 64 * per ? 64 : 256;
+  const int64_t pieces = (vocab + tpr * per - 1) / (tpr * per);
   const int64_t blocks = (rows * pieces + 256 / tpr - 1) / (256 / tpr);
   if (blocks > 0x7FFFFFFF)
     return pratchya_set_error(PRATCHYA_EUNSUPPORTED, "token_logprobs_bwd: more than 2^31 workgroups");

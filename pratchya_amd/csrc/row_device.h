@@ -21,79 +21,58 @@ __device__ __forceinline__ void store_param(void* p, bool bf16, int64_t i, float
   else static_cast<float*>(p)[i] = v;
 }
 
-// Eight consecutive elements as f32, and back.  The addresses are aligned for one
-// element only (rows of odd widths, slices): the vector types say so, and the
-// hardware takes 16-byte accesses at any element's address.
+// A vector is 16 bytes of a row: kN<T> = 8 bf16 or 4 f32 elements, so neighbouring
+// lanes load and store neighbouring pieces in both types (f32 rows in vectors of
+// 32 bytes took 417 us where these take 391, 2 GB of logits and their gradient).
+// Addresses are aligned for one element only (rows of odd widths, slices): the
+// vector types say so, and the hardware takes 16-byte accesses at any element's
+// address.
+template <typename T>
+constexpr int kN = 16 / (int)sizeof(T);
 typedef uint32_t u32x4_a2 __attribute__((ext_vector_type(4), aligned(2)));
 typedef uint32_t u32x4_a4 __attribute__((ext_vector_type(4), aligned(4)));
-constexpr int kVec = 8;
+template <typename T> struct Unaligned { typedef u32x4_a2 type; };
+template <> struct Unaligned<float> { typedef u32x4_a4 type; };
 
-struct Raw16 {
-  u32x4_t v;
-};
-struct Raw32 {
-  u32x4_t lo, hi;
-};
-template <typename T> struct RawOf;
-template <> struct RawOf<uint16_t> { typedef Raw16 type; };
-template <> struct RawOf<float> { typedef Raw32 type; };
-
-template <bool NT = false>
-__device__ __forceinline__ Raw16 load_raw(const uint16_t* p) {
-  const u32x4_a2* q = reinterpret_cast<const u32x4_a2*>(p);
-  if constexpr (NT) return {__builtin_nontemporal_load(q)};
-  else return {*q};
+template <bool NT = false, typename T>
+__device__ __forceinline__ u32x4_t load_raw(const T* p) {
+  const auto* q = reinterpret_cast<const typename Unaligned<T>::type*>(p);
+  if constexpr (NT) return __builtin_nontemporal_load(q);
+  else return *q;
 }
-template <bool NT = false>
-__device__ __forceinline__ Raw32 load_raw(const float* p) {
-  const u32x4_a4* q = reinterpret_cast<const u32x4_a4*>(p);
-  if constexpr (NT) return {__builtin_nontemporal_load(q), __builtin_nontemporal_load(q + 1)};
-  else return {q[0], q[1]};
-}
-__device__ __forceinline__ void widen(const Raw16& r, float (&v)[kVec]) {
+__device__ __forceinline__ void widen(const u32x4_t& r, float (&v)[8]) {
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    v[2 * i] = u2f(r.v[i] << 16);
-    v[2 * i + 1] = u2f(r.v[i] & 0xFFFF0000u);
+    v[2 * i] = u2f(r[i] << 16);
+    v[2 * i + 1] = u2f(r[i] & 0xFFFF0000u);
   }
 }
-__device__ __forceinline__ void widen(const Raw32& r, float (&v)[kVec]) {
+__device__ __forceinline__ void widen(const u32x4_t& r, float (&v)[4]) {
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    v[i] = u2f(r.lo[i]);
-    v[4 + i] = u2f(r.hi[i]);
-  }
+  for (int i = 0; i < 4; ++i) v[i] = u2f(r[i]);
 }
-template <bool NT = false>
-__device__ __forceinline__ void store_vec(uint16_t* p, const float (&v)[kVec]) {
-  const u32x4_t w = {pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]), pack_bf16x2(v[4], v[5]),
-                     pack_bf16x2(v[6], v[7])};
-  u32x4_a2* q = reinterpret_cast<u32x4_a2*>(p);
-  if constexpr (NT) __builtin_nontemporal_store(w, q);
-  else *q = w;
+__device__ __forceinline__ u32x4_t narrow(const float (&v)[8]) {
+  return u32x4_t{pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]), pack_bf16x2(v[4], v[5]), pack_bf16x2(v[6], v[7])};
 }
-template <bool NT = false>
-__device__ __forceinline__ void store_vec(float* p, const float (&v)[kVec]) {
-  const u32x4_t a = {f2u(v[0]), f2u(v[1]), f2u(v[2]), f2u(v[3])}, b = {f2u(v[4]), f2u(v[5]), f2u(v[6]), f2u(v[7])};
-  u32x4_a4* q = reinterpret_cast<u32x4_a4*>(p);
-  if constexpr (NT) {
-    __builtin_nontemporal_store(a, q);
-    __builtin_nontemporal_store(b, q + 1);
-  } else {
-    q[0] = a;
-    q[1] = b;
-  }
+__device__ __forceinline__ u32x4_t narrow(const float (&v)[4]) {
+  return u32x4_t{f2u(v[0]), f2u(v[1]), f2u(v[2]), f2u(v[3])};
 }
-// The first n (0 to 8) of eight elements; the others read as `fill`.
-template <typename T>
-__device__ __forceinline__ void load_some(const T* p, int64_t n, float fill, float (&v)[kVec]) {
+template <bool NT = false, typename T>
+__device__ __forceinline__ void store_vec(T* p, const float (&v)[kN<T>]) {
+  auto* q = reinterpret_cast<typename Unaligned<T>::type*>(p);
+  if constexpr (NT) __builtin_nontemporal_store(narrow(v), q);
+  else *q = narrow(v);
+}
+// The first n of a vector's elements; the others read as `fill`.
+template <typename T, int N>
+__device__ __forceinline__ void load_some(const T* p, int64_t n, float fill, float (&v)[N]) {
 #pragma unroll
-  for (int i = 0; i < kVec; ++i) v[i] = i < n ? load_elem(p + i) : fill;
+  for (int i = 0; i < N; ++i) v[i] = i < n ? load_elem(p + i) : fill;
 }
-template <typename T>
-__device__ __forceinline__ void store_some(T* p, int64_t n, const float (&v)[kVec]) {
+template <typename T, int N>
+__device__ __forceinline__ void store_some(T* p, int64_t n, const float (&v)[N]) {
 #pragma unroll
-  for (int i = 0; i < kVec; ++i)
+  for (int i = 0; i < N; ++i)
     if (i < n) store_elem(p + i, v[i]);
 }
 
@@ -153,47 +132,65 @@ __device__ __forceinline__ float block_add(float v, float* lds) {
 }
 
 // --------------------------------------------------------------------------
-// The 8-bit form of a row's values, eight consecutive ones per lane: blocks of
-// BLK elements are BLK / 8 neighbouring lanes, groups of BLK / 16 blocks (one
-// for 16) up to 32 lanes, or for BLK 128 the wave's 64 lanes of two vectors.
+// The 8-bit form of a row's values, a vector of N per lane: blocks of BLK
+// elements are BLK / N neighbouring lanes, groups of blocks more of them or the
+// same lanes of several vectors.
 // --------------------------------------------------------------------------
-__device__ __forceinline__ uint32_t absmax8(const float (&v)[kVec]) {
+template <int N>
+__device__ __forceinline__ uint32_t absmax(const float (&v)[N]) {
   uint32_t m = 0;
 #pragma unroll
-  for (int i = 0; i < kVec; ++i) m = umax(m, abs_bits(v[i]));
+  for (int i = 0; i < N; ++i) m = umax(m, abs_bits(v[i]));
   return m;
 }
 
-// The payload of eight values of a block with maximum mb in a group with
-// maximum Gb (f32 bits), and the block's e8m0 byte: quantize_impl's (fp8_math.h),
-// by the division-free cast of block_scale; values near a bf16 rounding
-// midpoint, and clamped blocks and groups that are not finite, by the exact
-// composition.
-__device__ __forceinline__ u32x2_t store_form(const float (&v)[kVec], uint32_t mb, uint32_t Gb, uint32_t& e) {
+// N payload bytes.
+template <int N> struct Payload;
+template <> struct Payload<8> { typedef u32x2_t type; };
+template <> struct Payload<4> { typedef uint32_t type; };
+__device__ __forceinline__ u32x2_t payload_of(uint32_t a, uint32_t b, u32x2_t) { return u32x2_t{a, b}; }
+__device__ __forceinline__ uint32_t payload_of(uint32_t a, uint32_t, uint32_t) { return a; }
+
+// The payload of a vector of a block with maximum mb in a group with maximum Gb
+// (f32 bits), and the block's e8m0 byte: quantize_impl's (fp8_math.h), by the
+// division-free cast of block_scale; values near a bf16 rounding midpoint, and
+// clamped blocks and groups that are not finite, by the exact composition.
+template <int N>
+__device__ __forceinline__ typename Payload<N>::type store_form(const float (&v)[N], uint32_t mb, uint32_t Gb,
+                                                                uint32_t& e) {
   const float G = u2f(Gb);
   const BlockScale b = block_scale(mb, Gb, __builtin_amdgcn_rcpf(G * 0.0078125f));
   e = b.e;
   bool fast = is_finite_f(G) && !b.clamped;
-  u32x2_t w = {0, 0};
+  uint32_t w[2] = {0, 0};
   if (fast) {
-    float t[kVec];
+    uint32_t mid = 0xFFFFFFFFu;
 #pragma unroll
-    for (int i = 0; i < kVec; ++i) t[i] = v[i] * b.y;
-    w = {cvt4_hw(t[0], t[1], t[2], t[3]), cvt4_hw(t[4], t[5], t[6], t[7])};
-    fast = umin(mid_key4(t[0], t[1], t[2], t[3]), mid_key4(t[4], t[5], t[6], t[7])) > kMidKey;
+    for (int i = 0; i < N; i += 4) {
+      const float t0 = v[i] * b.y, t1 = v[i + 1] * b.y, t2 = v[i + 2] * b.y, t3 = v[i + 3] * b.y;
+      w[i / 4] = cvt4_hw(t0, t1, t2, t3);
+      mid = umin(mid, mid_key4(t0, t1, t2, t3));
+    }
+    fast = mid > kMidKey;
   }
   if (!fast) {
     e = b.clamped || !is_finite_f(G) ? e8m0_of(u2f(mb), G) : b.e;
     const float S = quant_scale(e, G);
-    w = {cvt4_exact(v[0], v[1], v[2], v[3], S), cvt4_exact(v[4], v[5], v[6], v[7], S)};
+#pragma unroll
+    for (int i = 0; i < N; i += 4) w[i / 4] = cvt4_exact(v[i], v[i + 1], v[i + 2], v[i + 3], S);
   }
-  return w;
+  return payload_of(w[0], w[1], typename Payload<N>::type());
 }
 
-// What eight payload bytes of a block stand for.
-__device__ __forceinline__ void stored_values(u32x2_t w, float scale, float (&v)[kVec]) {
+// What a vector's payload bytes stand for.
+__device__ __forceinline__ void stored_values(u32x2_t w, float scale, float (&v)[8]) {
   fp8_word(w.x, v[0], v[1], v[2], v[3]);
   fp8_word(w.y, v[4], v[5], v[6], v[7]);
 #pragma unroll
-  for (int i = 0; i < kVec; ++i) v[i] = (v[i] * scale) * 0.0078125f;
+  for (int i = 0; i < 8; ++i) v[i] = (v[i] * scale) * 0.0078125f;
+}
+__device__ __forceinline__ void stored_values(uint32_t w, float scale, float (&v)[4]) {
+  fp8_word(w, v[0], v[1], v[2], v[3]);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) v[i] = (v[i] * scale) * 0.0078125f;
 }
