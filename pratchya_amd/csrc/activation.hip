@@ -158,18 +158,24 @@ __global__ __launch_bounds__(kThreads) void k_act(const T* __restrict__ x, Rows 
   constexpr int N = kN<T>, PER = kPer<T>;
   const int64_t vec = first_vec<T>();
   At at[PER];
+  u32x4_t raw[PER];
   float v[PER][N];
 #pragma unroll
   for (int u = 0; u < PER; ++u) {
     at[u] = place<N, ONE>(r, vec + u * 64);
     const T* p = x + at[u].row * r.ldx + at[u].c;
-    if (at[u].left == N) widen(load_raw<true>(p), v[u]);
-    else load_some(p, at[u].left, 0.0f, v[u]);
+    if (at[u].left == N) raw[u] = load_raw<true>(p);
+  }
+#pragma unroll
+  for (int u = 0; u < PER; ++u) {
+    if (at[u].left == N) widen(raw[u], v[u]);
+    else load_some(x + at[u].row * r.ldx + at[u].c, at[u].left, 0.0f, v[u]);
   }
   if constexpr (BLK != 0) {
     uint32_t m[PER], G[PER] = {};
 #pragma unroll
-    for (int u = 0; u < PER; ++u) m[u] = lane_group_max<BLK / N>(absmax(v[u]));
+    for (int u = 0; u < PER; ++u)
+      m[u] = lane_group_max<BLK / N>(at[u].left ? absmax<T>(raw[u]) : 0u);   // whole vectors or none
     group_max<BLK, N>(m, K, G);
 #pragma unroll
     for (int u = 0; u < PER; ++u) {
@@ -220,7 +226,7 @@ __global__ __launch_bounds__(kThreads) void k_act_bwd(const T* __restrict__ x, R
       if (at[u].left) {
         const int64_t e0 = (vec + u * 64) * N, n = e0 >> s.blk_log2;
         q[u] = __builtin_nontemporal_load(reinterpret_cast<const W*>(s.x8 + e0));
-        scale[u] = e8m0_decode(s.sc8[n]) * s.sc32[n >> s.K_log2];
+        scale[u] = stored_scale(s.sc8[n], s.sc32[n >> s.K_log2]);
       }
     } else {
       const T* px = x + at[u].row * r.ldx + at[u].c;
@@ -233,7 +239,11 @@ __global__ __launch_bounds__(kThreads) void k_act_bwd(const T* __restrict__ x, R
 #pragma unroll
   for (int u = 0; u < PER; ++u) {
     if (at[u].left == 0) continue;
-    if constexpr (STORED) stored_values(q[u], scale[u], v[u]);
+    if constexpr (STORED) {
+      payload_values(q[u], v[u]);
+#pragma unroll
+      for (int i = 0; i < N; ++i) v[u][i] *= scale[u];
+    }
     act_grad(v[u], g[u], kind);
     T* p = dx + at[u].row * r.width + at[u].c;
     if (at[u].left == N) store_vec<true>(p, g[u]);

@@ -122,6 +122,14 @@ __device__ __forceinline__ void load_params(const void* p, bool bf16, int64_t at
   }
 }
 
+// (x - mean) r.  For bf16 in one operation with shift = -mean r: the product's and
+// shift's roundings are 2^-24 of |x| r, far below bf16's step of x itself.
+template <typename T>
+__device__ __forceinline__ float normed(float x, float mean, float rstd, float shift) {
+  if constexpr (sizeof(T) == 2) return __builtin_fmaf(x, rstd, shift);
+  else return (x - mean) * rstd;
+}
+
 // y and the statistics of whole segments; with BLK, x's stored form beside them
 // (groups = 1).  Mean and squared deviations are taken within each wave, from
 // registers, and joined by counts, so a mean far from zero costs no digits.
@@ -178,10 +186,12 @@ __global__ __launch_bounds__(G::TB) void k_layer_norm(const T* __restrict__ x, i
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
       cur[j].get(v);
+      if (left[j] == N) {
 #pragma unroll
-      for (int i = 0; i < N; ++i) {
-        const float d = v[i] - mean;
-        q += i < left[j] ? d * d : 0.0f;
+        for (int i = 0; i < N; ++i) q += (v[i] - mean) * (v[i] - mean);
+      } else {
+#pragma unroll
+        for (int i = 0; i < N; ++i) q += i < left[j] ? (v[i] - mean) * (v[i] - mean) : 0.0f;
       }
     }
     q = lane_group_add<LANES>(q);
@@ -213,11 +223,12 @@ __global__ __launch_bounds__(G::TB) void k_layer_norm(const T* __restrict__ x, i
       stats[2 * (row * groups + me.g) + 1] = rstd;
     }
     T* yr = y + row * width + c0;
+    const float shift = -mean * rstd;
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
       cur[j].get(v);
 #pragma unroll
-      for (int i = 0; i < N; ++i) v[i] = (v[i] - mean) * rstd * w[j][i] + b[j][i];
+      for (int i = 0; i < N; ++i) v[i] = normed<T>(v[i], mean, rstd, shift) * w[j][i] + b[j][i];
       if (left[j] == N) store_vec<true>(yr + me.template at<N>(j), v);
       else if (left[j]) store_some(yr + me.template at<N>(j), left[j], v);
     }
@@ -227,8 +238,7 @@ __global__ __launch_bounds__(G::TB) void k_layer_norm(const T* __restrict__ x, i
       uint32_t mb[NV], Gb[NV];
 #pragma unroll
       for (int j = 0; j < NV; ++j) {
-        cur[j].get(v);
-        mb[j] = lane_group_max<LB>(absmax(v));
+        mb[j] = lane_group_max<LB>(absmax<T>(cur[j].raw));
         Gb[j] = lane_group_max<LR>(mb[j]);
       }
 #pragma unroll
@@ -312,7 +322,11 @@ template <typename T> struct HeldSource<T, false> {
   __device__ __forceinline__ void load(const Source<T>& s, int64_t row, int64_t c, int left) {
     x.load(s.x + row * s.ldx + c, left);
   }
-  __device__ __forceinline__ void get(float (&v)[kN<T>]) const { x.get(v); }
+  __device__ __forceinline__ void normed_values(float mean, float rstd, float shift, float (&v)[kN<T>]) const {
+    x.get(v);
+#pragma unroll
+    for (int i = 0; i < kN<T>; ++i) v[i] = normed<T>(v[i], mean, rstd, shift);
+  }
 };
 template <typename T> struct HeldSource<T, true> {
   typedef typename Payload<kN<T>>::type W;
@@ -330,7 +344,12 @@ template <typename T> struct HeldSource<T, true> {
       G = s.sc32[n >> s.K_log2];
     }
   }
-  __device__ __forceinline__ void get(float (&v)[kN<T>]) const { stored_values(w, e8m0_decode(e) * G, v); }
+  __device__ __forceinline__ void normed_values(float, float rstd, float shift, float (&v)[kN<T>]) const {
+    payload_values(w, v);
+    const float s = stored_scale(e, G) * rstd;
+#pragma unroll
+    for (int i = 0; i < kN<T>; ++i) v[i] = __builtin_fmaf(v[i], s, shift);
+  }
 };
 
 // dx of whole segments, and the sums of dy h and dy over the rows that a team
@@ -389,15 +408,14 @@ __global__ __launch_bounds__(G::TB) void k_layer_norm_bwd(typename SourceOf<T, S
     } else {
       fetch(row, cur);
     }
-    const float mean = cur.mean, rstd = cur.rstd;
+    const float mean = cur.mean, rstd = cur.rstd, shift = -mean * rstd;
     float s1 = 0.0f, s2 = 0.0f, h[N], g[N];
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
-      cur.x[j].get(h);
+      cur.x[j].normed_values(mean, rstd, shift, h);
       cur.g[j].get(g);
 #pragma unroll
       for (int i = 0; i < N; ++i) {
-        h[i] = (h[i] - mean) * rstd;
         aw[j][i] += g[i] * h[i];
         ab[j][i] += g[i];
         const float a = g[i] * w[j][i];
@@ -422,15 +440,15 @@ __global__ __launch_bounds__(G::TB) void k_layer_norm_bwd(typename SourceOf<T, S
           s2 += r[k][1];
         }
       }
-      const float m1 = s1 / (float)D, m2 = s2 / (float)D;
+      const float m1 = rstd * (s1 / (float)D), m2 = rstd * (s2 / (float)D);
       if (me.live && row < rows) {
         T* out = dx + row * width + c0;
 #pragma unroll
         for (int j = 0; j < NV; ++j) {
-          cur.x[j].get(h);
+          cur.x[j].normed_values(mean, rstd, shift, h);
           cur.g[j].get(g);
 #pragma unroll
-          for (int i = 0; i < N; ++i) g[i] = rstd * (g[i] * w[j][i] - m1 - (h[i] - mean) * rstd * m2);
+          for (int i = 0; i < N; ++i) g[i] = (g[i] * w[j][i]) * rstd - m1 - h[i] * m2;
           if (left[j] == N) store_vec(out + me.template at<N>(j), g);
           else if (left[j]) store_some(out + me.template at<N>(j), left[j], g);
         }

@@ -136,12 +136,10 @@ __device__ __forceinline__ float block_add(float v, float* lds) {
 // elements are BLK / N neighbouring lanes, groups of blocks more of them or the
 // same lanes of several vectors.
 // --------------------------------------------------------------------------
-template <int N>
-__device__ __forceinline__ uint32_t absmax(const float (&v)[N]) {
-  uint32_t m = 0;
-#pragma unroll
-  for (int i = 0; i < N; ++i) m = umax(m, abs_bits(v[i]));
-  return m;
+// max |x| of a vector, as f32 bits.
+template <typename T>
+__device__ __forceinline__ uint32_t absmax(const u32x4_t& r) {
+  return vec_absmax_bits<sizeof(T) == 2>(make_uint4(r[0], r[1], r[2], r[3]));
 }
 
 // N payload bytes.
@@ -154,7 +152,10 @@ __device__ __forceinline__ uint32_t payload_of(uint32_t a, uint32_t, uint32_t) {
 // The payload of a vector of a block with maximum mb in a group with maximum Gb
 // (f32 bits), and the block's e8m0 byte: quantize_impl's (fp8_math.h), by the
 // division-free cast of block_scale; values near a bf16 rounding midpoint, and
-// clamped blocks and groups that are not finite, by the exact composition.
+// clamped blocks and groups that are not finite, by the exact composition.  A
+// vector of eight is bf16, whose quotients x / S of two 8-bit significands are no
+// midpoint (9 bits) and at least 2^-17 of their size away from one: the cast's few
+// ulp do not reach it, and there is nothing to test.
 template <int N>
 __device__ __forceinline__ typename Payload<N>::type store_form(const float (&v)[N], uint32_t mb, uint32_t Gb,
                                                                 uint32_t& e) {
@@ -169,7 +170,7 @@ __device__ __forceinline__ typename Payload<N>::type store_form(const float (&v)
     for (int i = 0; i < N; i += 4) {
       const float t0 = v[i] * b.y, t1 = v[i + 1] * b.y, t2 = v[i + 2] * b.y, t3 = v[i + 3] * b.y;
       w[i / 4] = cvt4_hw(t0, t1, t2, t3);
-      mid = umin(mid, mid_key4(t0, t1, t2, t3));
+      if constexpr (N == 4) mid = umin(mid, mid_key4(t0, t1, t2, t3));
     }
     fast = mid > kMidKey;
   }
@@ -182,15 +183,11 @@ __device__ __forceinline__ typename Payload<N>::type store_form(const float (&v)
   return payload_of(w[0], w[1], typename Payload<N>::type());
 }
 
-// What a vector's payload bytes stand for.
-__device__ __forceinline__ void stored_values(u32x2_t w, float scale, float (&v)[8]) {
+// A vector's payload bytes as numbers; times its block's stored_scale they are what it stands for
+// ((q * scale) / 128 in one product: the same but for values beyond 2^118 or below 2^-110).
+__device__ __forceinline__ void payload_values(u32x2_t w, float (&v)[8]) {
   fp8_word(w.x, v[0], v[1], v[2], v[3]);
   fp8_word(w.y, v[4], v[5], v[6], v[7]);
-#pragma unroll
-  for (int i = 0; i < 8; ++i) v[i] = (v[i] * scale) * 0.0078125f;
 }
-__device__ __forceinline__ void stored_values(uint32_t w, float scale, float (&v)[4]) {
-  fp8_word(w, v[0], v[1], v[2], v[3]);
-#pragma unroll
-  for (int i = 0; i < 4; ++i) v[i] = (v[i] * scale) * 0.0078125f;
-}
+__device__ __forceinline__ void payload_values(uint32_t w, float (&v)[4]) { fp8_word(w, v[0], v[1], v[2], v[3]); }
+__device__ __forceinline__ float stored_scale(uint32_t e, float G) { return (e8m0_decode(e) * G) * 0.0078125f; }
