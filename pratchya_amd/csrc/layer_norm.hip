@@ -58,6 +58,8 @@ struct Shape {
   static constexpr int LANES = P_ < 64 ? P_ : 64;
 };
 
+// A thread's place.  What all lanes of a wave share (all but the lane's offset,
+// where a team has whole waves) is made a scalar, and with it rows' addresses.
 template <typename G>
 struct Place {
   int t, team;         // thread in its team, team in the workgroup
@@ -67,17 +69,24 @@ struct Place {
   __device__ __forceinline__ Place(int64_t groups) {
     t = threadIdx.x % G::P;
     team = threadIdx.x / G::P;
+    if constexpr (G::P >= 64) team = __builtin_amdgcn_readfirstlane(team);
     const int gt = groups < G::TEAMS ? (int)groups : G::TEAMS;
     rt = G::TEAMS / gt;
     rl = team / gt;
     g = (int64_t)blockIdx.y * gt + team % gt;
     live = rl < rt && g < groups;
   }
-  // first element of this thread's vector j, of N elements, in its segment
+  // first element of vector j, of N elements, in the segment: the wave's, and the lane's offset to it
   template <int N>
-  __device__ __forceinline__ int64_t at(int j) const {
-    return (int64_t)((t / G::LANES * G::NV + j) * G::LANES + t % G::LANES) * N;
+  __device__ __forceinline__ int64_t wave_at(int j) const {
+    int wave = t / G::LANES;
+    if constexpr (G::P >= 64) wave = __builtin_amdgcn_readfirstlane(wave);
+    return (int64_t)(wave * G::NV + j) * (G::LANES * N);
   }
+  template <int N>
+  __device__ __forceinline__ uint32_t lane_at() const { return (uint32_t)(t % G::LANES) * N; }
+  template <int N>
+  __device__ __forceinline__ int64_t at(int j) const { return wave_at<N>(j) + lane_at<N>(); }
 };
 
 // Elements of a vector that lie in the segment.
@@ -122,6 +131,14 @@ __device__ __forceinline__ void load_params(const void* p, bool bf16, int64_t at
   }
 }
 
+// 1 / sqrt(v): the hardware's approximation and one step of Newton's iteration,
+// but for values whose approximation may flush to zero.
+__device__ __forceinline__ float rsqrt_of(float v) {
+  if (!(v > 1e-30f)) return 1.0f / sqrtf(v);
+  const float r = __builtin_amdgcn_rsqf(v);
+  return r * (1.5f - 0.5f * v * r * r);
+}
+
 // (x - mean) r.  For bf16 in one operation with shift = -mean r: the product's and
 // shift's roundings are 2^-24 of |x| r, far below bf16's step of x itself.
 template <typename T>
@@ -139,9 +156,10 @@ __global__ __launch_bounds__(G::TB) void k_layer_norm(const T* __restrict__ x, i
                                                       float* __restrict__ stats, uint8_t* __restrict__ x8,
                                                       uint8_t* __restrict__ sc8, float* __restrict__ sc32) {
   constexpr int N = kN<T>, NV = G::NV, LANES = G::LANES, SPAN = NV * LANES * N;   // SPAN: elements of a wave
-  __shared__ float red[2][G::TEAMS * G::WAVES][2];
+  __shared__ float4 red[2][G::TEAMS * G::WAVES];
   const Place<G> me(groups);
   const int64_t D = width / groups, c0 = me.g * D;
+  const uint32_t lane_at = me.template lane_at<N>();
   int left[NV];
   float w[NV][N], b[NV][N];
 #pragma unroll
@@ -150,16 +168,17 @@ __global__ __launch_bounds__(G::TB) void k_layer_norm(const T* __restrict__ x, i
     load_params(p.w, p.w16, c0 + me.template at<N>(j), left[j], 1.0f, w[j]);
     load_params(p.b, p.b16, c0 + me.template at<N>(j), left[j], 0.0f, b[j]);
   }
-  // elements of the segment that this wave holds
-  const int64_t first = (int64_t)(me.t / LANES) * SPAN;
-  const float mine = (float)(D - first < 0 ? 0 : D - first < SPAN ? D - first : SPAN);
+  // elements of the segment in this wave, and its share of the segment
+  const int64_t held = D - me.template wave_at<N>(0);
+  const float mine = (float)(held < 0 ? 0 : held < SPAN ? held : SPAN), per_mine = mine > 0.0f ? 1.0f / mine : 0.0f;
+  const float per_D = 1.0f / (float)D;
   const int64_t step = (int64_t)gridDim.x * me.rt;
   int64_t row = (int64_t)blockIdx.x * me.rt + me.rl;
   // the next AHEAD rows are on their way while one is computed
   Held<T> cur[NV], next[AHEAD][NV];
   auto fetch = [&](int64_t r, Held<T> (&to)[NV]) {
 #pragma unroll
-    for (int j = 0; j < NV; ++j) to[j].load(x + r * ldx + c0 + me.template at<N>(j), r < rows ? left[j] : 0);
+    for (int j = 0; j < NV; ++j) to[j].load(x + (r * ldx + c0 + me.template wave_at<N>(j)) + lane_at, r < rows ? left[j] : 0);
   };
 #pragma unroll
   for (int d = 0; d < AHEAD; ++d) fetch(row + d * step, next[d]);
@@ -182,7 +201,7 @@ __global__ __launch_bounds__(G::TB) void k_layer_norm(const T* __restrict__ x, i
       for (int i = 0; i < N; ++i) s += v[i];
     }
     s = lane_group_add<LANES>(s);
-    float mean = mine > 0.0f ? s / mine : 0.0f;
+    float mean = s * per_mine;
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
       cur[j].get(v);
@@ -196,41 +215,31 @@ __global__ __launch_bounds__(G::TB) void k_layer_norm(const T* __restrict__ x, i
     }
     q = lane_group_add<LANES>(q);
     if constexpr (G::WAVES > 1) {
-      float (*r)[2] = &red[buf][me.team * G::WAVES];
-      if ((me.t & 63) == 0) {
-        r[me.t >> 6][0] = s;
-        r[me.t >> 6][1] = q;
-      }
+      float4* r = &red[buf][me.team * G::WAVES];
+      if ((me.t & 63) == 0) r[me.t >> 6] = make_float4(mean, q, mine * per_D, 0.0f);
       __syncthreads();
-      float sum = 0.0f;
-#pragma unroll
-      for (int k = 0; k < G::WAVES; ++k) sum += r[k][0];
-      mean = sum / (float)D;
-      q = 0.0f;
-#pragma unroll
-      for (int k = 0; k < G::WAVES; ++k) {
-        const int64_t from = (int64_t)k * SPAN;
-        if (from < D) {
-          const float n = (float)(D - from < SPAN ? D - from : SPAN), d = r[k][0] / n - mean;
-          q += r[k][1] + n * d * d;
-        }
-      }
+      // a wave's numbers per lane, all waves' in every group of lanes
+      const float4 k = r[me.t % G::WAVES];
+      mean = lane_group_add<G::WAVES>(k.z * k.x);
+      const float d = k.x - mean;
+      q = lane_group_add<G::WAVES>(k.y + (k.z * (float)D) * d * d);
     }
-    const float rstd = 1.0f / sqrtf(q / (float)D + eps);
+    const float rstd = rsqrt_of(q * per_D + eps);
     if (!on) continue;
     if (stats && me.t == 0) {
       stats[2 * (row * groups + me.g)] = mean;
       stats[2 * (row * groups + me.g) + 1] = rstd;
     }
-    T* yr = y + row * width + c0;
+    T* yr = y + (row * width + c0);
     const float shift = -mean * rstd;
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
       cur[j].get(v);
 #pragma unroll
       for (int i = 0; i < N; ++i) v[i] = normed<T>(v[i], mean, rstd, shift) * w[j][i] + b[j][i];
-      if (left[j] == N) store_vec<true>(yr + me.template at<N>(j), v);
-      else if (left[j]) store_some(yr + me.template at<N>(j), left[j], v);
+      T* to = yr + me.template wave_at<N>(j) + lane_at;
+      if (left[j] == N) store_vec<true>(to, v);
+      else if (left[j]) store_some(to, left[j], v);
     }
     if constexpr (BLK != 0) {
       // lanes of a block, of a group, and vectors that a group spans
@@ -253,11 +262,13 @@ __global__ __launch_bounds__(G::TB) void k_layer_norm(const T* __restrict__ x, i
         if (left[j] == 0) continue;
         cur[j].get(v);
         uint32_t e;
-        const int64_t at = row * width + me.template at<N>(j);
+        // groups divide rows: an element's place in its group is its place in the row's
+        const int64_t from = row * width + me.template wave_at<N>(j);
+        const uint32_t in = (uint32_t)me.template wave_at<N>(j) + lane_at;
         const auto q8 = store_form(v, mb[j], Gb[j], e);
-        __builtin_nontemporal_store(q8, reinterpret_cast<typename Payload<N>::type*>(x8 + at));
-        if (at % BLK == 0) sc8[at / BLK] = (uint8_t)e;
-        if (at % (BLK * K) == 0) sc32[at / (BLK * K)] = u2f(Gb[j]);
+        __builtin_nontemporal_store(q8, reinterpret_cast<typename Payload<N>::type*>(x8 + from + lane_at));
+        if (in % BLK == 0) sc8[(from + lane_at) / BLK] = (uint8_t)e;
+        if (in % (BLK * K) == 0) sc32[(from + lane_at) / (BLK * K)] = u2f(Gb[j]);
       }
     }
   }
@@ -319,8 +330,8 @@ template <typename T> struct SourceOf<T, true> { typedef Stored type; };
 template <typename T, bool STORED> struct HeldSource;
 template <typename T> struct HeldSource<T, false> {
   Held<T, true> x;
-  __device__ __forceinline__ void load(const Source<T>& s, int64_t row, int64_t c, int left) {
-    x.load(s.x + row * s.ldx + c, left);
+  __device__ __forceinline__ void load(const Source<T>& s, int64_t row, int64_t c, uint32_t lane_at, int left) {
+    x.load(s.x + (row * s.ldx + c) + lane_at, left);
   }
   __device__ __forceinline__ void normed_values(float mean, float rstd, float shift, float (&v)[kN<T>]) const {
     x.get(v);
@@ -333,13 +344,13 @@ template <typename T> struct HeldSource<T, true> {
   W w;
   uint32_t e;
   float G;
-  __device__ __forceinline__ void load(const Stored& s, int64_t row, int64_t c, int left) {
+  __device__ __forceinline__ void load(const Stored& s, int64_t row, int64_t c, uint32_t lane_at, int left) {
     w = W{};
     e = 0;
     G = 0.0f;
     if (left) {     // blocks are a multiple of a vector: it lies in one
-      const int64_t at = row * s.width + c, n = at >> s.blk_log2;
-      w = __builtin_nontemporal_load(reinterpret_cast<const W*>(s.x8 + at));
+      const int64_t from = row * s.width + c, n = (from + lane_at) >> s.blk_log2;
+      w = __builtin_nontemporal_load(reinterpret_cast<const W*>(s.x8 + from + lane_at));
       e = s.sc8[n];
       G = s.sc32[n >> s.K_log2];
     }
@@ -368,6 +379,8 @@ __global__ __launch_bounds__(G::TB) void k_layer_norm_bwd(typename SourceOf<T, S
   __shared__ float sums[G::TEAMS > 1 ? SUMS * (G::TB / 2) : 1];
   const Place<G> me(groups);
   const int64_t D = width / groups, c0 = me.g * D;
+  const uint32_t lane_at = me.template lane_at<N>();
+  const float per_D = 1.0f / (float)D;
   int left[NV];
   float w[NV][N], aw[NV][N], ab[NV][N];
 #pragma unroll
@@ -390,8 +403,9 @@ __global__ __launch_bounds__(G::TB) void k_layer_norm_bwd(typename SourceOf<T, S
     const bool on = me.live && r < rows;
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
-      to.x[j].load(src, r, c0 + me.template at<N>(j), on ? left[j] : 0);
-      to.g[j].load(dy + r * ldy + c0 + me.template at<N>(j), on ? left[j] : 0);
+      const int64_t c = c0 + me.template wave_at<N>(j);
+      to.x[j].load(src, r, c, lane_at, on ? left[j] : 0);
+      to.g[j].load(dy + (r * ldy + c) + lane_at, on ? left[j] : 0);
     }
     to.mean = on ? stats[2 * (r * groups + me.g)] : 0.0f;
     to.rstd = on ? stats[2 * (r * groups + me.g) + 1] : 0.0f;
@@ -433,24 +447,20 @@ __global__ __launch_bounds__(G::TB) void k_layer_norm_bwd(typename SourceOf<T, S
           r[me.t >> 6][1] = s2;
         }
         __syncthreads();
-        s1 = s2 = 0.0f;
-#pragma unroll
-        for (int k = 0; k < G::WAVES; ++k) {
-          s1 += r[k][0];
-          s2 += r[k][1];
-        }
+        s1 = lane_group_add<G::WAVES>(r[me.t % G::WAVES][0]);
+        s2 = lane_group_add<G::WAVES>(r[me.t % G::WAVES][1]);
       }
-      const float m1 = rstd * (s1 / (float)D), m2 = rstd * (s2 / (float)D);
+      const float m1 = rstd * (s1 * per_D), m2 = rstd * (s2 * per_D);
       if (me.live && row < rows) {
-        T* out = dx + row * width + c0;
 #pragma unroll
         for (int j = 0; j < NV; ++j) {
           cur.x[j].normed_values(mean, rstd, shift, h);
           cur.g[j].get(g);
 #pragma unroll
           for (int i = 0; i < N; ++i) g[i] = (g[i] * w[j][i]) * rstd - m1 - h[i] * m2;
-          if (left[j] == N) store_vec(out + me.template at<N>(j), g);
-          else if (left[j]) store_some(out + me.template at<N>(j), left[j], g);
+          T* to = dx + (row * width + c0 + me.template wave_at<N>(j)) + lane_at;
+          if (left[j] == N) store_vec(to, g);
+          else if (left[j]) store_some(to, left[j], g);
         }
       }
     }
