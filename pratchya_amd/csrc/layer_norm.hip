@@ -620,8 +620,8 @@ int check_shape(const char* what, int64_t rows, int64_t width, int64_t groups) {
 
 // Threads of a workgroup (more where a team is larger), workgroups of a launch,
 // rows on their way.
-constexpr int kFwdThreads = 256, kFwdAhead = 1, kBwdThreads = 1024, kBwdAhead = 1;
-constexpr int64_t kFwdBlocks = 2048, kBwdBlocks = 256;
+constexpr int kFwdThreads = 512, kFwdAhead = 1, kBwdThreads = 1024, kBwdAhead = 1;
+constexpr int64_t kFwdBlocks = 512, kBwdBlocks = 256;
 
 // Call f(Shape) with the smallest team that holds a segment of D elements: in the
 // forward pass of 16 elements a thread where a wave is full, in the backward pass,
@@ -636,7 +636,7 @@ auto with_fwd_shape(int64_t D, F f) {
   if (D <= 1024) return f(Shape<64, 2 * V, TB>());
   if (D <= 2048) return f(Shape<128, 2 * V, TB>());
   if (D <= 4096) return f(Shape<256, 2 * V, TB>());
-  if (D <= 8192) return f(Shape<512, 2 * V, 512>());
+  if (D <= 8192) return f(Shape<512, 2 * V, TB>());
   return f(Shape<1024, 2 * V, 1024>());
 }
 template <typename T, typename F>

@@ -36,8 +36,8 @@ bool is_float_dtype(int d) { return d == PRATCHYA_DT_F32 || d == PRATCHYA_DT_BF1
 // largest for every NaN.
 __device__ __forceinline__ uint32_t rank_bits(float x) {
   const uint32_t u = f2u(x + 0.0f);
-  if (is_nan_bits(u)) return 0xFFFFFFFEu;   // no key is ~0
-  return (u & 0x80000000u) ? ~u : (u | 0x80000000u);
+  const uint32_t r = u ^ ((uint32_t)((int32_t)u >> 31) | 0x80000000u);
+  return x != x ? 0xFFFFFFFEu : r;          // no key is ~0
 }
 __device__ __forceinline__ uint64_t rank_key(float x, int64_t i) {
   return ((uint64_t)rank_bits(x) << 32) | (uint32_t)(0xFFFFFFFFu - (uint32_t)i);
@@ -224,7 +224,7 @@ __device__ __forceinline__ void select_top(const uint64_t (&keys)[kKeys], int to
   sel.seen[tid] = best;
   if (tid == 0) {
     sel.found = 0;
-    sel.bound = 0;       // where fewer than `top` groups have a key, every key is collected
+    sel.bound = 1;       // where fewer than `top` groups have a key, every key is collected
   }
   __syncthreads();
   // every wave holds all groups, two per lane, and counts how many of a quarter of
@@ -258,14 +258,14 @@ __device__ __forceinline__ void select_top(const uint64_t (&keys)[kKeys], int to
   }
   __syncthreads();
   const uint64_t bound = sel.bound;
-  if (best != 0 && best >= bound) {
+  if (best >= bound) {
     int mine = 0;
 #pragma unroll
-    for (int i = 0; i < kKeys; ++i) mine += keys[i] != 0 && keys[i] >= bound;
+    for (int i = 0; i < kKeys; ++i) mine += keys[i] >= bound;
     int at = atomicAdd(&sel.found, mine);
 #pragma unroll
     for (int i = 0; i < kKeys; ++i)
-      if (keys[i] != 0 && keys[i] >= bound) {
+      if (keys[i] >= bound) {
         if (at < kCandidates) sel.cand[at] = keys[i];
         ++at;
       }
@@ -342,12 +342,16 @@ __global__ __launch_bounds__(kPartThreads) void k_logprobs_part(const T* __restr
       if (base + (u * kPartThreads + tid) * N < to) r.add(v[u]);
     uint64_t keys[kKeys];
 #pragma unroll
-    for (int u = 0; u < VECS; ++u)
+    for (int u = 0; u < VECS; ++u) {
+      const int64_t at = base + (u * kPartThreads + tid) * N;
 #pragma unroll
-      for (int j = 0; j < N; ++j) {
-        const int64_t i = base + (u * kPartThreads + tid) * N + j;
-        keys[u * N + j] = i < to ? rank_key(v[u][j], i) : 0;
+      for (int j = 0; j < N; ++j) keys[u * N + j] = rank_key(v[u][j], at + j);
+      if (at + N > to) {
+#pragma unroll
+        for (int j = 0; j < N; ++j)
+          if (at + j >= to) keys[u * N + j] = 0;
       }
+    }
     keys[kKeys - 1] = tid < top ? list[tid] : 0;
     select_top(keys, top, sel, list);
   }
