@@ -164,18 +164,19 @@ __global__ __launch_bounds__(kThreads) void k_act(const T* __restrict__ x, Rows 
   for (int u = 0; u < PER; ++u) {
     at[u] = place<N, ONE>(r, vec + u * 64);
     const T* p = x + at[u].row * r.ldx + at[u].c;
-    if (at[u].left == N) raw[u] = load_raw<true>(p);
-  }
-#pragma unroll
-  for (int u = 0; u < PER; ++u) {
-    if (at[u].left == N) widen(raw[u], v[u]);
-    else load_some(x + at[u].row * r.ldx + at[u].c, at[u].left, 0.0f, v[u]);
+    if (at[u].left == N) {
+      raw[u] = load_raw<true>(p);
+      widen(raw[u], v[u]);
+    } else {
+      load_some(p, at[u].left, 0.0f, v[u]);
+      raw[u] = narrow(v[u]);
+    }
   }
   if constexpr (BLK != 0) {
     uint32_t m[PER], G[PER] = {};
 #pragma unroll
     for (int u = 0; u < PER; ++u)
-      m[u] = lane_group_max<BLK / N>(at[u].left ? absmax<T>(raw[u]) : 0u);   // whole vectors or none
+      m[u] = lane_group_max<BLK / N>(absmax<T>(raw[u]));
     group_max<BLK, N>(m, K, G);
 #pragma unroll
     for (int u = 0; u < PER; ++u) {

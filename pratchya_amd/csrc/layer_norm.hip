@@ -48,10 +48,11 @@ struct Affine {
 // segment position of the row (its slice of w and b, and of dw and db) and walks
 // over rows: `gt` neighbouring segments side by side, the other teams on
 // further rows.  Thread t of a team holds vectors (t / L * NV + j) * L + t % L, L =
-// min(P, 64), j < NV: groups of stored blocks lie in one wave.  Streaming accesses where they measured faster, [16384, 4096] bf16:
-// the forward pass's stores (55.2 -> 52.3 us; its loads 55.2 -> 50.8, but 25.2 ->
-// 25.7 us and 11.0 -> 12.0 us where the caches hold x), the backward pass's
-// loads (84.3 -> 79.8 us; its stores 84.3 -> 83.4, with the loads 82.7 us).
+// min(P, 64), j < NV: groups of stored blocks lie in one wave. Streaming accesses where
+// they measured faster: the forward pass's stores ([16384, 2048] bf16 27.0 -> 23.9
+// us), its loads of an x that is stored and so not read again (with its backward
+// pass [16384, 4096] 138 -> 134.5 us; of other x 25.2 -> 25.7 us where the caches
+// hold it), the backward pass's loads (84.3 -> 79.8 us).
 template <int P_, int NV_, int TB_>
 struct Shape {
   static constexpr int P = P_, NV = NV_, TB = TB_, TEAMS = TB_ / P_, WAVES = P_ > 64 ? P_ / 64 : 1;
@@ -175,8 +176,9 @@ __global__ __launch_bounds__(G::TB) void k_layer_norm(const T* __restrict__ x, i
   const int64_t step = (int64_t)gridDim.x * me.rt;
   int64_t row = (int64_t)blockIdx.x * me.rt + me.rl;
   // the next AHEAD rows are on their way while one is computed
-  Held<T> cur[NV], next[AHEAD][NV];
-  auto fetch = [&](int64_t r, Held<T> (&to)[NV]) {
+  typedef Held<T, BLK != 0> Vec;
+  Vec cur[NV], next[AHEAD][NV];
+  auto fetch = [&](int64_t r, Vec (&to)[NV]) {
 #pragma unroll
     for (int j = 0; j < NV; ++j) to[j].load(x + (r * ldx + c0 + me.template wave_at<N>(j)) + lane_at, r < rows ? left[j] : 0);
   };
@@ -661,9 +663,18 @@ dim3 grid_of(int64_t rows, int64_t groups, int64_t most) {
   return dim3((unsigned)(gx < cap ? gx : cap), (unsigned)gy);
 }
 
+// The backward pass's workgroups.  Up to kOneBlockRounds rows a team it is one along
+// the rows, whose sums are the results without a second launch.
+constexpr int64_t kOneBlockRounds = 4;      // 64 x 512 bf16 11.3 -> 9.7 us; 8 rounds, 128 x 512: 11.1 -> 13.2
+template <typename G>
+dim3 bwd_grid_of(int64_t rows, int64_t groups) {
+  const int64_t rt = G::TEAMS / (groups < G::TEAMS ? groups : G::TEAMS);
+  return grid_of<G>(rows, groups, rows <= kOneBlockRounds * rt ? 1 : kBwdBlocks);
+}
+
 dim3 bwd_grid(int64_t rows, int64_t width, int64_t groups) {
   return with_bwd_shape<float>(width / groups, [&](auto shape) {      // the teams are the same for both types
-    return grid_of<decltype(shape)>(rows, groups, kBwdBlocks);
+    return bwd_grid_of<decltype(shape)>(rows, groups);
   });
 }
 
@@ -720,7 +731,7 @@ int layer_norm_bwd(typename SourceOf<T, STORED>::type src, const void* dy, int64
       typedef decltype(shape) G;
       // 16 elements a thread leave none of the 128 registers for a row ahead
       constexpr int AHEAD = G::NV * kN<T> == 8 ? kBwdAhead : 0;
-      const dim3 grid = grid_of<G>(rows, groups, kBwdBlocks);
+      const dim3 grid = bwd_grid_of<G>(rows, groups);
       slices = (int)grid.x;
       hipLaunchKernelGGL((k_layer_norm_bwd<T, G, STORED, AHEAD>), grid, dim3(G::TB), 0, stream, src, g, ldy, p, rows,
                          width, groups, stats, static_cast<T*>(dx), part, dw, dw16, db, db16);
@@ -754,6 +765,8 @@ extern "C" int pratchya_layer_norm(const void* x, int64_t ldx, int dtype, const 
                               w_dtype, b_dtype);
   if (rows == 0 || width == 0) return pratchya_set_error(PRATCHYA_OK, "");
   if (!x || !y || (x8 && (!sc8 || !sc32))) return pratchya_set_error(PRATCHYA_EINVAL, "layer_norm: null buffer");
+  if (reinterpret_cast<uintptr_t>(x8) % 8)
+    return pratchya_set_error(PRATCHYA_EINVAL, "layer_norm: the payload must be 8-byte aligned");
   const Affine p = {w, b, w_dtype == PRATCHYA_DT_BF16, b_dtype == PRATCHYA_DT_BF16};
   return dtype == PRATCHYA_DT_BF16
              ? layer_norm<uint16_t>(x, ldx, p, rows, width, groups, eps, y, stats, x8, sc8, sc32, blk, stream)

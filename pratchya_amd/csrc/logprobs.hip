@@ -195,8 +195,8 @@ constexpr int kPartThreads = 256, kPartElems = 16, kBlock = kPartThreads * kPart
 constexpr int kKeys = kPartElems + 1;                   // keys of a thread: a block's logits and one kept key
 
 // LDS of a selection among up to kKeys keys per thread.  kCandidates is what
-// leaves room for eight workgroups in a compute unit (with room for every key, four
-// fit, and 1280 rows' parts of 4096 logits took twice the time).
+// leaves room for as many workgroups in a compute unit as its registers hold,
+// seven (with room for every key four fit: 512 rows of 131072 bf16 117 -> 90 us).
 constexpr int kCandidates = 1024;
 struct Selection {
   uint64_t cand[kCandidates];
@@ -312,7 +312,7 @@ struct Out {
 // [rows][parts][3] and kept [rows][parts][top], or for a row of one part the
 // results themselves.
 template <typename T, bool ENTROPY>
-__global__ __launch_bounds__(kPartThreads) void k_logprobs_part(const T* __restrict__ x, int64_t ld,
+__global__ __launch_bounds__(kPartThreads, 7) void k_logprobs_part(const T* __restrict__ x, int64_t ld,
                                                                 const int64_t* __restrict__ tokens, int64_t vocab,
                                                                 int top, int parts, int64_t part_len,
                                                                 float* __restrict__ sums, uint64_t* __restrict__ kept,
@@ -485,10 +485,12 @@ int check_args(const char* what, int dtype, int64_t rows, int64_t vocab) {
   return PRATCHYA_OK;
 }
 
-// Logits that the last-level cache (256 MB) cannot hold are read, and their
-// gradient written, past it: forward 8192 x 65536 bf16 188 -> 167 us, backward 372
-// -> 357 us, but 1000 x 50021 f32, 200 MB, 37.6 -> 40.2 us and 82 -> 89 us.
-bool streams(int64_t rows, int64_t vocab, int size) { return rows * vocab > ((int64_t)256 << 20) / size; }
+// Accesses past the caches.  Forward, for logits that the last-level cache (256 MB)
+// cannot hold: 8192 x 65536 bf16 188 -> 167 us, but 1000 x 50021 f32, 200 MB, 37.6 ->
+// 40.2 us.  Backward, for more than the L2 caches hold: a gradient left in the
+// last-level cache is written back while the next pass's logits are read; both
+// passes over 1000 x 50021 f32 one after the other 119 -> 97 us.
+constexpr int64_t kFwdStream = (int64_t)256 << 20, kBwdStream = (int64_t)32 << 20;
 
 // How a row with alternatives is cut.
 struct Cut {
@@ -524,7 +526,7 @@ int launch(const void* logits, int64_t ld, const int64_t* tokens, int64_t rows, 
                      dim3((unsigned)((rows + (WPR < 4 ? 4 / WPR : 1) - 1) / (WPR < 4 ? 4 / WPR : 1))),                \
                      dim3(WPR < 4 ? 256 : WPR * 64), 0, stream, x, ld, tokens, rows, vocab, o.logprobs, o.entropy,    \
                      o.stats)
-  const bool nt = streams(rows, vocab, sizeof(T));
+  const bool nt = rows * vocab > kFwdStream / (int64_t)sizeof(T);
   if (vocab <= 2048) PRATCHYA_LP(1, false);
   else if (rows < 512) PRATCHYA_LP(16, false);
   else if (nt) PRATCHYA_LP(4, true);
@@ -547,7 +549,7 @@ int launch_bwd(const void* logits, int64_t ld, const int64_t* tokens, const floa
                      static_cast<const T*>(logits), ld, tokens, stats, g, gh, rows, vocab, (unsigned)pieces,          \
                      static_cast<T*>(dx))
   if (tpr == 64) PRATCHYA_LPB(64, false);
-  else if (streams(rows, vocab, sizeof(T))) PRATCHYA_LPB(256, true);
+  else if (rows * vocab > kBwdStream / (int64_t)sizeof(T)) PRATCHYA_LPB(256, true);
   else PRATCHYA_LPB(256, false);
 #undef PRATCHYA_LPB
   return check_launch("token_logprobs_bwd");

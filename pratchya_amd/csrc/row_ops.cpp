@@ -8,6 +8,7 @@
 #include <Python.h>
 
 #include <ATen/ATen.h>
+#include <ATen/hip/EmptyTensor.h>
 #include <ATen/hip/impl/HIPStreamMasqueradingAsCUDA.h>
 #include <c10/core/DeviceGuard.h>
 #include <torch/csrc/Dtype.h>
@@ -64,8 +65,9 @@ hipStream_t stream_of(const Tensor& t) {
   return at::hip::getCurrentHIPStreamMasqueradingAsCUDA(t.device().index()).stream();
 }
 
+// Straight from the device's allocator: at::empty's dispatch costs as much again.
 Tensor new_empty(at::IntArrayRef shape, at::ScalarType type, const Tensor& like) {
-  return at::empty(shape, at::TensorOptions().dtype(type).device(like.device()));
+  return at::detail::empty_cuda(shape, type, like.device(), std::nullopt);
 }
 
 void* address(const Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
