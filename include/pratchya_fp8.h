@@ -671,7 +671,8 @@ int pratchya_debug_f32_to_bf16(const float* in, uint16_t* out, int64_t n, int mo
  * (f32 [rows * groups][2]), which the backward pass reads.  x8 / sc8 / sc32, if
  * x8 is not null, receive x quantized with tgrid (1, blk) as
  * pratchya_quantize(x [rows, width]) in the same pass, for the layouts
- * pratchya_layer_norm_stores takes (PRATCHYA_EUNSUPPORTED for others). */
+ * pratchya_layer_norm_stores takes (PRATCHYA_EUNSUPPORTED for others); x8 is
+ * 8-byte aligned. */
 int pratchya_layer_norm(const void* x, int64_t ldx, int dtype, const void* w, int w_dtype, const void* b, int b_dtype,
                         int64_t rows, int64_t width, int64_t groups, float eps, void* y, float* stats, uint8_t* x8,
                         uint8_t* sc8, float* sc32, int64_t blk, hipStream_t stream);
@@ -681,7 +682,8 @@ int pratchya_layer_norm_stores(int64_t width, int64_t groups, int64_t blk);
 
 /* Gradients of pratchya_layer_norm.  x as the forward pass read it (x_dtype =
  * dtype, ldx), or its quantized form (x_dtype PRATCHYA_DT_E4M3, payload
- * contiguous, with sc8 / sc32 and blk; ldx unused); dy of dtype, rows ldy
+ * contiguous, 8-byte aligned, with sc8 / sc32 and blk, a power of two of 8 or more;
+ * segments of a multiple of 8 elements; ldx unused); dy of dtype, rows ldy
  * elements apart; stats of the forward pass.  Writes dx (contiguous, dtype), dw
  * and db ([width], f32 or bf16); each may be null.  dw and db need a workspace
  * of pratchya_layer_norm_bwd_workspace_bytes, 4-byte aligned; they are sums of a

@@ -795,6 +795,9 @@ extern "C" int pratchya_layer_norm_bwd(const void* x, int64_t ldx, int x_dtype, 
                               (long long)width);
   if (stored && reinterpret_cast<uintptr_t>(x) % 8)
     return pratchya_set_error(PRATCHYA_EINVAL, "layer_norm_bwd: the payload must be 8-byte aligned");
+  if (stored && (width / groups) % 8)      // a vector of a segment would lie in two blocks
+    return pratchya_set_error(PRATCHYA_EUNSUPPORTED, "layer_norm_bwd: stored segments of %lld elements, not of eights",
+                              (long long)(width / groups));
   if (rows == 0 || width == 0) return pratchya_set_error(PRATCHYA_OK, "");
   if (!x || !dy || !stats || (stored && (!sc8 || !sc32)))
     return pratchya_set_error(PRATCHYA_EINVAL, "layer_norm_bwd: null buffer");

@@ -173,7 +173,11 @@ Normed layer_norm_fwd(const Tensor& x, const MaybeTensor& weight, const MaybeTen
   const RowArray r = as_rows(x, what);
   TORCH_CHECK_VALUE(groups >= 1 && r.width % groups == 0, what, ": ", groups, " groups do not divide rows of ", r.width);
   const Param w = param(weight, r.width, x, "layer_norm: weight"), b = param(bias, r.width, x, "layer_norm: bias");
-  if (grid.b) check_block(grid.a, grid.b, r.width, what);
+  if (grid.b) {
+    check_block(grid.a, grid.b, r.width, what);
+    TORCH_CHECK_VALUE(r.width / groups % 8 == 0, what, ": block grid for ", groups, " groups of ", r.width / groups,
+                      " elements; an 8-bit input needs groups of a multiple of 8");
+  }
   const c10::DeviceGuard guard(x.device());
   const hipStream_t stream = stream_of(x);
   Normed out;

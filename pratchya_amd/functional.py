@@ -34,8 +34,9 @@ def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, bias: Opt
     """``(x - mean) / sqrt(var + eps) * weight + bias`` over the last axis of x
     [..., C], or over each of ``groups`` equal segments of it (the heads of a norm
     over heads); weight and bias [C] or None.  With ``tgrid=(1, b)``, b 16, 32, 64 or
-    128 dividing C, x is kept for the backward pass in 8 bits with that block
-    grid (its mean and deviation in f32, of x itself).  Without a gradient to
+    128 dividing C, and segments of a multiple of 8 elements, x is kept for the
+    backward pass in 8 bits with that block grid (its mean and deviation in f32, of
+    x itself).  Without a gradient to
     compute nothing is kept, and ``tgrid`` has no effect."""
     return _ops.layer_norm(x, weight, bias, eps, groups, tgrid)
 

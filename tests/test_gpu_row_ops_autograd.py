@@ -133,3 +133,19 @@ def test_library_errors():
     from pratchya_amd import _lib
     with pytest.raises(_lib.PratchyaUnsupported, match="2\\^20"):
         _F().layer_norm(torch.zeros((1, 1 << 21), device="cuda"), groups=1 << 21)
+
+
+def test_stored_segments_of_eights():
+    """A segment of an 8-bit input starts at a vector's boundary, so that no vector lies in two blocks or beyond
+    the array: other segments are refused before any launch, by the binding and by the library."""
+    from pratchya_amd import _kernels as K
+    from pratchya_amd import _lib
+    x = torch.zeros((4, 96), device="cuda", requires_grad=True)
+    with pytest.raises(ValueError, match="multiple of 8"):
+        _F().layer_norm(x, groups=8, tgrid=(1, 32))
+    stats = torch.zeros((32, 2), device="cuda")
+    with pytest.raises(_lib.PratchyaUnsupported, match="not of eights"):
+        K.layer_norm_bwd(K.quantize(x.detach(), (1, 32)), torch.zeros((4, 96), device="cuda"), None, stats, 8, (1, 32))
+    y = _F().layer_norm(x, groups=4, tgrid=(1, 32))          # segments of 24
+    y.sum().backward()
+    assert x.grad is not None
