@@ -151,6 +151,9 @@ __device__ __forceinline__ float normed(float x, float mean, float rstd, float s
 // y and the statistics of whole segments; with BLK, x's stored form beside them
 // (groups = 1).  Mean and squared deviations are taken within each wave, from
 // registers, and joined by counts, so a mean far from zero costs no digits.
+// Bound by HBM, with some 20 vector instructions an element beside it: [16384,
+// 4096] bf16 49 us (268 MB, 5.4 TB/s), with its 8-bit form 64 us (335 MB, 5.2
+// TB/s), heads of 64 over [8192, 4096] 23 us (5.8 TB/s); one row of 4096 4 us.
 template <typename T, typename G, int BLK, int AHEAD>
 __global__ __launch_bounds__(G::TB) void k_layer_norm(const T* __restrict__ x, int64_t ldx, Affine p, int64_t rows,
                                                       int64_t width, int64_t groups, float eps, T* __restrict__ y,
@@ -276,31 +279,65 @@ __global__ __launch_bounds__(G::TB) void k_layer_norm(const T* __restrict__ x, i
   }
 }
 
-// Segments longer than a workgroup's registers: three passes over the row, the
-// later ones from the caches.
+// Segments of more than kLongest elements, which a workgroup's registers do not
+// hold: a workgroup a segment, kLongVecs vectors a thread in flight, three passes
+// over the row of which the later two come from the L2 cache.  [2048, 32768] bf16
+// 88 us, its backward pass 180 us (3.0 and 2.2 TB/s of what goes through HBM once).
+constexpr int kLongThreads = 1024, kLongVecs = 4;
+
+// Calls f(first element, elements there) for this thread's vectors of a segment,
+// after load has been called for up to kLongVecs of them.
+template <int N, typename Load, typename Use>
+__device__ __forceinline__ void sweep(int64_t D, Load load, Use use) {
+  for (int64_t i = (int64_t)threadIdx.x * N; i < D; i += (int64_t)kLongVecs * kLongThreads * N) {
+#pragma unroll
+    for (int u = 0; u < kLongVecs; ++u) {
+      const int64_t at = i + (int64_t)u * kLongThreads * N;
+      load(u, at, part_of<N>(D - at));
+    }
+#pragma unroll
+    for (int u = 0; u < kLongVecs; ++u) {
+      const int64_t at = i + (int64_t)u * kLongThreads * N;
+      const int left = part_of<N>(D - at);
+      if (left) use(u, at, left);
+    }
+  }
+}
+
 template <typename T>
-__global__ __launch_bounds__(256) void k_layer_norm_long(const T* __restrict__ x, int64_t ldx, Affine p, int64_t width,
-                                                         int64_t groups, float eps, T* __restrict__ y,
-                                                         float* __restrict__ stats) {
-  __shared__ float lds[4];
-  const int64_t D = width / groups, row = blockIdx.x / groups, c0 = (blockIdx.x - row * groups) * D;
-  const T* xs = x + row * ldx + c0;
-  T* ys = y + row * width + c0;
-  float s = 0.0f;
-  for (int64_t i = threadIdx.x; i < D; i += 256) s += load_elem(xs + i);
-  const float mean = block_add<4>(s, lds) / (float)D;
-  float q = 0.0f;
-  for (int64_t i = threadIdx.x; i < D; i += 256) {
-    const float d = load_elem(xs + i) - mean;
-    q += d * d;
-  }
-  const float rstd = 1.0f / sqrtf(block_add<4>(q, lds) / (float)D + eps);
-  for (int64_t i = threadIdx.x; i < D; i += 256) {
-    float v = (load_elem(xs + i) - mean) * rstd;
-    if (p.w) v *= load_param(p.w, p.w16, c0 + i);
-    if (p.b) v += load_param(p.b, p.b16, c0 + i);
-    store_elem(ys + i, v);
-  }
+__global__ __launch_bounds__(kLongThreads) void k_layer_norm_long(const T* __restrict__ x, int64_t ldx, Affine p,
+                                                                  int64_t width, int64_t groups, float eps,
+                                                                  T* __restrict__ y, float* __restrict__ stats) {
+  constexpr int N = kN<T>;
+  __shared__ float lds[kLongThreads / 64];
+  const int64_t D = width / groups, row = blockIdx.x / (unsigned)groups, c0 = (blockIdx.x - row * groups) * D;
+  const T* xs = x + (row * ldx + c0);
+  T* ys = y + (row * width + c0);
+  Held<T> h[kLongVecs];
+  const auto load = [&](int u, int64_t at, int left) { h[u].load(xs + at, left); };
+  float v[N], s = 0.0f, q = 0.0f;
+  sweep<N>(D, load, [&](int u, int64_t, int) {
+    h[u].get(v);
+#pragma unroll
+    for (int i = 0; i < N; ++i) s += v[i];
+  });
+  const float mean = block_add<kLongThreads / 64>(s, lds) / (float)D;
+  sweep<N>(D, load, [&](int u, int64_t, int left) {
+    h[u].get(v);
+#pragma unroll
+    for (int i = 0; i < N; ++i) q += i < left ? (v[i] - mean) * (v[i] - mean) : 0.0f;
+  });
+  const float rstd = rsqrt_of(block_add<kLongThreads / 64>(q, lds) / (float)D + eps), shift = -mean * rstd;
+  sweep<N>(D, load, [&](int u, int64_t at, int left) {
+    float w[N], b[N];
+    load_params(p.w, p.w16, c0 + at, left, 1.0f, w);
+    load_params(p.b, p.b16, c0 + at, left, 0.0f, b);
+    h[u].get(v);
+#pragma unroll
+    for (int i = 0; i < N; ++i) v[i] = normed<T>(v[i], mean, rstd, shift) * w[i] + b[i];
+    if (left == N) store_vec(ys + at, v);
+    else store_some(ys + at, left, v);
+  });
   if (stats && threadIdx.x == 0) {
     stats[2 * (int64_t)blockIdx.x] = mean;
     stats[2 * (int64_t)blockIdx.x + 1] = rstd;
@@ -312,7 +349,6 @@ template <typename X>
 struct Source {
   const X* x;
   int64_t ldx;
-  __device__ __forceinline__ float at(int64_t row, int64_t i) const { return load_elem(x + row * ldx + i); }
 };
 struct Stored {
   const uint8_t* x8;
@@ -320,10 +356,6 @@ struct Stored {
   const float* sc32;
   int64_t width;
   int blk_log2, K_log2;      // elements per block and blocks per group are powers of two
-  __device__ __forceinline__ float at(int64_t row, int64_t i) const {
-    const int64_t e = row * width + i, n = e >> blk_log2;
-    return (e4m3fn_to_f32(x8[e]) * (e8m0_decode(sc8[n]) * sc32[n >> K_log2])) * 0.0078125f;
-  }
 };
 template <typename T, bool STORED> struct SourceOf { typedef Source<T> type; };
 template <typename T> struct SourceOf<T, true> { typedef Stored type; };
@@ -368,7 +400,9 @@ template <typename T> struct HeldSource<T, true> {
 // dx of whole segments, and the sums of dy h and dy over the rows that a team
 // has walked: joined over the workgroup's row lanes and written to
 // part[blockIdx.x][0 / 1][width], or as the results where there is one workgroup
-// per column.
+// per column.  Bound by HBM; the partial sums, 2 kB a column over 256 workgroups,
+// are 5% of it: with the join [16384, 4096] bf16 79 us (402 MB, 5.1 TB/s), from the
+// 8-bit form 71 us (335 MB), heads of 64 over [8192, 4096] 41 us (201 MB).
 template <typename T, typename G, bool STORED, int AHEAD>
 __global__ __launch_bounds__(G::TB) void k_layer_norm_bwd(typename SourceOf<T, STORED>::type src,
                                                           const T* __restrict__ dy, int64_t ldy, Affine p,
@@ -526,51 +560,85 @@ __global__ __launch_bounds__(G::TB) void k_layer_norm_bwd(typename SourceOf<T, S
   }
 }
 
-template <typename T, typename S>
-__global__ __launch_bounds__(256) void k_layer_norm_long_dx(S src, const T* __restrict__ dy, int64_t ldy, Affine p,
-                                                       int64_t width, int64_t groups, const float* __restrict__ stats,
-                                                       T* __restrict__ dx) {
-  __shared__ float lds[4];
-  const int64_t D = width / groups, row = blockIdx.x / groups, c0 = (blockIdx.x - row * groups) * D;
-  const float mean = stats[2 * (int64_t)blockIdx.x], rstd = stats[2 * (int64_t)blockIdx.x + 1];
-  float s1 = 0.0f, s2 = 0.0f;
-  for (int64_t i = threadIdx.x; i < D; i += 256) {
-    const float h = (src.at(row, c0 + i) - mean) * rstd;
-    float a = load_elem(dy + row * ldy + c0 + i);
-    if (p.w) a *= load_param(p.w, p.w16, c0 + i);
-    s1 += a;
-    s2 += a * h;
-  }
-  const float m1 = block_add<4>(s1, lds) / (float)D, m2 = block_add<4>(s2, lds) / (float)D;
-  for (int64_t i = threadIdx.x; i < D; i += 256) {
-    const float h = (src.at(row, c0 + i) - mean) * rstd;
-    float a = load_elem(dy + row * ldy + c0 + i);
-    if (p.w) a *= load_param(p.w, p.w16, c0 + i);
-    store_elem(dx + row * width + c0 + i, rstd * (a - m1 - h * m2));
-  }
+// dx of long segments, a workgroup each: two passes.
+template <typename T, bool STORED>
+__global__ __launch_bounds__(kLongThreads) void k_layer_norm_long_dx(typename SourceOf<T, STORED>::type src,
+                                                                     const T* __restrict__ dy, int64_t ldy, Affine p,
+                                                                     int64_t width, int64_t groups,
+                                                                     const float* __restrict__ stats,
+                                                                     T* __restrict__ dx) {
+  constexpr int N = kN<T>;
+  __shared__ float lds[kLongThreads / 64];
+  const int64_t D = width / groups, row = blockIdx.x / (unsigned)groups, c0 = (blockIdx.x - row * groups) * D;
+  const float mean = stats[2 * (int64_t)blockIdx.x], rstd = stats[2 * (int64_t)blockIdx.x + 1], shift = -mean * rstd;
+  const T* gs = dy + (row * ldy + c0);
+  T* out = dx + (row * width + c0);
+  HeldSource<T, STORED> hx[kLongVecs];
+  Held<T> hg[kLongVecs];
+  const auto load = [&](int u, int64_t at, int left) {
+    hx[u].load(src, row, c0, (uint32_t)at, left);
+    hg[u].load(gs + at, left);
+  };
+  float h[N], g[N], w[N], s1 = 0.0f, s2 = 0.0f;
+  sweep<N>(D, load, [&](int u, int64_t at, int left) {
+    load_params(p.w, p.w16, c0 + at, left, 1.0f, w);
+    hx[u].normed_values(mean, rstd, shift, h);
+    hg[u].get(g);
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      s1 += g[i] * w[i];
+      s2 += g[i] * w[i] * h[i];
+    }
+  });
+  const float m1 = rstd * (block_add<kLongThreads / 64>(s1, lds) / (float)D);
+  const float m2 = rstd * (block_add<kLongThreads / 64>(s2, lds) / (float)D);
+  sweep<N>(D, load, [&](int u, int64_t at, int left) {
+    load_params(p.w, p.w16, c0 + at, left, 1.0f, w);
+    hx[u].normed_values(mean, rstd, shift, h);
+    hg[u].get(g);
+#pragma unroll
+    for (int i = 0; i < N; ++i) g[i] = (g[i] * w[i]) * rstd - m1 - h[i] * m2;
+    if (left == N) store_vec(out + at, g);
+    else store_some(out + at, left, g);
+  });
 }
 
-// Column sums over the rows of one of gridDim.y slices: part[slice][0 / 1][width].
-template <typename T, typename S>
-__global__ __launch_bounds__(256) void k_layer_norm_long_dp(S src, const T* __restrict__ dy, int64_t ldy, int64_t rows,
-                                                       int64_t width, int64_t groups,
-                                                       const float* __restrict__ stats, float* __restrict__ part) {
-  const int64_t c = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  if (c >= width) return;
-  const int64_t g = c / (width / groups);
-  float dw = 0.0f, db = 0.0f;
+// Column sums of long segments over the rows of one of gridDim.y slices, a vector
+// of columns per thread: part[slice][0 / 1][width].
+template <typename T, bool STORED>
+__global__ __launch_bounds__(256) void k_layer_norm_long_dp(typename SourceOf<T, STORED>::type src,
+                                                            const T* __restrict__ dy, int64_t ldy, int64_t rows,
+                                                            int64_t width, int64_t groups, int64_t tiles,
+                                                            const float* __restrict__ stats,
+                                                            float* __restrict__ part) {
+  constexpr int N = kN<T>;
+  const int64_t D = width / groups, g0 = blockIdx.x / (unsigned)tiles, c0 = g0 * D;
+  const int64_t at = ((blockIdx.x - g0 * tiles) * 256 + threadIdx.x) * N;
+  const int left = part_of<N>(D - at);
+  if (!left) return;
+  float dw[N] = {}, db[N] = {}, h[N], g[N];
+#pragma unroll 4
   for (int64_t row = blockIdx.y; row < rows; row += gridDim.y) {
-    const float* st = stats + 2 * (row * groups + g);
-    const float v = load_elem(dy + row * ldy + c);
-    dw += v * ((src.at(row, c) - st[0]) * st[1]);
-    db += v;
+    HeldSource<T, STORED> hx;
+    Held<T> hg;
+    hx.load(src, row, c0, (uint32_t)at, left);
+    hg.load(dy + (row * ldy + c0) + at, left);
+    const float mean = stats[2 * (row * groups + g0)], rstd = stats[2 * (row * groups + g0) + 1];
+    hx.normed_values(mean, rstd, -mean * rstd, h);
+    hg.get(g);
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      dw[i] += g[i] * h[i];
+      db[i] += g[i];
+    }
   }
-  part[(2 * (int64_t)blockIdx.y) * width + c] = dw;
-  part[(2 * (int64_t)blockIdx.y + 1) * width + c] = db;
+  float* to = part + 2 * (int64_t)blockIdx.y * width + c0 + at;
+  store_some(to, left, dw);
+  store_some(to + width, left, db);
 }
 
 // dw and db from the slices' sums: kJoinCols columns per workgroup, its waves on
-// different slices.
+// different slices.  256 slices of 4096 columns 4 us, the launch among them.
 constexpr int kJoinCols = 64, kJoinWaves = 16, kJoinThreads = kJoinWaves * 64;
 __global__ __launch_bounds__(kJoinThreads) void k_layer_norm_join(const float* __restrict__ part, int slices,
                                                                   int64_t width, void* dw, bool dw16, void* db,
@@ -615,8 +683,8 @@ int check_shape(const char* what, int64_t rows, int64_t width, int64_t groups) {
   if (rows < 0 || width < 0 || groups < 1 || width % groups)
     return pratchya_set_error(PRATCHYA_EINVAL, "%s: %lld groups do not divide rows of %lld (%lld rows)", what,
                               (long long)groups, (long long)width, (long long)rows);
-  if (rows > 0x7FFFFFFF || groups > (1 << 20) || rows * groups > 0x7FFFFFFF || width > ((int64_t)1 << 38))
-    return pratchya_set_error(PRATCHYA_EUNSUPPORTED, "%s: more than 2^31 segments, or 2^20 in a row", what);
+  if (rows > 0x7FFFFFFF || groups > (1 << 20) || rows * groups > 0x7FFFFFFF || width > ((int64_t)1 << 31))
+    return pratchya_set_error(PRATCHYA_EUNSUPPORTED, "%s: more than 2^31 segments, 2^20 in a row or 2^31 elements in one", what);
   return PRATCHYA_OK;
 }
 
@@ -699,8 +767,8 @@ int layer_norm(const void* x, int64_t ldx, const Affine& p, int64_t rows, int64_
   const T* xt = static_cast<const T*>(x);
   T* yt = static_cast<T*>(y);
   if (width / groups > kLongest)
-    hipLaunchKernelGGL((k_layer_norm_long<T>), dim3((unsigned)(rows * groups)), dim3(256), 0, stream, xt, ldx, p, width,
-                       groups, eps, yt, stats);
+    hipLaunchKernelGGL((k_layer_norm_long<T>), dim3((unsigned)(rows * groups)), dim3(kLongThreads), 0, stream, xt, ldx,
+                       p, width, groups, eps, yt, stats);
   else
     with_fwd_shape<T>(width / groups, [&](auto shape) {
       launch_fwd<T>(shape, xt, ldx, p, rows, width, groups, eps, yt, stats, x8, sc8, sc32, blk, stream);
@@ -712,19 +780,19 @@ template <typename T, bool STORED>
 int layer_norm_bwd(typename SourceOf<T, STORED>::type src, const void* dy, int64_t ldy, const void* w, int w_dtype,
                    const float* stats, int64_t rows, int64_t width, int64_t groups, void* dx, void* dw, int dw_dtype,
                    void* db, int db_dtype, float* part, hipStream_t stream) {
-  typedef typename SourceOf<T, STORED>::type S;
   const T* g = static_cast<const T*>(dy);
   const Affine p = {w, nullptr, w_dtype == PRATCHYA_DT_BF16, false};
   const bool dw16 = dw_dtype == PRATCHYA_DT_BF16, db16 = db_dtype == PRATCHYA_DT_BF16;
   int slices = 1;
   if (width / groups > kLongest) {
     if (dx)
-      hipLaunchKernelGGL((k_layer_norm_long_dx<T, S>), dim3((unsigned)(rows * groups)), dim3(256), 0, stream, src, g,
-                         ldy, p, width, groups, stats, static_cast<T*>(dx));
+      hipLaunchKernelGGL((k_layer_norm_long_dx<T, STORED>), dim3((unsigned)(rows * groups)), dim3(kLongThreads), 0,
+                         stream, src, g, ldy, p, width, groups, stats, static_cast<T*>(dx));
     if (dw || db) {
       slices = rows < kSlices ? (int)rows : kSlices;
-      hipLaunchKernelGGL((k_layer_norm_long_dp<T, S>), dim3((unsigned)((width + 255) / 256), (unsigned)slices),
-                         dim3(256), 0, stream, src, g, ldy, rows, width, groups, stats, part);
+      const int64_t tiles = (width / groups + 256 * kN<T> - 1) / (256 * kN<T>);
+      hipLaunchKernelGGL((k_layer_norm_long_dp<T, STORED>), dim3((unsigned)(groups * tiles), (unsigned)slices),
+                         dim3(256), 0, stream, src, g, ldy, rows, width, groups, tiles, stats, part);
     }
   } else {
     with_bwd_shape<T>(width / groups, [&](auto shape) {

@@ -67,5 +67,6 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, entropy: bool = F
 
     A negative token stands for none: its log probability is 0 and has no
     gradient.  A token of V or more gives NaN.  Logits of -inf are masked; a row of
-    nothing else has log probabilities of -inf, entropy 0 and no gradient."""
+    nothing else has log probabilities of -inf and entropy 0, and in its gradient,
+    as for any masked logit, the probability 0."""
     return TokenLogprobs(*_ops.token_logprobs(logits, tokens, entropy, top))
