@@ -133,9 +133,9 @@ __device__ __forceinline__ void load_params(const void* p, bool bf16, int64_t at
 }
 
 // 1 / sqrt(v): the hardware's approximation and one step of Newton's iteration,
-// but for values whose approximation may flush to zero.
+// but for values near the ends of f32's range, where either may not be finite.
 __device__ __forceinline__ float rsqrt_of(float v) {
-  if (!(v > 1e-30f)) return 1.0f / sqrtf(v);
+  if (!(v > 1e-30f && v < 1e30f)) return 1.0f / sqrtf(v);
   const float r = __builtin_amdgcn_rsqf(v);
   return r * (1.5f - 0.5f * v * r * r);
 }
