@@ -94,16 +94,35 @@ struct Place {
 template <int N>
 __device__ __forceinline__ int part_of(int64_t n) { return n < 0 ? 0 : n < N ? (int)n : N; }
 
+// A thread's vector of a segment of D elements: the last `own` of the n elements
+// loaded and stored at `off`.  The vector at the end of a segment of an odd length
+// is moved back to end with it: its first elements are the thread's before it, left
+// out of sums and stored by both, with the same value.  By its elements, each
+// load waited for where it was issued, [8192, 4095] bf16 took 34.5 us for 23.9, in the
+// backward pass 99.9 for 51.1.  Segments below a vector (whole: false) go by elements.
+template <int N>
+struct Part {
+  uint32_t off;
+  int own;
+  __device__ __forceinline__ void set(int64_t D, int64_t at, bool whole) {
+    own = part_of<N>(D - at);
+    off = (uint32_t)(at - (own && whole ? N - own : 0));
+  }
+  __device__ __forceinline__ int n(bool whole) const { return own && whole ? N : own; }
+  __device__ __forceinline__ bool owns(int i, bool whole) const { return whole ? i >= N - own : i < own; }
+};
+
 // A vector of a row in registers, in its type.
 template <typename T, bool NT = false>
 struct Held {
   u32x4_t raw;
-  __device__ __forceinline__ void load(const T* p, int left) {
-    if (left == kN<T>) {
-      raw = load_raw<NT>(p);
+  __device__ __forceinline__ void load(const T* p, const Part<kN<T>>& at, bool whole) {
+    if (whole) {
+      raw = u32x4_t{0, 0, 0, 0};
+      if (at.own) raw = load_raw<NT>(p + at.off);
     } else {
       float v[kN<T>];
-      load_some(p, left, 0.0f, v);
+      load_some(p + at.off, at.own, 0.0f, v);
       raw = narrow(v);
     }
   }
@@ -163,14 +182,14 @@ __global__ __launch_bounds__(G::TB) void k_layer_norm(const T* __restrict__ x, i
   __shared__ float4 red[2][G::TEAMS * G::WAVES];
   const Place<G> me(groups);
   const int64_t D = width / groups, c0 = me.g * D;
-  const uint32_t lane_at = me.template lane_at<N>();
-  int left[NV];
+  const bool whole = G::P > 8 || D >= N;    // wider teams hold segments of more than 64
+  Part<N> at[NV];
   float w[NV][N], b[NV][N];
 #pragma unroll
   for (int j = 0; j < NV; ++j) {
-    left[j] = me.live ? part_of<N>(D - me.template at<N>(j)) : 0;
-    load_params(p.w, p.w16, c0 + me.template at<N>(j), left[j], 1.0f, w[j]);
-    load_params(p.b, p.b16, c0 + me.template at<N>(j), left[j], 0.0f, b[j]);
+    at[j].set(me.live ? D : 0, me.template at<N>(j), whole);
+    load_params(p.w, p.w16, c0 + at[j].off, at[j].n(whole), 1.0f, w[j]);
+    load_params(p.b, p.b16, c0 + at[j].off, at[j].n(whole), 0.0f, b[j]);
   }
   // elements of the segment in this wave, and its share of the segment
   const int64_t held = D - me.template wave_at<N>(0);
@@ -183,7 +202,11 @@ __global__ __launch_bounds__(G::TB) void k_layer_norm(const T* __restrict__ x, i
   Vec cur[NV], next[AHEAD][NV];
   auto fetch = [&](int64_t r, Vec (&to)[NV]) {
 #pragma unroll
-    for (int j = 0; j < NV; ++j) to[j].load(x + (r * ldx + c0 + me.template wave_at<N>(j)) + lane_at, r < rows ? left[j] : 0);
+    for (int j = 0; j < NV; ++j) {
+      Part<N> a = at[j];
+      if (r >= rows) a.own = 0;
+      to[j].load(x + (r * ldx + c0), a, whole);
+    }
   };
 #pragma unroll
   for (int d = 0; d < AHEAD; ++d) fetch(row + d * step, next[d]);
@@ -202,20 +225,25 @@ __global__ __launch_bounds__(G::TB) void k_layer_norm(const T* __restrict__ x, i
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
       cur[j].get(v);
+      if (at[j].own == N) {
 #pragma unroll
-      for (int i = 0; i < N; ++i) s += v[i];
+        for (int i = 0; i < N; ++i) s += v[i];
+      } else {
+#pragma unroll
+        for (int i = 0; i < N; ++i) s += at[j].owns(i, whole) ? v[i] : 0.0f;
+      }
     }
     s = lane_group_add<LANES>(s);
     float mean = s * per_mine;
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
       cur[j].get(v);
-      if (left[j] == N) {
+      if (at[j].own == N) {
 #pragma unroll
         for (int i = 0; i < N; ++i) q += (v[i] - mean) * (v[i] - mean);
       } else {
 #pragma unroll
-        for (int i = 0; i < N; ++i) q += i < left[j] ? (v[i] - mean) * (v[i] - mean) : 0.0f;
+        for (int i = 0; i < N; ++i) q += at[j].owns(i, whole) ? (v[i] - mean) * (v[i] - mean) : 0.0f;
       }
     }
     q = lane_group_add<LANES>(q);
@@ -242,9 +270,8 @@ __global__ __launch_bounds__(G::TB) void k_layer_norm(const T* __restrict__ x, i
       cur[j].get(v);
 #pragma unroll
       for (int i = 0; i < N; ++i) v[i] = normed<T>(v[i], mean, rstd, shift) * w[j][i] + b[j][i];
-      T* to = yr + me.template wave_at<N>(j) + lane_at;
-      if (left[j] == N) store_vec<true>(to, v);
-      else if (left[j]) store_some(to, left[j], v);
+      if (at[j].n(whole) == N) store_vec<true>(yr + at[j].off, v);
+      else if (at[j].own) store_some(yr + at[j].off, at[j].own, v);
     }
     if constexpr (BLK != 0) {
       // lanes of a block, of a group, and vectors that a group spans
@@ -264,16 +291,16 @@ __global__ __launch_bounds__(G::TB) void k_layer_norm(const T* __restrict__ x, i
       }
 #pragma unroll
       for (int j = 0; j < NV; ++j) {
-        if (left[j] == 0) continue;
+        if (at[j].own == 0) continue;
         cur[j].get(v);
         uint32_t e;
         // groups divide rows: an element's place in its group is its place in the row's
-        const int64_t from = row * width + me.template wave_at<N>(j);
-        const uint32_t in = (uint32_t)me.template wave_at<N>(j) + lane_at;
+        const int64_t from = row * width;
+        const uint32_t in = at[j].off;
         const auto q8 = store_form(v, mb[j], Gb[j], e);
-        __builtin_nontemporal_store(q8, reinterpret_cast<typename Payload<N>::type*>(x8 + from + lane_at));
-        if (in % BLK == 0) sc8[(from + lane_at) / BLK] = (uint8_t)e;
-        if (in % (BLK * K) == 0) sc32[(from + lane_at) / (BLK * K)] = u2f(Gb[j]);
+        __builtin_nontemporal_store(q8, reinterpret_cast<typename Payload<N>::type*>(x8 + from + in));
+        if (in % BLK == 0) sc8[(from + in) / BLK] = (uint8_t)e;
+        if (in % (BLK * K) == 0) sc32[(from + in) / (BLK * K)] = u2f(Gb[j]);
       }
     }
   }
@@ -285,22 +312,20 @@ __global__ __launch_bounds__(G::TB) void k_layer_norm(const T* __restrict__ x, i
 // 88 us, its backward pass 180 us (3.0 and 2.2 TB/s of what goes through HBM once).
 constexpr int kLongThreads = 1024, kLongVecs = 4;
 
-// Calls f(first element, elements there) for this thread's vectors of a segment,
-// after load has been called for up to kLongVecs of them.
+// Calls use(u, part) for this thread's vectors of a segment, after load has been
+// called for up to kLongVecs of them.
 template <int N, typename Load, typename Use>
 __device__ __forceinline__ void sweep(int64_t D, Load load, Use use) {
   for (int64_t i = (int64_t)threadIdx.x * N; i < D; i += (int64_t)kLongVecs * kLongThreads * N) {
+    Part<N> at[kLongVecs];
 #pragma unroll
     for (int u = 0; u < kLongVecs; ++u) {
-      const int64_t at = i + (int64_t)u * kLongThreads * N;
-      load(u, at, part_of<N>(D - at));
+      at[u].set(D, i + (int64_t)u * kLongThreads * N, true);
+      load(u, at[u]);
     }
 #pragma unroll
-    for (int u = 0; u < kLongVecs; ++u) {
-      const int64_t at = i + (int64_t)u * kLongThreads * N;
-      const int left = part_of<N>(D - at);
-      if (left) use(u, at, left);
-    }
+    for (int u = 0; u < kLongVecs; ++u)
+      if (at[u].own) use(u, at[u]);
   }
 }
 
@@ -314,29 +339,28 @@ __global__ __launch_bounds__(kLongThreads) void k_layer_norm_long(const T* __res
   const T* xs = x + (row * ldx + c0);
   T* ys = y + (row * width + c0);
   Held<T> h[kLongVecs];
-  const auto load = [&](int u, int64_t at, int left) { h[u].load(xs + at, left); };
+  const auto load = [&](int u, const Part<N>& at) { h[u].load(xs, at, true); };
   float v[N], s = 0.0f, q = 0.0f;
-  sweep<N>(D, load, [&](int u, int64_t, int) {
+  sweep<N>(D, load, [&](int u, const Part<N>& at) {
     h[u].get(v);
 #pragma unroll
-    for (int i = 0; i < N; ++i) s += v[i];
+    for (int i = 0; i < N; ++i) s += at.owns(i, true) ? v[i] : 0.0f;
   });
   const float mean = block_add<kLongThreads / 64>(s, lds) / (float)D;
-  sweep<N>(D, load, [&](int u, int64_t, int left) {
+  sweep<N>(D, load, [&](int u, const Part<N>& at) {
     h[u].get(v);
 #pragma unroll
-    for (int i = 0; i < N; ++i) q += i < left ? (v[i] - mean) * (v[i] - mean) : 0.0f;
+    for (int i = 0; i < N; ++i) q += at.owns(i, true) ? (v[i] - mean) * (v[i] - mean) : 0.0f;
   });
   const float rstd = rsqrt_of(block_add<kLongThreads / 64>(q, lds) / (float)D + eps), shift = -mean * rstd;
-  sweep<N>(D, load, [&](int u, int64_t at, int left) {
+  sweep<N>(D, load, [&](int u, const Part<N>& at) {
     float w[N], b[N];
-    load_params(p.w, p.w16, c0 + at, left, 1.0f, w);
-    load_params(p.b, p.b16, c0 + at, left, 0.0f, b);
+    load_params(p.w, p.w16, c0 + at.off, N, 1.0f, w);
+    load_params(p.b, p.b16, c0 + at.off, N, 0.0f, b);
     h[u].get(v);
 #pragma unroll
     for (int i = 0; i < N; ++i) v[i] = normed<T>(v[i], mean, rstd, shift) * w[i] + b[i];
-    if (left == N) store_vec(ys + at, v);
-    else store_some(ys + at, left, v);
+    store_vec(ys + at.off, v);
   });
   if (stats && threadIdx.x == 0) {
     stats[2 * (int64_t)blockIdx.x] = mean;
@@ -364,8 +388,8 @@ template <typename T> struct SourceOf<T, true> { typedef Stored type; };
 template <typename T, bool STORED> struct HeldSource;
 template <typename T> struct HeldSource<T, false> {
   Held<T, true> x;
-  __device__ __forceinline__ void load(const Source<T>& s, int64_t row, int64_t c, uint32_t lane_at, int left) {
-    x.load(s.x + (row * s.ldx + c) + lane_at, left);
+  __device__ __forceinline__ void load(const Source<T>& s, int64_t row, int64_t c, const Part<kN<T>>& at, bool whole) {
+    x.load(s.x + (row * s.ldx + c), at, whole);
   }
   __device__ __forceinline__ void normed_values(float mean, float rstd, float shift, float (&v)[kN<T>]) const {
     x.get(v);
@@ -378,13 +402,13 @@ template <typename T> struct HeldSource<T, true> {
   W w;
   uint32_t e;
   float G;
-  __device__ __forceinline__ void load(const Stored& s, int64_t row, int64_t c, uint32_t lane_at, int left) {
+  __device__ __forceinline__ void load(const Stored& s, int64_t row, int64_t c, const Part<kN<T>>& at, bool) {
     w = W{};
     e = 0;
     G = 0.0f;
-    if (left) {     // blocks are a multiple of a vector: it lies in one
-      const int64_t from = row * s.width + c, n = (from + lane_at) >> s.blk_log2;
-      w = __builtin_nontemporal_load(reinterpret_cast<const W*>(s.x8 + from + lane_at));
+    if (at.own) {   // segments and blocks are multiples of a vector: it lies in one
+      const int64_t from = row * s.width + c, n = (from + at.off) >> s.blk_log2;
+      w = __builtin_nontemporal_load(reinterpret_cast<const W*>(s.x8 + from + at.off));
       e = s.sc8[n];
       G = s.sc32[n >> s.K_log2];
     }
@@ -415,14 +439,14 @@ __global__ __launch_bounds__(G::TB) void k_layer_norm_bwd(typename SourceOf<T, S
   __shared__ float sums[G::TEAMS > 1 ? SUMS * (G::TB / 2) : 1];
   const Place<G> me(groups);
   const int64_t D = width / groups, c0 = me.g * D;
-  const uint32_t lane_at = me.template lane_at<N>();
+  const bool whole = G::P > 8 || D >= N;
   const float per_D = 1.0f / (float)D;
-  int left[NV];
+  Part<N> at[NV];
   float w[NV][N], aw[NV][N], ab[NV][N];
 #pragma unroll
   for (int j = 0; j < NV; ++j) {
-    left[j] = me.live ? part_of<N>(D - me.template at<N>(j)) : 0;
-    load_params(p.w, p.w16, c0 + me.template at<N>(j), left[j], 1.0f, w[j]);
+    at[j].set(me.live ? D : 0, me.template at<N>(j), whole);
+    load_params(p.w, p.w16, c0 + at[j].off, at[j].n(whole), 1.0f, w[j]);
 #pragma unroll
     for (int i = 0; i < N; ++i) aw[j][i] = ab[j][i] = 0.0f;
   }
@@ -439,9 +463,10 @@ __global__ __launch_bounds__(G::TB) void k_layer_norm_bwd(typename SourceOf<T, S
     const bool on = me.live && r < rows;
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
-      const int64_t c = c0 + me.template wave_at<N>(j);
-      to.x[j].load(src, r, c, lane_at, on ? left[j] : 0);
-      to.g[j].load(dy + (r * ldy + c) + lane_at, on ? left[j] : 0);
+      Part<N> a = at[j];
+      if (!on) a.own = 0;
+      to.x[j].load(src, r, c0, a, whole);
+      to.g[j].load(dy + (r * ldy + c0), a, whole);
     }
     to.mean = on ? stats[2 * (r * groups + me.g)] : 0.0f;
     to.rstd = on ? stats[2 * (r * groups + me.g) + 1] : 0.0f;
@@ -468,9 +493,21 @@ __global__ __launch_bounds__(G::TB) void k_layer_norm_bwd(typename SourceOf<T, S
       for (int i = 0; i < N; ++i) {
         aw[j][i] += g[i] * h[i];
         ab[j][i] += g[i];
-        const float a = g[i] * w[j][i];
-        s1 += a;
-        s2 += a * h[i];
+      }
+      if (at[j].own == N) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+          const float a = g[i] * w[j][i];
+          s1 += a;
+          s2 += a * h[i];
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+          const float a = at[j].owns(i, whole) ? g[i] * w[j][i] : 0.0f;
+          s1 += a;
+          s2 += a * h[i];
+        }
       }
     }
     if (dx) {
@@ -494,9 +531,9 @@ __global__ __launch_bounds__(G::TB) void k_layer_norm_bwd(typename SourceOf<T, S
           cur.g[j].get(g);
 #pragma unroll
           for (int i = 0; i < N; ++i) g[i] = (g[i] * w[j][i]) * rstd - m1 - h[i] * m2;
-          T* to = dx + (row * width + c0 + me.template wave_at<N>(j)) + lane_at;
-          if (left[j] == N) store_vec(to, g);
-          else if (left[j]) store_some(to, left[j], g);
+          T* to = dx + (row * width + c0) + at[j].off;
+          if (at[j].n(whole) == N) store_vec(to, g);
+          else if (at[j].own) store_some(to, at[j].own, g);
         }
       }
     }
@@ -534,10 +571,10 @@ __global__ __launch_bounds__(G::TB) void k_layer_norm_bwd(typename SourceOf<T, S
   if (!me.live || me.rl) return;
 #pragma unroll
   for (int j = 0; j < NV; ++j) {
-    const int64_t c = c0 + me.template at<N>(j);
+    const int64_t c = c0 + at[j].off;
     if (gridDim.x > 1) {
       float* to = part + 2 * (int64_t)blockIdx.x * width + c;
-      if (left[j] == N) {
+      if (at[j].own == N) {
 #pragma unroll
         for (int i = 0; i < N; i += 4) {
           *reinterpret_cast<u32x4_a4*>(to + i) =
@@ -546,13 +583,17 @@ __global__ __launch_bounds__(G::TB) void k_layer_norm_bwd(typename SourceOf<T, S
               u32x4_t{f2u(ab[j][i]), f2u(ab[j][i + 1]), f2u(ab[j][i + 2]), f2u(ab[j][i + 3])};
         }
       } else {
-        store_some(to, left[j], aw[j]);
-        store_some(to + width, left[j], ab[j]);
+#pragma unroll
+        for (int i = 0; i < N; ++i)
+          if (at[j].owns(i, whole)) {
+            to[i] = aw[j][i];
+            to[width + i] = ab[j][i];
+          }
       }
     } else {
 #pragma unroll
       for (int i = 0; i < N; ++i)
-        if (i < left[j]) {
+        if (at[j].owns(i, whole)) {
           if (dw) store_param(dw, dw16, c + i, aw[j][i]);
           if (db) store_param(db, db16, c + i, ab[j][i]);
         }
@@ -575,31 +616,31 @@ __global__ __launch_bounds__(kLongThreads) void k_layer_norm_long_dx(typename So
   T* out = dx + (row * width + c0);
   HeldSource<T, STORED> hx[kLongVecs];
   Held<T> hg[kLongVecs];
-  const auto load = [&](int u, int64_t at, int left) {
-    hx[u].load(src, row, c0, (uint32_t)at, left);
-    hg[u].load(gs + at, left);
+  const auto load = [&](int u, const Part<N>& at) {
+    hx[u].load(src, row, c0, at, true);
+    hg[u].load(gs, at, true);
   };
   float h[N], g[N], w[N], s1 = 0.0f, s2 = 0.0f;
-  sweep<N>(D, load, [&](int u, int64_t at, int left) {
-    load_params(p.w, p.w16, c0 + at, left, 1.0f, w);
+  sweep<N>(D, load, [&](int u, const Part<N>& at) {
+    load_params(p.w, p.w16, c0 + at.off, N, 1.0f, w);
     hx[u].normed_values(mean, rstd, shift, h);
     hg[u].get(g);
 #pragma unroll
     for (int i = 0; i < N; ++i) {
-      s1 += g[i] * w[i];
-      s2 += g[i] * w[i] * h[i];
+      const float a = at.owns(i, true) ? g[i] * w[i] : 0.0f;
+      s1 += a;
+      s2 += a * h[i];
     }
   });
   const float m1 = rstd * (block_add<kLongThreads / 64>(s1, lds) / (float)D);
   const float m2 = rstd * (block_add<kLongThreads / 64>(s2, lds) / (float)D);
-  sweep<N>(D, load, [&](int u, int64_t at, int left) {
-    load_params(p.w, p.w16, c0 + at, left, 1.0f, w);
+  sweep<N>(D, load, [&](int u, const Part<N>& at) {
+    load_params(p.w, p.w16, c0 + at.off, N, 1.0f, w);
     hx[u].normed_values(mean, rstd, shift, h);
     hg[u].get(g);
 #pragma unroll
     for (int i = 0; i < N; ++i) g[i] = (g[i] * w[i]) * rstd - m1 - h[i] * m2;
-    if (left == N) store_vec(out + at, g);
-    else store_some(out + at, left, g);
+    store_vec(out + at.off, g);
   });
 }
 
@@ -613,16 +654,16 @@ __global__ __launch_bounds__(256) void k_layer_norm_long_dp(typename SourceOf<T,
                                                             float* __restrict__ part) {
   constexpr int N = kN<T>;
   const int64_t D = width / groups, g0 = blockIdx.x / (unsigned)tiles, c0 = g0 * D;
-  const int64_t at = ((blockIdx.x - g0 * tiles) * 256 + threadIdx.x) * N;
-  const int left = part_of<N>(D - at);
-  if (!left) return;
+  Part<N> at;
+  at.set(D, ((blockIdx.x - g0 * tiles) * 256 + threadIdx.x) * N, true);
+  if (!at.own) return;
   float dw[N] = {}, db[N] = {}, h[N], g[N];
 #pragma unroll 4
   for (int64_t row = blockIdx.y; row < rows; row += gridDim.y) {
     HeldSource<T, STORED> hx;
     Held<T> hg;
-    hx.load(src, row, c0, (uint32_t)at, left);
-    hg.load(dy + (row * ldy + c0) + at, left);
+    hx.load(src, row, c0, at, true);
+    hg.load(dy + (row * ldy + c0), at, true);
     const float mean = stats[2 * (row * groups + g0)], rstd = stats[2 * (row * groups + g0) + 1];
     hx.normed_values(mean, rstd, -mean * rstd, h);
     hg.get(g);
@@ -632,9 +673,13 @@ __global__ __launch_bounds__(256) void k_layer_norm_long_dp(typename SourceOf<T,
       db[i] += g[i];
     }
   }
-  float* to = part + 2 * (int64_t)blockIdx.y * width + c0 + at;
-  store_some(to, left, dw);
-  store_some(to + width, left, db);
+  float* to = part + 2 * (int64_t)blockIdx.y * width + c0 + at.off;
+#pragma unroll
+  for (int i = 0; i < N; ++i)
+    if (at.owns(i, true)) {
+      to[i] = dw[i];
+      to[width + i] = db[i];
+    }
 }
 
 // dw and db from the slices' sums: kJoinCols columns per workgroup, its waves on
