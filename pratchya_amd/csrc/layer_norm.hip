@@ -57,6 +57,7 @@ template <int P_, int NV_, int TB_>
 struct Shape {
   static constexpr int P = P_, NV = NV_, TB = TB_, TEAMS = TB_ / P_, WAVES = P_ > 64 ? P_ / 64 : 1;
   static constexpr int LANES = P_ < 64 ? P_ : 64;
+  static constexpr int JOIN = WAVES <= 2 ? WAVES : WAVES <= 4 ? 4 : WAVES <= 8 ? 8 : 16;    // lanes that join them
 };
 
 // A thread's place.  What all lanes of a wave share (all but the lane's offset,
@@ -520,8 +521,9 @@ __global__ __launch_bounds__(G::TB) void k_layer_norm_bwd(typename SourceOf<T, S
           r[me.t >> 6][1] = s2;
         }
         __syncthreads();
-        s1 = lane_group_add<G::WAVES>(r[me.t % G::WAVES][0]);
-        s2 = lane_group_add<G::WAVES>(r[me.t % G::WAVES][1]);
+        const int wave = me.t % G::JOIN;
+        s1 = lane_group_add<G::JOIN>(wave < G::WAVES ? r[wave][0] : 0.0f);
+        s2 = lane_group_add<G::JOIN>(wave < G::WAVES ? r[wave][1] : 0.0f);
       }
       const float m1 = rstd * (s1 * per_D), m2 = rstd * (s2 * per_D);
       if (me.live && row < rows) {
@@ -737,10 +739,18 @@ int check_shape(const char* what, int64_t rows, int64_t width, int64_t groups) {
 // rows on their way.
 constexpr int kFwdThreads = 512, kFwdAhead = 1, kBwdThreads = 1024, kBwdAhead = 1;
 constexpr int64_t kFwdBlocks = 512, kBwdBlocks = 256;
+// The backward pass's workgroups of 12 waves: two a compute unit from this many rows
+// a team on (2048 x 5120, 4 rows: 23.7 -> 25.2 us; 8 rows 35.1 -> 33.9; 16 rows 58.2 -> 52.3)
+constexpr int kBwdThin = 768;
+constexpr int64_t kThinRows = 8;
 
 // Call f(Shape) with the smallest team that holds a segment of D elements: in the
 // forward pass of 16 elements a thread where a wave is full, in the backward pass,
-// where an element takes five registers more for its sums and weight, of 8.
+// where an element takes five registers more for its sums and weight, of 8.  bf16's
+// backward pass also has teams of 3, 6 and 12 waves in workgroups of 12 waves, two a
+// compute unit: [8192, 5120] 59.3 -> 52.3 us, [16384, 1280] 35.4 -> 31.8.  f32's, of
+// more registers, does not fit twice and loses 5% (97.5 -> 102.6 us), and the
+// forward pass, of two vectors a thread, gains nothing by them (29.6 -> 28.6, 40.7 -> 42.0).
 template <typename T, typename F>
 auto with_fwd_shape(int64_t D, F f) {
   constexpr int TB = kFwdThreads, V = 8 / kN<T>;      // vectors of 8 elements
@@ -762,6 +772,11 @@ auto with_bwd_shape(int64_t D, F f) {
   if (D <= 256) return f(Shape<32, V, TB>());
   if (D <= 512) return f(Shape<64, V, TB>());
   if (D <= 1024) return f(Shape<128, V, TB>());
+  if constexpr (sizeof(T) == 2) {
+    if (D > 1024 && D <= 192 * 8) return f(Shape<192, V, kBwdThin>());
+    if (D > 2048 && D <= 384 * 8) return f(Shape<384, V, kBwdThin>());
+    if (D > 4096 && D <= 768 * 8) return f(Shape<768, V, kBwdThin>());
+  }
   if (D <= 2048) return f(Shape<256, V, TB>());
   if (D <= 4096) return f(Shape<512, V, TB>());
   if (D <= 8192) return f(Shape<1024, V, TB>());
@@ -782,13 +797,15 @@ constexpr int64_t kOneBlockRounds = 4;      // 64 x 512 bf16 11.3 -> 9.7 us; 8 r
 template <typename G>
 dim3 bwd_grid_of(int64_t rows, int64_t groups) {
   const int64_t rt = G::TEAMS / (groups < G::TEAMS ? groups : G::TEAMS);
-  return grid_of<G>(rows, groups, rows <= kOneBlockRounds * rt ? 1 : kBwdBlocks);
+  int64_t most = kBwdBlocks;
+  if (rows <= kOneBlockRounds * rt) most = 1;
+  else if (G::TB == kBwdThin && rows >= kThinRows * 2 * kBwdBlocks * rt) most = 2 * kBwdBlocks;
+  return grid_of<G>(rows, groups, most);
 }
 
+template <typename T>
 dim3 bwd_grid(int64_t rows, int64_t width, int64_t groups) {
-  return with_bwd_shape<float>(width / groups, [&](auto shape) {      // the teams are the same for both types
-    return bwd_grid_of<decltype(shape)>(rows, groups);
-  });
+  return with_bwd_shape<T>(width / groups, [&](auto shape) { return bwd_grid_of<decltype(shape)>(rows, groups); });
 }
 
 template <typename T, typename G>
@@ -888,7 +905,12 @@ extern "C" int pratchya_layer_norm(const void* x, int64_t ldx, int dtype, const 
 
 extern "C" int64_t pratchya_layer_norm_bwd_workspace_bytes(int64_t rows, int64_t width, int64_t groups) {
   if (rows < 1 || width < 1 || groups < 1 || width % groups) return 0;
-  const int64_t slices = width / groups > kLongest ? (rows < kSlices ? rows : kSlices) : bwd_grid(rows, width, groups).x;
+  int64_t slices = rows < kSlices ? rows : kSlices;
+  if (width / groups <= kLongest) {      // the larger of the two types' grids
+    const int64_t s = bwd_grid<float>(rows, width, groups).x;
+    slices = bwd_grid<uint16_t>(rows, width, groups).x;
+    if (s > slices) slices = s;
+  }
   return slices * 2 * width * (int64_t)sizeof(float);
 }
 

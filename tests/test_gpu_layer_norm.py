@@ -353,3 +353,44 @@ def test_refusals():
     q = K.quantize(x.detach(), (1, 32))
     with pytest.raises(ValueError, match="stored"):
         K.layer_norm_bwd(q, torch.zeros((2, 192), device="cuda"), None, torch.zeros((2, 2), device="cuda"), 1, (1, 32))
+
+
+@pytest.mark.parametrize("dt", ["bf16", "f32"])
+@pytest.mark.parametrize("rows,width,groups", [
+    (70, 1025, 1), (33, 1536, 1), (21, 1537, 1), (40, 2048, 1), (19, 2049, 1), (9, 4097, 1), (30, 5120, 1),
+    (5, 6144, 1), (7, 6151, 1), (37, 3300, 3), (11, 5002, 2), (6, 8190, 6), (13, 9, 1), (13, 15, 1), (50, 30, 2)])
+def test_teams(rows, width, groups, dt):
+    """Segments around the sizes at which teams grow, and ones that end inside a vector."""
+    x, w, b, dy = _inputs(rows, width, dt, rows * 11 + width, w=torch.bfloat16)
+    _check(x, w, b, dy, groups, what=f"{rows}x{width}/{groups}")
+
+
+@pytest.mark.parametrize("rows,width,groups,blk", [(4100, 4097, 1, 0), (8200, 2050, 1, 0), (16390, 1029, 1, 0),
+                                                   (8193, 2058, 2, 0), (4097, 4160, 1, 32)])
+def test_many_rows(rows, width, groups, blk):
+    """Rows enough for the backward pass's largest grids."""
+    x, w, b, dy = _inputs(rows, width, "bf16", rows + width)
+    _check(x, w, b, dy, groups, blk, what=f"{rows}x{width}/{groups}")
+
+
+def test_an_odd_end_and_its_neighbours():
+    """The vector moved back to a segment's end reads and writes nothing outside the segment: what lies
+    around it is NaN going in and untouched coming out, and infinities stay in their segment."""
+    for dt in (torch.bfloat16, torch.float32):
+        for D in (9, 13, 65, 67, 1027, 4097, 16391):
+            gen = torch.Generator().manual_seed(D)
+            big = torch.full((6, 3 * D), float("nan"), dtype=dt)
+            big[1:5, D:2 * D] = torch.randn((4, D), generator=gen).to(dt)
+            x, dy = big.cuda()[1:5, D:2 * D], torch.randn((4, D), generator=gen).to(dt)
+            y = _F().layer_norm(x)
+            want, bound = R.layer_norm(x.cpu(), None, None, EPS, 1)
+            R.close(y, want[0], bound[0], f"{dt} {D}")
+            x = x.detach().requires_grad_(True)
+            (dx,) = torch.autograd.grad(_F().layer_norm(x), x, dy.cuda())
+            want, bound = R.layer_norm(x.detach().cpu(), None, None, EPS, 1, dy)
+            R.close(dx, want[1], bound[1], f"{dt} {D}")
+            three = torch.randn((4, 3 * D), generator=gen).to(dt)
+            three[2, D - 1] = float("inf")
+            y3 = _F().layer_norm(three.cuda(), groups=3).float().cpu()
+            assert torch.isfinite(y3[2, D:]).all() and torch.isfinite(y3[[0, 1, 3]]).all()
+            assert not torch.isfinite(y3[2, :D]).any()
