@@ -172,8 +172,8 @@ __device__ __forceinline__ float normed(float x, float mean, float rstd, float s
 // (groups = 1).  Mean and squared deviations are taken within each wave, from
 // registers, and joined by counts, so a mean far from zero costs no digits.
 // Bound by HBM, with some 20 vector instructions an element beside it: [16384,
-// 4096] bf16 49 us (268 MB, 5.4 TB/s), with its 8-bit form 64 us (335 MB, 5.2
-// TB/s), heads of 64 over [8192, 4096] 23 us (5.8 TB/s); one row of 4096 4 us.
+// 4096] bf16 49 us (268 MB, 5.4 TB/s), with its 8-bit form 63 us (335 MB, 5.3
+// TB/s), heads of 64 over [8192, 4096] 22 us (6.0 TB/s); one row of 4096 4 us.
 template <typename T, typename G, int BLK, int AHEAD>
 __global__ __launch_bounds__(G::TB) void k_layer_norm(const T* __restrict__ x, int64_t ldx, Affine p, int64_t rows,
                                                       int64_t width, int64_t groups, float eps, T* __restrict__ y,
@@ -310,7 +310,8 @@ __global__ __launch_bounds__(G::TB) void k_layer_norm(const T* __restrict__ x, i
 // Segments of more than kLongest elements, which a workgroup's registers do not
 // hold: a workgroup a segment, kLongVecs vectors a thread in flight, three passes
 // over the row of which the later two come from the L2 cache.  [2048, 32768] bf16
-// 88 us, its backward pass 180 us (3.0 and 2.2 TB/s of what goes through HBM once).
+// 85 us, its backward pass 179 us (3.2 and 2.2 TB/s of what goes through HBM once);
+// of 32769, on no address of 16 bytes, 111 and 225 us.
 constexpr int kLongThreads = 1024, kLongVecs = 4;
 
 // Calls use(u, part) for this thread's vectors of a segment, after load has been
@@ -426,8 +427,8 @@ template <typename T> struct HeldSource<T, true> {
 // has walked: joined over the workgroup's row lanes and written to
 // part[blockIdx.x][0 / 1][width], or as the results where there is one workgroup
 // per column.  Bound by HBM; the partial sums, 2 kB a column over 256 workgroups,
-// are 5% of it: with the join [16384, 4096] bf16 79 us (402 MB, 5.1 TB/s), from the
-// 8-bit form 71 us (335 MB), heads of 64 over [8192, 4096] 41 us (201 MB).
+// are 5% of it: with the join [16384, 4096] bf16 78 us (402 MB, 5.2 TB/s), from the
+// 8-bit form 72 us (335 MB), heads of 64 over [8192, 4096] 41 us (201 MB).
 template <typename T, typename G, bool STORED, int AHEAD>
 __global__ __launch_bounds__(G::TB) void k_layer_norm_bwd(typename SourceOf<T, STORED>::type src,
                                                           const T* __restrict__ dy, int64_t ldy, Affine p,
