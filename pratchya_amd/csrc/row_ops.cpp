@@ -461,6 +461,15 @@ bool wants_grad(const Tensor& t) { return t.requires_grad(); }
 bool wants_grad(const MaybeTensor& t) { return t && t->requires_grad(); }
 Tensor or_none(const MaybeTensor& t) { return t ? *t : Tensor(); }
 
+// The nodes hold reverse-mode gradients only.  An input with a forward-mode tangent
+// would give an output without one, whose derivative counts as 0.
+void refuse_tangent(const Tensor& t, const char* what) {
+  TORCH_CHECK_NOT_IMPLEMENTED(!t._fw_grad(0).defined(), what, ": no forward-mode derivative; the input has a tangent");
+}
+void refuse_tangent(const MaybeTensor& t, const char* what) {
+  if (t) refuse_tangent(*t, what);
+}
+
 template <typename N>
 std::shared_ptr<N> new_node() {
   return std::shared_ptr<N>(new N(), torch::autograd::deleteNode);
@@ -468,6 +477,9 @@ std::shared_ptr<N> new_node() {
 
 Tensor layer_norm(const Tensor& x, const MaybeTensor& weight, const MaybeTensor& bias, double eps, int64_t groups,
                   Grid grid) {
+  refuse_tangent(x, "layer_norm");
+  refuse_tangent(weight, "layer_norm: weight");
+  refuse_tangent(bias, "layer_norm: bias");
   const bool grad = at::GradMode::is_enabled() && (wants_grad(x) || wants_grad(weight) || wants_grad(bias));
   if (!grad) return layer_norm_fwd(x, weight, bias, eps, groups, false, {}).y;
   Normed r;
@@ -489,6 +501,7 @@ Tensor layer_norm(const Tensor& x, const MaybeTensor& weight, const MaybeTensor&
 }
 
 Tensor activation(const Tensor& x, int kind, const Grid& grid) {
+  refuse_tangent(x, "activation");
   if (!(at::GradMode::is_enabled() && wants_grad(x))) return activation_fwd(x, kind, {}).y;
   Activated r;
   {
@@ -504,6 +517,7 @@ Tensor activation(const Tensor& x, int kind, const Grid& grid) {
 }
 
 Scored token_logprobs(const Tensor& logits, const Tensor& tokens, bool entropy, int64_t top) {
+  refuse_tangent(logits, "token_logprobs");
   const bool grad = at::GradMode::is_enabled() && wants_grad(logits);
   Scored r;
   {

@@ -15,7 +15,9 @@ to the backward pass, as the quantized Linear holds its own input.
     loss = -functional.token_logprobs(logits, tokens).logprobs.mean()
 
 Arrays are bf16 or f32 on the GPU; rows may be a stride apart (slices of a wider
-array).  Arithmetic is f32, with one rounding to a result's type.
+array).  Arithmetic is f32, with one rounding to a result's type.  Gradients are
+reverse-mode and of first order: inputs with a forward-mode tangent are refused, and
+so is the gradient of a gradient.
 """
 from __future__ import annotations
 
