@@ -160,17 +160,21 @@ __device__ __forceinline__ float rsqrt_of(float v) {
   return r * (1.5f - 0.5f * v * r * r);
 }
 
-// (x - mean) r.  For bf16 in one operation with shift = -mean r: the product's and
-// shift's roundings are 2^-24 of |x| r, far below bf16's step of x itself.
-template <typename T>
-__device__ __forceinline__ float normed(float x, float mean, float rstd, float shift) {
-  if constexpr (sizeof(T) == 2) return __builtin_fmaf(x, rstd, shift);
-  else return (x - mean) * rstd;
-}
+// Squared deviations q from a mean that was off, about the corrected one: less its
+// square, `by` times the deviations' sum.  Not below 0; NaN stays.
+__device__ __forceinline__ float without(float q, float less) { return q - less < 0.0f ? 0.0f : q - less; }
+
+// (x - mean) r, the difference first: x r - mean r in one operation would leave the
+// roundings of mean r in a segment of equal values, r = 1 / sqrt(eps) there (0.4 for
+// 29952 where 0 is right).
+__device__ __forceinline__ float normed(float x, float mean, float rstd) { return (x - mean) * rstd; }
 
 // y and the statistics of whole segments; with BLK, x's stored form beside them
 // (groups = 1).  Mean and squared deviations are taken within each wave, from
-// registers, and joined by counts, so a mean far from zero costs no digits.
+// registers, and joined by counts, so a mean far from zero costs no digits.  The mean
+// of equal values is that value: up to 2^16 bf16 values' sum is exact and the
+// quotient's rounding the only one; f32's mean is corrected by the mean of the
+// deviations from it, and waves are joined by their distance from the first.
 // Bound by HBM, with some 20 vector instructions an element beside it: [16384,
 // 4096] bf16 49 us (268 MB, 5.4 TB/s), with its 8-bit form 63 us (335 MB, 5.3
 // TB/s), heads of 64 over [8192, 4096] 22 us (6.0 TB/s); one row of 4096 4 us.
@@ -194,7 +198,7 @@ __global__ __launch_bounds__(G::TB) void k_layer_norm(const T* __restrict__ x, i
   }
   // elements of the segment in this wave, and its share of the segment
   const int64_t held = D - me.template wave_at<N>(0);
-  const float mine = (float)(held < 0 ? 0 : held < SPAN ? held : SPAN), per_mine = mine > 0.0f ? 1.0f / mine : 0.0f;
+  const float mine = (float)(held < 0 ? 0 : held < SPAN ? held : SPAN), count = mine > 0.0f ? mine : 1.0f;
   const float per_D = 1.0f / (float)D;
   const int64_t step = (int64_t)gridDim.x * me.rt;
   int64_t row = (int64_t)blockIdx.x * me.rt + me.rl;
@@ -235,26 +239,38 @@ __global__ __launch_bounds__(G::TB) void k_layer_norm(const T* __restrict__ x, i
       }
     }
     s = lane_group_add<LANES>(s);
-    float mean = s * per_mine;
+    constexpr bool EXACT = sizeof(T) == 2;      // the sum of equal values
+    float mean = s / count, rest = 0.0f;
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
       cur[j].get(v);
-      if (at[j].own == N) {
 #pragma unroll
-        for (int i = 0; i < N; ++i) q += (v[i] - mean) * (v[i] - mean);
-      } else {
+      for (int i = 0; i < N; ++i) v[i] -= mean;
+      if (at[j].own != N) {
 #pragma unroll
-        for (int i = 0; i < N; ++i) q += at[j].owns(i, whole) ? (v[i] - mean) * (v[i] - mean) : 0.0f;
+        for (int i = 0; i < N; ++i) v[i] = at[j].owns(i, whole) ? v[i] : 0.0f;
+      }
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        q += v[i] * v[i];
+        if constexpr (!EXACT) rest += v[i];
       }
     }
     q = lane_group_add<LANES>(q);
+    if constexpr (!EXACT) {
+      rest = lane_group_add<LANES>(rest);
+      const float by = rest / count;      // equal deviations: exact, and so is what q loses
+      mean += by;
+      q = without(q, by * rest);
+    }
     if constexpr (G::WAVES > 1) {
       float4* r = &red[buf][me.team * G::WAVES];
       if ((me.t & 63) == 0) r[me.t >> 6] = make_float4(mean, q, mine * per_D, 0.0f);
       __syncthreads();
       // a wave's numbers per lane, all waves' in every group of lanes
       const float4 k = r[me.t % G::WAVES];
-      mean = lane_group_add<G::WAVES>(k.z * k.x);
+      const float first = r[0].x;
+      mean = first + lane_group_add<G::WAVES>(k.z * (k.x - first));
       const float d = k.x - mean;
       q = lane_group_add<G::WAVES>(k.y + (k.z * (float)D) * d * d);
     }
@@ -265,12 +281,11 @@ __global__ __launch_bounds__(G::TB) void k_layer_norm(const T* __restrict__ x, i
       stats[2 * (row * groups + me.g) + 1] = rstd;
     }
     T* yr = y + (row * width + c0);
-    const float shift = -mean * rstd;
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
       cur[j].get(v);
 #pragma unroll
-      for (int i = 0; i < N; ++i) v[i] = normed<T>(v[i], mean, rstd, shift) * w[j][i] + b[j][i];
+      for (int i = 0; i < N; ++i) v[i] = normed(v[i], mean, rstd) * w[j][i] + b[j][i];
       if (at[j].n(whole) == N) store_vec<true>(yr + at[j].off, v);
       else if (at[j].own) store_some(yr + at[j].off, at[j].own, v);
     }
@@ -348,20 +363,28 @@ __global__ __launch_bounds__(kLongThreads) void k_layer_norm_long(const T* __res
 #pragma unroll
     for (int i = 0; i < N; ++i) s += at.owns(i, true) ? v[i] : 0.0f;
   });
-  const float mean = block_add<kLongThreads / 64>(s, lds) / (float)D;
+  float mean = block_add<kLongThreads / 64>(s, lds) / (float)D, rest = 0.0f;
   sweep<N>(D, load, [&](int u, const Part<N>& at) {
     h[u].get(v);
 #pragma unroll
-    for (int i = 0; i < N; ++i) q += at.owns(i, true) ? (v[i] - mean) * (v[i] - mean) : 0.0f;
+    for (int i = 0; i < N; ++i) {
+      const float d = at.owns(i, true) ? v[i] - mean : 0.0f;
+      q += d * d;
+      rest += d;
+    }
   });
-  const float rstd = rsqrt_of(block_add<kLongThreads / 64>(q, lds) / (float)D + eps), shift = -mean * rstd;
+  q = block_add<kLongThreads / 64>(q, lds);
+  rest = block_add<kLongThreads / 64>(rest, lds);
+  const float by = rest / (float)D;       // of a mean of so many values a step or two may be missing
+  mean += by;
+  const float rstd = rsqrt_of(without(q, by * rest) / (float)D + eps);
   sweep<N>(D, load, [&](int u, const Part<N>& at) {
     float w[N], b[N];
     load_params(p.w, p.w16, c0 + at.off, N, 1.0f, w);
     load_params(p.b, p.b16, c0 + at.off, N, 0.0f, b);
     h[u].get(v);
 #pragma unroll
-    for (int i = 0; i < N; ++i) v[i] = normed<T>(v[i], mean, rstd, shift) * w[i] + b[i];
+    for (int i = 0; i < N; ++i) v[i] = normed(v[i], mean, rstd) * w[i] + b[i];
     store_vec(ys + at.off, v);
   });
   if (stats && threadIdx.x == 0) {
@@ -393,10 +416,10 @@ template <typename T> struct HeldSource<T, false> {
   __device__ __forceinline__ void load(const Source<T>& s, int64_t row, int64_t c, const Part<kN<T>>& at, bool whole) {
     x.load(s.x + (row * s.ldx + c), at, whole);
   }
-  __device__ __forceinline__ void normed_values(float mean, float rstd, float shift, float (&v)[kN<T>]) const {
+  __device__ __forceinline__ void normed_values(float mean, float rstd, float (&v)[kN<T>]) const {
     x.get(v);
 #pragma unroll
-    for (int i = 0; i < kN<T>; ++i) v[i] = normed<T>(v[i], mean, rstd, shift);
+    for (int i = 0; i < kN<T>; ++i) v[i] = normed(v[i], mean, rstd);
   }
 };
 template <typename T> struct HeldSource<T, true> {
@@ -415,11 +438,11 @@ template <typename T> struct HeldSource<T, true> {
       G = s.sc32[n >> s.K_log2];
     }
   }
-  __device__ __forceinline__ void normed_values(float, float rstd, float shift, float (&v)[kN<T>]) const {
+  __device__ __forceinline__ void normed_values(float mean, float rstd, float (&v)[kN<T>]) const {
     payload_values(w, v);
-    const float s = stored_scale(e, G) * rstd;
+    const float s = stored_scale(e, G);
 #pragma unroll
-    for (int i = 0; i < kN<T>; ++i) v[i] = __builtin_fmaf(v[i], s, shift);
+    for (int i = 0; i < kN<T>; ++i) v[i] = __builtin_fmaf(v[i], s, -mean) * rstd;
   }
 };
 
@@ -485,11 +508,11 @@ __global__ __launch_bounds__(G::TB) void k_layer_norm_bwd(typename SourceOf<T, S
     } else {
       fetch(row, cur);
     }
-    const float mean = cur.mean, rstd = cur.rstd, shift = -mean * rstd;
+    const float mean = cur.mean, rstd = cur.rstd;
     float s1 = 0.0f, s2 = 0.0f, h[N], g[N];
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
-      cur.x[j].normed_values(mean, rstd, shift, h);
+      cur.x[j].normed_values(mean, rstd, h);
       cur.g[j].get(g);
 #pragma unroll
       for (int i = 0; i < N; ++i) {
@@ -503,7 +526,7 @@ __global__ __launch_bounds__(G::TB) void k_layer_norm_bwd(typename SourceOf<T, S
           s1 += a;
           s2 += a * h[i];
         }
-      } else {
+      } else if (!STORED) {      // a stored segment has whole vectors or none
 #pragma unroll
         for (int i = 0; i < N; ++i) {
           const float a = at[j].owns(i, whole) ? g[i] * w[j][i] : 0.0f;
@@ -530,7 +553,7 @@ __global__ __launch_bounds__(G::TB) void k_layer_norm_bwd(typename SourceOf<T, S
       if (me.live && row < rows) {
 #pragma unroll
         for (int j = 0; j < NV; ++j) {
-          cur.x[j].normed_values(mean, rstd, shift, h);
+          cur.x[j].normed_values(mean, rstd, h);
           cur.g[j].get(g);
 #pragma unroll
           for (int i = 0; i < N; ++i) g[i] = (g[i] * w[j][i]) * rstd - m1 - h[i] * m2;
@@ -614,7 +637,7 @@ __global__ __launch_bounds__(kLongThreads) void k_layer_norm_long_dx(typename So
   constexpr int N = kN<T>;
   __shared__ float lds[kLongThreads / 64];
   const int64_t D = width / groups, row = blockIdx.x / (unsigned)groups, c0 = (blockIdx.x - row * groups) * D;
-  const float mean = stats[2 * (int64_t)blockIdx.x], rstd = stats[2 * (int64_t)blockIdx.x + 1], shift = -mean * rstd;
+  const float mean = stats[2 * (int64_t)blockIdx.x], rstd = stats[2 * (int64_t)blockIdx.x + 1];
   const T* gs = dy + (row * ldy + c0);
   T* out = dx + (row * width + c0);
   HeldSource<T, STORED> hx[kLongVecs];
@@ -626,7 +649,7 @@ __global__ __launch_bounds__(kLongThreads) void k_layer_norm_long_dx(typename So
   float h[N], g[N], w[N], s1 = 0.0f, s2 = 0.0f;
   sweep<N>(D, load, [&](int u, const Part<N>& at) {
     load_params(p.w, p.w16, c0 + at.off, N, 1.0f, w);
-    hx[u].normed_values(mean, rstd, shift, h);
+    hx[u].normed_values(mean, rstd, h);
     hg[u].get(g);
 #pragma unroll
     for (int i = 0; i < N; ++i) {
@@ -639,7 +662,7 @@ __global__ __launch_bounds__(kLongThreads) void k_layer_norm_long_dx(typename So
   const float m2 = rstd * (block_add<kLongThreads / 64>(s2, lds) / (float)D);
   sweep<N>(D, load, [&](int u, const Part<N>& at) {
     load_params(p.w, p.w16, c0 + at.off, N, 1.0f, w);
-    hx[u].normed_values(mean, rstd, shift, h);
+    hx[u].normed_values(mean, rstd, h);
     hg[u].get(g);
 #pragma unroll
     for (int i = 0; i < N; ++i) g[i] = (g[i] * w[i]) * rstd - m1 - h[i] * m2;
@@ -668,7 +691,7 @@ __global__ __launch_bounds__(256) void k_layer_norm_long_dp(typename SourceOf<T,
     hx.load(src, row, c0, at, true);
     hg.load(dy + (row * ldy + c0), at, true);
     const float mean = stats[2 * (row * groups + g0)], rstd = stats[2 * (row * groups + g0) + 1];
-    hx.normed_values(mean, rstd, -mean * rstd, h);
+    hx.normed_values(mean, rstd, h);
     hg.get(g);
 #pragma unroll
     for (int i = 0; i < N; ++i) {
