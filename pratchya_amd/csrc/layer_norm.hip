@@ -160,9 +160,12 @@ __device__ __forceinline__ float rsqrt_of(float v) {
   return r * (1.5f - 0.5f * v * r * r);
 }
 
-// Squared deviations q from a mean that was off, about the corrected one: less its
-// square, `by` times the deviations' sum.  Not below 0; NaN stays.
-__device__ __forceinline__ float without(float q, float less) { return q - less < 0.0f ? 0.0f : q - less; }
+// Squared deviations q from a mean that was off, about the corrected one: less the
+// correction times the deviations' sum.  Not below 0; infinite sums (values whose
+// squares overflow) and NaN stay.
+__device__ __forceinline__ float without(float q, float less) {
+  return less < q ? q - less : q <= 3.4028234663852886e38f ? 0.0f : q;
+}
 
 // (x - mean) r, the difference first: x r - mean r in one operation would leave the
 // roundings of mean r in a segment of equal values, r = 1 / sqrt(eps) there (0.4 for

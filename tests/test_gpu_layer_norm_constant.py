@@ -51,3 +51,19 @@ def test_equal_values(rows, width, groups, dt):
     (4, 34816, 1, 128), (10, 2048, 16, 128), (10, 768, 12, 32)])
 def test_equal_values_in_8_bits(rows, width, groups, blk, dt):
     _run(rows, width, groups, blk, dt)
+
+
+@pytest.mark.parametrize("dt", ["bf16", "f32"])
+@pytest.mark.parametrize("width,groups", [(96, 1), (1000, 1), (4096, 1), (2057, 1), (512, 8), (20000, 1)])
+def test_squares_that_overflow(width, groups, dt):
+    """Values whose squared deviations are infinite in 32 bits: 1 / sqrt(inf) = 0, the result is the bias and x has
+    no gradient, as the same formula gives it in plain 32-bit operations."""
+    from pratchya_amd import functional as F
+    gen = torch.Generator().manual_seed(width)
+    x = (torch.randn((4, width), generator=gen) * 1e30 + 1e29).to(DT[dt])
+    w, b = torch.randn(width, generator=gen), torch.randn(width, generator=gen)
+    args = [t.cuda().requires_grad_(True) for t in (x, w, b)]
+    y = F.layer_norm(*args, groups=groups)
+    assert torch.equal(y.cpu(), b.to(DT[dt]).expand(4, width))
+    dx, dw, db = torch.autograd.grad(y, args, torch.randn((4, width), generator=gen).to(DT[dt]).cuda())
+    assert not bool(dx.any()) and not bool(dw.any()) and bool(torch.isfinite(db).all())
