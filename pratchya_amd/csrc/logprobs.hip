@@ -49,11 +49,11 @@ __device__ __forceinline__ uint64_t shfl_xor_u64(uint64_t v, int m) {
   return (uint64_t)__shfl_xor((unsigned long long)v, m, 64);
 }
 
-// A thread's running sums over the logits it has seen, relative to m: s = sum
-// 2^((x - m) log2 e), t = sum of the same times (x - m) log2 e.  m follows the
-// largest logit within kSlack only: a larger step of the sums is rare, and
-// e^kSlack times a row's length is far from f32's range.
-constexpr float kSlack = 8.0f;
+// A thread's running sums over the logits it has seen, relative to the largest, m:
+// s = sum 2^((x - m) log2 e), t = sum of the same times (x - m) log2 e.  m moves
+// before a larger logit is added, once for several vectors, so the largest one's term
+// is 1 and a row's sum 1 or more: no log probability comes out above 0, no entropy
+// below, and near 0 they keep a sum's digits.
 template <bool ENTROPY>
 struct Running {
   float m = kLowest, s = 0.0f, t = 0.0f;
@@ -65,20 +65,27 @@ struct Running {
     s *= f;
     m = to;
   }
+  // NaN is passed over here; its term makes the sum NaN
   template <int N>
-  __device__ __forceinline__ void add(const float (&v)[N]) {
-    float c = v[0];
+  __device__ __forceinline__ void raise(const float (&v)[N], float& c) const {
 #pragma unroll
-    for (int i = 1; i < N; ++i) c = fmaxf(c, v[i]);
-    if (__any(c > m + kSlack)) {
-      if (c > m) move(c);
-    }
+    for (int i = 0; i < N; ++i) c = fmaxf(c, v[i]);
+  }
+  template <int N>
+  __device__ __forceinline__ void sum(const float (&v)[N]) {
 #pragma unroll
     for (int i = 0; i < N; ++i) {
       const float d = (v[i] - m) * kLog2e, e = __builtin_amdgcn_exp2f(d);
       s += e;
       if constexpr (ENTROPY) t += e * fmaxf(d, kLowest);   // 0, not NaN, for a masked logit
     }
+  }
+  template <int N>
+  __device__ __forceinline__ void add(const float (&v)[N]) {
+    float c = m;
+    raise(v, c);
+    if (c > m) move(c);
+    sum(v);
   }
 };
 
@@ -164,11 +171,17 @@ __global__ __launch_bounds__(WPR < 4 ? 256 : WPR * 64) void k_logprobs(
     u32x4_t raw[U];
 #pragma unroll
     for (int u = 0; u < U; ++u) raw[u] = load_raw<NT>(xr + (i + u * THREADS) * N);
+    float v[N], c = r.m;
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      float v[N];
       widen(raw[u], v);
-      r.add(v);
+      r.raise(v, c);
+    }
+    if (c > r.m) r.move(c);
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      widen(raw[u], v);
+      r.sum(v);
     }
   }
   for (; i < vecs; i += THREADS) {
@@ -344,9 +357,14 @@ __global__ __launch_bounds__(kPartThreads, 7) void k_logprobs_part(const T* __re
       if (at + N <= to) widen(load_raw(xr + at), v[u]);
       else load_some(xr + at, to - at, -__builtin_inff(), v[u]);
     }
+    // what lies beyond the part reads as masked
+    float c = r.m;
+#pragma unroll
+    for (int u = 0; u < VECS; ++u) r.raise(v[u], c);
+    if (c > r.m) r.move(c);
 #pragma unroll
     for (int u = 0; u < VECS; ++u)
-      if (base + (u * kPartThreads + tid) * N < to) r.add(v[u]);
+      if (base + (u * kPartThreads + tid) * N < to) r.sum(v[u]);
     uint64_t keys[kKeys];
 #pragma unroll
     for (int u = 0; u < VECS; ++u) {
