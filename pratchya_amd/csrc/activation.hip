@@ -39,10 +39,35 @@ bool is_float_dtype(int d) { return d == PRATCHYA_DT_F32 || d == PRATCHYA_DT_BF1
 
 constexpr float kLog2e = 1.4426950408889634f;
 
-// P(x) and p(x) of the normal distribution: with z = |x| / sqrt 2 and t = 1 / (1 +
-// 0.3275911 z), erfc(z) = (a1 t + ... + a5 t^5) e^(-z^2) to 1.5e-7 (Abramowitz and
-// Stegun, Handbook of Mathematical Functions, 7.1.26); p shares the exponential.
+// P(x) and p(x) of the normal distribution, which share e^(-x^2 / 2).  For a result in
+// bf16: with z = |x| / sqrt 2 and t = 1 / (1 + 0.3275911 z), erfc(z) = (a1 t + ... + a5
+// t^5) e^(-z^2) to 1.5e-7 (Abramowitz and Stegun, Handbook of Mathematical Functions,
+// 7.1.26).  For one in f32, where that is up to 5 times what the roundings of
+// x (1 + erf(z)) / 2 leave: P(-|x|) = e^(-x^2 / 2) t Q(t), t = 1 / (1 + 0.35 |x|), with Q
+// of degree 8, to 3.2e-8 of itself for |x| up to 14, and for |x| < 1 P = 1/2 + x R(x^2),
+// R of degree 5, to 3e-10; Q and R are fitted to the functions' values (least squares,
+// weights raised where the error is largest).  The library's erfc in place of both was
+// as exact, and a quarter to a third slower in the passes with an 8-bit input ([8192,
+// 8192] 131 and 129 us where these take 105 and 99, the shorter form 105 and 98).
+template <bool F32>
 __device__ __forceinline__ void normal(float x, float& P, float& p) {
+  if constexpr (F32) {
+    const float a = fabsf(x), sq = x * x;
+    const float t = __builtin_amdgcn_rcpf(__builtin_fmaf(0.35f, a, 1.0f));
+    const float e = __builtin_amdgcn_exp2f(sq * (-0.5f * kLog2e));
+    const float Q[] = {0.1396214f, 0.13986185f, 0.119833045f, 0.105507225f, -0.02310781f, 0.15917094f,
+                       -0.2557112f, 0.14397009f, -0.029145574f};
+    const float R[] = {0.3989423f, -0.06649036f, 0.009973331f, -0.001186353f, 1.13512666e-04f, -7.664675e-06f};
+    float c = Q[8], r = R[5];
+#pragma unroll
+    for (int i = 7; i >= 0; --i) c = __builtin_fmaf(c, t, Q[i]);
+#pragma unroll
+    for (int i = 4; i >= 0; --i) r = __builtin_fmaf(r, sq, R[i]);
+    const float tail = (c * t) * e;
+    P = a < 1.0f ? __builtin_fmaf(x, r, 0.5f) : x < 0.0f ? tail : 1.0f - tail;
+    p = 0.39894228040143268f * e;
+    return;
+  }
   const float z = fabsf(x) * 0.70710678118654752f;
   const float t = __builtin_amdgcn_rcpf(__builtin_fmaf(0.3275911f, z, 1.0f));
   const float e = __builtin_amdgcn_exp2f(-z * z * kLog2e);
@@ -74,7 +99,7 @@ __device__ __forceinline__ void act(float (&v)[N], int kind) {
 #pragma unroll
     for (int i = 0; i < N; ++i) {
       float P, p;
-      normal(v[i], P, p);
+      normal<N == 4>(v[i], P, p);
       v[i] *= P;
     }
   }
@@ -96,7 +121,7 @@ __device__ __forceinline__ void act_grad(const float (&v)[N], float (&g)[N], int
 #pragma unroll
     for (int i = 0; i < N; ++i) {
       float P, p;
-      normal(v[i], P, p);
+      normal<N == 4>(v[i], P, p);
       g[i] *= P + v[i] * p;
     }
   }
