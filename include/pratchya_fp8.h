@@ -719,8 +719,9 @@ int pratchya_activation_bwd(const void* x, int64_t ldx, int x_dtype, const uint8
  * the `top` (0 to 64, at most vocab) largest logits' log probabilities and
  * indices [rows, top], in falling order, equal logits by index, NaN above all
  * numbers.  A token below 0 stands for none (log probability 0); one of vocab or
- * more gives NaN.  Logits of -inf are masked; a row of nothing else has log
- * probabilities of -inf and entropy 0.  Alternatives may need a workspace of
+ * more gives NaN, and in the backward pass the gradient of the sum alone (-p g).
+ * Logits of -inf are masked; a row of nothing else has log probabilities of -inf
+ * and entropy 0.  Alternatives may need a workspace of
  * pratchya_token_logprobs_workspace_bytes, 8-byte aligned.  stats hold the
  * entropy only if entropy is not null. */
 int64_t pratchya_token_logprobs_workspace_bytes(int64_t rows, int64_t vocab, int top);

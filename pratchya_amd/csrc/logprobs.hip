@@ -7,7 +7,8 @@
 // A logit of -inf is masked: p = 0, and it adds nothing to H or dx.  A row that is
 // masked everywhere holds no distribution: its log probabilities are -inf, H and
 // every p in dx are 0.  A negative token stands for no token: log probability 0,
-// without a gradient; a token beyond the vocabulary gives NaN.
+// without a gradient; a token beyond the vocabulary gives NaN (x_token is a NaN that
+// no logit holds, so dx is the formula's without its first term, and 0 for g = 0).
 // Alternatives are ranked by their logit (NaN above all numbers), equal ones by
 // index; ranking keys hold both in 64 bits, so no two are equal.
 #include <hip/hip_runtime.h>

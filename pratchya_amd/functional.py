@@ -68,7 +68,9 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, entropy: bool = F
     differentiable in the logits, the alternatives are not.
 
     A negative token stands for none: its log probability is 0 and has no
-    gradient.  A token of V or more gives NaN.  Logits of -inf are masked; a row of
+    gradient.  A token of V or more gives NaN, as no logit stands for it; its gradient
+    is that of the sum alone, -p times the cotangent, so a position that the loss leaves
+    out (``nansum``, ``where``, ``clamp``) has none.  Logits of -inf are masked; a row of
     nothing else has log probabilities of -inf and entropy 0, and in its gradient,
     as for any masked logit, the probability 0."""
     return TokenLogprobs(*_ops.token_logprobs(logits, tokens, entropy, top))
