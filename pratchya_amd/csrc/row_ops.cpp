@@ -22,6 +22,7 @@
 #include <torch/csrc/utils/pybind.h>
 
 #include <array>
+#include <mutex>
 #include <numeric>
 #include <optional>
 
@@ -380,6 +381,8 @@ variable_list once(variable_list&& grads, const char* what) {
   return (*error)(std::move(grads));
 }
 
+// A node's saved arrays are read and given up under its mutex: backward passes of
+// several threads may share a graph, and run without the interpreter's lock.
 struct KeptNode : torch::autograd::Node {
   SavedVariable x_, sc8_, sc32_;
   int64_t blk_ = 0;
@@ -402,6 +405,12 @@ struct KeptNode : torch::autograd::Node {
     return k;
   }
   void release_variables() override {
+    const std::lock_guard<std::mutex> lock(mutex_);
+    release();
+  }
+
+ protected:
+  virtual void release() {
     x_.reset_data();
     sc8_.reset_data();
     sc32_.reset_data();
@@ -416,17 +425,26 @@ struct PratchyaLayerNormBackward : KeptNode {
   variable_list apply(variable_list&& grads) override {
     variable_list out(3);
     if (!grads[0].defined()) return out;
+    Kept x;
     MaybeTensor weight;
-    if (has_weight_) weight = weight_.unpack();
-    auto got = layer_norm_bwd(kept(), grads[0], weight, stats_.unpack(), groups_,
+    Tensor stats;
+    {
+      const std::lock_guard<std::mutex> lock(mutex_);
+      x = kept();
+      if (has_weight_) weight = weight_.unpack();
+      stats = stats_.unpack();
+    }
+    auto got = layer_norm_bwd(x, grads[0], weight, stats, groups_,
                               {task_should_compute_output(0), task_should_compute_output(1),
                                task_should_compute_output(2)},
                               bias_type_);
     for (int i = 0; i < 3; ++i) out[i] = std::move(got[i]);
     return once(std::move(out), "layer_norm");
   }
-  void release_variables() override {
-    KeptNode::release_variables();
+
+ protected:
+  void release() override {
+    KeptNode::release();
     weight_.reset_data();
     stats_.reset_data();
   }
@@ -436,8 +454,14 @@ struct PratchyaActivationBackward : KeptNode {
   int kind_ = 0;
   variable_list apply(variable_list&& grads) override {
     variable_list out(1);
-    if (grads[0].defined()) out[0] = activation_bwd(kept(), grads[0], kind_);
-    return grads[0].defined() ? once(std::move(out), "activation") : out;
+    if (!grads[0].defined()) return out;
+    Kept x;
+    {
+      const std::lock_guard<std::mutex> lock(mutex_);
+      x = kept();
+    }
+    out[0] = activation_bwd(x, grads[0], kind_);
+    return once(std::move(out), "activation");
   }
 };
 
@@ -447,10 +471,18 @@ struct PratchyaTokenLogprobsBackward : torch::autograd::Node {
     variable_list out(1);
     const Tensor g = grads[0], gh = grads.size() > 1 ? grads[1] : Tensor();
     if (!g.defined() && !gh.defined()) return out;
-    out[0] = token_logprobs_bwd(logits_.unpack(), tokens_.unpack(), stats_.unpack(), g, gh);
+    Tensor logits, tokens, stats;
+    {
+      const std::lock_guard<std::mutex> lock(mutex_);
+      logits = logits_.unpack();
+      tokens = tokens_.unpack();
+      stats = stats_.unpack();
+    }
+    out[0] = token_logprobs_bwd(logits, tokens, stats, g, gh);
     return once(std::move(out), "token_logprobs");
   }
   void release_variables() override {
+    const std::lock_guard<std::mutex> lock(mutex_);
     logits_.reset_data();
     tokens_.reset_data();
     stats_.reset_data();
