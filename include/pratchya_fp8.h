@@ -662,6 +662,12 @@ int pratchya_debug_f32_to_bf16(const float* in, uint16_t* out, int64_t n, int mo
                                hipStream_t stream);
 
 /* ---- row operators around the quantized linears ------------------------ */
+/* A call is one launch or two, and a launch holds fewer than 2^32 threads and 65535
+ * workgroups along its second axis.  Larger calls are PRATCHYA_EUNSUPPORTED: log
+ * probabilities of 2^26 rows (2^24 of more than 2048 logits, 2^24 parts of up to
+ * 4096 logits with alternatives, 2^24 pieces of 4096 in the gradient), activations
+ * of 2^36 elements, norms of 2^22 segments of more than 16384 elements, gradients
+ * of 2^28 columns of such, and rows of some 2^20 segments of 256 elements or more. */
 
 /* Layer norm over segments of a row: `rows` rows of `width` elements (dtype f32
  * or bf16, `ldx` elements apart) hold `groups` segments of D = width / groups

@@ -15,6 +15,7 @@
 
 #include "pratchya_fp8.h"
 #include "row_device.h"
+#include "row_host.h"
 
 int pratchya_set_error(int code, const char* fmt, ...);
 
@@ -319,8 +320,8 @@ int launch(const void* x, int64_t ldx, int kind, int64_t rows, int64_t width, vo
   bool one;
   const Rows r = make_rows<T>(ldx, width, rows, width, one);
   const int K = x8 ? (int)gcd64(blk / 16, rows * width / blk) : 1;
-  if (workgroups<T>(r) > 0x7FFFFFFF)
-    return pratchya_set_error(PRATCHYA_EUNSUPPORTED, "activation: more than 2^31 workgroups");
+  if (!fits_launch(workgroups<T>(r), kThreads))
+    return pratchya_set_error(PRATCHYA_EUNSUPPORTED, "activation: more elements than a launch has threads for (2^36)");
 #define PRATCHYA_ACT(B)                                                                                              \
   if (one)                                                                                                           \
     hipLaunchKernelGGL((k_act<T, B, true>), dim3((unsigned)workgroups<T>(r)), dim3(kThreads), 0, stream,                \
@@ -342,8 +343,8 @@ int launch_bwd(const void* x, int64_t ldx, const StoredX& s, const void* dy, int
                int64_t width, void* dx, hipStream_t stream) {
   bool one;
   const Rows r = make_rows<T>(STORED ? width : ldx, ldy, rows, width, one);
-  if (workgroups<T>(r) > 0x7FFFFFFF)
-    return pratchya_set_error(PRATCHYA_EUNSUPPORTED, "activation_bwd: more than 2^31 workgroups");
+  if (!fits_launch(workgroups<T>(r), kThreads))
+    return pratchya_set_error(PRATCHYA_EUNSUPPORTED, "activation_bwd: more elements than a launch has threads for (2^36)");
   const dim3 grid((unsigned)workgroups<T>(r));
   const T* xt = STORED ? nullptr : static_cast<const T*>(x);
   if (one)

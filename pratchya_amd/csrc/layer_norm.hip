@@ -15,6 +15,7 @@
 
 #include "pratchya_fp8.h"
 #include "row_device.h"
+#include "row_host.h"
 
 int pratchya_set_error(int code, const char* fmt, ...);
 
@@ -835,10 +836,15 @@ dim3 bwd_grid(int64_t rows, int64_t width, int64_t groups) {
   return with_bwd_shape<T>(width / groups, [&](auto shape) { return bwd_grid_of<decltype(shape)>(rows, groups); });
 }
 
+int too_many(const char* what) {
+  return pratchya_set_error(PRATCHYA_EUNSUPPORTED, "%s: more segments or columns than a launch has workgroups for", what);
+}
+
 template <typename T, typename G>
-void launch_fwd(G, const T* x, int64_t ldx, const Affine& p, int64_t rows, int64_t width, int64_t groups, float eps,
+int launch_fwd(G, const T* x, int64_t ldx, const Affine& p, int64_t rows, int64_t width, int64_t groups, float eps,
                 T* y, float* stats, uint8_t* x8, uint8_t* sc8, float* sc32, int64_t blk, hipStream_t stream) {
   const dim3 grid = grid_of<G>(rows, groups, kFwdBlocks * kFwdThreads / G::TB);
+  if (!fits_launch(grid.x, G::TB, grid.y)) return too_many("layer_norm");
 #define PRATCHYA_LN(B)                                                                                              \
   hipLaunchKernelGGL((k_layer_norm<T, G, B, kFwdAhead>), grid, dim3(G::TB), 0, stream, x, ldx, p, rows, width, groups, eps, y, \
                      stats, x8, sc8, sc32)
@@ -848,6 +854,7 @@ void launch_fwd(G, const T* x, int64_t ldx, const Affine& p, int64_t rows, int64
   else if (blk == 64) { if constexpr (G::P >= 32) PRATCHYA_LN(64); }
   else { if constexpr (G::P >= 64 && G::NV * kN<T> >= 16) PRATCHYA_LN(128); }
 #undef PRATCHYA_LN
+  return check_launch("layer_norm");
 }
 
 template <typename T>
@@ -855,13 +862,13 @@ int layer_norm(const void* x, int64_t ldx, const Affine& p, int64_t rows, int64_
                void* y, float* stats, uint8_t* x8, uint8_t* sc8, float* sc32, int64_t blk, hipStream_t stream) {
   const T* xt = static_cast<const T*>(x);
   T* yt = static_cast<T*>(y);
-  if (width / groups > kLongest)
-    hipLaunchKernelGGL((k_layer_norm_long<T>), dim3((unsigned)(rows * groups)), dim3(kLongThreads), 0, stream, xt, ldx,
-                       p, width, groups, eps, yt, stats);
-  else
-    with_fwd_shape<T>(width / groups, [&](auto shape) {
-      launch_fwd<T>(shape, xt, ldx, p, rows, width, groups, eps, yt, stats, x8, sc8, sc32, blk, stream);
+  if (width / groups <= kLongest)
+    return with_fwd_shape<T>(width / groups, [&](auto shape) {
+      return launch_fwd<T>(shape, xt, ldx, p, rows, width, groups, eps, yt, stats, x8, sc8, sc32, blk, stream);
     });
+  if (!fits_launch(rows * groups, kLongThreads)) return too_many("layer_norm");
+  hipLaunchKernelGGL((k_layer_norm_long<T>), dim3((unsigned)(rows * groups)), dim3(kLongThreads), 0, stream, xt, ldx, p,
+                     width, groups, eps, yt, stats);
   return check_launch("layer_norm");
 }
 
@@ -873,7 +880,11 @@ int layer_norm_bwd(typename SourceOf<T, STORED>::type src, const void* dy, int64
   const Affine p = {w, nullptr, w_dtype == PRATCHYA_DT_BF16, false};
   const bool dw16 = dw_dtype == PRATCHYA_DT_BF16, db16 = db_dtype == PRATCHYA_DT_BF16;
   int slices = 1;
+  const int64_t joins = (width + kJoinCols - 1) / kJoinCols;
   if (width / groups > kLongest) {
+    // both limits before the first launch; the other form joins rows of 2^22 columns at most
+    if ((dx && !fits_launch(rows * groups, kLongThreads)) || ((dw || db) && !fits_launch(joins, kJoinThreads)))
+      return too_many("layer_norm_bwd");
     if (dx)
       hipLaunchKernelGGL((k_layer_norm_long_dx<T, STORED>), dim3((unsigned)(rows * groups)), dim3(kLongThreads), 0,
                          stream, src, g, ldy, p, width, groups, stats, static_cast<T*>(dx));
@@ -884,20 +895,23 @@ int layer_norm_bwd(typename SourceOf<T, STORED>::type src, const void* dy, int64
                          dim3(256), 0, stream, src, g, ldy, rows, width, groups, tiles, stats, part);
     }
   } else {
-    with_bwd_shape<T>(width / groups, [&](auto shape) {
+    const bool fits = with_bwd_shape<T>(width / groups, [&](auto shape) {
       typedef decltype(shape) G;
       // 16 elements a thread leave none of the 128 registers for a row ahead
       constexpr int AHEAD = G::NV * kN<T> == 8 ? kBwdAhead : 0;
       const dim3 grid = bwd_grid_of<G>(rows, groups);
+      if (!fits_launch(grid.x, G::TB, grid.y)) return false;
       slices = (int)grid.x;
       hipLaunchKernelGGL((k_layer_norm_bwd<T, G, STORED, AHEAD>), grid, dim3(G::TB), 0, stream, src, g, ldy, p, rows,
                          width, groups, stats, static_cast<T*>(dx), part, dw, dw16, db, db16);
+      return true;
     });
+    if (!fits) return too_many("layer_norm_bwd");
     if (slices == 1) return check_launch("layer_norm_bwd");
   }
   if (dw || db)
-    hipLaunchKernelGGL(k_layer_norm_join, dim3((unsigned)((width + kJoinCols - 1) / kJoinCols)), dim3(kJoinThreads), 0,
-                       stream, part, slices, width, dw, dw16, db, db16);
+    hipLaunchKernelGGL(k_layer_norm_join, dim3((unsigned)joins), dim3(kJoinThreads), 0, stream, part, slices,
+                       width, dw, dw16, db, db16);
   return check_launch("layer_norm_bwd");
 }
 

@@ -16,6 +16,7 @@
 
 #include "pratchya_fp8.h"
 #include "row_device.h"
+#include "row_host.h"
 
 int pratchya_set_error(int code, const char* fmt, ...);
 
@@ -512,6 +513,9 @@ int check_args(const char* what, int dtype, int64_t rows, int64_t vocab) {
   return PRATCHYA_OK;
 }
 
+// Logits of a row that one wave takes, four rows a workgroup.
+constexpr int64_t kOneWave = 2048;
+
 // Accesses past the caches.  Forward, for logits that the last-level cache (256 MB)
 // cannot hold: 8192 x 65536 bf16 188 -> 167 us, but 1000 x 50021 f32, 200 MB, 37.6 ->
 // 40.2 us.  Backward, for more than the L2 caches hold: a gradient left in the
@@ -537,8 +541,8 @@ int launch(const void* logits, int64_t ld, const int64_t* tokens, int64_t rows, 
   const T* x = static_cast<const T*>(logits);
   if (top) {
     const Cut cut = cut_row(vocab);
-    if (rows * cut.parts > 0x7FFFFFFF)
-      return pratchya_set_error(PRATCHYA_EUNSUPPORTED, "token_logprobs: more than 2^31 parts of rows");
+    if (!fits_launch(rows * cut.parts, kPartThreads))
+      return pratchya_set_error(PRATCHYA_EUNSUPPORTED, "token_logprobs: more parts of rows than a launch has threads for (2^24)");
     uint64_t* kept = static_cast<uint64_t*>(workspace);
     float* sums = reinterpret_cast<float*>(static_cast<char*>(workspace) + keys_bytes(rows, cut.parts, top));
     hipLaunchKernelGGL((k_logprobs_part<T, ENTROPY>), dim3((unsigned)(rows * cut.parts)), dim3(kPartThreads), 0, stream,
@@ -548,13 +552,17 @@ int launch(const void* logits, int64_t ld, const int64_t* tokens, int64_t rows, 
                          tokens, vocab, top, cut.parts, sums, kept, o);
     return check_launch("token_logprobs");
   }
+  const int rows_per = vocab <= kOneWave ? 4 : 1;
+  const int64_t groups = (rows + rows_per - 1) / rows_per;
+  if (!fits_launch(groups, 256))
+    return pratchya_set_error(PRATCHYA_EUNSUPPORTED, "token_logprobs: more rows than a launch has threads for (2^%d)",
+                              rows_per == 4 ? 26 : 24);
 #define PRATCHYA_LP(WPR, NT)                                                                                          \
-  hipLaunchKernelGGL((k_logprobs<T, WPR, ENTROPY, NT>),                                                               \
-                     dim3((unsigned)((rows + (WPR < 4 ? 4 / WPR : 1) - 1) / (WPR < 4 ? 4 / WPR : 1))),                \
+  hipLaunchKernelGGL((k_logprobs<T, WPR, ENTROPY, NT>), dim3((unsigned)groups),                                       \
                      dim3(WPR < 4 ? 256 : WPR * 64), 0, stream, x, ld, tokens, rows, vocab, o.logprobs, o.entropy,    \
                      o.stats)
   const bool nt = rows * vocab > kFwdStream / (int64_t)sizeof(T);
-  if (vocab <= 2048) PRATCHYA_LP(1, false);
+  if (vocab <= kOneWave) PRATCHYA_LP(1, false);
   else if (rows < 512) PRATCHYA_LP(16, false);
   else if (nt) PRATCHYA_LP(4, true);
   else PRATCHYA_LP(4, false);
@@ -569,8 +577,8 @@ int launch_bwd(const void* logits, int64_t ld, const int64_t* tokens, const floa
   const int tpr = vocab <= 64 * per ? 64 : 256;
   const int64_t pieces = (vocab + tpr * per - 1) / (tpr * per);
   const int64_t blocks = (rows * pieces + 256 / tpr - 1) / (256 / tpr);
-  if (blocks > 0x7FFFFFFF)
-    return pratchya_set_error(PRATCHYA_EUNSUPPORTED, "token_logprobs_bwd: more than 2^31 workgroups");
+  if (!fits_launch(blocks, 256))
+    return pratchya_set_error(PRATCHYA_EUNSUPPORTED, "token_logprobs_bwd: more pieces of rows than a launch has threads for (2^24)");
 #define PRATCHYA_LPB(TPR, NT)                                                                                         \
   hipLaunchKernelGGL((k_logprobs_bwd<T, TPR, NT>), dim3((unsigned)blocks), dim3(256), 0, stream,                      \
                      static_cast<const T*>(logits), ld, tokens, stats, g, gh, rows, vocab, (unsigned)pieces,          \
