@@ -3,12 +3,15 @@ compiled binding of the row operators, ``pratchya_amd/_row_ops.so``.
 
 The library is built in-tree with ``hipcc --offload-arch=gfx950`` so that it
 travels with the source tree to the GPU machine; the binding holds no GPU code and
-is built with the host compiler against torch's headers.  Usage::
+is built with the host compiler against torch's headers.  The library itself needs no
+torch: where none is installed (another host of its C ABI), only the library is built.
+Usage::
 
     python -m pratchya_amd.build          # or pratchya_amd.build.build()
 """
 from __future__ import annotations
 
+import importlib.util
 import os
 import subprocess
 import sys
@@ -62,7 +65,11 @@ def build(verbose: bool = False) -> Path:
     tmp = LIB.with_suffix(".so.tmp")
     _run([HIPCC, "--offload-arch=gfx950", "-shared", "-fPIC", *objs, "-o", str(tmp)])
     os.replace(tmp, LIB)
-    build_row_ops()
+    if importlib.util.find_spec("torch"):
+        build_row_ops()
+    else:
+        ROW_OPS.unlink(missing_ok=True)      # of an older library
+        print("no torch here: the Python binding of the row operators is not built", file=sys.stderr)
     return LIB
 
 
