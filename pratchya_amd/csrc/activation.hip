@@ -17,26 +17,7 @@
 #include "row_device.h"
 #include "row_host.h"
 
-int pratchya_set_error(int code, const char* fmt, ...);
-
 namespace {
-
-int64_t gcd64(int64_t x, int64_t y) {
-  while (y) {
-    const int64_t t = x % y;
-    x = y;
-    y = t;
-  }
-  return x;
-}
-
-int check_launch(const char* what) {
-  const hipError_t e = hipGetLastError();
-  if (e != hipSuccess) return pratchya_set_error(PRATCHYA_EHIP, "%s: launch failed: %s", what, hipGetErrorString(e));
-  return pratchya_set_error(PRATCHYA_OK, "");
-}
-
-bool is_float_dtype(int d) { return d == PRATCHYA_DT_F32 || d == PRATCHYA_DT_BF16; }
 
 constexpr float kLog2e = 1.4426950408889634f;
 
@@ -298,15 +279,6 @@ Rows make_rows(int64_t ldx, int64_t ldy, int64_t rows, int64_t width, bool& one)
   one = rows == 1 || (ldx == width && ldy == width);
   const int64_t w = one ? rows * width : width, per = (w + kN<T> - 1) / kN<T>;
   return {ldx, w, per, one ? per : rows * per};
-}
-
-int log2_of(int64_t v) {
-  int n = 0;
-  while (v > 1) {
-    v >>= 1;
-    ++n;
-  }
-  return n;
 }
 
 template <typename T>

@@ -17,26 +17,7 @@
 #include "row_device.h"
 #include "row_host.h"
 
-int pratchya_set_error(int code, const char* fmt, ...);
-
 namespace {
-
-int64_t gcd64(int64_t x, int64_t y) {
-  while (y) {
-    const int64_t t = x % y;
-    x = y;
-    y = t;
-  }
-  return x;
-}
-
-int check_launch(const char* what) {
-  const hipError_t e = hipGetLastError();
-  if (e != hipSuccess) return pratchya_set_error(PRATCHYA_EHIP, "%s: launch failed: %s", what, hipGetErrorString(e));
-  return pratchya_set_error(PRATCHYA_OK, "");
-}
-
-bool is_float_dtype(int d) { return d == PRATCHYA_DT_F32 || d == PRATCHYA_DT_BF16; }
 
 struct Affine {
   const void* w;
@@ -745,14 +726,6 @@ constexpr int64_t kLongest = 16384;     // elements of a segment held in registe
 constexpr int kSlices = 64;             // row slices of the long segments' column sums
 
 bool power_of_two(int64_t v) { return v > 0 && (v & (v - 1)) == 0; }
-int log2_of(int64_t v) {
-  int n = 0;
-  while (v > 1) {
-    v >>= 1;
-    ++n;
-  }
-  return n;
-}
 
 int check_shape(const char* what, int64_t rows, int64_t width, int64_t groups) {
   if (rows < 0 || width < 0 || groups < 1 || width % groups)

@@ -18,21 +18,11 @@
 #include "row_device.h"
 #include "row_host.h"
 
-int pratchya_set_error(int code, const char* fmt, ...);
-
 namespace {
 
 constexpr int kMaxTop = 64;
 constexpr float kLowest = -3.4028234663852886e38f;
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.69314718055994531f;
-
-int check_launch(const char* what) {
-  const hipError_t e = hipGetLastError();
-  if (e != hipSuccess) return pratchya_set_error(PRATCHYA_EHIP, "%s: launch failed: %s", what, hipGetErrorString(e));
-  return pratchya_set_error(PRATCHYA_OK, "");
-}
-
-bool is_float_dtype(int d) { return d == PRATCHYA_DT_F32 || d == PRATCHYA_DT_BF16; }
 
 // 32-bit rank of a logit: larger for larger values, equal for 0 and -0, the
 // largest for every NaN.

@@ -11,11 +11,7 @@ __device__ __forceinline__ float load_elem(const uint16_t* p) { return u2f((uint
 __device__ __forceinline__ void store_elem(float* p, float v) { *p = v; }
 __device__ __forceinline__ void store_elem(uint16_t* p, float v) { *p = (uint16_t)f32_to_bf16_rne(v); }
 
-// Element i of an array whose type is known at run time (parameters: [width]
-// vectors that stay in the caches).
-__device__ __forceinline__ float load_param(const void* p, bool bf16, int64_t i) {
-  return bf16 ? load_elem(static_cast<const uint16_t*>(p) + i) : static_cast<const float*>(p)[i];
-}
+// Element i of an array whose type is known at run time (a parameter's gradient, [width]).
 __device__ __forceinline__ void store_param(void* p, bool bf16, int64_t i, float v) {
   if (bf16) store_elem(static_cast<uint16_t*>(p) + i, v);
   else static_cast<float*>(p)[i] = v;
