@@ -6,10 +6,15 @@
 // The forward pass computes f from x itself; the backward pass is dx = f'(x) dy
 // with x read as it is or from its quantized form with block grid (1, blk)
 // (fp8_math.h).  Arithmetic in f32, one rounding to the result's type.
-// Both passes are bound by HBM and read and write past the caches.  [16384, 16384]
-// bf16, forward with the 8-bit form 216 us (1.35 GB, 6.2 TB/s), backward from it 209
-// us (6.4 TB/s); without it 170 and 259 us (6.3 and 6.2 TB/s).  gelu's 20 operations
-// an element show a little: [8192, 8192] 61 to 64 us each way (5.4 TB/s).
+// Both passes are bound by HBM and read and write past the caches.  With the
+// quantizer of the Linear behind it, that reads y at once, this against plain stores:
+// 2 MB of bf16 the same, 8 and 16 MB 10.9 -> 9.2 and 16.6 -> 13.0 us, 32 to 192 MB within
+// 6% either way, 256 MB 136 -> 149, 512 MB and 1 GB within 2%; f32 and the backward
+// pass alike.  One form is kept: only at 256 MB are plain stores clearly ahead.
+// [16384, 16384] bf16, forward with the 8-bit form 216 us (1.35 GB, 6.2 TB/s), backward
+// from it 209 us (6.4 TB/s); without it 170 and 259 us (6.3 and 6.2 TB/s).  gelu's 20
+// operations an element in bf16 show a little: [8192, 8192] 61 to 64 us each way (5.4
+// TB/s).
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 

@@ -30,11 +30,11 @@ struct Affine {
 // segment position of the row (its slice of w and b, and of dw and db) and walks
 // over rows: `gt` neighbouring segments side by side, the other teams on
 // further rows.  Thread t of a team holds vectors (t / L * NV + j) * L + t % L, L =
-// min(P, 64), j < NV: groups of stored blocks lie in one wave. Streaming accesses where
-// they measured faster: the forward pass's stores ([16384, 2048] bf16 27.0 -> 23.9
-// us), its loads of an x that is stored and so not read again (with its backward
-// pass [16384, 4096] 138 -> 134.5 us; of other x 25.2 -> 25.7 us where the caches
-// hold it), the backward pass's loads (84.3 -> 79.8 us).
+// min(P, 64), j < NV: groups of stored blocks lie in one wave.  Streaming accesses
+// where they measured faster: the forward pass's stores of results up to kFwdPast, its
+// loads of an x that is stored and so not read again (with its backward pass [16384,
+// 4096] 138 -> 134.5 us; of other x 25.2 -> 25.7 us where the caches hold it), the
+// backward pass's loads (84.3 -> 79.8 us).
 template <int P_, int NV_, int TB_>
 struct Shape {
   static constexpr int P = P_, NV = NV_, TB = TB_, TEAMS = TB_ / P_, WAVES = P_ > 64 ? P_ / 64 : 1;
@@ -163,7 +163,7 @@ __device__ __forceinline__ float normed(float x, float mean, float rstd) { retur
 // Bound by HBM, with some 20 vector instructions an element beside it: [16384,
 // 4096] bf16 49 us (268 MB, 5.4 TB/s), with its 8-bit form 63 us (335 MB, 5.3
 // TB/s), heads of 64 over [8192, 4096] 22 us (6.0 TB/s); one row of 4096 4 us.
-template <typename T, typename G, int BLK, int AHEAD>
+template <typename T, typename G, int BLK, int AHEAD, bool PAST>
 __global__ __launch_bounds__(G::TB) void k_layer_norm(const T* __restrict__ x, int64_t ldx, Affine p, int64_t rows,
                                                       int64_t width, int64_t groups, float eps, T* __restrict__ y,
                                                       float* __restrict__ stats, uint8_t* __restrict__ x8,
@@ -271,7 +271,7 @@ __global__ __launch_bounds__(G::TB) void k_layer_norm(const T* __restrict__ x, i
       cur[j].get(v);
 #pragma unroll
       for (int i = 0; i < N; ++i) v[i] = normed(v[i], mean, rstd) * w[j][i] + b[j][i];
-      if (at[j].n(whole) == N) store_vec<true>(yr + at[j].off, v);
+      if (at[j].n(whole) == N) store_vec<PAST>(yr + at[j].off, v);
       else if (at[j].own) store_some(yr + at[j].off, at[j].own, v);
     }
     if constexpr (BLK != 0) {
@@ -740,6 +740,12 @@ int check_shape(const char* what, int64_t rows, int64_t width, int64_t groups) {
 // rows on their way.
 constexpr int kFwdThreads = 512, kFwdAhead = 1, kBwdThreads = 1024, kBwdAhead = 1;
 constexpr int64_t kFwdBlocks = 512, kBwdBlocks = 256;
+// Bytes of y up to which the forward pass stores it past the caches.  With the
+// quantizer of the Linear behind it, that reads y at once (bf16, rows of 4096, with
+// the 8-bit form or without): 2 MB as fast, 8 and 16 MB 13.2 -> 12.1 and 18.6 -> 14.0 us
+// (14.4 -> 11.9, 21.7 -> 17.8), 32 and 64 MB within 3%; 96 to 256 MB 4 to 9% slower
+// (64.3 for 59.8, 83 for 76, 162 for 153 us), 512 MB 4%.  f32 the same.
+constexpr int64_t kFwdPast = (int64_t)64 << 20;
 // The backward pass's workgroups of 12 waves: two a compute unit from this many rows
 // a team on (2048 x 5120, 4 rows: 23.7 -> 25.2 us; 8 rows 35.1 -> 33.9; 16 rows 58.2 -> 52.3)
 constexpr int kBwdThin = 768;
@@ -818,15 +824,21 @@ int launch_fwd(G, const T* x, int64_t ldx, const Affine& p, int64_t rows, int64_
                 T* y, float* stats, uint8_t* x8, uint8_t* sc8, float* sc32, int64_t blk, hipStream_t stream) {
   const dim3 grid = grid_of<G>(rows, groups, kFwdBlocks * kFwdThreads / G::TB);
   if (!fits_launch(grid.x, G::TB, grid.y)) return too_many("layer_norm");
+#define PRATCHYA_LNP(B, PAST)                                                                                       \
+  hipLaunchKernelGGL((k_layer_norm<T, G, B, kFwdAhead, PAST>), grid, dim3(G::TB), 0, stream, x, ldx, p, rows, width,   \
+                     groups, eps, y, stats, x8, sc8, sc32)
 #define PRATCHYA_LN(B)                                                                                              \
-  hipLaunchKernelGGL((k_layer_norm<T, G, B, kFwdAhead>), grid, dim3(G::TB), 0, stream, x, ldx, p, rows, width, groups, eps, y, \
-                     stats, x8, sc8, sc32)
-  if (!x8) PRATCHYA_LN(0);
-  else if (blk == 16) PRATCHYA_LN(16);
-  else if (blk == 32) PRATCHYA_LN(32);
-  else if (blk == 64) { if constexpr (G::P >= 32) PRATCHYA_LN(64); }
-  else { if constexpr (G::P >= 64 && G::NV * kN<T> >= 16) PRATCHYA_LN(128); }
+  {                                                                                                                 \
+    if (rows * width * (int64_t)sizeof(T) <= kFwdPast) PRATCHYA_LNP(B, true);                                       \
+    else PRATCHYA_LNP(B, false);                                                                                    \
+  }
+  if (!x8) PRATCHYA_LN(0)
+  else if (blk == 16) PRATCHYA_LN(16)
+  else if (blk == 32) PRATCHYA_LN(32)
+  else if (blk == 64) { if constexpr (G::P >= 32) PRATCHYA_LN(64) }
+  else { if constexpr (G::P >= 64 && G::NV * kN<T> >= 16) PRATCHYA_LN(128) }
 #undef PRATCHYA_LN
+#undef PRATCHYA_LNP
   return check_launch("layer_norm");
 }
 
