@@ -66,8 +66,11 @@ __device__ __forceinline__ void normal(float x, float& P, float& p) {
   P = x < 0.0f ? tail : 1.0f - tail;
   p = 0.39894228040143268f * e;
 }
+// For a result in f32 by the library's exponential, whose argument is not rounded to x
+// log2 e first: that rounding is one of |x| units of the sigmoid below 0.
+template <bool F32>
 __device__ __forceinline__ float sigmoid(float x) {
-  return __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(-x * kLog2e));
+  return __builtin_amdgcn_rcpf(1.0f + (F32 ? expf(-x) : __builtin_amdgcn_exp2f(-x * kLog2e)));
 }
 
 // f of a vector; the kind is the same for the whole launch.
@@ -81,7 +84,7 @@ __device__ __forceinline__ void act(float (&v)[N], int kind) {
     }
   } else if (kind == PRATCHYA_ACT_SILU) {
 #pragma unroll
-    for (int i = 0; i < N; ++i) v[i] *= sigmoid(v[i]);
+    for (int i = 0; i < N; ++i) v[i] *= sigmoid<N == 4>(v[i]);
   } else {
 #pragma unroll
     for (int i = 0; i < N; ++i) {
@@ -101,7 +104,7 @@ __device__ __forceinline__ void act_grad(const float (&v)[N], float (&g)[N], int
   } else if (kind == PRATCHYA_ACT_SILU) {
 #pragma unroll
     for (int i = 0; i < N; ++i) {
-      const float s = sigmoid(v[i]);
+      const float s = sigmoid<N == 4>(v[i]);
       g[i] *= s * (1.0f + v[i] * (1.0f - s));
     }
   } else {
