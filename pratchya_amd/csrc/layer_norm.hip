@@ -742,13 +742,11 @@ constexpr int kFwdThreads = 512, kFwdAhead = 1, kBwdThreads = 1024, kBwdAhead = 
 constexpr int64_t kFwdBlocks = 512, kBwdBlocks = 256;
 // Bytes of y up to which the forward pass stores it past the caches.  With the
 // quantizer of the Linear behind it, that reads y at once (bf16, rows of 4096): 2 MB as
-// fast, 8 and 16 MB 13.2 -> 12.1 and 18.6 -> 14.0 us, 32 and 64 MB within 3%; 96 to 256 MB 4
-// to 9% slower (64.3 for 59.8, 83 for 76, 162 for 153 us), 512 MB 4%.  f32 the same.  Where
-// the 8-bit form is stored beside it 8 and 16 MB 14.4 -> 11.9 and 21.7 -> 17.8, 96 and 128 MB
-// within 3%, 160 MB 122 for 116, 256 MB 190 for 177.  Without a reader of y, the
-// backward pass right behind, streaming is the faster form at every size to 256 MB (128
-// MB 125 for 135 us); a step has the reader.
-constexpr int64_t kFwdPast = (int64_t)64 << 20, kFwdPastStored = (int64_t)128 << 20;
+// fast, 8 and 16 MB 13.2 -> 12.1 and 18.6 -> 14.0 us (with the 8-bit form 14.4 -> 11.9 and
+// 21.7 -> 17.8), 32 and 64 MB within 3%.  Between a residual addition before and that
+// quantizer, other work and the backward pass behind, 96 and 128 MB are within 1%,
+// but 192 MB take 514 us for 501, 256 MB 684 for 667, 512 MB 1332 for 1311; f32 alike.
+constexpr int64_t kFwdPast = (int64_t)128 << 20;
 // The backward pass's workgroups of 12 waves: two a compute unit from this many rows
 // a team on (2048 x 5120, 4 rows: 23.7 -> 25.2 us; 8 rows 35.1 -> 33.9; 16 rows 58.2 -> 52.3)
 constexpr int kBwdThin = 768;
@@ -832,7 +830,7 @@ int launch_fwd(G, const T* x, int64_t ldx, const Affine& p, int64_t rows, int64_
                      groups, eps, y, stats, x8, sc8, sc32)
 #define PRATCHYA_LN(B)                                                                                              \
   {                                                                                                                 \
-    if (rows * width * (int64_t)sizeof(T) <= (B ? kFwdPastStored : kFwdPast)) PRATCHYA_LNP(B, true);                                       \
+    if (rows * width * (int64_t)sizeof(T) <= kFwdPast) PRATCHYA_LNP(B, true);                                       \
     else PRATCHYA_LNP(B, false);                                                                                    \
   }
   if (!x8) PRATCHYA_LN(0)
