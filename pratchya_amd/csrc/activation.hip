@@ -11,10 +11,10 @@
 // 2 MB of bf16 the same, 8 and 16 MB 10.9 -> 9.2 and 16.6 -> 13.0 us, 32 to 192 MB within
 // 6% either way, 256 MB 136 -> 149, 512 MB and 1 GB within 2%; f32 and the backward
 // pass alike.  One form is kept: only at 256 MB are plain stores clearly ahead.
-// [16384, 16384] bf16, forward with the 8-bit form 216 us (1.35 GB, 6.2 TB/s), backward
-// from it 209 us (6.4 TB/s); without it 170 and 259 us (6.3 and 6.2 TB/s).  gelu's 20
-// operations an element in bf16 show a little: [8192, 8192] 61 to 64 us each way (5.4
-// TB/s).
+// [16384, 16384] bf16, forward with the 8-bit form 217 us (1.35 GB, 6.2 TB/s), backward
+// from it 211 us (6.4 TB/s); without it 169 and 255 us (6.4 and 6.3 TB/s).  gelu's 20
+// operations an element in bf16 show a little with it: [8192, 8192] 61 and 60 us (5.5 and
+// 5.6 TB/s); in f32, 31 of them, 104 and 101 us (5.8 and 5.9 TB/s).
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 

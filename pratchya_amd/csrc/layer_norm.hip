@@ -81,8 +81,8 @@ __device__ __forceinline__ int part_of(int64_t n) { return n < 0 ? 0 : n < N ? (
 // loaded and stored at `off`.  The vector at the end of a segment of an odd length
 // is moved back to end with it: its first elements are the thread's before it, left
 // out of sums and stored by both, with the same value.  By its elements, each
-// load waited for where it was issued, [8192, 4095] bf16 took 34.5 us for 23.9, in the
-// backward pass 99.9 for 51.1.  Segments below a vector (whole: false) go by elements.
+// load waited for where it was issued, [8192, 4095] bf16 took 34.5 us where it takes 29, in
+// the backward pass 99.9 for 50.  Segments below a vector (whole: false) go by elements.
 template <int N>
 struct Part {
   uint32_t off;
@@ -160,9 +160,10 @@ __device__ __forceinline__ float normed(float x, float mean, float rstd) { retur
 // of equal values is that value: up to 2^16 bf16 values' sum is exact and the
 // quotient's rounding the only one; f32's mean is corrected by the mean of the
 // deviations from it, and waves are joined by their distance from the first.
-// Bound by HBM, with some 20 vector instructions an element beside it: [16384,
-// 4096] bf16 49 us (268 MB, 5.4 TB/s), with its 8-bit form 63 us (335 MB, 5.3
-// TB/s), heads of 64 over [8192, 4096] 22 us (6.0 TB/s); one row of 4096 4 us.
+// Bound by HBM, with 16 to 24 vector instructions an element beside it (medians of
+// kernel traces): [16384, 4096] bf16 49.5 us (268 MB, 5.4 TB/s), with its 8-bit form 64 us
+// (337 MB, 5.3 TB/s), f32 [8192, 4096] 48.5 us (5.5 TB/s), heads of 64 over [8192, 4096]
+// 26 to 27 us (134 MB, 5.1 TB/s); one row of 4096 3.4 us.
 template <typename T, typename G, int BLK, int AHEAD, bool PAST>
 __global__ __launch_bounds__(G::TB) void k_layer_norm(const T* __restrict__ x, int64_t ldx, Affine p, int64_t rows,
                                                       int64_t width, int64_t groups, float eps, T* __restrict__ y,
@@ -308,10 +309,11 @@ __global__ __launch_bounds__(G::TB) void k_layer_norm(const T* __restrict__ x, i
 }
 
 // Segments of more than kLongest elements, which a workgroup's registers do not
-// hold: a workgroup a segment, kLongVecs vectors a thread in flight, three passes
-// over the row of which the later two come from the L2 cache.  [2048, 32768] bf16
-// 85 us, its backward pass 179 us (3.2 and 2.2 TB/s of what goes through HBM once);
-// of 32769, on no address of 16 bytes, 111 and 225 us.
+// hold beside their weights and biases in f32: a workgroup a segment, kLongVecs vectors
+// a thread in flight, three passes over the row of which the later two come from the L2
+// cache.  [2048, 32768] bf16 90 us, its backward pass 183 us (3.0 and 2.2 TB/s of what goes
+// through HBM once); of 32769, on no address of 16 bytes, 117 and 224 us.  Held as raw
+// vectors, with the parameters loaded where they are used, 65536 bf16 would fit.
 constexpr int kLongThreads = 1024, kLongVecs = 4;
 
 // Calls use(u, part) for this thread's vectors of a segment, after load has been
@@ -435,8 +437,9 @@ template <typename T> struct HeldSource<T, true> {
 // has walked: joined over the workgroup's row lanes and written to
 // part[blockIdx.x][0 / 1][width], or as the results where there is one workgroup
 // per column.  Bound by HBM; the partial sums, 2 kB a column over 256 workgroups,
-// are 5% of it: with the join [16384, 4096] bf16 78 us (402 MB, 5.2 TB/s), from the
-// 8-bit form 72 us (335 MB), heads of 64 over [8192, 4096] 41 us (201 MB).
+// are 5% of it: with the join [16384, 4096] bf16 77 us (402 MB, 5.2 TB/s), from the
+// 8-bit form 73 us (337 MB), f32 [8192, 4096] 71 us (402 MB), heads of 64 over [8192, 4096]
+// bf16 41 us (201 MB).
 template <typename T, typename G, bool STORED, int AHEAD>
 __global__ __launch_bounds__(G::TB) void k_layer_norm_bwd(typename SourceOf<T, STORED>::type src,
                                                           const T* __restrict__ dy, int64_t ldy, Affine p,

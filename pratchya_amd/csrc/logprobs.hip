@@ -141,10 +141,11 @@ template <typename T>
 constexpr int kBwdUnroll = 16 / kN<T>;
 
 // One row per WPR waves, 4 / WPR rows (at least one) per workgroup: one pass, bound
-// by HBM where rows fill the device (8192 x 65536 bf16 165 to 174 us, 1.07 GB at 6.2
-// to 6.5 TB/s; the exponential's quarter rate and six operations more a logit are
-// some two thirds of that time), by one compute unit's loads for few rows (one row
-// of 131072 in 9 us), which the 16 waves of a row are for.
+// by HBM where rows fill the device (8192 x 65536 bf16 167 us, 1.07 GB at 6.4 TB/s, with
+// entropies 177 to 213 from run to run and 165 at best; the exponential's quarter rate and
+// six operations more a logit are some two thirds of that time), by one compute unit's
+// loads for few rows (one row of 131072 in 10 us, whatever the other compute units do),
+// which the 16 waves of a row are for.
 template <typename T, int WPR, bool ENTROPY, bool NT>
 __global__ __launch_bounds__(WPR < 4 ? 256 : WPR * 64) void k_logprobs(
     const T* __restrict__ x, int64_t ld, const int64_t* __restrict__ tokens, int64_t rows, int64_t vocab,
@@ -201,8 +202,8 @@ __global__ __launch_bounds__(WPR < 4 ? 256 : WPR * 64) void k_logprobs(
 // alone would take longer over a row than all parts and the join together; a part
 // stays in registers, so its logits are read once for the sums and the selection.
 // Bound by the selection's instructions and barriers: 20 of one row of 65536 bf16
-// 7 us and 5 us for the join, 5 of 256 rows of 32768 f32 15 and 5 us, 20 of 512 rows
-// of 131072 bf16 81 us together (1.6 TB/s).
+// 7 us and 5 us for the join, 5 of 256 rows of 32768 f32 14 and 5 us (34 instructions a
+// logit), 20 of 512 rows of 131072 bf16 79 us together (1.7 TB/s).
 constexpr int kPartThreads = 256, kPartElems = 16, kBlock = kPartThreads * kPartElems, kParts = 64;
 constexpr int kKeys = kPartElems + 1;                   // keys of a thread: a block's logits and one kept key
 
@@ -436,8 +437,8 @@ __global__ __launch_bounds__(kPartThreads) void k_logprobs_join(const T* __restr
 }
 
 // dx of 16 TPR logits of a row per TPR threads: elementwise, one
-// read and one write of each logit, bound by HBM: 8192 x 65536 bf16 348 us (2.15 GB,
-// 6.2 TB/s).
+// read and one write of each logit, bound by HBM: 8192 x 65536 bf16 347 to 367 us (2.15 GB,
+// 5.9 to 6.2 TB/s), 1000 x 50021 f32 61 us (6.6 TB/s).
 template <typename T, int TPR, bool NT>
 __global__ __launch_bounds__(256) void k_logprobs_bwd(const T* __restrict__ x, int64_t ld,
                                                       const int64_t* __restrict__ tokens,
