@@ -742,6 +742,25 @@ int pratchya_token_logprobs_bwd(const void* logits, int64_t ld, int dtype, const
                                 const float* g_logprobs, const float* g_entropy, int64_t rows, int64_t vocab,
                                 void* d_logits, hipStream_t stream);
 
+/* ---- a model's ends and its time mixing -------------------------------- */
+
+/* Embedding lookup: y_i = scale * table[tokens_i] for n tokens and a table of
+ * [vocab, width] elements (f32 or bf16, rows ld elements apart); y contiguous [n,
+ * width], of the table's dtype.  A token below 0 stands for none: its row is 0; one of
+ * vocab or more has no row: NaN.  n and vocab below 2^31, up to 2^26 pieces of rows (of
+ * 1024 bf16 or 512 f32 elements). */
+int pratchya_embedding(const void* table, int64_t ld, int dtype, const int64_t* tokens, int64_t n, int64_t vocab,
+                       int64_t width, float scale, void* y, hipStream_t stream);
+
+/* Its table's gradient: dtable_v = scale * the sum of dy_i over tokens_i = v, 0 for
+ * rows without tokens; dy of dtype, rows ldy elements apart, dtable contiguous
+ * [vocab, width] of dtype.  f32 sums in the tokens' order.  workspace:
+ * pratchya_embedding_bwd_workspace_bytes, 16-byte aligned. */
+int64_t pratchya_embedding_bwd_workspace_bytes(int64_t n, int64_t vocab, int64_t width);
+int pratchya_embedding_bwd(const void* dy, int64_t ldy, int dtype, const int64_t* tokens, int64_t n, int64_t vocab,
+                           int64_t width, float scale, void* dtable, void* workspace, int64_t workspace_bytes,
+                           hipStream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

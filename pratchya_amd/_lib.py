@@ -143,6 +143,10 @@ SIGNATURES = {
                                          _c_p, _c_p, _c_i64, _c_p]),
     "pratchya_token_logprobs_bwd": (_c_int, [_c_p, _c_i64, _c_int, _c_p, _c_p, _c_p, _c_p, _c_i64, _c_i64, _c_p,
                                              _c_p]),
+    "pratchya_embedding": (_c_int, [_c_p, _c_i64, _c_int, _c_p, _c_i64, _c_i64, _c_i64, ctypes.c_float, _c_p, _c_p]),
+    "pratchya_embedding_bwd_workspace_bytes": (_c_i64, [_c_i64, _c_i64, _c_i64]),
+    "pratchya_embedding_bwd": (_c_int, [_c_p, _c_i64, _c_int, _c_p, _c_i64, _c_i64, _c_i64, ctypes.c_float, _c_p, _c_p,
+                                        _c_i64, _c_p]),
     "pratchya_mfma_ceiling": (_c_int, [_c_p, _c_p, _c_i64, _c_int, _c_i64, _c_p, ctypes.POINTER(_c_i64), _c_p]),
     "pratchya_debug_bf16_to_e4m3": (_c_int, [_c_p, _c_p, _c_i64, _c_int, _c_p]),
     "pratchya_debug_f32_to_bf16": (_c_int, [_c_p, _c_p, _c_i64, _c_int, _c_p]),

@@ -370,12 +370,68 @@ Tensor token_logprobs_bwd(const Tensor& logits, const Tensor& tokens, const Tens
 }
 
 // --------------------------------------------------------------------------
+// embedding
+// --------------------------------------------------------------------------
+// Tokens as the kernels read them: int64, contiguous.
+Tensor token_array(const Tensor& tokens, const Tensor& like, const char* what) {
+  TORCH_CHECK_VALUE(tokens.device() == like.device(), what, ": tokens on ", tokens.device(), " for an array on ",
+                    like.device());
+  TORCH_CHECK_TYPE(tokens.scalar_type() == at::kLong || tokens.scalar_type() == at::kInt, what, ": tokens of ",
+                   tokens.scalar_type(), "; expected int64 or int32");
+  return tokens.scalar_type() == at::kLong && tokens.is_contiguous() ? tokens : tokens.to(at::kLong).contiguous();
+}
+
+struct Embedded {
+  Tensor y, tokens;
+};
+
+Embedded embedding_fwd(const Tensor& table, const Tensor& tokens, double scale) {
+  const char* what = "embedding";
+  require_gpu(table);
+  require_gpu(tokens);
+  const int code = float_code(table, what);
+  TORCH_CHECK_VALUE(table.dim() == 2 && table.size(0) >= 1, what, ": a table of ", table.sizes(),
+                    "; expected [vocabulary, width]");
+  const c10::DeviceGuard guard(table.device());
+  Embedded out;
+  out.tokens = token_array(tokens, table, what);
+  const RowArray r = as_rows(table, what);
+  c10::DimVector shape(tokens.sizes());
+  shape.push_back(table.size(1));
+  out.y = new_empty(shape, table.scalar_type(), table);
+  check(pratchya_embedding(r.t.data_ptr(), r.ld, code, static_cast<const int64_t*>(out.tokens.data_ptr()),
+                           tokens.numel(), table.size(0), table.size(1), (float)scale, out.y.data_ptr(),
+                           stream_of(table)),
+        what);
+  return out;
+}
+
+Tensor embedding_bwd(const Tensor& cotangent, const Tensor& tokens, int64_t vocab, double scale) {
+  const char* what = "embedding_bwd";
+  require_gpu(cotangent);
+  const int code = float_code(cotangent, what);
+  const c10::DeviceGuard guard(cotangent.device());
+  const int64_t width = cotangent.size(-1), n = tokens.numel();
+  const RowArray dy = as_rows(cotangent, what);
+  const Tensor dtable = new_empty({vocab, width}, cotangent.scalar_type(), cotangent);
+  const int64_t bytes = pratchya_embedding_bwd_workspace_bytes(n, vocab, width);
+  const Tensor ws = new_empty({bytes}, at::kByte, cotangent);
+  check(pratchya_embedding_bwd(dy.t.data_ptr(), dy.ld, code, static_cast<const int64_t*>(tokens.data_ptr()), n, vocab,
+                               width, (float)scale, dtable.data_ptr(), ws.data_ptr(), bytes, stream_of(cotangent)),
+        what);
+  return dtable;
+}
+
+// --------------------------------------------------------------------------
 // autograd nodes
 // --------------------------------------------------------------------------
 // Gradients of gradients are not computed: with create_graph the results are
-// differentiable into an error, as torch's once_differentiable has it.
+// differentiable into an error, as torch's once_differentiable has it (they count as
+// differentiable, since the error's node is attached to those only).
 variable_list once(variable_list&& grads, const char* what) {
   if (!at::GradMode::is_enabled()) return std::move(grads);
+  for (Tensor& g : grads)
+    if (g.defined()) g.set_requires_grad(true);
   auto error = std::make_shared<torch::autograd::DelayedError>(
       std::string(what) + ": its gradient cannot be differentiated again", (int)grads.size());
   return (*error)(std::move(grads));
@@ -489,6 +545,27 @@ struct PratchyaTokenLogprobsBackward : torch::autograd::Node {
   }
 };
 
+struct PratchyaEmbeddingBackward : torch::autograd::Node {
+  SavedVariable tokens_;
+  int64_t vocab_ = 0;
+  double scale_ = 1.0;
+  variable_list apply(variable_list&& grads) override {
+    variable_list out(1);
+    if (!grads[0].defined()) return out;
+    Tensor tokens;
+    {
+      const std::lock_guard<std::mutex> lock(mutex_);
+      tokens = tokens_.unpack();
+    }
+    out[0] = embedding_bwd(grads[0], tokens, vocab_, scale_);
+    return once(std::move(out), "embedding");
+  }
+  void release_variables() override {
+    const std::lock_guard<std::mutex> lock(mutex_);
+    tokens_.reset_data();
+  }
+};
+
 bool wants_grad(const Tensor& t) { return t.requires_grad(); }
 bool wants_grad(const MaybeTensor& t) { return t && t->requires_grad(); }
 Tensor or_none(const MaybeTensor& t) { return t ? *t : Tensor(); }
@@ -565,6 +642,24 @@ Scored token_logprobs(const Tensor& logits, const Tensor& tokens, bool entropy, 
   torch::autograd::set_history(r.logprobs, node);
   if (entropy) torch::autograd::set_history(r.entropy, node);
   return r;
+}
+
+Tensor embedding(const Tensor& table, const Tensor& tokens, double scale) {
+  refuse_tangent(table, "embedding");
+  const bool grad = at::GradMode::is_enabled() && wants_grad(table);
+  Embedded r;
+  {
+    at::NoGradGuard no;
+    r = embedding_fwd(table, tokens, scale);
+  }
+  if (!grad) return r.y;
+  auto node = new_node<PratchyaEmbeddingBackward>();
+  node->set_next_edges(torch::autograd::collect_next_edges(table));
+  node->tokens_ = SavedVariable(r.tokens, false);
+  node->vocab_ = table.size(0);
+  node->scale_ = scale;
+  torch::autograd::set_history(r.y, node);
+  return r.y;
 }
 
 // --------------------------------------------------------------------------
@@ -738,13 +833,22 @@ PyObject* py_token_logprobs_bwd(PyObject*, PyObject* const* a, Py_ssize_t n) {
   });
 }
 
+PyObject* py_embedding(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  return method<3>("embedding", n, [&] {
+    const Tensor &table = tensor_arg(a[0], "embedding"), &tokens = tensor_arg(a[1], "embedding");
+    const double scale = float_arg(a[2]);
+    return wrap(unlocked([&] { return embedding(table, tokens, scale); }));
+  });
+}
+
 #define PRATCHYA_METHOD(name) \
   {#name, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(py_##name)), METH_FASTCALL, nullptr}
 PyMethodDef methods[] = {PRATCHYA_METHOD(layer_norm),         PRATCHYA_METHOD(layer_norm_fwd),
                          PRATCHYA_METHOD(layer_norm_bwd),     PRATCHYA_METHOD(activation),
                          PRATCHYA_METHOD(activation_fwd),     PRATCHYA_METHOD(activation_bwd),
                          PRATCHYA_METHOD(token_logprobs),     PRATCHYA_METHOD(token_logprobs_fwd),
-                         PRATCHYA_METHOD(token_logprobs_bwd), {nullptr, nullptr, 0, nullptr}};
+                         PRATCHYA_METHOD(token_logprobs_bwd), PRATCHYA_METHOD(embedding),
+                         {nullptr, nullptr, 0, nullptr}};
 #undef PRATCHYA_METHOD
 
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_row_ops", "Row operators over libpratchya_fp8.", -1, methods,

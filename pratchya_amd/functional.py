@@ -52,6 +52,16 @@ def activation(x: torch.Tensor, kind: str = "relu2", tgrid: Optional[Tuple[int, 
     return _ops.activation(x, K._activation_code(kind), tgrid)
 
 
+def embedding(table: torch.Tensor, tokens: torch.Tensor, scale: float = 1.0) -> torch.Tensor:
+    """``scale * table[tokens]`` for a table [V, C] and tokens [...] (int64 or int32),
+    [..., C] in the table's dtype, differentiable in the table: its gradient is dense,
+    f32 sums over a token's occurrences in their order, rounded once.
+
+    A negative token stands for none: its row is 0 and it has no gradient.  A token of V
+    or more gives NaN, as no row stands for it, and has no gradient."""
+    return _ops.embedding(table, tokens, scale)
+
+
 class TokenLogprobs(NamedTuple):
     """Results of ``token_logprobs``; what was not asked for is None."""
     logprobs: torch.Tensor                      # f32 [...]
