@@ -748,7 +748,7 @@ int pratchya_token_logprobs_bwd(const void* logits, int64_t ld, int dtype, const
  * [vocab, width] elements (f32 or bf16, rows ld elements apart); y contiguous [n,
  * width], of the table's dtype.  A token below 0 stands for none: its row is 0; one of
  * vocab or more has no row: NaN.  n and vocab below 2^31, up to 2^26 pieces of rows (of
- * 1024 bf16 or 512 f32 elements). */
+ * 512 bf16 or 256 f32 elements). */
 int pratchya_embedding(const void* table, int64_t ld, int dtype, const int64_t* tokens, int64_t n, int64_t vocab,
                        int64_t width, float scale, void* y, hipStream_t stream);
 
@@ -760,6 +760,34 @@ int64_t pratchya_embedding_bwd_workspace_bytes(int64_t n, int64_t vocab, int64_t
 int pratchya_embedding_bwd(const void* dy, int64_t ldy, int dtype, const int64_t* tokens, int64_t n, int64_t vocab,
                            int64_t width, float scale, void* dtable, void* workspace, int64_t workspace_bytes,
                            hipStream_t stream);
+
+/* Cross entropy of an output head, without keeping the logits z = x W: x [n, width]
+ * (f32 or bf16, rows ldx elements apart), W of x's dtype, [width, vocab] (w_rows 0) or
+ * the transpose of a table [vocab, width] (w_rows 1), rows ldw apart;
+ *   loss_i = (1 - smoothing) (lse - z_t) + smoothing (lse - mean z),  lse = log sum e^z,
+ * f32 [n], for targets t.  A target below 0 stands for none: its loss is 0, without a
+ * gradient; one of vocab or more gives NaN, its gradient is the formula's without the
+ * target's term.  stats, if not null, [n][2] f32 for the backward pass.  workspace:
+ * pratchya_linear_cross_entropy_workspace_bytes of the same arguments (backward_dx and
+ * backward_dw 0 for the forward pass, else whether that gradient is wanted), 256-byte
+ * aligned: the f32 logits of a piece of the vocabulary (256 MB at most, but for 64 Ki
+ * rows or more), and copies of operands whose sizes are no multiples of 64 or that are
+ * f32 (three bf16 planes).  Rows and one piece's planes lie within 2^32 bytes
+ * (PRATCHYA_EUNSUPPORTED otherwise). */
+int64_t pratchya_linear_cross_entropy_workspace_bytes(const void* x, int64_t ldx, const void* w, int64_t ldw, int dtype,
+                                                      int w_rows, int64_t n, int64_t width, int64_t vocab,
+                                                      int backward_dx, int backward_dw);
+int pratchya_linear_cross_entropy(const void* x, int64_t ldx, const void* w, int64_t ldw, int dtype, int w_rows,
+                                  const int64_t* targets, int64_t n, int64_t width, int64_t vocab, float smoothing,
+                                  float* loss, float* stats, void* workspace, int64_t workspace_bytes,
+                                  hipStream_t stream);
+
+/* Its gradients from the losses' cotangents g [n] (f32) and the forward pass's stats:
+ * dx contiguous [n, width], dw contiguous in W's layout; either may be null. */
+int pratchya_linear_cross_entropy_bwd(const void* x, int64_t ldx, const void* w, int64_t ldw, int dtype, int w_rows,
+                                      const int64_t* targets, const float* stats, const float* g, int64_t n,
+                                      int64_t width, int64_t vocab, float smoothing, void* dx, void* dw,
+                                      void* workspace, int64_t workspace_bytes, hipStream_t stream);
 
 #ifdef __cplusplus
 }

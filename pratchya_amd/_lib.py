@@ -147,6 +147,12 @@ SIGNATURES = {
     "pratchya_embedding_bwd_workspace_bytes": (_c_i64, [_c_i64, _c_i64, _c_i64]),
     "pratchya_embedding_bwd": (_c_int, [_c_p, _c_i64, _c_int, _c_p, _c_i64, _c_i64, _c_i64, ctypes.c_float, _c_p, _c_p,
                                         _c_i64, _c_p]),
+    "pratchya_linear_cross_entropy_workspace_bytes": (_c_i64, [_c_p, _c_i64, _c_p, _c_i64, _c_int, _c_int, _c_i64,
+                                                               _c_i64, _c_i64, _c_int, _c_int]),
+    "pratchya_linear_cross_entropy": (_c_int, [_c_p, _c_i64, _c_p, _c_i64, _c_int, _c_int, _c_p, _c_i64, _c_i64, _c_i64,
+                                               ctypes.c_float, _c_p, _c_p, _c_p, _c_i64, _c_p]),
+    "pratchya_linear_cross_entropy_bwd": (_c_int, [_c_p, _c_i64, _c_p, _c_i64, _c_int, _c_int, _c_p, _c_p, _c_p, _c_i64,
+                                                   _c_i64, _c_i64, ctypes.c_float, _c_p, _c_p, _c_p, _c_i64, _c_p]),
     "pratchya_mfma_ceiling": (_c_int, [_c_p, _c_p, _c_i64, _c_int, _c_i64, _c_p, ctypes.POINTER(_c_i64), _c_p]),
     "pratchya_debug_bf16_to_e4m3": (_c_int, [_c_p, _c_p, _c_i64, _c_int, _c_p]),
     "pratchya_debug_f32_to_bf16": (_c_int, [_c_p, _c_p, _c_i64, _c_int, _c_p]),

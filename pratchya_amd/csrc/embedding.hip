@@ -6,10 +6,10 @@
 // token of the vocabulary's size or more has no row: its y is NaN, without a gradient.
 // Sums are f32 in the tokens' order, the same bits for the same inputs.
 //
-// Gradient.  The tokens are sorted by value first (k_sort_tokens), so that each row
-// of the table is summed and written once, rows without tokens as zeros: no atomics
-// and no f32 copy of the table.  Bound: HBM, dy read once and the table's gradient
-// written once.
+// Gradient.  One launch sorts the tokens by value (k_sort_tokens) while its other
+// workgroups fill the gradient with zeros; then each row that has tokens is summed
+// once: no atomics and no f32 copy of the table.  Bound: HBM, dy read and the table's
+// gradient written.
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
@@ -78,8 +78,37 @@ struct Sorted {
   int32_t* offs;     // [vocab + 1] first place of each row
 };
 
-__global__ __launch_bounds__(kSortWaves * 64) void k_sort_tokens(const int64_t* __restrict__ tokens, int n, int vocab,
-                                                                  int rows, Sorted out) {
+// The gradient's bytes as a fill sees them: `vectors` of 16 from the first 16-byte
+// boundary on, `head` and `tail` elements around them.
+struct Fill {
+  uint8_t *first, *vec, *last;
+  int64_t vectors;
+  int head, tail;
+};
+
+constexpr int kSortThreads = kSortWaves * 64, kFillUnroll = 4;
+
+__device__ __forceinline__ void fill_zero(const Fill& f, int64_t block) {
+  auto* v = reinterpret_cast<u32x4_t*>(f.vec);
+  const int64_t at = block * (kSortThreads * kFillUnroll) + threadIdx.x;
+#pragma unroll
+  for (int u = 0; u < kFillUnroll; ++u) {
+    const int64_t i = at + u * kSortThreads;
+    if (i < f.vectors) v[i] = u32x4_t{};
+  }
+  if (block == 0 && threadIdx.x < 32) {
+    const int e = threadIdx.x & 15;
+    uint8_t* p = threadIdx.x < 16 ? f.first + e : f.last + e;
+    if (e < (threadIdx.x < 16 ? f.head : f.tail)) *p = 0;
+  }
+}
+
+__global__ __launch_bounds__(kSortThreads) void k_sort_tokens(const int64_t* __restrict__ tokens, int n, int vocab,
+                                                              int rows, int sorters, Sorted out, Fill fill) {
+  if ((int)blockIdx.x >= sorters) {
+    fill_zero(fill, (int64_t)blockIdx.x - sorters);
+    return;
+  }
   __shared__ int count[kSortWaves][kSortRows];
   __shared__ int part[kSortWaves], first[kSortWaves];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
@@ -167,7 +196,7 @@ __global__ __launch_bounds__(kSortWaves * 64) void k_sort_tokens(const int64_t* 
 
 // Sum of dy's rows pos[first .. first + count), count up to 64, over the lane's
 // vectors: the row numbers come in one load, the rows kAhead at a time.
-constexpr int kAhead = 4;
+constexpr int kAhead = 8;
 template <typename T, int U>
 __device__ __forceinline__ void sum_rows(const T* __restrict__ dy, int64_t ldy, const int32_t* __restrict__ pos,
                                          int first, int count, int64_t c0, int64_t width, float (&acc)[U][kN<T>]) {
@@ -203,23 +232,31 @@ __device__ __forceinline__ void sum_rows(const T* __restrict__ dy, int64_t ldy, 
   }
 }
 
-// Rows of up to kRun tokens are summed by one wave a piece.  Longer ones are cut at
-// the multiples of kRun of the sorted order: a tile of kRun sorted tokens holds
-// parts of at most two such rows, whose sums go to the tile's first partial (the
-// part that holds its first token) or its second; k_join_rows adds a row's partials.
-constexpr int kRun = 64;
+// Rows of up to kRun tokens are summed by one wave a piece, that of the row's first
+// token in sorted order.  Longer ones are cut at the multiples of kRun of that order:
+// a tile of kRun sorted tokens holds parts of at most two such rows, whose sums go to
+// the tile's first partial (the part that holds its first token) or its second;
+// k_join_rows adds a row's partials.
+//
+// Measured, gradient of [65536, 2048] bf16 from 16384 tokens as text has them (a tenth
+// of them the same): fill and sort 36 us (7.4 TB/s), sums 34, join 6; of [50021, 2057]
+// f32 from 1001: 68 (6 TB/s), 15, 4.  One vector a lane and 8 rows ahead: two and 4
+// ahead took 0.3 and 3% more time of both passes, runs of 64 and 16 instead of 32 3 to
+// 8% and -3 to 3%.  With the zeros written by the waves that sum, whose registers
+// leave few of them on a compute unit, both passes took 134 us instead of 104.
+constexpr int kRun = 32;
 
 template <typename T, int U>
-__global__ __launch_bounds__(256) void k_embedding_grad(const T* __restrict__ dy, int64_t ldy, Sorted s, int n,
+__global__ __launch_bounds__(256) void k_embedding_grad(const T* __restrict__ dy, int64_t ldy, Sorted s,
                                                         int64_t vocab, int64_t width, int pieces, int64_t tile_units,
                                                         float scale, float* __restrict__ partial,
                                                         T* __restrict__ dtable) {
   constexpr int N = kN<T>;
   int64_t unit = (int64_t)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int lane = threadIdx.x & 63;
+  const int lane = threadIdx.x & 63, total = s.offs[vocab];
   if (unit < tile_units) {
     const int64_t tile = unit / pieces, c0 = (unit - tile * pieces) * kPiece<T, U> + lane * N;
-    const int at = (int)tile * kRun, total = s.offs[vocab];
+    const int at = (int)tile * kRun;
     if (at >= total) return;
     const int here = min(kRun, total - at);
     const int v = lane < here ? s.key[at + lane] : -1;
@@ -243,12 +280,12 @@ __global__ __launch_bounds__(256) void k_embedding_grad(const T* __restrict__ dy
     return;
   }
   unit -= tile_units;
-  const int64_t row = unit / pieces, c0 = (unit - row * pieces) * kPiece<T, U> + lane * N;
-  if (row >= vocab) return;
-  const int first = s.offs[row], count = s.offs[row + 1] - first;
-  if (count > kRun) return;
+  const int64_t at = unit / pieces, c0 = (unit - at * pieces) * kPiece<T, U> + lane * N;
+  if (at >= total) return;
+  const int row = s.key[at], first = s.offs[row], count = s.offs[row + 1] - first;
+  if (first != at || count > kRun) return;
   float acc[U][N] = {};
-  if (count) sum_rows<T, U>(dy, ldy, s.pos, first, count, c0, width, acc);
+  sum_rows<T, U>(dy, ldy, s.pos, first, count, c0, width, acc);
   T* out = dtable + row * width;
 #pragma unroll
   for (int u = 0; u < U; ++u) {
@@ -301,8 +338,8 @@ int check_args(const char* what, int dtype, int64_t n, int64_t vocab, int64_t wi
   return PRATCHYA_OK;
 }
 
-// Vectors of a lane.
-constexpr int kU = 2;
+// Vectors of a lane (see k_embedding_grad; the lookup takes 22 us for 16384 rows of 4 KB, 5.8 TB/s).
+constexpr int kU = 1;
 
 template <typename T>
 int64_t pieces_of(int64_t width) {
@@ -338,7 +375,7 @@ template <typename T>
 int launch_bwd(const void* dy, int64_t ldy, const int64_t* tokens, int64_t n, int64_t vocab, int64_t width, float scale,
                void* dtable, char* ws, hipStream_t stream) {
   const int64_t pieces = pieces_of<T>(width), tiles = n > kRun ? (n + kRun - 1) / kRun : 0;
-  const int64_t units = (tiles + vocab) * pieces, columns = (width + 255) / 256;
+  const int64_t units = (tiles + n) * pieces, columns = (width + 255) / 256;
   if (pieces > 0x7FFFFFFF || !fits_launch((units + 3) / 4, 256) || !fits_launch(tiles, 256, columns))
     return pratchya_set_error(PRATCHYA_EUNSUPPORTED, "embedding_bwd: more pieces of rows than a launch has threads for (2^26)");
   const Layout l(n, vocab, width);
@@ -347,12 +384,25 @@ int launch_bwd(const void* dy, int64_t ldy, const int64_t* tokens, int64_t n, in
   float* partial = reinterpret_cast<float*>(ws + l.partial);
   // one workgroup a compute unit, or as many as the rows need
   const int64_t rows = (vocab + 255) / 256 < kSortRows ? (vocab + 255) / 256 : kSortRows;
-  hipLaunchKernelGGL(k_sort_tokens, dim3((unsigned)((vocab + rows - 1) / rows)), dim3(kSortWaves * 64), 0, stream,
-                     tokens, (int)n, (int)vocab, (int)rows, s);
+  const int64_t sorters = (vocab + rows - 1) / rows;
+  Fill fill;
+  const int64_t size = vocab * width * (int64_t)sizeof(T);
+  fill.first = static_cast<uint8_t*>(dtable);
+  fill.head = (int)(-reinterpret_cast<intptr_t>(dtable) & 15);
+  if (fill.head > size) fill.head = (int)size;
+  fill.vec = fill.first + fill.head;
+  fill.vectors = (size - fill.head) / 16;
+  fill.last = fill.vec + fill.vectors * 16;
+  fill.tail = (int)((size - fill.head) % 16);
+  const int64_t fillers = (fill.vectors + kSortThreads * kFillUnroll - 1) / (kSortThreads * kFillUnroll);
+  if (!fits_launch(sorters + fillers + 1, kSortThreads))
+    return pratchya_set_error(PRATCHYA_EUNSUPPORTED, "embedding_bwd: a table of more than 2^38 bytes");
+  hipLaunchKernelGGL(k_sort_tokens, dim3((unsigned)(sorters + (fillers ? fillers : 1))), dim3(kSortThreads), 0, stream,
+                     tokens, (int)n, (int)vocab, (int)rows, (int)sorters, s, fill);
   int rc = check_launch("embedding_bwd");
-  if (rc) return rc;
+  if (rc || n == 0) return rc;
   hipLaunchKernelGGL((k_embedding_grad<T, kU>), dim3((unsigned)((units + 3) / 4)), dim3(256), 0, stream,
-                     static_cast<const T*>(dy), ldy, s, (int)n, vocab, width, (int)pieces, tiles * pieces, scale, partial,
+                     static_cast<const T*>(dy), ldy, s, vocab, width, (int)pieces, tiles * pieces, scale, partial,
                      static_cast<T*>(dtable));
   rc = check_launch("embedding_bwd");
   if (rc || !tiles) return rc;

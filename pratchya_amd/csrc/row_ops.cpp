@@ -423,6 +423,93 @@ Tensor embedding_bwd(const Tensor& cotangent, const Tensor& tokens, int64_t voca
 }
 
 // --------------------------------------------------------------------------
+// cross entropy of an output head
+// --------------------------------------------------------------------------
+// A weight [C, V] as the library reads it: its rows, or those of the table [V, C]
+// whose transposed view it is.
+struct HeadWeight {
+  Tensor t;
+  int64_t ld;
+  bool rows;
+};
+HeadWeight head_weight(const Tensor& w) {
+  if (w.stride(1) == 1 || w.size(1) == 1) {
+    if (w.stride(1) == 1 && (w.size(0) == 1 || w.stride(0) >= w.size(1)))
+      return {w, w.size(0) == 1 ? w.size(1) : w.stride(0), false};
+  }
+  if (w.stride(0) == 1 && (w.size(1) == 1 || w.stride(1) >= w.size(0)))
+    return {w, w.size(1) == 1 ? w.size(0) : w.stride(1), true};
+  return {w.contiguous(), w.size(1), false};
+}
+
+struct HeadLoss {
+  Tensor loss, stats, targets;
+};
+
+HeadLoss head_loss_fwd(const Tensor& x, const Tensor& weight, const Tensor& targets, double smoothing, bool want_stats) {
+  const char* what = "linear_cross_entropy";
+  require_gpu(x);
+  require_gpu(weight);
+  require_gpu(targets);
+  const int code = float_code(x, what);
+  TORCH_CHECK_TYPE(weight.scalar_type() == x.scalar_type(), what, ": a weight of ", weight.scalar_type(), " for x of ",
+                   x.scalar_type());
+  TORCH_CHECK_VALUE(x.dim() > 0 && weight.dim() == 2 && weight.size(0) == x.size(-1) && weight.size(0) >= 1 &&
+                        weight.size(1) >= 1 && weight.device() == x.device(),
+                    what, ": a weight of ", weight.sizes(), " on ", weight.device(), " for x of ", x.sizes(), " on ",
+                    x.device());
+  TORCH_CHECK_VALUE(targets.sizes() == x.sizes().slice(0, x.dim() - 1), what, ": targets of ", targets.sizes(),
+                    " for x of ", x.sizes());
+  TORCH_CHECK_VALUE(smoothing >= 0.0 && smoothing <= 1.0, what, ": label smoothing of ", smoothing, "; expected 0 to 1");
+  const c10::DeviceGuard guard(x.device());
+  HeadLoss out;
+  out.targets = token_array(targets, x, what);
+  const RowArray r = as_rows(x, what);
+  const HeadWeight w = head_weight(weight);
+  out.loss = new_empty(targets.sizes(), at::kFloat, x);
+  if (want_stats) out.stats = new_empty({r.rows, 2}, at::kFloat, x);
+  const int64_t bytes = pratchya_linear_cross_entropy_workspace_bytes(
+      r.t.data_ptr(), r.ld, w.t.data_ptr(), w.ld, code, w.rows, r.rows, r.width, weight.size(1), 0, 0);
+  const Tensor ws = bytes ? new_empty({bytes}, at::kByte, x) : Tensor();
+  check(pratchya_linear_cross_entropy(r.t.data_ptr(), r.ld, w.t.data_ptr(), w.ld, code, w.rows,
+                                      static_cast<const int64_t*>(out.targets.data_ptr()), r.rows, r.width,
+                                      weight.size(1), (float)smoothing, static_cast<float*>(out.loss.data_ptr()),
+                                      static_cast<float*>(address(out.stats)), address(ws), bytes, stream_of(x)),
+        what);
+  return out;
+}
+
+// dx and dw, undefined where not needed; dw has the weight's layout.
+std::array<Tensor, 2> head_loss_bwd(const Tensor& x, const Tensor& weight, const Tensor& targets, const Tensor& stats,
+                                    Tensor g, double smoothing, std::array<bool, 2> need) {
+  const char* what = "linear_cross_entropy_bwd";
+  const int code = float_code(x, what);
+  const c10::DeviceGuard guard(x.device());
+  const RowArray r = as_rows(x, what);
+  const HeadWeight w = head_weight(weight);
+  const int64_t vocab = weight.size(1);
+  TORCH_CHECK_VALUE(g.numel() == r.rows && g.scalar_type() == at::kFloat && g.device() == x.device(), what,
+                    ": a cotangent of ", g.sizes(), " ", g.scalar_type(), " for ", r.rows, " rows");
+  g = g.contiguous();
+  std::array<Tensor, 2> out;
+  if (need[0]) out[0] = new_empty(x.sizes(), x.scalar_type(), x);
+  Tensor dw;
+  if (need[1]) dw = w.rows ? new_empty({vocab, r.width}, x.scalar_type(), x) : new_empty({r.width, vocab}, x.scalar_type(), x);
+  const int64_t bytes = pratchya_linear_cross_entropy_workspace_bytes(
+      r.t.data_ptr(), r.ld, w.t.data_ptr(), w.ld, code, w.rows, r.rows, r.width, vocab, need[0], need[1]);
+  const Tensor ws = bytes ? new_empty({bytes}, at::kByte, x) : Tensor();
+  check(pratchya_linear_cross_entropy_bwd(r.t.data_ptr(), r.ld, w.t.data_ptr(), w.ld, code, w.rows,
+                                          static_cast<const int64_t*>(targets.data_ptr()),
+                                          static_cast<const float*>(stats.data_ptr()),
+                                          static_cast<const float*>(g.data_ptr()), r.rows, r.width, vocab,
+                                          (float)smoothing, address(out[0]), address(dw), address(ws), bytes,
+                                          stream_of(x)),
+        what);
+  if (need[1]) out[1] = w.rows ? dw.t() : dw;
+  return out;
+}
+
+// --------------------------------------------------------------------------
 // autograd nodes
 // --------------------------------------------------------------------------
 // Gradients of gradients are not computed: with create_graph the results are
@@ -566,6 +653,37 @@ struct PratchyaEmbeddingBackward : torch::autograd::Node {
   }
 };
 
+struct PratchyaLinearCrossEntropyBackward : torch::autograd::Node {
+  SavedVariable x_, weight_, targets_, stats_;
+  double smoothing_ = 0.0;
+  variable_list apply(variable_list&& grads) override {
+    variable_list out(2);
+    if (!grads[0].defined()) return out;
+    Tensor x, weight, targets, stats;
+    {
+      const std::lock_guard<std::mutex> lock(mutex_);
+      x = x_.unpack();
+      weight = weight_.unpack();
+      targets = targets_.unpack();
+      stats = stats_.unpack();
+    }
+    auto got = [&] {
+      at::NoGradGuard no;
+      return head_loss_bwd(x, weight, targets, stats, grads[0], smoothing_,
+                           {task_should_compute_output(0), task_should_compute_output(1)});
+    }();
+    for (int i = 0; i < 2; ++i) out[i] = std::move(got[i]);
+    return once(std::move(out), "linear_cross_entropy");
+  }
+  void release_variables() override {
+    const std::lock_guard<std::mutex> lock(mutex_);
+    x_.reset_data();
+    weight_.reset_data();
+    targets_.reset_data();
+    stats_.reset_data();
+  }
+};
+
 bool wants_grad(const Tensor& t) { return t.requires_grad(); }
 bool wants_grad(const MaybeTensor& t) { return t && t->requires_grad(); }
 Tensor or_none(const MaybeTensor& t) { return t ? *t : Tensor(); }
@@ -660,6 +778,27 @@ Tensor embedding(const Tensor& table, const Tensor& tokens, double scale) {
   node->scale_ = scale;
   torch::autograd::set_history(r.y, node);
   return r.y;
+}
+
+Tensor linear_cross_entropy(const Tensor& x, const Tensor& weight, const Tensor& targets, double smoothing) {
+  refuse_tangent(x, "linear_cross_entropy");
+  refuse_tangent(weight, "linear_cross_entropy: weight");
+  const bool grad = at::GradMode::is_enabled() && (wants_grad(x) || wants_grad(weight));
+  HeadLoss r;
+  {
+    at::NoGradGuard no;
+    r = head_loss_fwd(x, weight, targets, smoothing, grad);
+  }
+  if (!grad) return r.loss;
+  auto node = new_node<PratchyaLinearCrossEntropyBackward>();
+  node->set_next_edges(torch::autograd::collect_next_edges(x, weight));
+  node->x_ = SavedVariable(x, false);
+  node->weight_ = SavedVariable(weight, false);
+  node->targets_ = SavedVariable(r.targets, false);
+  node->stats_ = SavedVariable(r.stats, false);
+  node->smoothing_ = smoothing;
+  torch::autograd::set_history(r.loss, node);
+  return r.loss;
 }
 
 // --------------------------------------------------------------------------
@@ -841,6 +980,15 @@ PyObject* py_embedding(PyObject*, PyObject* const* a, Py_ssize_t n) {
   });
 }
 
+PyObject* py_linear_cross_entropy(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  return method<4>("linear_cross_entropy", n, [&] {
+    const char* what = "linear_cross_entropy";
+    const Tensor &x = tensor_arg(a[0], what), &w = tensor_arg(a[1], what), &targets = tensor_arg(a[2], what);
+    const double smoothing = float_arg(a[3]);
+    return wrap(unlocked([&] { return linear_cross_entropy(x, w, targets, smoothing); }));
+  });
+}
+
 #define PRATCHYA_METHOD(name) \
   {#name, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(py_##name)), METH_FASTCALL, nullptr}
 PyMethodDef methods[] = {PRATCHYA_METHOD(layer_norm),         PRATCHYA_METHOD(layer_norm_fwd),
@@ -848,6 +996,7 @@ PyMethodDef methods[] = {PRATCHYA_METHOD(layer_norm),         PRATCHYA_METHOD(la
                          PRATCHYA_METHOD(activation_fwd),     PRATCHYA_METHOD(activation_bwd),
                          PRATCHYA_METHOD(token_logprobs),     PRATCHYA_METHOD(token_logprobs_fwd),
                          PRATCHYA_METHOD(token_logprobs_bwd), PRATCHYA_METHOD(embedding),
+                         PRATCHYA_METHOD(linear_cross_entropy),
                          {nullptr, nullptr, 0, nullptr}};
 #undef PRATCHYA_METHOD
 

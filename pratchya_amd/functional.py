@@ -84,3 +84,18 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, entropy: bool = F
     nothing else has log probabilities of -inf and entropy 0, and in its gradient,
     as for any masked logit, the probability 0."""
     return TokenLogprobs(*_ops.token_logprobs(logits, tokens, entropy, top))
+
+
+def linear_cross_entropy(x: torch.Tensor, weight: torch.Tensor, targets: torch.Tensor,
+                         label_smoothing: float = 0.0) -> torch.Tensor:
+    """Softmax cross entropy of the output head ``z = x @ weight``, for x [..., C],
+    weight [C, V] of x's dtype and targets [...] (int64 or int32): f32 [...],
+    ``(1 - a) (lse - z_t) + a (lse - mean z)`` with a the label smoothing,
+    differentiable in x and weight.  The logits are not kept: both passes compute them
+    in pieces of the vocabulary, in f32.  An embedding table [V, C] serves as weight
+    through its transposed view ``table.t()``, which is read as it lies.
+
+    A negative target stands for none: its loss is 0 and has no gradient.  A target of V
+    or more gives NaN, as no logit stands for it; its gradient is that of the other
+    terms."""
+    return _ops.linear_cross_entropy(x, weight, targets, label_smoothing)

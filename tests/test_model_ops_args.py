@@ -33,6 +33,46 @@ def test_embedding():
                 dict(ws_bytes=8), dict(ws=ctypes.c_void_p((1 << 20) + 8))):
         assert bwd(**bad) == L.EINVAL, bad
         assert b"embedding_bwd" in lib.pratchya_last_error()
-    assert bwd(vocab=1 << 27) == L.EUNSUPPORTED and bwd(n=100, width=1 << 25) == L.EUNSUPPORTED
+    assert bwd(vocab=1 << 30, width=1 << 10) == L.EUNSUPPORTED and bwd(n=1 << 27) == L.EUNSUPPORTED and bwd(n=100, width=1 << 25) == L.EUNSUPPORTED
     need = lib.pratchya_embedding_bwd_workspace_bytes
     assert need(0, 1, 8) > 0 and need(1000, 50, 64) >= 8 * 1000 + 4 * 51 and need(1 << 31, 5, 8) == 0
+
+
+def test_linear_cross_entropy():
+    L, lib = _L()
+
+    def fwd(x=FAKE, ldx=64, w=FAKE, ldw=128, dtype=1, rows=0, t=FAKE, n=64, C=64, V=128, a=0.0, loss=FAKE, ws=FAKE,
+            ws_bytes=1 << 60):
+        return lib.pratchya_linear_cross_entropy(x, ldx, w, ldw, dtype, rows, t, n, C, V, a, loss, None, ws, ws_bytes, None)
+    assert fwd(n=0) == L.OK
+    for bad in (dict(dtype=2), dict(n=-1), dict(C=0), dict(V=0), dict(ldx=-1), dict(a=-0.5), dict(a=1.5),
+                dict(a=float("nan")), dict(x=None), dict(w=None), dict(t=None), dict(loss=None), dict(ws=None),
+                dict(ws_bytes=8), dict(ws=ctypes.c_void_p((1 << 20) + 16))):
+        assert fwd(**bad) == L.EINVAL, bad
+        assert b"linear_cross_entropy" in lib.pratchya_last_error()
+    for big in (dict(n=1 << 24), dict(n=1 << 20, C=4096), dict(V=1 << 31), dict(C=1 << 31), dict(n=1 << 21, dtype=0)):
+        assert fwd(**big) == L.EUNSUPPORTED, big
+
+    def bwd(x=FAKE, w=FAKE, dtype=1, t=FAKE, stats=FAKE, g=FAKE, n=64, C=64, V=128, a=0.0, dx=FAKE, dw=FAKE, ws=FAKE,
+            ws_bytes=1 << 60):
+        return lib.pratchya_linear_cross_entropy_bwd(x, C, w, V, dtype, 0, t, stats, g, n, C, V, a, dx, dw, ws, ws_bytes,
+                                                     None)
+    assert bwd(dx=None, dw=None) == L.OK and bwd(n=0, dw=None) == L.OK
+    for bad in (dict(dtype=2), dict(a=2.0), dict(x=None), dict(t=None), dict(stats=None), dict(g=None), dict(ws=None),
+                dict(ws_bytes=64)):
+        assert bwd(**bad) == L.EINVAL, bad
+        assert b"linear_cross_entropy_bwd" in lib.pratchya_last_error()
+    need = lib.pratchya_linear_cross_entropy_workspace_bytes
+    # a large vocabulary's logits are never whole
+    assert 0 < need(FAKE, 4096, FAKE, 65536, 1, 0, 8192, 4096, 65536, 0, 0) < 1 << 29
+    assert need(FAKE, 4096, FAKE, 65536, 1, 0, 8192, 4096, 65536, 1, 1) < 3 << 29
+
+
+def test_names_without_gpu():
+    """Arguments that a user can get wrong are refused before the library is asked."""
+    import torch
+    from pratchya_amd import functional as F
+    x, t = torch.zeros((2, 8)), torch.zeros(2).long()
+    for call in (lambda: F.embedding(x, t), lambda: F.linear_cross_entropy(x, x.t(), t)):
+        with pytest.raises(RuntimeError, match="GPU only"):
+            call()
