@@ -789,6 +789,50 @@ int pratchya_linear_cross_entropy_bwd(const void* x, int64_t ldx, const void* w,
                                       int64_t width, int64_t vocab, float smoothing, void* dx, void* dw,
                                       void* workspace, int64_t workspace_bytes, hipStream_t stream);
 
+/* Linear attention with a decay for each head and token: per sequence and head, with
+ * S [dk, dv] in f32,
+ *   S_t = e^(log_decay_t) S_(t-1) + k_t^T v_t,   out_t = scale q_t S_t.
+ * q, k [batch, length, heads, dk] and v [.., dv] (f32 or bf16, dtype), log_decay
+ * [batch, length, heads] (f32 or bf16, g_dtype), heads of up to 128; strides: the
+ * elements from one sequence, token and head to the next of q, k, v and log_decay (12
+ * numbers, host memory), the last axis of q, k and v contiguous.  lengths [batch]
+ * (device memory) or null: tokens from a sequence's length on are not read (0 and
+ * `length` bound it), their outputs are 0.  state: S before the first token, f32
+ * contiguous [batch, heads, dk, dv], or null for 0.  out: contiguous [batch, length,
+ * heads, dv] of dtype; state_out: S behind the last token, f32 as state (not state
+ * itself).  starts: pratchya_linear_attention_starts_floats of f32, 16-byte aligned
+ * (null where that is 0): the states before the segments that a long sequence is cut
+ * into, which the backward pass reads.  A decay of 0 (log_decay -inf) forgets all. */
+int64_t pratchya_linear_attention_starts_floats(int64_t batch, int64_t length, int64_t heads, int64_t dk, int64_t dv,
+                                                int dtype);
+int pratchya_linear_attention(const void* q, const void* k, const void* v, int dtype, const void* log_decay, int g_dtype,
+                              const int64_t* strides, const int64_t* lengths, const float* state, int64_t batch,
+                              int64_t length, int64_t heads, int64_t dk, int64_t dv, float scale, void* out,
+                              float* state_out, float* starts, hipStream_t stream);
+
+/* Its gradients from the cotangents dout (of dtype, strides[12 .. 14], last axis
+ * contiguous) and dstate_out (f32 as state, or null for 0), with the forward pass's
+ * starts and, if dlog_decay and dstate_out are given, its state_out: dq, dk, dv
+ * contiguous of dtype, dlog_decay contiguous of g_dtype (may be null: its sums are then
+ * left out), dstate f32 (may be null).  workspace:
+ * pratchya_linear_attention_bwd_workspace_bytes, 16-byte aligned. */
+int64_t pratchya_linear_attention_bwd_workspace_bytes(int64_t batch, int64_t length, int64_t heads, int64_t dk,
+                                                      int64_t dv, int dtype);
+int pratchya_linear_attention_bwd(const void* q, const void* k, const void* v, int dtype, const void* log_decay,
+                                  int g_dtype, const int64_t* strides, const int64_t* lengths, const float* state,
+                                  const float* state_out, const float* starts, const void* dout,
+                                  const float* dstate_out, int64_t batch, int64_t length, int64_t heads, int64_t dk,
+                                  int64_t dv, float scale, void* dq, void* dk_out, void* dv_out, void* dlog_decay,
+                                  float* dstate, void* workspace, int64_t workspace_bytes, hipStream_t stream);
+
+/* One token of each sequence: q, k [batch, heads, dk], v [batch, heads, dv], log_decay
+ * [batch, heads]; strides: elements from one sequence and head to the next of q, k, v
+ * and log_decay (8 numbers, host memory).  state (f32 contiguous, 16-byte aligned) is
+ * updated in place; out contiguous [batch, heads, dv]. */
+int pratchya_linear_attention_step(const void* q, const void* k, const void* v, int dtype, const void* log_decay,
+                                   int g_dtype, const int64_t* strides, float* state, int64_t batch, int64_t heads,
+                                   int64_t dk, int64_t dv, float scale, void* out, hipStream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -26,7 +26,7 @@ LIB = PKG / "libpratchya_fp8.so"
 ROW_OPS = PKG / "_row_ops.so"
 SOURCES = ["quantize.hip", "quantize_t.hip", "gemm.hip", "gemm_t128.hip", "optim.hip", "elementwise.hip",
            "layer_norm.hip", "activation.hip", "logprobs.hip",
-           "embedding.hip", "head_loss.hip"]
+           "embedding.hip", "head_loss.hip", "linear_attention.hip"]
 
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
 CXX = os.environ.get("CXX", "g++")

@@ -510,6 +510,120 @@ std::array<Tensor, 2> head_loss_bwd(const Tensor& x, const Tensor& weight, const
 }
 
 // --------------------------------------------------------------------------
+// linear attention
+// --------------------------------------------------------------------------
+// Arguments of the kernels from arrays [B, T, H, D] (or [B, H, D], one token).
+struct Mix {
+  Tensor q, k, v, decay, lengths, state;
+  int code = 0, g_code = 0;
+  int64_t B = 0, T = 0, H = 0, dk = 0, dv = 0;
+  std::array<int64_t, 15> strides{};
+
+  const int64_t* length_ptr() const { return static_cast<const int64_t*>(address(lengths)); }
+  const float* state_ptr() const { return static_cast<const float*>(address(state)); }
+};
+
+// Itself where its last axis is contiguous, else a contiguous copy.
+Tensor last_contiguous(const Tensor& t) { return t.size(-1) <= 1 || t.stride(-1) == 1 ? t : t.contiguous(); }
+
+Mix mix_args(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& decay, const MaybeTensor& state,
+             const MaybeTensor& lengths, bool one, const char* what) {
+  for (const Tensor* t : {&q, &k, &v, &decay}) require_gpu(*t);
+  Mix m;
+  m.code = float_code(q, what);
+  m.g_code = float_code(decay, what);
+  const int64_t axes = one ? 3 : 4;
+  TORCH_CHECK_VALUE(q.dim() == axes && k.sizes() == q.sizes() && v.dim() == axes &&
+                        v.sizes().slice(0, axes - 1) == q.sizes().slice(0, axes - 1) &&
+                        decay.sizes() == q.sizes().slice(0, axes - 1),
+                    what, ": q of ", q.sizes(), ", k of ", k.sizes(), ", v of ", v.sizes(), ", log_decay of ",
+                    decay.sizes(), "; expected [batch", one ? "" : ", length", ", heads, width], decays without a width");
+  TORCH_CHECK_TYPE(k.scalar_type() == q.scalar_type() && v.scalar_type() == q.scalar_type(), what, ": q, k and v of ",
+                   q.scalar_type(), ", ", k.scalar_type(), " and ", v.scalar_type());
+  TORCH_CHECK_VALUE(k.device() == q.device() && v.device() == q.device() && decay.device() == q.device(), what,
+                    ": arrays on different devices");
+  m.B = q.size(0);
+  m.T = one ? 1 : q.size(1);
+  m.H = q.size(axes - 2);
+  m.dk = q.size(-1);
+  m.dv = v.size(-1);
+  TORCH_CHECK_VALUE(m.H >= 1 && m.dk >= 1 && m.dv >= 1, what, ": q of ", q.sizes(), " and v of ", v.sizes());
+  m.q = last_contiguous(q);
+  m.k = last_contiguous(k);
+  m.v = last_contiguous(v);
+  m.decay = decay;
+  int i = 0;
+  for (const Tensor* t : {&m.q, &m.k, &m.v, &m.decay})
+    for (int64_t d = 0; d < axes - 1; ++d) m.strides[i++] = t->stride(d);
+  if (state) {
+    TORCH_CHECK_VALUE(state->dim() == 4 && state->size(0) == m.B && state->size(1) == m.H && state->size(2) == m.dk &&
+                          state->size(3) == m.dv && state->device() == q.device(),
+                      what, ": a state of ", state->sizes(), " on ", state->device(), "; expected [", m.B, ", ", m.H, ", ",
+                      m.dk, ", ", m.dv, "] on ", q.device());
+    TORCH_CHECK_TYPE(state->scalar_type() == at::kFloat, what, ": a state of ", state->scalar_type(),
+                     "; expected float32");
+    m.state = one ? *state : state->contiguous();
+  }
+  if (lengths) {
+    require_gpu(*lengths);
+    TORCH_CHECK_VALUE(lengths->dim() == 1 && lengths->size(0) == m.B && lengths->device() == q.device(), what,
+                      ": lengths of ", lengths->sizes(), " on ", lengths->device(), " for ", m.B, " sequences");
+    TORCH_CHECK_TYPE(lengths->scalar_type() == at::kLong || lengths->scalar_type() == at::kInt, what, ": lengths of ",
+                     lengths->scalar_type(), "; expected int64 or int32");
+    m.lengths = lengths->to(at::kLong).contiguous();
+  }
+  return m;
+}
+
+struct Mixed {
+  Tensor out, state, starts;
+};
+
+Mixed linear_attention_fwd(const Mix& m, double scale) {
+  Mixed r;
+  r.out = new_empty({m.B, m.T, m.H, m.dv}, m.q.scalar_type(), m.q);
+  r.state = new_empty({m.B, m.H, m.dk, m.dv}, at::kFloat, m.q);
+  const int64_t floats = pratchya_linear_attention_starts_floats(m.B, m.T, m.H, m.dk, m.dv, m.code);
+  if (floats) r.starts = new_empty({floats}, at::kFloat, m.q);
+  check(pratchya_linear_attention(m.q.data_ptr(), m.k.data_ptr(), m.v.data_ptr(), m.code, m.decay.data_ptr(), m.g_code,
+                                  m.strides.data(), m.length_ptr(), m.state_ptr(), m.B, m.T, m.H, m.dk, m.dv,
+                                  (float)scale, r.out.data_ptr(), static_cast<float*>(r.state.data_ptr()),
+                                  static_cast<float*>(address(r.starts)), stream_of(m.q)),
+        "linear_attention");
+  return r;
+}
+
+// dq, dk, dv, the decays' and the state's gradient, the last two undefined where not needed.
+std::array<Tensor, 5> linear_attention_bwd(Mix m, const Tensor& starts, const Tensor& state_out, const Tensor& dout,
+                                           const Tensor& dstate_out, double scale, bool want_decay, bool want_state) {
+  const char* what = "linear_attention_bwd";
+  // a cotangent of one output only: the other one's is 0
+  Tensor d = dout.defined() ? dout : at::zeros({}, m.q.options()).expand({m.B, m.T, m.H, m.dv});
+  TORCH_CHECK_VALUE(d.dim() == 4 && d.size(0) == m.B && d.size(1) == m.T && d.size(2) == m.H && d.size(3) == m.dv &&
+                        d.scalar_type() == m.q.scalar_type() && d.device() == m.q.device(),
+                    what, ": a cotangent of ", d.sizes(), " ", d.scalar_type());
+  d = last_contiguous(d);
+  for (int i = 0; i < 3; ++i) m.strides[12 + i] = d.stride(i);
+  const Tensor ds = dstate_out.defined() ? dstate_out.to(at::kFloat).contiguous() : Tensor();
+  std::array<Tensor, 5> out;
+  out[0] = new_empty({m.B, m.T, m.H, m.dk}, m.q.scalar_type(), m.q);
+  out[1] = new_empty({m.B, m.T, m.H, m.dk}, m.q.scalar_type(), m.q);
+  out[2] = new_empty({m.B, m.T, m.H, m.dv}, m.q.scalar_type(), m.q);
+  if (want_decay) out[3] = new_empty({m.B, m.T, m.H}, m.decay.scalar_type(), m.q);
+  if (want_state) out[4] = new_empty({m.B, m.H, m.dk, m.dv}, at::kFloat, m.q);
+  const int64_t bytes = pratchya_linear_attention_bwd_workspace_bytes(m.B, m.T, m.H, m.dk, m.dv, m.code);
+  const Tensor ws = bytes ? new_empty({bytes}, at::kByte, m.q) : Tensor();
+  check(pratchya_linear_attention_bwd(
+            m.q.data_ptr(), m.k.data_ptr(), m.v.data_ptr(), m.code, m.decay.data_ptr(), m.g_code, m.strides.data(),
+            m.length_ptr(), m.state_ptr(), static_cast<const float*>(address(state_out)),
+            static_cast<const float*>(address(starts)), d.data_ptr(), static_cast<const float*>(address(ds)), m.B, m.T,
+            m.H, m.dk, m.dv, (float)scale, out[0].data_ptr(), out[1].data_ptr(), out[2].data_ptr(), address(out[3]),
+            static_cast<float*>(address(out[4])), address(ws), bytes, stream_of(m.q)),
+        what);
+  return out;
+}
+
+// --------------------------------------------------------------------------
 // autograd nodes
 // --------------------------------------------------------------------------
 // Gradients of gradients are not computed: with create_graph the results are
@@ -684,6 +798,45 @@ struct PratchyaLinearCrossEntropyBackward : torch::autograd::Node {
   }
 };
 
+struct PratchyaLinearAttentionBackward : torch::autograd::Node {
+  SavedVariable q_, k_, v_, decay_, state_, lengths_, starts_, state_out_;
+  bool has_state_ = false, has_lengths_ = false;
+  double scale_ = 1.0;
+  variable_list apply(variable_list&& grads) override {
+    variable_list out(5);
+    const Tensor dout = grads[0], dstate = grads.size() > 1 ? grads[1] : Tensor();
+    if (!dout.defined() && !dstate.defined()) return out;
+    Tensor q, k, v, decay, starts, state_out;
+    MaybeTensor state, lengths;
+    {
+      const std::lock_guard<std::mutex> lock(mutex_);
+      q = q_.unpack();
+      k = k_.unpack();
+      v = v_.unpack();
+      decay = decay_.unpack();
+      if (has_state_) state = state_.unpack();
+      if (has_lengths_) lengths = lengths_.unpack();
+      starts = starts_.unpack();
+      // read where it meets a cotangent of its own
+      if (dstate.defined()) state_out = state_out_.unpack(shared_from_this());
+    }
+    auto got = [&] {
+      at::NoGradGuard no;
+      const c10::DeviceGuard guard(q.device());
+      const Mix m = mix_args(q, k, v, decay, state, lengths, false, "linear_attention_bwd");
+      return linear_attention_bwd(m, starts, state_out, dout, dstate, scale_, task_should_compute_output(3),
+                                  has_state_ && task_should_compute_output(4));
+    }();
+    for (int i = 0; i < 5; ++i)
+      if (task_should_compute_output(i)) out[i] = std::move(got[i]);
+    return once(std::move(out), "linear_attention");
+  }
+  void release_variables() override {
+    const std::lock_guard<std::mutex> lock(mutex_);
+    for (SavedVariable* s : {&q_, &k_, &v_, &decay_, &state_, &lengths_, &starts_, &state_out_}) s->reset_data();
+  }
+};
+
 bool wants_grad(const Tensor& t) { return t.requires_grad(); }
 bool wants_grad(const MaybeTensor& t) { return t && t->requires_grad(); }
 Tensor or_none(const MaybeTensor& t) { return t ? *t : Tensor(); }
@@ -799,6 +952,63 @@ Tensor linear_cross_entropy(const Tensor& x, const Tensor& weight, const Tensor&
   node->smoothing_ = smoothing;
   torch::autograd::set_history(r.loss, node);
   return r.loss;
+}
+
+Mixed linear_attention(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& decay, const MaybeTensor& state,
+                       const MaybeTensor& lengths, double scale) {
+  const char* what = "linear_attention";
+  for (const Tensor* t : {&q, &k, &v, &decay}) refuse_tangent(*t, what);
+  refuse_tangent(state, what);
+  const bool grad = at::GradMode::is_enabled() &&
+                    (wants_grad(q) || wants_grad(k) || wants_grad(v) || wants_grad(decay) || wants_grad(state));
+  Mixed r;
+  Tensor lens;
+  {
+    at::NoGradGuard no;
+    const c10::DeviceGuard guard(q.device());
+    const Mix m = mix_args(q, k, v, decay, state, lengths, false, what);
+    lens = m.lengths;
+    r = linear_attention_fwd(m, scale);
+  }
+  if (!grad) return r;
+  auto node = new_node<PratchyaLinearAttentionBackward>();
+  node->set_next_edges(torch::autograd::collect_next_edges(q, k, v, decay, or_none(state)));
+  node->q_ = SavedVariable(q, false);
+  node->k_ = SavedVariable(k, false);
+  node->v_ = SavedVariable(v, false);
+  node->decay_ = SavedVariable(decay, false);
+  node->has_state_ = state.has_value();
+  if (state) node->state_ = SavedVariable(*state, false);
+  node->has_lengths_ = lengths.has_value();
+  if (lengths) node->lengths_ = SavedVariable(lens, false);
+  node->starts_ = SavedVariable(r.starts, false);
+  node->scale_ = scale;
+  torch::autograd::set_history(r.out, node);
+  torch::autograd::set_history(r.state, node);
+  node->state_out_ = SavedVariable(r.state, true);
+  return r;
+}
+
+Tensor linear_attention_step(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& decay, const Tensor& state,
+                             double scale) {
+  const char* what = "linear_attention_step";
+  for (const Tensor* t : {&q, &k, &v, &decay, &state}) {
+    refuse_tangent(*t, what);
+    TORCH_CHECK_VALUE(!(at::GradMode::is_enabled() && t->requires_grad()), what,
+                      ": no gradient (the state is updated in place); linear_attention has one");
+  }
+  require_gpu(state);
+  const c10::DeviceGuard guard(q.device());
+  const Mix m = mix_args(q, k, v, decay, state, std::nullopt, true, what);
+  TORCH_CHECK_VALUE(m.state.is_contiguous() && reinterpret_cast<uintptr_t>(m.state.data_ptr()) % 16 == 0, what,
+                    ": the state must be contiguous and 16-byte aligned");
+  const Tensor out = new_empty({m.B, m.H, m.dv}, q.scalar_type(), q);
+  check(pratchya_linear_attention_step(m.q.data_ptr(), m.k.data_ptr(), m.v.data_ptr(), m.code, m.decay.data_ptr(),
+                                       m.g_code, m.strides.data(), static_cast<float*>(m.state.data_ptr()), m.B, m.H,
+                                       m.dk, m.dv, (float)scale, out.data_ptr(), stream_of(q)),
+        what);
+  if (!state.is_inference()) state.unsafeGetTensorImpl()->bump_version();
+  return out;
 }
 
 // --------------------------------------------------------------------------
@@ -989,6 +1199,27 @@ PyObject* py_linear_cross_entropy(PyObject*, PyObject* const* a, Py_ssize_t n) {
   });
 }
 
+PyObject* py_linear_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  return method<7>("linear_attention", n, [&] {
+    const char* what = "linear_attention";
+    const Tensor &q = tensor_arg(a[0], what), &k = tensor_arg(a[1], what), &v = tensor_arg(a[2], what),
+                 &decay = tensor_arg(a[3], what);
+    const MaybeTensor state = maybe_arg(a[4], what), lengths = maybe_arg(a[5], what);
+    const double scale = float_arg(a[6]);
+    const Mixed r = unlocked([&] { return linear_attention(q, k, v, decay, state, lengths, scale); });
+    return wrap_all({wrap(r.out), wrap(r.state)});
+  });
+}
+PyObject* py_linear_attention_step(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  return method<6>("linear_attention_step", n, [&] {
+    const char* what = "linear_attention_step";
+    const Tensor &q = tensor_arg(a[0], what), &k = tensor_arg(a[1], what), &v = tensor_arg(a[2], what),
+                 &decay = tensor_arg(a[3], what), &state = tensor_arg(a[4], what);
+    const double scale = float_arg(a[5]);
+    return wrap(unlocked([&] { return linear_attention_step(q, k, v, decay, state, scale); }));
+  });
+}
+
 #define PRATCHYA_METHOD(name) \
   {#name, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(py_##name)), METH_FASTCALL, nullptr}
 PyMethodDef methods[] = {PRATCHYA_METHOD(layer_norm),         PRATCHYA_METHOD(layer_norm_fwd),
@@ -996,7 +1227,8 @@ PyMethodDef methods[] = {PRATCHYA_METHOD(layer_norm),         PRATCHYA_METHOD(la
                          PRATCHYA_METHOD(activation_fwd),     PRATCHYA_METHOD(activation_bwd),
                          PRATCHYA_METHOD(token_logprobs),     PRATCHYA_METHOD(token_logprobs_fwd),
                          PRATCHYA_METHOD(token_logprobs_bwd), PRATCHYA_METHOD(embedding),
-                         PRATCHYA_METHOD(linear_cross_entropy),
+                         PRATCHYA_METHOD(linear_cross_entropy), PRATCHYA_METHOD(linear_attention),
+                         PRATCHYA_METHOD(linear_attention_step),
                          {nullptr, nullptr, 0, nullptr}};
 #undef PRATCHYA_METHOD
 

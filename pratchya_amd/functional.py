@@ -99,3 +99,37 @@ def linear_cross_entropy(x: torch.Tensor, weight: torch.Tensor, targets: torch.T
     or more gives NaN, as no logit stands for it; its gradient is that of the other
     terms."""
     return _ops.linear_cross_entropy(x, weight, targets, label_smoothing)
+
+
+class LinearAttention(NamedTuple):
+    """Results of ``linear_attention``."""
+    out: torch.Tensor                           # [B, T, H, E], of q's dtype
+    state: torch.Tensor                         # f32 [B, H, D, E]
+
+
+def linear_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log_decay: torch.Tensor,
+                     state: Optional[torch.Tensor] = None, lengths: Optional[torch.Tensor] = None,
+                     scale: float = 1.0) -> LinearAttention:
+    """Linear attention with a decay for each head and token: with a state S [D, E] per
+    sequence and head,
+
+        S_t = exp(log_decay_t) S_(t-1) + k_t^T v_t,      out_t = scale * q_t S_t
+
+    for q, k [B, T, H, D] and v [B, T, H, E] (bf16 or f32, heads of up to 128, rows at
+    any strides) and log_decay [B, T, H] (bf16 or f32; decays that are the same for all
+    tokens are an expanded array; -inf forgets all).  ``state`` is S before the first
+    token, f32 [B, H, D, E], or None for 0; the result holds S behind the last one.
+    Differentiable in all of them, states included.
+
+    ``lengths`` [B] (int64 or int32): tokens from a sequence's length on are padding.
+    They are not read, their outputs and gradients are 0, and the state is that behind
+    the last token before them.  States are f32 throughout."""
+    return LinearAttention(*_ops.linear_attention(q, k, v, log_decay, state, lengths, scale))
+
+
+def linear_attention_step(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log_decay: torch.Tensor,
+                          state: torch.Tensor, scale: float = 1.0) -> torch.Tensor:
+    """One token of ``linear_attention`` for each sequence: q, k [B, H, D], v [B, H, E],
+    log_decay [B, H]; ``state`` (f32 [B, H, D, E], contiguous) is updated in place, and
+    the result is [B, H, E].  For generation: it has no gradient."""
+    return _ops.linear_attention_step(q, k, v, log_decay, state, scale)

@@ -76,3 +76,39 @@ def test_names_without_gpu():
     for call in (lambda: F.embedding(x, t), lambda: F.linear_cross_entropy(x, x.t(), t)):
         with pytest.raises(RuntimeError, match="GPU only"):
             call()
+
+
+def test_linear_attention():
+    L, lib = _L()
+    st = (ctypes.c_int64 * 15)(*[8] * 15)
+
+    def fwd(q=FAKE, dtype=1, g=FAKE, gdt=0, st=st, B=2, T=5, H=3, dk=8, dv=8, out=FAKE, s=FAKE, starts=None):
+        return lib.pratchya_linear_attention(q, q, q, dtype, g, gdt, st, None, None, B, T, H, dk, dv, 1.0, out, s, starts,
+                                             None)
+    assert fwd(B=0) == L.OK
+    for bad in (dict(dtype=2), dict(gdt=2), dict(B=-1), dict(T=-1), dict(H=0), dict(dk=0), dict(dv=0), dict(q=None),
+                dict(g=None), dict(st=None), dict(out=None), dict(s=None), dict(T=4096)):
+        assert fwd(**bad) == L.EINVAL, bad
+        assert b"linear_attention" in lib.pratchya_last_error()
+    for big in (dict(dk=129), dict(dv=129), dict(T=1 << 31), dict(B=1 << 24), dict(B=1 << 25, H=1)):
+        assert fwd(**big) == L.EUNSUPPORTED, big
+    assert lib.pratchya_linear_attention_starts_floats(1, 200, 1, 8, 8, 1) == 0
+    assert lib.pratchya_linear_attention_starts_floats(1, 4096, 1, 8, 8, 1) > 0
+
+    def bwd(q=FAKE, dtype=1, T=5, dk=8, dq=FAKE, dg=FAKE, s=FAKE, ds=FAKE, starts=None, ws=FAKE, ws_bytes=1 << 60):
+        return lib.pratchya_linear_attention_bwd(q, q, q, dtype, FAKE, 0, st, None, None, s, starts, FAKE, ds, 2, T, 3, dk,
+                                                 8, 1.0, dq, FAKE, FAKE, dg, None, ws, ws_bytes, None)
+    for bad in (dict(dtype=2), dict(dk=0), dict(q=None), dict(dq=None), dict(s=None), dict(T=4096), dict(ws=None),
+                dict(ws_bytes=8)):
+        assert bwd(**bad) == L.EINVAL, bad
+        assert b"linear_attention_bwd" in lib.pratchya_last_error()
+    assert bwd(dk=129) == L.EUNSUPPORTED
+
+    def step(q=FAKE, dtype=1, B=2, H=3, dk=8, s=FAKE, out=FAKE):
+        return lib.pratchya_linear_attention_step(q, q, q, dtype, FAKE, 0, st, s, B, H, dk, 8, 1.0, out, None)
+    assert step(B=0) == L.OK
+    for bad in (dict(dtype=3), dict(B=-1), dict(H=0), dict(dk=0), dict(q=None), dict(s=None), dict(out=None),
+                dict(s=ctypes.c_void_p((1 << 20) + 4))):
+        assert step(**bad) == L.EINVAL, bad
+        assert b"linear_attention_step" in lib.pratchya_last_error()
+    assert step(dk=200) == L.EUNSUPPORTED
