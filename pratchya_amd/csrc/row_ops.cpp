@@ -579,15 +579,15 @@ struct Mixed {
   Tensor out, state, starts;
 };
 
-Mixed linear_attention_fwd(const Mix& m, double scale) {
+Mixed linear_attention_fwd(const Mix& m, double scale, bool train) {
   Mixed r;
   r.out = new_empty({m.B, m.T, m.H, m.dv}, m.q.scalar_type(), m.q);
   r.state = new_empty({m.B, m.H, m.dk, m.dv}, at::kFloat, m.q);
-  const int64_t floats = pratchya_linear_attention_starts_floats(m.B, m.T, m.H, m.dk, m.dv, m.code);
+  const int64_t floats = pratchya_linear_attention_starts_floats(m.B, m.T, m.H, m.dk, m.dv, m.code, train);
   if (floats) r.starts = new_empty({floats}, at::kFloat, m.q);
   check(pratchya_linear_attention(m.q.data_ptr(), m.k.data_ptr(), m.v.data_ptr(), m.code, m.decay.data_ptr(), m.g_code,
                                   m.strides.data(), m.length_ptr(), m.state_ptr(), m.B, m.T, m.H, m.dk, m.dv,
-                                  (float)scale, r.out.data_ptr(), static_cast<float*>(r.state.data_ptr()),
+                                  (float)scale, train, r.out.data_ptr(), static_cast<float*>(r.state.data_ptr()),
                                   static_cast<float*>(address(r.starts)), stream_of(m.q)),
         "linear_attention");
   return r;
@@ -968,7 +968,7 @@ Mixed linear_attention(const Tensor& q, const Tensor& k, const Tensor& v, const 
     const c10::DeviceGuard guard(q.device());
     const Mix m = mix_args(q, k, v, decay, state, lengths, false, what);
     lens = m.lengths;
-    r = linear_attention_fwd(m, scale);
+    r = linear_attention_fwd(m, scale, grad);
   }
   if (!grad) return r;
   auto node = new_node<PratchyaLinearAttentionBackward>();

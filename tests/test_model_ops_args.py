@@ -83,7 +83,7 @@ def test_linear_attention():
     st = (ctypes.c_int64 * 15)(*[8] * 15)
 
     def fwd(q=FAKE, dtype=1, g=FAKE, gdt=0, st=st, B=2, T=5, H=3, dk=8, dv=8, out=FAKE, s=FAKE, starts=None):
-        return lib.pratchya_linear_attention(q, q, q, dtype, g, gdt, st, None, None, B, T, H, dk, dv, 1.0, out, s, starts,
+        return lib.pratchya_linear_attention(q, q, q, dtype, g, gdt, st, None, None, B, T, H, dk, dv, 1.0, 1, out, s, starts,
                                              None)
     assert fwd(B=0) == L.OK
     for bad in (dict(dtype=2), dict(gdt=2), dict(B=-1), dict(T=-1), dict(H=0), dict(dk=0), dict(dv=0), dict(q=None),
@@ -92,8 +92,8 @@ def test_linear_attention():
         assert b"linear_attention" in lib.pratchya_last_error()
     for big in (dict(dk=129), dict(dv=129), dict(T=1 << 31), dict(B=1 << 24), dict(B=1 << 25, H=1)):
         assert fwd(**big) == L.EUNSUPPORTED, big
-    assert lib.pratchya_linear_attention_starts_floats(1, 200, 1, 8, 8, 1) == 0
-    assert lib.pratchya_linear_attention_starts_floats(1, 4096, 1, 8, 8, 1) > 0
+    assert lib.pratchya_linear_attention_starts_floats(1, 200, 1, 8, 8, 1, 1) == 0
+    assert lib.pratchya_linear_attention_starts_floats(1, 4096, 1, 8, 8, 1, 1) > 0
 
     def bwd(q=FAKE, dtype=1, T=5, dk=8, dq=FAKE, dg=FAKE, s=FAKE, ds=FAKE, starts=None, ws=FAKE, ws_bytes=1 << 60):
         return lib.pratchya_linear_attention_bwd(q, q, q, dtype, FAKE, 0, st, None, None, s, starts, FAKE, ds, 2, T, 3, dk,
