@@ -46,6 +46,7 @@
 #include <numeric>
 #include <type_traits>
 
+#include "gemm_head.h"
 #include "pratchya_fp8.h"
 #include "quant_device.h"
 
@@ -1427,12 +1428,219 @@ __device__ __forceinline__ void store_tile_ns(const v16f (&acc)[2][4], uint8_t* 
   }
 }
 
+// --------------------------------------------------------------------------
+// Products of an output head's loss (gemm_head.h; FQ 7: store, 8: row statistics,
+// 9: gradient of the logits)
+// --------------------------------------------------------------------------
+struct HeadArgs : FqArgs {
+  uint32_t planes_a, planes_b;       // plane of segment s: 4 bits at 4 s
+  uint32_t pstride_a, pstride_b;     // bytes from a plane to the next
+  int segs;
+  int splits;                        // slices of K, each to a C of its own, split_c elements apart
+  int64_t split_c;
+  int rows, cols;                    // what is stored of C
+  int64_t plane_c;
+  const float* sums;
+  int64_t ld_sums;
+  const int64_t* targets;
+  int64_t v0;
+  float keep, even;                  // 1 - smoothing, smoothing / vocabulary
+  float2* hpart;
+  float* part_sum;
+  float* target_value;
+  int64_t ld_part;
+  const float *stats, *cot;
+};
+
+__device__ __forceinline__ float head_top(float v) { return u2f(f2u(v) & 0xFFFF0000u); }
+
+// This wave's 64 x 128 values at (row0, col0), its rows from row_lo and columns from
+// col_lo on (an edge tile moved back computes its neighbour's again) up to (rows, cols),
+// at any element's address.  The values go through the wave's slice of LDS 16 rows at a
+// time, so that neighbouring lanes store neighbouring pieces of 16 bytes.  PLANE: the
+// value's bf16 piece of that number, the last (LAST) one rounded.
+template <bool OUT_BF16, int PLANE, bool LAST>
+__device__ __forceinline__ void store_tile_head(const v16f (&acc)[2][4], uint8_t* stage, int wave, int lane, void* C,
+                                                int64_t ldc, const float* sums, int64_t ld_sums, int row0, int col0,
+                                                int row_lo, int col_lo, int rows, int cols) {
+  typedef uint32_t u32x4_a2 __attribute__((ext_vector_type(4), aligned(2)));
+  constexpr int ESZ = OUT_BF16 ? 2 : 4, PITCH = 128 * 4 + 16, RP = 16, PER = 16 / ESZ, CHUNKS = 128 / PER;
+  const int l32 = lane & 31, lhi = lane >> 5;
+  uint8_t* stg = stage + wave * (RP * PITCH);
+  __syncthreads();                          // every wave is done with the stage buffer
+#pragma unroll
+  for (int mi = 0; mi < 2; ++mi)
+#pragma unroll
+    for (int p = 0; p < 2; ++p) {
+      if ((l32 / RP) == p) {
+#pragma unroll
+        for (int ni = 0; ni < 4; ++ni)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            float o[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              o[i] = acc[mi][ni][4 * j + i];
+#pragma unroll
+              for (int q = 0; q < PLANE; ++q) o[i] -= head_top(o[i]);
+              if (!LAST) o[i] = head_top(o[i]);
+            }
+            *reinterpret_cast<float4*>(stg + (l32 % RP) * PITCH + (ni * 32 + 8 * j + 4 * lhi) * 4) =
+                make_float4(o[0], o[1], o[2], o[3]);
+          }
+      }
+      __builtin_amdgcn_s_waitcnt(0xC07F);   // lgkmcnt(0): this wave's staging writes are done
+#pragma unroll
+      for (int it = 0; it < RP * CHUNKS / 64; ++it) {
+        const int q = it * 64 + lane, c = q % CHUNKS * PER, r = q / CHUNKS;
+        const int row = row0 + mi * 32 + p * RP + r, col = col0 + c;
+        const uint8_t* from = stg + r * PITCH + c * 4;
+        float v[PER];
+#pragma unroll
+        for (int i = 0; i < PER; i += 4) {
+          const float4 w = *reinterpret_cast<const float4*>(from + i * 4);
+          v[i] = w.x;
+          v[i + 1] = w.y;
+          v[i + 2] = w.z;
+          v[i + 3] = w.w;
+        }
+        if (row < row_lo || row >= rows || col >= cols) continue;
+        if (sums) {
+#pragma unroll
+          for (int i = 0; i < PER; i += 4) {
+            const float4 w = *reinterpret_cast<const float4*>(sums + (int64_t)row * ld_sums + col + i);
+            v[i] += w.x;
+            v[i + 1] += w.y;
+            v[i + 2] += w.z;
+            v[i + 3] += w.w;
+          }
+        }
+        u32x4_a2 o;
+        if constexpr (OUT_BF16) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) o[i] = pack_bf16x2(v[2 * i], v[2 * i + 1]);
+        } else {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) o[i] = f2u(v[i]);
+        }
+        uint8_t* to = static_cast<uint8_t*>(C) + ((int64_t)row * ldc + col) * ESZ;
+        if (col >= col_lo && col + PER <= cols) {
+          *reinterpret_cast<u32x4_a2*>(to) = o;
+        } else {
+#pragma unroll
+          for (int i = 0; i < PER; ++i)
+            if (col + i >= col_lo && col + i < cols) {
+              if constexpr (OUT_BF16) reinterpret_cast<uint16_t*>(to)[i] = (uint16_t)(i & 1 ? o[i >> 1] >> 16 : o[i >> 1]);
+              else reinterpret_cast<uint32_t*>(to)[i] = o[i];
+            }
+        }
+      }
+      __builtin_amdgcn_s_waitcnt(0xC07F);   // staging reads done before the next pass overwrites
+    }
+}
+
+// Row statistics of this wave's 64 x 128 logits: per row the maximum m, the sum of
+// e^(z - m), both without the target's, and the sum of all (label smoothing); the
+// target's logit apart, so that a loss near 0 keeps its digits.  A lane holds half of
+// two rows' columns, lane + 32 the other half.
+__device__ __forceinline__ void head_rows(v16f (&acc)[2][4], const HeadArgs& p, int lane, int row0, int col0,
+                                          int col_lo, int half) {
+  const int l32 = lane & 31, lhi = lane >> 5;
+#pragma unroll
+  for (int mi = 0; mi < 2; ++mi) {
+    const int row = row0 + mi * 32 + l32;
+    const int64_t target = p.targets[min(row, p.rows - 1)];
+    // columns of the 128 that count, and the target's place among them (or none)
+    const int lo = max(col_lo - col0, 0), hi = min(p.cols - col0, 128);
+    const int64_t rel = target < 0 ? -1 : target - p.v0 - col0;
+    const int tc = rel >= lo && rel < hi ? (int)rel : -1;
+    float sum = 0.0f;
+    if (lo == 0 && hi == 128 && !__any(tc >= 0)) {
+      if (p.part_sum) {
+#pragma unroll
+        for (int ni = 0; ni < 4; ++ni)
+#pragma unroll
+          for (int v = 0; v < 16; ++v) sum += acc[mi][ni][v];
+      }
+    } else {
+      const int first = lo - 4 * lhi, end = hi - 4 * lhi, at = tc < 0 ? -8 : tc - 4 * lhi;
+      float value = 0.0f;
+#pragma unroll
+      for (int ni = 0; ni < 4; ++ni)
+#pragma unroll
+        for (int v = 0; v < 16; ++v) {
+          const int c = ni * 32 + 8 * (v >> 2) + (v & 3);
+          float z = acc[mi][ni][v];
+          const bool in = c >= first && c < end;
+          sum += in ? z : 0.0f;
+          value = c == at ? z : value;
+          z = in && c != at ? z : -__builtin_inff();
+          asm volatile("" : "+v"(z));       // one after the other: no 128 results of comparisons at once
+          acc[mi][ni][v] = z;
+        }
+      if (tc >= 0 && ((tc >> 2) & 1) == lhi && row < p.rows) p.target_value[row] = value;
+    }
+    sum += __shfl_xor(sum, 32, 64);
+    float m = -3.4028234663852886e38f;
+#pragma unroll
+    for (int ni = 0; ni < 4; ++ni)
+#pragma unroll
+      for (int v = 0; v < 16; ++v) m = fmaxf(m, acc[mi][ni][v]);
+    m = fmaxf(m, __shfl_xor(m, 32, 64));
+    float s = 0.0f;
+#pragma unroll
+    for (int ni = 0; ni < 4; ++ni)
+#pragma unroll
+      for (int v = 0; v < 16; ++v) s += __expf(acc[mi][ni][v] - m);
+    s += __shfl_xor(s, 32, 64);
+    if (lhi == 0 && row < p.rows) {
+      const int64_t at = (int64_t)row * p.ld_part + half;
+      p.hpart[at] = make_float2(m, s);
+      if (p.part_sum) p.part_sum[at] = sum;
+    }
+  }
+}
+
+// The logits of this wave's 64 x 128 turned into the loss's gradient of them.
+__device__ __forceinline__ void head_grad(v16f (&acc)[2][4], const HeadArgs& p, int lane, int row0, int col0) {
+  const int l32 = lane & 31, lhi = lane >> 5;
+#pragma unroll
+  for (int mi = 0; mi < 2; ++mi) {
+    const int row = min(row0 + mi * 32 + l32, p.rows - 1);
+    const int64_t target = p.targets[row], rel = target - p.v0 - col0;
+    const float m = p.stats[2 * row], logs = p.stats[2 * row + 1] * 1.44269504f, g = target < 0 ? 0.0f : p.cot[row];
+    const int tc = target >= 0 && rel >= 0 && rel < 128 ? (int)rel : -1, hi = p.cols - col0;
+    const float ge = g * p.even, gt = g * p.keep;
+#pragma unroll
+    for (int ni = 0; ni < 4; ++ni)
+#pragma unroll
+      for (int v = 0; v < 16; ++v) {
+        const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(acc[mi][ni][v] - m, 1.44269504f, -logs));
+        acc[mi][ni][v] = __builtin_fmaf(g, e, -ge);
+      }
+    if (hi < 128 || __any(tc >= 0 || target < 0)) {
+      const int end = target < 0 ? -8 : hi - 4 * lhi, at = tc < 0 ? -8 : tc - 4 * lhi;
+#pragma unroll
+      for (int ni = 0; ni < 4; ++ni)
+#pragma unroll
+        for (int v = 0; v < 16; ++v) {
+          const int c = ni * 32 + 8 * (v >> 2) + (v & 3);
+          float d = acc[mi][ni][v];
+          d -= c == at ? gt : 0.0f;
+          d = c < end ? d : 0.0f;
+          asm volatile("" : "+v"(d));
+          acc[mi][ni][v] = d;
+        }
+    }
+  }
+}
+
 template <bool OUT_BF16, int BG, int FQ, bool BF = false, int KM = 0, bool QA = false>
 __global__ __launch_bounds__(NTHREADS, 1) void k_gemm_bs_nt(
     const uint8_t* __restrict__ A, int64_t lda, const uint8_t* __restrict__ B, int64_t ldb,
     Scales sa, Scales sb, void* __restrict__ C, int64_t ldc, int K, int span, int tiles_m,
     int tiles_n, uint32_t a_bytes, uint32_t b_bytes, uint32_t ea_bytes, uint32_t eb_bytes,
-    uint32_t ga_bytes, uint32_t gb_bytes, int M, int N, FqArgs fq,
+    uint32_t ga_bytes, uint32_t gb_bytes, int M, int N, std::conditional_t<(FQ >= 7), HeadArgs, FqArgs> fq,
     std::conditional_t<QA, QaArgs, QaNone> qa) {
   static_assert(!QA || (!BF && KM == 0 && FQ <= 2), "the quantize prologue feeds an FP8 A operand");
   __shared__ __attribute__((aligned(1024))) uint8_t lds[LDS_BYTES + ((FQ == 1 || FQ == 2) ? FQ_TABLE_BYTES : 0) +
@@ -1446,7 +1654,17 @@ __global__ __launch_bounds__(NTHREADS, 1) void k_gemm_bs_nt(
   const int grp = wave >> 2;              // ping-pong group
   const int wm = wave & 3, wn = grp;      // 64-row band wm, 128-column half wn
   int nk = K / BK;                        // K steps of the current unit
+  // Products of an output head: segments of planes one after the other.  A wave loads
+  // its operand's stages in order, so their offsets advance from one to the next.
+  constexpr bool HEAD = FQ >= 7;
+  static_assert(!HEAD || BF, "an output head's operands are bf16");
+  const int spp = nk;                     // K steps of a segment
   const int T = tiles_m * tiles_n;
+  int units = T;                          // tiles times slices of K, slice by slice
+  if constexpr (HEAD) {
+    nk = nk * fq.segs / fq.splits;
+    units = T * fq.splits;
+  }
   // the Gram product (upper-triangle tiles by stream-K, FQ 4); operands
   // given K-major (KM bit 0: A, bit 1: B; read through the LDS transposing
   // loads) or K-contiguous
@@ -1493,6 +1711,44 @@ __global__ __launch_bounds__(NTHREADS, 1) void k_gemm_bs_nt(
     r.e_word = (uint32_t)blk_index(so, (int64_t)rb0 + w4 * 64 + lane, 0);
     r.kb = kb_;
     return r;
+  };
+  uint32_t head_at = 0;                   // bytes to the next stage's K values in the operand
+  int head_k = 0, head_seg = 0, head_left = nk, head_unit = (int)blockIdx.x;
+  auto head_plane = [&] {
+    if constexpr (HEAD)
+      head_at = grp == 0 ? ((fq.planes_a >> (4 * head_seg)) & 15u) * fq.pstride_a
+                         : ((fq.planes_b >> (4 * head_seg)) & 15u) * fq.pstride_b;
+  };
+  auto head_start = [&] {                 // at the first step of head_unit's slice
+    if constexpr (HEAD) {
+      const int first = head_unit < units ? head_unit / T * nk : 0;
+      head_seg = first / spp;
+      head_k = first - head_seg * spp;
+      head_plane();
+      head_at += (uint32_t)head_k * (kmaj ? 64u * h.ld : (uint32_t)BK);
+    }
+  };
+  auto head_next = [&] {                  // the next stage's offset: this one's, then on
+    const uint32_t at = head_at;
+    if constexpr (HEAD) {
+      head_at += kmaj ? 64u * h.ld : (uint32_t)BK;
+      if (--head_left == 0) {
+        head_left = nk;
+        head_unit += (int)gridDim.x;
+        head_start();
+      } else if (++head_k == spp) {
+        head_k = 0;
+        ++head_seg;
+        head_plane();
+      }
+    }
+    return at;
+  };
+  head_start();
+  auto head_stage = [&](const DmaRows& r, uint8_t* st) {
+    const uint32_t at = head_next() + (kmaj ? r.row0 * 2u + h.krow0 * h.ld : r.row0 * h.ld);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) dma_rows_at(h, at, st + h.lds_pay, i, kmaj ? 2u : 8u);
   };
   // K block of a unit's first step: 0 except for the segments of a Gram range
   auto kb_of = [&](const DmaRows& r) { return GRAM ? r.kb : 0; };
@@ -1545,7 +1801,7 @@ __global__ __launch_bounds__(NTHREADS, 1) void k_gemm_bs_nt(
   int64_t g = 0, g_end = 0;               // Gram: the range's next and end steps
   auto next_tile = [&](int t_, int* tm_, int* tn_) {
     if constexpr (FQ == 1 || FQ == 2) tile_of_fq(t_, tiles_m, tiles_n, fq.xcd != 0, tm_, tn_);
-    else tile_of(t_, tiles_m, tiles_n, tm_, tn_);
+    else tile_of(HEAD ? t_ % T : t_, tiles_m, tiles_n, tm_, tn_);
   };
   // Gram unit starting at step g_: tile q_, its K blocks [kb_, kb_ + nk_)
   auto gram_unit = [&](int64_t g_, int* q_, int* tm_, int* tn_, int* kb_, int* nk_) {
@@ -1575,8 +1831,12 @@ __global__ __launch_bounds__(NTHREADS, 1) void k_gemm_bs_nt(
   // (it is one stage ahead of group 0 throughout).  The wave's last stage
   // DMA, not yet published: g_pub (a span start), its group max g_ld, its
   // buffer g_st, g_first (a tile's K block 0).
+  if constexpr (HEAD) {
+    head_stage(cur, lds);
+  } else {
 #pragma unroll
-  for (int i = 0; i < 8; ++i) stage_rows(cur, lds, kb_of(cur), i);
+    for (int i = 0; i < 8; ++i) stage_rows(cur, lds, kb_of(cur), i);
+  }
   float g_ld = 0.0f, u_prev = 1.0f;
   if constexpr (!BF) {
     dma_scales(h, cur, lds, 0);
@@ -1593,7 +1853,7 @@ __global__ __launch_bounds__(NTHREADS, 1) void k_gemm_bs_nt(
     int t_next = t + (int)gridDim.x, kb2 = 0, nk2 = nk;
     bool has_next;
     if constexpr (GRAM) has_next = g + nk < g_end;
-    else has_next = t_next < T;
+    else has_next = t_next < units;
     int tm2 = 0, tn2 = 0;
     DmaRows nxt = cur;
     if (has_next) {
@@ -1604,8 +1864,12 @@ __global__ __launch_bounds__(NTHREADS, 1) void k_gemm_bs_nt(
     if (grp == 1) {
       if (1 < nk) {
         uint8_t* s1 = lds + ((1 + par) & 1) * STAGE_BYTES;
+        if constexpr (HEAD) {
+          head_stage(cur, s1);
+        } else {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) stage_rows(cur, s1, 1 + kb_of(cur), i);
+          for (int i = 0; i < 8; ++i) stage_rows(cur, s1, 1 + kb_of(cur), i);
+        }
         if constexpr (!BF) {
           dma_scales(h, cur, s1, 1);
           g_pub = span == 1;
@@ -1730,8 +1994,14 @@ __global__ __launch_bounds__(NTHREADS, 1) void k_gemm_bs_nt(
         const int lkt = to_next ? 0 : dkt;            // K block inside the tile loaded
         uint8_t* dst = lds + ((dkt + par) & 1) * STAGE_BYTES;
         constexpr uint32_t KESZ = BF ? 2u : 1u, KROWS = BK / KESZ, KRPI = 1024 / (256 * KESZ);
-        const uint32_t soff0 = kmaj ? dr.row0 * KESZ + ((uint32_t)(lkt + kb_of(dr)) * KROWS + h.krow0) * h.ld
-                                    : dr.row0 * h.ld + (uint32_t)(lkt + kb_of(dr)) * BK;
+        uint32_t soff0;
+        if constexpr (HEAD) {
+          soff0 = kmaj ? dr.row0 * KESZ + h.krow0 * h.ld : dr.row0 * h.ld;
+          if (dma_now) soff0 += head_next();
+        } else {
+          soff0 = kmaj ? dr.row0 * KESZ + ((uint32_t)(lkt + kb_of(dr)) * KROWS + h.krow0) * h.ld
+                       : dr.row0 * h.ld + (uint32_t)(lkt + kb_of(dr)) * BK;
+        }
         const uint32_t drows = kmaj ? KRPI : 8u;
         uint8_t* const lds0 = dst + h.lds_pay;
         pin_frags(fa, fb);
@@ -1795,6 +2065,25 @@ __global__ __launch_bounds__(NTHREADS, 1) void k_gemm_bs_nt(
         gram_add_partials(acc, fq, (int)blockIdx.x, (int)gridDim.x, t, wave, lane);
         store_tile_gram(acc, lds + ((nk - 1 + par) & 1) * STAGE_BYTES, wave, lane, C, ldc, m0 + wm * 64,
                         n0 + wn * 128, tm != tn);
+      }
+    } else if constexpr (HEAD) {
+      uint8_t* stage = lds + ((nk - 1 + par) & 1) * STAGE_BYTES;
+      const int row0 = m0 + wm * 64, col0 = n0 + wn * 128, col_lo = tn * BN;
+      if constexpr (FQ == 7) {
+        uint8_t* c = static_cast<uint8_t*>(C) + t / T * fq.split_c * (OUT_BF16 ? 2 : 4);
+        store_tile_head<OUT_BF16, 0, true>(acc, stage, wave, lane, c, ldc, fq.sums, fq.ld_sums, row0, col0, tm * BM, col_lo,
+                                           fq.rows, fq.cols);
+      } else if constexpr (FQ == 8) {
+        head_rows(acc, fq, lane, row0, col0, col_lo, 2 * tn + wn);
+      } else {
+        head_grad(acc, fq, lane, row0, col0);
+        uint16_t* c = static_cast<uint16_t*>(C);
+        constexpr bool ONE = FQ == 9;
+        store_tile_head<true, 0, ONE>(acc, stage, wave, lane, c, ldc, nullptr, 0, row0, col0, 0, 0, fq.rows, N);
+        if constexpr (!ONE) {
+          store_tile_head<true, 1, false>(acc, stage, wave, lane, c + fq.plane_c, ldc, nullptr, 0, row0, col0, 0, 0, fq.rows, N);
+          store_tile_head<true, 2, true>(acc, stage, wave, lane, c + 2 * fq.plane_c, ldc, nullptr, 0, row0, col0, 0, 0, fq.rows, N);
+        }
       }
     } else if constexpr (FQ == 3) {
       static_assert(BF && OUT_BF16, "the Newton-Schulz epilogue combines bf16 products");
@@ -2459,6 +2748,86 @@ extern "C" int pratchya_gemm_bf16_nt_ns(const void* A, int64_t lda, const void* 
   if (b_kmajor) bf16_launch<true, 3, 2>(P, A, lda, B, ldb, C, ldc, M, N, K, fq, stream);
   else bf16_launch<true, 3>(P, A, lda, B, ldb, C, ldc, M, N, K, fq, stream);
   return launch_status("gemm_bf16_ns");
+}
+
+// --------------------------------------------------------------------------
+// Products of an output head's loss
+// --------------------------------------------------------------------------
+bool head_product_fits(const HeadProduct& p) {
+  const int64_t a_last = p.a_kmajor ? (p.K - 1) * p.lda + p.M : (p.M - 1) * p.lda + p.K;
+  const int64_t b_last = p.b_kmajor ? (p.K - 1) * p.ldb + p.N : (p.N - 1) * p.ldb + p.K;
+  const int64_t held = p.segs > 1 ? 2 : 0;          // planes behind the first
+  return p.M >= BM && p.N >= BN && p.M <= INT32_MAX / 2 && p.N <= INT32_MAX / 2 && p.K >= 64 && p.K % 64 == 0 &&
+         (!p.a_kmajor || p.M % 8 == 0) && (!p.b_kmajor || p.N % 8 == 0) &&
+         p.lda >= (p.a_kmajor ? p.M : p.K) && p.ldb >= (p.b_kmajor ? p.N : p.K) && p.lda % 8 == 0 && p.ldb % 8 == 0 &&
+         p.a_plane % 8 == 0 && p.b_plane % 8 == 0 && !((uintptr_t)p.a % 16) && !((uintptr_t)p.b % 16) &&
+         2 * (held * p.a_plane + a_last) <= INT32_MAX && 2 * (held * p.b_plane + b_last) <= INT32_MAX &&
+         p.segs * (p.K / 64) <= (1 << 24) && p.splits >= 1 && p.segs * (p.K / 64) % p.splits == 0;
+}
+
+namespace {
+
+template <bool OB, int FQ, int KM>
+void head_launch(const HeadProduct& p, const HeadArgs& h, int64_t a_bytes, int64_t b_bytes, hipStream_t stream) {
+  const int64_t tm = (p.M + BM - 1) / BM, tn = (p.N + BN - 1) / BN, cus = gemm_num_cus();
+  const int64_t units = tm * tn * p.splits;
+  hipLaunchKernelGGL((k_gemm_bs_nt<OB, 0, FQ, true, KM>), dim3((unsigned)(units < cus ? units : cus)), dim3(NTHREADS), 0,
+                     stream, reinterpret_cast<const uint8_t*>(p.a), p.lda * 2, reinterpret_cast<const uint8_t*>(p.b),
+                     p.ldb * 2, Scales{nullptr, nullptr, 1, 0, 0, 1}, Scales{nullptr, nullptr, 1, 0, 0, 1}, p.c, p.ldc,
+                     (int)(p.K * 2), 1, (int)tm, (int)tn, (uint32_t)a_bytes, (uint32_t)b_bytes, 0u, 0u, 0u, 0u, (int)p.M,
+                     (int)p.N, h, QaNone{});
+}
+
+}  // namespace
+
+int head_product(const HeadProduct& p, hipStream_t stream) {
+  const char* who = "linear_cross_entropy";
+  if (!head_product_fits(p)) return pratchya_set_error(PRATCHYA_EUNSUPPORTED, "%s: a product's operands", who);
+  HeadArgs h{};
+  h.planes_a = p.a_planes;
+  h.planes_b = p.b_planes;
+  h.pstride_a = (uint32_t)(2 * p.a_plane);
+  h.pstride_b = (uint32_t)(2 * p.b_plane);
+  h.segs = p.segs;
+  h.splits = p.splits;
+  h.split_c = p.split_c;
+  h.rows = (int)p.rows;
+  h.cols = (int)p.cols;
+  h.plane_c = p.plane_c;
+  h.sums = p.sums;
+  h.ld_sums = p.ld_sums;
+  h.targets = p.targets;
+  h.v0 = p.v0;
+  h.keep = 1.0f - p.smooth;
+  h.even = p.smooth / (float)p.vocab;
+  h.hpart = p.part;
+  h.part_sum = p.part_sum;
+  h.target_value = p.target_value;
+  h.ld_part = p.ld_part;
+  h.stats = p.stats;
+  h.cot = p.g;
+  const int64_t held = p.segs > 1 ? 2 : 0;
+  const int64_t ab = 2 * (held * p.a_plane + (p.a_kmajor ? (p.K - 1) * p.lda + p.M : (p.M - 1) * p.lda + p.K));
+  const int64_t bb = 2 * (held * p.b_plane + (p.b_kmajor ? (p.K - 1) * p.ldb + p.N : (p.N - 1) * p.ldb + p.K));
+  const int km = (p.a_kmajor ? 1 : 0) | (p.b_kmajor ? 2 : 0);
+  if (km == 1) return pratchya_set_error(PRATCHYA_EUNSUPPORTED, "%s: a K-major left operand alone", who);
+  if (p.epilogue == kHeadStore) {
+    if (km == 0) p.c_bf16 ? head_launch<true, 7, 0>(p, h, ab, bb, stream) : head_launch<false, 7, 0>(p, h, ab, bb, stream);
+    else if (km == 2) p.c_bf16 ? head_launch<true, 7, 2>(p, h, ab, bb, stream) : head_launch<false, 7, 2>(p, h, ab, bb, stream);
+    else p.c_bf16 ? head_launch<true, 7, 3>(p, h, ab, bb, stream) : head_launch<false, 7, 3>(p, h, ab, bb, stream);
+  } else if (km == 3) {
+    return pratchya_set_error(PRATCHYA_EUNSUPPORTED, "%s: a K-major left operand", who);
+  } else if (p.epilogue == kHeadRows) {
+    if (km == 0) head_launch<false, 8, 0>(p, h, ab, bb, stream);
+    else head_launch<false, 8, 2>(p, h, ab, bb, stream);
+  } else if (p.planes == 1) {
+    if (km == 0) head_launch<true, 9, 0>(p, h, ab, bb, stream);
+    else head_launch<true, 9, 2>(p, h, ab, bb, stream);
+  } else {
+    if (km == 0) head_launch<true, 10, 0>(p, h, ab, bb, stream);
+    else head_launch<true, 10, 2>(p, h, ab, bb, stream);
+  }
+  return launch_status(who);
 }
 
 // --------------------------------------------------------------------------

@@ -8,13 +8,21 @@
 // A negative target stands for none: l = 0 and dz = 0.  A target of V or more has no
 // logit: l is NaN and dz the formula's without its second term.
 //
-// The vocabulary is taken in pieces: a piece's logits are computed in f32, enter the
-// rows' running maxima and sums (forward) or turn into dz (backward, from lse), and
-// are overwritten by the next piece's.  In f32 every operand of a product is the sum
-// of three exact bf16 planes and a product six products of planes.
+// From 256 rows on, logits are not written: the product's epilogue (head_product) takes
+// each row's maximum and sum of 128 columns, which k_head_join joins, or turns its tile
+// into dz (backward, from lse), of which a piece of the vocabulary is held at a time.
+// Below, a piece's f32 logits are computed, read by k_head_rows or k_head_grad and
+// overwritten by the next piece's.  In f32 every operand of a product is the sum of three
+// exact bf16 planes and a product six products of planes.
+//
+// Bound: the MFMAs' rate on 256-row tiles, 1.1 PFLOP/s of four products (logits twice) where
+// a large product alone reaches 1.27 and the library's 1.5: [8192, 4096] . [4096, 65536] in
+// bf16, both passes, 16.0 ms (19.4 with the logits written and 128-row tiles); f32
+// [1000, 1027] . [1027, 50021] 3.2 ms, the tiles' last of four rounds nearly empty.
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
+#include "gemm_head.h"
 #include "pratchya_fp8.h"
 #include "row_device.h"
 #include "row_host.h"
@@ -97,71 +105,92 @@ __device__ __forceinline__ void finish_row(const Seen& a, int64_t target, int64_
   }
 }
 
-// A piece's logits [rows, cols], columns v0 .. of the vocabulary, into the rows'
-// states: one workgroup a row.  The last piece's call finishes them.
-constexpr int kRowThreads = 256;
-
-__device__ __forceinline__ Seen join_seen(Seen a, float* lds) {
-  const float m = wave_max(a.m);
-  if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = m;
-  __syncthreads();
-  float M = lds[0];
-#pragma unroll
-  for (int w = 1; w < kRowThreads / 64; ++w) M = fmaxf(M, lds[w]);
-  a.s = a.s == 0.0f ? 0.0f : a.s * expf(fmaxf(a.m - M, kLowest));
-  a.m = M;
-  a.s = block_add<kRowThreads / 64>(a.s, lds);
-  a.sum = block_add<kRowThreads / 64>(a.sum, lds);
-  return a;
-}
+// Statistics of kRowColumns of a row's logits, as the products' epilogue gives them of 128
+// (gemm_head.h): one workgroup a row and part of a piece [rows, cols], whose column 0 is
+// v0 of the vocabulary.  (128 rows of 32768 by a workgroup each took 22 us.)
+constexpr int kRowThreads = 256, kRowColumns = 4096;
 
 __global__ __launch_bounds__(kRowThreads) void k_head_rows(const float* __restrict__ z, int64_t ld, int64_t cols,
                                                            const int64_t* __restrict__ targets, int64_t v0,
-                                                           int64_t vocab, float smooth, float4* __restrict__ state,
-                                                           int first, int last, float* __restrict__ loss,
-                                                           float* __restrict__ stats) {
+                                                           float2* __restrict__ part, float* __restrict__ part_sum,
+                                                           int64_t ld_part, float* __restrict__ target_value) {
   __shared__ float lds[kRowThreads / 64];
-  __shared__ float shared_zt;
-  const int64_t row = blockIdx.x, target = targets[row];
+  const int64_t row = blockIdx.x, target = targets[row], tc = target < 0 ? -1 : target - v0;
+  const int64_t lo = (int64_t)blockIdx.y * kRowColumns, hi = lo + kRowColumns < cols ? lo + kRowColumns : cols;
   const float* p = z + row * ld;
-  // the target's column in this piece, or none
-  const int64_t tc = target >= 0 && target < vocab ? target - v0 : -1;
-  Seen a;
-  for (int64_t c = threadIdx.x * 4; c < cols; c += kRowThreads * 4) {
-    float v[4];
-    if (c + 4 <= cols) widen(load_raw(p + c), v);
-    else load_some(p + c, cols - c, -__builtin_inff(), v);
-    float top = a.m;
+  float v[kRowColumns / kRowThreads / 4][4], m = kLowest, s = 0.0f, sum = 0.0f;
+#pragma unroll
+  for (int i = 0; i < kRowColumns / kRowThreads / 4; ++i) {
+    const int64_t c = lo + (i * kRowThreads + threadIdx.x) * 4;
+    if (c + 4 <= hi) widen(load_raw(p + c), v[i]);
+    else load_some(p + c, hi - c, -__builtin_inff(), v[i]);
+  }
+#pragma unroll
+  for (int i = 0; i < kRowColumns / kRowThreads / 4; ++i) {
+    const int64_t c = lo + (i * kRowThreads + threadIdx.x) * 4;
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
-      if (c + k < cols) a.sum += v[k];
-      if (c + k == tc) {
-        shared_zt = v[k];
-        v[k] = -__builtin_inff();
+      if (c + k < hi) sum += v[i][k];
+      if (c + k == tc && c + k < hi) {
+        target_value[row] = v[i][k];
+        v[i][k] = -__builtin_inff();
       }
-      top = fmaxf(top, v[k]);
+      m = fmaxf(m, v[i][k]);
     }
-    if (top > a.m) {
-      a.s *= expf(fmaxf(a.m - top, kLowest));
-      a.m = top;
-    }
+  }
+  m = wave_max(m);
+  if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = m;
+  __syncthreads();
 #pragma unroll
-    for (int k = 0; k < 4; ++k) a.s += expf(v[k] - a.m);
-  }
-  a = join_seen(a, lds);
+  for (int w = 0; w < kRowThreads / 64; ++w) m = fmaxf(m, lds[w]);
+#pragma unroll
+  for (int i = 0; i < kRowColumns / kRowThreads / 4; ++i)
+#pragma unroll
+    for (int k = 0; k < 4; ++k) s += expf(v[i][k] - m);
+  s = block_add<kRowThreads / 64>(s, lds);
+  if (part_sum) sum = block_add<kRowThreads / 64>(sum, lds);
   if (threadIdx.x) return;
-  if (tc >= 0 && tc < cols) a.zt = shared_zt;
-  if (!first) {
-    const float4 b = state[row];
-    const float M = fmaxf(a.m, b.x);
-    a.s = (a.s == 0.0f ? 0.0f : a.s * expf(fmaxf(a.m - M, kLowest))) +
-          (b.y == 0.0f ? 0.0f : b.y * expf(fmaxf(b.x - M, kLowest)));
-    a.m = M;
-    if (!(tc >= 0 && tc < cols)) a.zt = b.z;
-    a.sum += b.w;
+  const int64_t at = row * ld_part + blockIdx.y;
+  part[at] = make_float2(m, s);
+  if (part_sum) part_sum[at] = sum;
+}
+
+// The rows' losses from the statistics of their parts: one wave a row.
+__global__ __launch_bounds__(256) void k_head_join(const float2* __restrict__ part, const float* __restrict__ part_sum,
+                                                   int64_t ld, int64_t held, const float* __restrict__ target_value,
+                                                   int64_t n,
+                                                   const int64_t* __restrict__ targets, int64_t vocab, float smooth,
+                                                   float* __restrict__ loss, float* __restrict__ stats) {
+  const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+  const int lane = threadIdx.x & 63;
+  if (row >= n) return;
+  const float2* p = part + row * ld;
+  float m = kLowest;
+  for (int64_t i = lane; i < held; i += 64) m = fmaxf(m, p[i].x);
+  Seen a;
+  a.m = wave_max(m);
+  for (int64_t i = lane; i < held; i += 64) {
+    const float2 v = p[i];
+    if (v.y != 0.0f) a.s += v.y * expf(fmaxf(v.x - a.m, kLowest));
+    if (part_sum) a.sum += part_sum[row * ld + i];
   }
-  if (last) finish_row(a, target, vocab, smooth, loss + row, stats ? stats + 2 * row : nullptr);
-  else state[row] = make_float4(a.m, a.s, a.zt, a.sum);
+#pragma unroll
+  for (int k = 32; k; k >>= 1) {
+    a.s += __shfl_xor(a.s, k, 64);
+    a.sum += __shfl_xor(a.sum, k, 64);
+  }
+  if (lane) return;
+  const int64_t target = targets[row];
+  if (target >= 0 && target < vocab) a.zt = target_value[row];
+  finish_row(a, target, vocab, smooth, loss + row, stats ? stats + 2 * row : nullptr);
+}
+
+// Zeros in the planes' rows [rows, rows_to), which the product of the gradients reads.
+__global__ __launch_bounds__(256) void k_head_zero_rows(uint16_t* __restrict__ dst, int64_t plane, int64_t ld, int64_t rows,
+                                                        int64_t rows_to) {
+  const int64_t per = ld / 8, i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (i >= (rows_to - rows) * per) return;
+  *reinterpret_cast<u32x4_t*>(dst + blockIdx.y * plane + (rows + i / per) * ld + i % per * 8) = u32x4_t{};
 }
 
 // dz of a piece's logits as planes [P][rows_to][cols_to], zeros around [rows, cols].
@@ -203,17 +232,24 @@ __global__ __launch_bounds__(256) void k_head_grad(const float* __restrict__ z, 
   }
 }
 
-// out [rows, cols] (contiguous, or ld_out apart) = src [rows, cols], f32 ld_src apart,
+// out [rows, cols] (contiguous, or ld_out apart) = src [slices][rows, cols], f32 ld_src
+// apart, summed,
 // plus the sums of the pieces before (sum, if add); not the last piece: into sum.
 template <typename T>
 __global__ __launch_bounds__(256) void k_head_out(const float* __restrict__ src, int64_t ld_src, int64_t rows,
                                                   int64_t cols, float* __restrict__ sum, int add, int last,
-                                                  T* __restrict__ out, int64_t ld_out) {
+                                                  T* __restrict__ out, int64_t ld_out, int slices) {
   const int64_t per = (cols + 3) / 4, i = (int64_t)blockIdx.x * 256 + threadIdx.x;
   if (i >= rows * per) return;
   const int64_t r = i / per, c = (i - r * per) * 4;
   float v[4];
   widen(load_raw(src + r * ld_src + c), v);
+  for (int s = 1; s < slices; ++s) {
+    float o[4];
+    widen(load_raw(src + s * rows * ld_src + r * ld_src + c), o);
+#pragma unroll
+    for (int k = 0; k < 4; ++k) v[k] += o[k];
+  }
   if (add) {
     float o[4];
     widen(load_raw(sum + r * ld_src + c), o);
@@ -248,11 +284,46 @@ struct Head {
   int P;
   int64_t n64, C64, piece;       // piece: columns of a vocabulary piece, a multiple of 64
   bool x_direct, w_direct;
+  // rows of dz lie apart from each other's memory channels ([4096, 65536] . [65536, 2048]
+  // 4183 us of a step without, 4117 with)
+  int64_t pad() const { return fused ? 64 : 0; }
+  bool fused;                    // logits on 256-row tiles, what follows them in the product's epilogue
+  int64_t parts, ld_part;        // of a row of a piece, of the whole row: what statistics are taken of
+  int64_t parts_of(int64_t cols) const { return fused ? 2 * ((cols + 255) / 256) : (cols + kRowColumns - 1) / kRowColumns; }
   // workspace
-  int64_t xp, wp, z, dzp, dx_sum, dx_tmp, dw_tmp, split, split_bytes, state, bytes;
+  int64_t part, part_sum, zt;
+  int64_t xp, wp, z, dzp, dx_sum, dx_tmp, dw_tmp, split, split_bytes, bytes;
 };
 
 bool aligned16(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
+
+// Slices of K for which a product of [M, N] over `steps` goes to the 256-row tiles, 0 if it
+// does not.  One workgroup a compute unit takes one tile of one slice after the other; where
+// 3/10 of the last round are idle, the 128-row tiles are as fast ([4096, 65536] . [65536,
+// 2048] in bf16: 1186 us there, 128 tiles in two slices here).
+int on256(const Head& h, int64_t M, int64_t N, int64_t steps, int most) {
+  if (!h.fused || M < 256 || N < 256) return 0;
+  const int64_t tiles = ((M + 255) / 256) * ((N + 255) / 256);
+  int best = 0;
+  double best_use = 0.699;
+  for (int s = 1; s <= most && (s == 1 || steps / s >= 16); ++s) {
+    if (steps % s) continue;
+    const int64_t units = tiles * s, rounds = (units + 255) / 256;
+    const double use = (double)units / (double)(rounds * 256);
+    if (use > best_use + 0.03) {
+      best = s;
+      best_use = use;
+    }
+  }
+  return best;
+}
+
+// The gradient of x from a piece of Vp columns.
+int dx256(const Head& h, int64_t Vp) { return on256(h, h.n, h.C64, (h.P == 1 ? 1 : 6) * (Vp / 64), 16); }
+// The weight's gradient of a piece of Vp columns.
+bool dw256(const Head& h, int64_t Vp) {
+  return on256(h, h.rows ? Vp : h.C64, h.rows ? h.C64 : Vp, 1, 1) != 0;
+}
 
 // Sizes and workspace of a call; direct: whether x and w themselves are operands.
 int plan(const char* what, bool bwd, bool want_dx, bool want_dw, Head* h) {
@@ -275,15 +346,26 @@ int plan(const char* what, bool bwd, bool want_dx, bool want_dw, Head* h) {
                 2 * (h->n + 128) * h->ldx <= kMaxOffset;
   h->w_direct = bf && h->C % 64 == 0 && h->V % 64 == 0 && h->ldw % 8 == 0 && h->ldw >= (h->rows ? h->C : h->V) &&
                 aligned16(h->w) && 2 * ((h->rows ? 1152 : h->C + 1) * h->ldw + 128) <= kMaxOffset;
-  int64_t piece = kPieceBytes / 4 / (h->n64 ? h->n64 : 64) / 64 * 64;
-  const int64_t by_w = 2 * kPieceBytes / (2 * h->P * h->C64) / 64 * 64;       // its planes: 512 MB
-  if (!h->w_direct && by_w < piece) piece = by_w;
-  const int64_t by_ld = (kMaxOffset / 2 / h->P / (h->n64 > h->C64 ? h->n64 + 128 : h->C64 + 128)) / 64 * 64;
-  if (by_ld < piece) piece = by_ld;
+  // on 256-row tiles, whose operands' offsets have 31 bits
+  const int64_t planes = 2 * h->P, segs = h->P == 1 ? 1 : 6, wide = h->n64 > h->C64 ? h->n64 : h->C64;
+  h->fused = h->n >= 256 && h->C64 >= 256 && V64 >= 256 && planes * wide * 2560 <= INT32_MAX &&
+             planes * h->n64 * h->C64 <= INT32_MAX && (!h->x_direct || 2 * h->n * h->ldx <= INT32_MAX) &&
+             (!h->w_direct || 2 * (h->rows ? 2560 : h->C) * h->ldw <= INT32_MAX);
+  const int64_t unit = h->fused ? 256 : 64;
+  // what of a piece is kept: f32 logits, or only the planes of their gradient; the planes
+  // of its weight: 512 MB
+  int64_t piece = !h->fused ? kPieceBytes / 4 / (h->n64 ? h->n64 : 64) : bwd ? 2 * kPieceBytes / planes / h->n64 : V64;
+  auto bound = [&](int64_t by) { piece = by < piece ? by : piece; };
+  if (!h->w_direct) bound(2 * kPieceBytes / planes / h->C64);
+  if (!h->fused) bound(kMaxOffset / planes / (wide + 128));
+  else if (h->w_direct && h->rows) bound(INT32_MAX / 4 / h->ldw);
+  if (piece < V64) piece = piece / unit * unit;
   if (piece < 1024) piece = 1024;
   // pieces of one size
   const int64_t pieces = (V64 + piece - 1) / piece;
-  h->piece = up64((V64 + pieces - 1) / pieces);
+  h->piece = ((V64 + pieces - 1) / pieces + unit - 1) / unit * unit;
+  if (h->fused)
+    while (h->piece < V64 && (V64 - 1) % h->piece + 1 < 256) h->piece += 256;      // the last one: a tile or more
   if (h->piece > V64) h->piece = V64;
   int64_t at = 0;
   auto take = [&](int64_t bytes) {
@@ -291,11 +373,14 @@ int plan(const char* what, bool bwd, bool want_dx, bool want_dw, Head* h) {
     at += round256(bytes);
     return p;
   };
-  const int64_t planes = 2 * h->P, segs = h->P == 1 ? 1 : 6;
   h->xp = take(planes * h->n64 * h->C64);
   h->wp = take(h->w_direct ? 0 : planes * h->C64 * h->piece);
-  h->z = take(4 * h->n * h->piece);
-  h->state = take(16 * h->n);
+  h->parts = h->parts_of(h->piece);
+  h->ld_part = (V64 + h->piece - 1) / h->piece * h->parts;
+  h->part = take(bwd ? 0 : 8 * h->n * h->ld_part);
+  h->part_sum = take(bwd ? 0 : 4 * h->n * h->ld_part);
+  h->zt = take(bwd ? 0 : 4 * h->n);
+  h->z = take(h->fused ? 0 : 4 * h->n * h->piece);
   h->split_bytes = 0;
   auto split = [&](int64_t M, int64_t N, int64_t K) {
     const int64_t b = pratchya_gemm_t128_workspace_bytes(M, N, segs * (K / 64), 1);
@@ -303,21 +388,27 @@ int plan(const char* what, bool bwd, bool want_dx, bool want_dw, Head* h) {
   };
   const int64_t rest = V64 - (V64 - 1) / h->piece * h->piece;      // the last piece
   for (int64_t Vp : {h->piece, rest}) {
-    split(h->n, Vp, h->C64);
-    if (bwd && want_dx) split(h->n, h->C64, Vp);
-    if (bwd && want_dw) {
+    if (!h->fused) split(h->n, Vp, h->C64);
+    if (bwd && want_dx && !dx256(*h, Vp)) split(h->n, h->C64, Vp);
+    if (bwd && want_dw && !dw256(*h, Vp)) {
       split(h->rows ? Vp : h->C64, h->rows ? h->C64 : Vp, h->n64);
       split(h->rows ? Vp : h->C, h->rows ? h->C : Vp, h->n64);
     }
   }
   h->dzp = h->dx_sum = h->dx_tmp = h->dw_tmp = 0;
   if (bwd) {
-    h->dzp = take(planes * h->n64 * h->piece);
+    h->dzp = take(planes * h->n64 * (h->piece + h->pad()));
     if (want_dx) {
-      h->dx_tmp = take(4 * h->n * h->C64);
+      int64_t slices = 0;
+      for (int64_t Vp : {h->piece, rest}) {
+        const int s = dx256(*h, Vp);
+        const int64_t need = s == 1 ? 0 : s ? s : 1;
+        if (need > slices) slices = need;
+      }
+      h->dx_tmp = take(4 * slices * h->n * h->C64);
       h->dx_sum = take(h->piece < h->V ? 4 * h->n * h->C64 : 0);
     }
-    if (want_dw) h->dw_tmp = take(4 * h->C64 * h->piece);
+    if (want_dw && !(dw256(*h, h->piece) && dw256(*h, rest))) h->dw_tmp = take(4 * h->C64 * h->piece);
   }
   h->split = take(h->split_bytes);
   h->bytes = at;
@@ -343,6 +434,30 @@ struct Call {
       hipLaunchKernelGGL((k_head_planes<float, 3>), dim3((unsigned)blocks), dim3(256), 0, stream,
                          static_cast<const float*>(src), ld, rows, cols, rows_to, cols_to, dst);
     return check_launch("linear_cross_entropy");
+  }
+  // The same on 256-row tiles.
+  HeadProduct product256(const uint16_t* A, int64_t lda, int64_t a_rows, bool a_kmajor, const uint16_t* B, int64_t ldb,
+                         int64_t b_rows, bool b_kmajor, int64_t M, int64_t N, int64_t K) const {
+    HeadProduct p{};
+    p.a = A;
+    p.b = B;
+    p.lda = lda;
+    p.ldb = ldb;
+    p.a_plane = h.P == 1 ? 0 : a_rows * lda;
+    p.b_plane = h.P == 1 ? 0 : b_rows * ldb;
+    p.a_kmajor = a_kmajor;
+    p.b_kmajor = b_kmajor;
+    p.a_planes = h.P == 1 ? 0 : kPairsA;
+    p.b_planes = h.P == 1 ? 0 : kPairsB;
+    p.segs = h.P == 1 ? 1 : 6;
+    p.splits = 1;
+    p.planes = h.P;
+    p.M = M;
+    p.N = N;
+    p.K = K;
+    p.rows = M;
+    p.cols = N;
+    return p;
   }
   // C [M, N] = A . B over K; a plane's rows lie lda / ldb apart, planes a_rows * lda.
   int product(const uint16_t* A, int64_t lda, int64_t a_rows, int a_kmajor, const uint16_t* B, int64_t ldb,
@@ -397,19 +512,51 @@ int logits(const Call& c, const Operands& o, int64_t Vp) {
                    PRATCHYA_DT_F32);
 }
 
+HeadProduct logits_product(const Call& c, const Operands& o, int64_t v0, int64_t cols, const int64_t* targets,
+                           float smooth) {
+  const Head& h = c.h;
+  HeadProduct p = c.product256(o.x, o.ldx, o.x_rows, false, o.w, o.ldw, o.w_rows, !h.rows, h.n, up64(cols), h.C64);
+  p.rows = h.n;
+  p.cols = cols;
+  p.targets = targets;
+  p.v0 = v0;
+  p.vocab = h.V;
+  p.smooth = smooth;
+  return p;
+}
+
 int forward(const Call& c, const int64_t* targets, float smooth, float* loss, float* stats) {
   const Head& h = c.h;
   Operands o;
   int rc = operand_x(c, &o);
   for (int64_t v0 = 0; v0 < h.V && !rc; v0 += h.piece) {
     const int64_t cols = h.V - v0 < h.piece ? h.V - v0 : h.piece, Vp = up64(cols);
-    if ((rc = operand_w(c, v0, cols, Vp, &o)) || (rc = logits(c, o, Vp))) break;
-    hipLaunchKernelGGL(k_head_rows, dim3((unsigned)h.n), dim3(kRowThreads), 0, c.stream, c.floats_at(h.z), Vp, cols,
-                       targets, v0, h.V, smooth, reinterpret_cast<float4*>(c.ws + h.state), v0 == 0,
-                       v0 + h.piece >= h.V, loss, stats);
-    rc = check_launch("linear_cross_entropy");
+    if ((rc = operand_w(c, v0, cols, Vp, &o))) break;
+    const int64_t at = v0 / h.piece * h.parts;
+    float2* part = reinterpret_cast<float2*>(c.ws + h.part) + at;
+    float* part_sum = smooth != 0.0f ? c.floats_at(h.part_sum) + at : nullptr;
+    if (h.fused) {
+      HeadProduct p = logits_product(c, o, v0, cols, targets, smooth);
+      p.epilogue = kHeadRows;
+      p.part = part;
+      p.part_sum = part_sum;
+      p.target_value = c.floats_at(h.zt);
+      p.ld_part = h.ld_part;
+      rc = head_product(p, c.stream);
+    } else if (!(rc = logits(c, o, Vp))) {
+      hipLaunchKernelGGL(k_head_rows, dim3((unsigned)h.n, (unsigned)h.parts_of(cols)), dim3(kRowThreads), 0, c.stream,
+                         c.floats_at(h.z), Vp, cols, targets, v0, part, part_sum, h.ld_part, c.floats_at(h.zt));
+      rc = check_launch("linear_cross_entropy");
+    }
   }
-  return rc;
+  if (rc) return rc;
+  // the last piece may have fewer parts than the others
+  const int64_t last = (h.V - 1) / h.piece, rest = h.V - last * h.piece;
+  const int64_t held = last * h.parts + h.parts_of(h.fused ? up64(rest) : rest);
+  hipLaunchKernelGGL(k_head_join, dim3((unsigned)((h.n + 3) / 4)), dim3(256), 0, c.stream,
+                     reinterpret_cast<const float2*>(c.ws + h.part), smooth != 0.0f ? c.floats_at(h.part_sum) : nullptr,
+                     h.ld_part, held, c.floats_at(h.zt), h.n, targets, h.V, smooth, loss, stats);
+  return check_launch("linear_cross_entropy");
 }
 
 template <typename T>
@@ -421,37 +568,91 @@ int backward(const Call& c, const int64_t* targets, float smooth, const float* s
   int rc = operand_x(c, &o);
   for (int64_t v0 = 0; v0 < h.V && !rc; v0 += h.piece) {
     const int64_t cols = h.V - v0 < h.piece ? h.V - v0 : h.piece, Vp = up64(cols);
-    if ((rc = operand_w(c, v0, cols, Vp, &o)) || (rc = logits(c, o, Vp))) break;
+    if ((rc = operand_w(c, v0, cols, Vp, &o))) break;
+    const int64_t ldz = Vp + h.pad();
     uint16_t* dz = c.planes_at(h.dzp);
-    const int64_t blocks = (h.n64 * (Vp / 8) + 255) / 256;
-    if (!fits_launch(blocks, 256)) return pratchya_set_error(PRATCHYA_EUNSUPPORTED, "%s: too large", what);
-    auto grad = h.P == 1 ? k_head_grad<1> : k_head_grad<3>;
-    hipLaunchKernelGGL(grad, dim3((unsigned)blocks), dim3(256), 0, c.stream, c.floats_at(h.z), Vp, h.n, cols, h.n64, Vp,
-                       targets, v0, h.V, smooth, stats, g, dz);
-    if ((rc = check_launch(what))) break;
-    if (dx) {
+    if (h.fused) {
+      HeadProduct p = logits_product(c, o, v0, cols, targets, smooth);
+      p.epilogue = kHeadGrad;
+      p.c = dz;
+      p.ldc = ldz;
+      p.plane_c = h.n64 * ldz;
+      p.stats = stats;
+      p.g = g;
+      if ((rc = head_product(p, c.stream))) break;
+      if (h.n64 > h.n) {
+        hipLaunchKernelGGL(k_head_zero_rows, dim3((unsigned)(((h.n64 - h.n) * (ldz / 8) + 255) / 256), (unsigned)h.P), dim3(256),
+                           0, c.stream, dz, p.plane_c, ldz, h.n, h.n64);
+        if ((rc = check_launch(what))) break;
+      }
+    } else {
+      if ((rc = logits(c, o, Vp))) break;
+      const int64_t blocks = (h.n64 * (Vp / 8) + 255) / 256;
+      if (!fits_launch(blocks, 256)) return pratchya_set_error(PRATCHYA_EUNSUPPORTED, "%s: too large", what);
+      auto grad = h.P == 1 ? k_head_grad<1> : k_head_grad<3>;
+      hipLaunchKernelGGL(grad, dim3((unsigned)blocks), dim3(256), 0, c.stream, c.floats_at(h.z), Vp, h.n, cols, h.n64, Vp,
+                         targets, v0, h.V, smooth, stats, g, dz);
+      if ((rc = check_launch(what))) break;
+    }
+    const int slices = dx ? dx256(h, Vp) : 0;
+    if (slices) {
+      const bool first = v0 == 0, last = v0 + h.piece >= h.V;
+      HeadProduct p = c.product256(dz, ldz, h.n64, false, o.w, o.ldw, o.w_rows, h.rows, h.n, h.C64, Vp);
+      p.epilogue = kHeadStore;
+      if (slices > 1) {
+        p.splits = slices;
+        p.c = c.floats_at(h.dx_tmp);
+        p.ldc = h.C64;
+        p.split_c = h.n * h.C64;
+      } else {
+        p.cols = last ? h.C : h.C64;
+        p.c = last ? static_cast<void*>(dx) : c.floats_at(h.dx_sum);
+        p.ldc = last ? h.C : h.C64;
+        p.c_bf16 = last && h.P == 1;
+        p.sums = first ? nullptr : c.floats_at(h.dx_sum);
+        p.ld_sums = h.C64;
+      }
+      if ((rc = head_product(p, c.stream))) break;
+      if (slices > 1) {
+        hipLaunchKernelGGL((k_head_out<T>), dim3((unsigned)((h.n * ((h.C + 3) / 4) + 255) / 256)), dim3(256), 0, c.stream,
+                           c.floats_at(h.dx_tmp), h.C64, h.n, h.C, c.floats_at(h.dx_sum), !first, last, dx, h.C, slices);
+        if ((rc = check_launch(what))) break;
+      }
+    } else if (dx) {
       float* tmp = c.floats_at(h.dx_tmp);
-      rc = c.product(dz, Vp, h.n64, 0, o.w, o.ldw, o.w_rows, h.rows ? 1 : 0, h.n, h.C64, Vp, tmp, h.C64, PRATCHYA_DT_F32);
+      rc = c.product(dz, ldz, h.n64, 0, o.w, o.ldw, o.w_rows, h.rows ? 1 : 0, h.n, h.C64, Vp, tmp, h.C64, PRATCHYA_DT_F32);
       if (rc) break;
       hipLaunchKernelGGL((k_head_out<T>), dim3((unsigned)((h.n * ((h.C + 3) / 4) + 255) / 256)), dim3(256), 0, c.stream,
-                         tmp, h.C64, h.n, h.C, c.floats_at(h.dx_sum), v0 > 0, v0 + h.piece >= h.V, dx, h.C);
+                         tmp, h.C64, h.n, h.C, c.floats_at(h.dx_sum), v0 > 0, v0 + h.piece >= h.V, dx, h.C, 1);
       if ((rc = check_launch(what))) break;
     }
     if (dw) {
       // [C, V]: rows C, columns cols of them; [V, C]: rows cols, columns C
       const int64_t M = h.rows ? cols : h.C, N = h.rows ? h.C : cols, ld = h.rows ? h.C : h.V;
       T* to = dw + (h.rows ? v0 * h.C : v0);
+      if (dw256(h, Vp)) {
+        HeadProduct p = h.rows ? c.product256(dz, ldz, h.n64, true, o.x, o.ldx, o.x_rows, true, Vp, h.C64, h.n64)
+                               : c.product256(o.x, o.ldx, o.x_rows, true, dz, ldz, h.n64, true, h.C64, Vp, h.n64);
+        p.epilogue = kHeadStore;
+        p.rows = M;
+        p.cols = N;
+        p.c = to;
+        p.ldc = ld;
+        p.c_bf16 = h.P == 1;
+        if ((rc = head_product(p, c.stream))) break;
+        continue;
+      }
       const bool direct = M > 32 && M % 8 == 0 && N % 8 == 0 && ld % chunk == 0 && aligned16(to);
       const int64_t Mt = direct ? M : up64(M), Nt = direct ? N : up64(N);
       void* out = direct ? static_cast<void*>(to) : c.ws + h.dw_tmp;
       const int type = direct ? h.dtype : PRATCHYA_DT_F32;
       const int64_t ldo = direct ? ld : Nt;
-      rc = h.rows ? c.product(dz, Vp, h.n64, 1, o.x, o.ldx, o.x_rows, 1, Mt, Nt, h.n64, out, ldo, type)
-                  : c.product(o.x, o.ldx, o.x_rows, 1, dz, Vp, h.n64, 1, Mt, Nt, h.n64, out, ldo, type);
+      rc = h.rows ? c.product(dz, ldz, h.n64, 1, o.x, o.ldx, o.x_rows, 1, Mt, Nt, h.n64, out, ldo, type)
+                  : c.product(o.x, o.ldx, o.x_rows, 1, dz, ldz, h.n64, 1, Mt, Nt, h.n64, out, ldo, type);
       if (rc) break;
       if (!direct) {
         hipLaunchKernelGGL((k_head_out<T>), dim3((unsigned)((M * ((N + 3) / 4) + 255) / 256)), dim3(256), 0, c.stream,
-                           c.floats_at(h.dw_tmp), Nt, M, N, nullptr, 0, 1, to, ld);
+                           c.floats_at(h.dw_tmp), Nt, M, N, nullptr, 0, 1, to, ld, 1);
         rc = check_launch(what);
       }
     }
