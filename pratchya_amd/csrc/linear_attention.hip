@@ -65,12 +65,14 @@ struct MixArgs {
   int g_bf16;
   const int64_t* lengths;          // [B], or null
   const float* init;               // state before a segment: [B H][nseg] of [.., ..], or null
-  float* last;                     // state after the walk; without outputs: of every segment but its last
-  float* decay;                    // without outputs: e^(sum of a segment's log decays), [B H][nseg]
+  float* last;                     // state after the walk; without outputs: of the parts of every segment but the
+                                   // walk's last, in the walk's order
+  float* decay;                    // without outputs: e^(sum of a part's log decays)
   float* dot;                      // [B H][T]: x times what the output has from the state before the chunk
   int64_t init_seg, last_seg;      // elements from a segment's state to the next one's
   int init_r, init_c, last_r, last_c;   // strides of a state's query and value axes
   int B, T, H, dq, dv, nseg, per;  // per: chunks of a segment
+  int parts, per_part;             // without outputs: parts of a segment, chunks of a part
   int rev;
   float scale, kscale;             // of outputs, of what enters the state
 };
@@ -534,12 +536,24 @@ __global__ __launch_bounds__(kThreads, NS == 1 && DP + EP == 128 ? 3 : 2) void k
   __shared__ M m;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int l16 = lane & 15, g4 = lane >> 4;
-  const int segs = OUT ? p.nseg : p.nseg - 1;      // OUT false: the walk's last segment is not needed
-  const int bh = blockIdx.x / segs, walk = blockIdx.x - bh * segs;
+  const int units = OUT ? p.nseg : (p.nseg - 1) * p.parts;      // OUT false: the walk's last segment is not needed
+  const int bh = blockIdx.x / units, unit = blockIdx.x - bh * units, walk = OUT ? unit : unit / p.parts;
   const int b = bh / p.H, h = bh - b * p.H, seg = p.rev ? p.nseg - 1 - walk : walk;
   int64_t length = p.T;
   if (p.lengths) length = min(max(p.lengths[b], (int64_t)0), (int64_t)p.T);
-  const int chunks = (p.T + L - 1) / L, c_lo = seg * p.per, c_hi = min(c_lo + p.per, chunks), n = max(c_hi - c_lo, 0);
+  const int chunks = (p.T + L - 1) / L;
+  int c_lo = seg * p.per, c_hi = min(c_lo + p.per, chunks);
+  if constexpr (!OUT) {
+    const int before = (unit - walk * p.parts) * p.per_part;
+    if (p.rev) {
+      c_hi -= before;
+      c_lo = max(c_lo, c_hi - p.per_part);
+    } else {
+      c_lo += before;
+      c_hi = min(c_hi, c_lo + p.per_part);
+    }
+  }
+  const int n = max(c_hi - c_lo, 0);
   auto first_of = [&](int i) { return (p.rev ? c_hi - 1 - i : c_lo + i) * L; };     // chunk i of the walk
 
   Rows<T, L, DP, kThreads, FULL> rq(OUT ? p.q : p.k, b, h, length, p.dq), rk(p.k, b, h, length, p.dq);
@@ -668,25 +682,28 @@ __global__ __launch_bounds__(kThreads, NS == 1 && DP + EP == 128 ? 3 : 2) void k
   }
 
   if (p.last && (!OUT || walk == p.nseg - 1)) {
-    float* to = p.last + (OUT ? (int64_t)bh * p.last_seg : ((int64_t)bh * p.nseg + seg) * p.last_seg);
+    float* to = p.last + (OUT ? (int64_t)bh : (int64_t)blockIdx.x) * p.last_seg;
     S.each(p.dq, p.dv, wave, lane, [&](float& s, int d, int e) { to[(int64_t)d * p.last_r + (int64_t)e * p.last_c] = s; });
   }
-  if (!OUT && threadIdx.x == 0) p.decay[(int64_t)bh * p.nseg + seg] = (float)exp(sum_all);
+  if (!OUT && threadIdx.x == 0) p.decay[blockIdx.x] = (float)exp(sum_all);
 }
 
-// The states before the segments from the segments' own: states[walk] holds what its
-// segment adds and becomes the state before it.
-__global__ __launch_bounds__(256) void k_mix_join(float* __restrict__ states, const float* __restrict__ decay,
-                                                  const float* __restrict__ init, int64_t size, int nseg, int rev) {
+// The states before the segments, in the walk's order, from the parts' own.
+__global__ __launch_bounds__(256) void k_mix_join(float* __restrict__ states, const float* __restrict__ parts,
+                                                  const float* __restrict__ decay, const float* __restrict__ init,
+                                                  int64_t size, int nseg, int per, int rev) {
   const int64_t bh = blockIdx.x, e = (int64_t)blockIdx.y * 256 + threadIdx.x;
   if (e >= size) return;
+  const int64_t first = bh * (nseg - 1) * per;
   float s = init ? init[bh * size + e] : 0.0f;
-  for (int w = 0; w < nseg; ++w) {
-    const int seg = rev ? nseg - 1 - w : w;
-    float* at = states + (bh * nseg + seg) * size + e;
-    const float add = w + 1 < nseg ? *at : 0.0f;
-    *at = s;
-    if (w + 1 < nseg) s = decay[bh * nseg + seg] * s + add;
+  for (int w = 0;; ++w) {
+    states[(bh * nseg + (rev ? nseg - 1 - w : w)) * size + e] = s;
+    if (w + 1 == nseg) return;
+#pragma unroll 4
+    for (int i = 0; i < per; ++i) {
+      const int64_t at = first + w * per + i;
+      s = decay[at] * s + parts[at * size + e];
+    }
   }
 }
 
@@ -1056,10 +1073,20 @@ struct Shape {
     return (chunks() + n - 1) / n;
   }
   int64_t state() const { return dk * dv; }
-  // states before the segments, and the segments' decays
+  // Parts of a segment whose states are taken at once: about four workgroups a compute
+  // unit, of two chunks or more.
+  int64_t parts() const {
+    const int64_t units = B * H * (segments() - 1), most = per() / 2;
+    if (units < 1) return 1;
+    int64_t n = 1024 / units;
+    if (n > most) n = most;
+    return n < 1 ? 1 : n;
+  }
+  // states before the segments; of their parts, with their decays
+  int64_t states_floats() const { return B * H * segments() * state(); }
   int64_t starts_floats() const {
     const int64_t n = segments();
-    return n > 1 ? B * H * n * (state() + 1) : 0;
+    return n > 1 ? states_floats() + B * H * (n - 1) * parts() * (state() + 1) : 0;
   }
 };
 
@@ -1070,7 +1097,7 @@ int check_shape(const char* what, const Shape& s, int g_dtype) {
     return pratchya_set_error(PRATCHYA_EINVAL, "%s: [%lld, %lld, %lld] of heads of %lld and %lld", what, (long long)s.B,
                               (long long)s.T, (long long)s.H, (long long)s.dk, (long long)s.dv);
   if (s.dk > kMaxHead || s.dv > kMaxHead || s.T > 0x7FFFFF00 || s.B > (1 << 24) || s.H > (1 << 24) ||
-      !fits_launch(s.B * s.H * s.segments(), kThreads))
+      !fits_launch(s.B * s.H * s.segments() * s.parts(), 2 * kThreads))
     return pratchya_set_error(PRATCHYA_EUNSUPPORTED, "%s: heads of more than %d, or 2^24 heads of segments", what, kMaxHead);
   return PRATCHYA_OK;
 }
@@ -1108,7 +1135,7 @@ void launch_mix_as(const MixArgs& a, unsigned blocks, hipStream_t stream) {
 }
 
 int launch_mix(const Shape& s, const MixArgs& a, bool out, hipStream_t stream) {
-  const int64_t blocks = s.B * s.H * (out ? a.nseg : a.nseg - 1);
+  const int64_t blocks = s.B * s.H * (out ? a.nseg : (a.nseg - 1) * a.parts);
   if (!blocks) return PRATCHYA_OK;
   if (s.dtype == PRATCHYA_DT_BF16) {
     if (!out) launch_mix_as<uint16_t, 1, 1, 64, false>(a, (unsigned)blocks, stream);
@@ -1133,13 +1160,6 @@ int launch_back(const Shape& s, const BackArgs& a, hipStream_t stream) {
     else hipLaunchKernelGGL((k_mix_back<T, L, D, V, false>), dim3(blocks), dim3(2 * kThreads), 0, stream, a);
   });
   return check_launch("linear_attention_bwd");
-}
-
-int join(const Shape& s, float* starts, const float* init, int rev, hipStream_t stream) {
-  const int64_t n = s.segments(), size = s.state();
-  hipLaunchKernelGGL(k_mix_join, dim3((unsigned)(s.B * s.H), (unsigned)((size + 255) / 256)), dim3(256), 0, stream,
-                     starts, starts + s.B * s.H * n * size, init, size, (int)n, rev);
-  return check_launch("linear_attention");
 }
 
 // What all walks of a call share.
@@ -1167,14 +1187,19 @@ Array packed(const Shape& s, const void* p, int64_t d) {
 // The states before the segments (rev: behind them), where there are several.
 int segment_states(const Shape& s, MixArgs a, float* starts, const float* init, hipStream_t stream) {
   if (a.nseg < 2) return PRATCHYA_OK;
-  const int64_t size = s.state();
-  a.last = starts;
+  const int64_t size = s.state(), n = s.B * s.H * (a.nseg - 1) * s.parts();
+  a.parts = (int)s.parts();
+  a.per_part = (a.per + a.parts - 1) / a.parts;
+  a.last = starts + s.states_floats();
   a.last_seg = size;
   a.last_r = a.dv;
   a.last_c = 1;
-  a.decay = starts + s.B * s.H * a.nseg * size;
+  a.decay = a.last + n * size;
   const int rc = launch_mix(s, a, false, stream);
-  return rc ? rc : join(s, starts, init, a.rev, stream);
+  if (rc) return rc;
+  hipLaunchKernelGGL(k_mix_join, dim3((unsigned)(s.B * s.H), (unsigned)((size + 255) / 256)), dim3(256), 0, stream,
+                     starts, a.last, a.decay, init, size, a.nseg, a.parts, a.rev);
+  return check_launch("linear_attention");
 }
 
 // Outputs from the states before the segments.  transposed: the state is held as
