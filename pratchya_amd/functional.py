@@ -91,8 +91,9 @@ def linear_cross_entropy(x: torch.Tensor, weight: torch.Tensor, targets: torch.T
     """Softmax cross entropy of the output head ``z = x @ weight``, for x [..., C],
     weight [C, V] of x's dtype and targets [...] (int64 or int32): f32 [...],
     ``(1 - a) (lse - z_t) + a (lse - mean z)`` with a the label smoothing,
-    differentiable in x and weight.  The logits are not kept: both passes compute them
-    in pieces of the vocabulary, in f32.  An embedding table [V, C] serves as weight
+    differentiable in x and weight.  The logits are not kept: both passes compute them,
+    in f32; their gradient, of a piece of the vocabulary at a time, is rounded to x's dtype
+    before the products that give the gradients of x and weight.  An embedding table [V, C] serves as weight
     through its transposed view ``table.t()``, which is read as it lies.
 
     A negative target stands for none: its loss is 0 and has no gradient.  A target of V
@@ -123,7 +124,9 @@ def linear_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log_deca
 
     ``lengths`` [B] (int64 or int32): tokens from a sequence's length on are padding.
     They are not read, their outputs and gradients are 0, and the state is that behind
-    the last token before them.  States are f32 throughout."""
+    the last token before them.  States are f32 throughout.  Long sequences are cut into
+    segments, into more of them where no gradient is recorded: the results then differ in
+    roundings."""
     return LinearAttention(*_ops.linear_attention(q, k, v, log_decay, state, lengths, scale))
 
 
