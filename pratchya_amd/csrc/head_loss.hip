@@ -38,16 +38,18 @@ __device__ __forceinline__ float top_piece(float v) { return u2f(f2u(v) & 0xFFFF
 
 // Planes [P][rows_to][cols_to] of src [rows, cols] (rows ld elements apart, at any
 // element's address), zeros around it: bf16 as it is (P 1) or an f32 value's three
-// pieces (P 3), 8 columns a thread.
+// pieces (P 3), 8 columns a thread.  Rows whose target (targets, if not null) is negative
+// are zeros: 0 times what padding holds would be NaN in the weight's gradient.
 template <typename T, int P>
 __global__ __launch_bounds__(256) void k_head_planes(const T* __restrict__ src, int64_t ld, int64_t rows, int64_t cols,
-                                                     int64_t rows_to, int64_t cols_to, uint16_t* __restrict__ dst) {
+                                                     int64_t rows_to, int64_t cols_to,
+                                                     const int64_t* __restrict__ targets, uint16_t* __restrict__ dst) {
   const int64_t per = cols_to / 8, i = (int64_t)blockIdx.x * 256 + threadIdx.x;
   if (i >= rows_to * per) return;
   const int64_t r = i / per, c = (i - r * per) * 8;
   uint16_t* to = dst + r * cols_to + c;
   float v[8] = {};
-  if (r < rows && c < cols) {
+  if (r < rows && c < cols && !(targets && targets[r] < 0)) {
     const T* p = src + r * ld + c;
     if (c + 8 <= cols) {
       constexpr int N = kN<T>;
@@ -342,7 +344,7 @@ int plan(const char* what, bool bwd, bool want_dx, bool want_dw, Head* h) {
     return pratchya_set_error(PRATCHYA_EUNSUPPORTED, "%s: rows or weights beyond 32-bit offsets", what);
   const bool bf = h->dtype == PRATCHYA_DT_BF16;
   if (!fits_launch(h->n, kRowThreads)) return pratchya_set_error(PRATCHYA_EUNSUPPORTED, "%s: 2^24 rows or more", what);
-  h->x_direct = bf && h->n % 64 == 0 && h->C % 64 == 0 && h->ldx % 8 == 0 && h->ldx >= h->C && aligned16(h->x) &&
+  h->x_direct = bf && !(bwd && want_dw) && h->n % 64 == 0 && h->C % 64 == 0 && h->ldx % 8 == 0 && h->ldx >= h->C && aligned16(h->x) &&
                 2 * (h->n + 128) * h->ldx <= kMaxOffset;
   h->w_direct = bf && h->C % 64 == 0 && h->V % 64 == 0 && h->ldw % 8 == 0 && h->ldw >= (h->rows ? h->C : h->V) &&
                 aligned16(h->w) && 2 * ((h->rows ? 1152 : h->C + 1) * h->ldw + 128) <= kMaxOffset;
@@ -424,15 +426,15 @@ struct Call {
   float* floats_at(int64_t off) const { return reinterpret_cast<float*>(ws + off); }
 
   int planes(const void* src, int64_t ld, int64_t rows, int64_t cols, int64_t rows_to, int64_t cols_to,
-             uint16_t* dst) const {
+             const int64_t* targets, uint16_t* dst) const {
     const int64_t blocks = (rows_to * (cols_to / 8) + 255) / 256;
     if (!fits_launch(blocks, 256)) return pratchya_set_error(PRATCHYA_EUNSUPPORTED, "linear_cross_entropy: too large");
     if (h.P == 1)
       hipLaunchKernelGGL((k_head_planes<uint16_t, 1>), dim3((unsigned)blocks), dim3(256), 0, stream,
-                         static_cast<const uint16_t*>(src), ld, rows, cols, rows_to, cols_to, dst);
+                         static_cast<const uint16_t*>(src), ld, rows, cols, rows_to, cols_to, targets, dst);
     else
       hipLaunchKernelGGL((k_head_planes<float, 3>), dim3((unsigned)blocks), dim3(256), 0, stream,
-                         static_cast<const float*>(src), ld, rows, cols, rows_to, cols_to, dst);
+                         static_cast<const float*>(src), ld, rows, cols, rows_to, cols_to, targets, dst);
     return check_launch("linear_cross_entropy");
   }
   // The same on 256-row tiles.
@@ -476,7 +478,7 @@ struct Operands {
   int64_t ldx, ldw, x_rows, w_rows;
 };
 
-int operand_x(const Call& c, Operands* o) {
+int operand_x(const Call& c, const int64_t* targets, Operands* o) {
   const Head& h = c.h;
   o->x_rows = h.n64;
   if (h.x_direct) {
@@ -486,7 +488,7 @@ int operand_x(const Call& c, Operands* o) {
   }
   o->x = c.planes_at(h.xp);
   o->ldx = h.C64;
-  return c.planes(h.x, h.ldx, h.n, h.C, h.n64, h.C64, c.planes_at(h.xp));
+  return c.planes(h.x, h.ldx, h.n, h.C, h.n64, h.C64, targets, c.planes_at(h.xp));
 }
 
 int operand_w(const Call& c, int64_t v0, int64_t cols, int64_t Vp, Operands* o) {
@@ -501,8 +503,8 @@ int operand_w(const Call& c, int64_t v0, int64_t cols, int64_t Vp, Operands* o) 
   }
   o->w = c.planes_at(h.wp);
   o->ldw = h.rows ? h.C64 : Vp;
-  return h.rows ? c.planes(src, h.ldw, cols, h.C, Vp, h.C64, c.planes_at(h.wp))
-                : c.planes(src, h.ldw, h.C, cols, h.C64, Vp, c.planes_at(h.wp));
+  return h.rows ? c.planes(src, h.ldw, cols, h.C, Vp, h.C64, nullptr, c.planes_at(h.wp))
+                : c.planes(src, h.ldw, h.C, cols, h.C64, Vp, nullptr, c.planes_at(h.wp));
 }
 
 // A piece's logits into the workspace.
@@ -528,7 +530,7 @@ HeadProduct logits_product(const Call& c, const Operands& o, int64_t v0, int64_t
 int forward(const Call& c, const int64_t* targets, float smooth, float* loss, float* stats) {
   const Head& h = c.h;
   Operands o;
-  int rc = operand_x(c, &o);
+  int rc = operand_x(c, nullptr, &o);
   for (int64_t v0 = 0; v0 < h.V && !rc; v0 += h.piece) {
     const int64_t cols = h.V - v0 < h.piece ? h.V - v0 : h.piece, Vp = up64(cols);
     if ((rc = operand_w(c, v0, cols, Vp, &o))) break;
@@ -565,7 +567,7 @@ int backward(const Call& c, const int64_t* targets, float smooth, const float* s
   const char* what = "linear_cross_entropy_bwd";
   constexpr int64_t chunk = 16 / sizeof(T);
   Operands o;
-  int rc = operand_x(c, &o);
+  int rc = operand_x(c, dw ? targets : nullptr, &o);
   for (int64_t v0 = 0; v0 < h.V && !rc; v0 += h.piece) {
     const int64_t cols = h.V - v0 < h.piece ? h.V - v0 : h.piece, Vp = up64(cols);
     if ((rc = operand_w(c, v0, cols, Vp, &o))) break;

@@ -73,7 +73,7 @@ struct MixArgs {
   int init_r, init_c, last_r, last_c;   // strides of a state's query and value axes
   int B, T, H, dq, dv, nseg, per;  // per: chunks of a segment
   int parts, per_part;             // without outputs: parts of a segment, chunks of a part
-  int rev;
+  int rev;                         // without outputs: from the last token to the first
   float scale, kscale;             // of outputs, of what enters the state
 };
 
@@ -538,7 +538,7 @@ __global__ __launch_bounds__(kThreads, NS == 1 && DP + EP == 128 ? 3 : 2) void k
   const int l16 = lane & 15, g4 = lane >> 4;
   const int units = OUT ? p.nseg : (p.nseg - 1) * p.parts;      // OUT false: the walk's last segment is not needed
   const int bh = blockIdx.x / units, unit = blockIdx.x - bh * units, walk = OUT ? unit : unit / p.parts;
-  const int b = bh / p.H, h = bh - b * p.H, seg = p.rev ? p.nseg - 1 - walk : walk;
+  const int b = bh / p.H, h = bh - b * p.H, seg = !OUT && p.rev ? p.nseg - 1 - walk : walk;
   int64_t length = p.T;
   if (p.lengths) length = min(max(p.lengths[b], (int64_t)0), (int64_t)p.T);
   const int chunks = (p.T + L - 1) / L;
@@ -554,7 +554,7 @@ __global__ __launch_bounds__(kThreads, NS == 1 && DP + EP == 128 ? 3 : 2) void k
     }
   }
   const int n = max(c_hi - c_lo, 0);
-  auto first_of = [&](int i) { return (p.rev ? c_hi - 1 - i : c_lo + i) * L; };     // chunk i of the walk
+  auto first_of = [&](int i) { return (!OUT && p.rev ? c_hi - 1 - i : c_lo + i) * L; };     // chunk i of the walk
 
   Rows<T, L, DP, kThreads, FULL> rq(OUT ? p.q : p.k, b, h, length, p.dq), rk(p.k, b, h, length, p.dq);
   Rows<T, L, EP, kThreads, FULL> rv(p.v, b, h, length, p.dv);
@@ -655,7 +655,7 @@ __global__ __launch_bounds__(kThreads, NS == 1 && DP + EP == 128 ? 3 : 2) void k
     }
     bf16x8_t val[KS][ET][NPI];
     read_values(m.v, M::PE, wave, lane, val);
-    S.update(m.k, M::PD, val, p.rev ? m.gates.start[par] : m.gates.rest[par], p.kscale, m.gates.total[par], lane);
+    S.update(m.k, M::PD, val, !OUT && p.rev ? m.gates.start[par] : m.gates.rest[par], p.kscale, m.gates.total[par], lane);
     __syncthreads();                    // scores are whole
     if constexpr (OUT) {
       add_scores<false>(m.t, M::PT, val, lane, acc);

@@ -100,6 +100,27 @@ def test_rows_apart(dt):
     assert not bool(dx.any()) and not bool(dw.any())
 
 
+@pytest.mark.parametrize("dt", ["bf16", "f32"])
+@pytest.mark.parametrize("n,V,C", [(40, 100, 64), (64, 1024, 256), (300, 512, 256), (512, 1024, 320)])
+@pytest.mark.parametrize("tied", [False, True])
+def test_padding_that_is_not_finite(n, V, C, tied, dt):
+    """Rows without a target may hold anything: no loss, no gradient of theirs, none of the weight from them."""
+    F = _F()
+    x, w = _normal((n, C), DT[dt], 1), _normal((C, V), DT[dt], 2, 0.2)
+    targets = torch.randint(0, V, (n,), generator=torch.Generator().manual_seed(3))
+    rows = torch.tensor([0, 3, 17, n - 1])
+    targets[rows] = -1
+    g = _normal((n,), torch.float32, 4)
+    want = _check(x, w, targets, 0.1, g, tied)
+    bad = x.clone()
+    bad[rows[0]], bad[rows[1], 2], bad[rows[2]], bad[rows[3], C - 1] = math.nan, math.inf, -math.inf, math.nan
+    g[rows[1]] = math.nan
+    xd, wd = bad.cuda().requires_grad_(True), (w.t().contiguous() if tied else w).cuda().requires_grad_(True)
+    y = F.linear_cross_entropy(xd, wd.t() if tied else wd, targets.cuda(), label_smoothing=0.1)
+    got = (y,) + torch.autograd.grad(y, (xd, wd), g.cuda())
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
 def test_near_and_far():
     """Losses near 0 keep the digits of the others' sum; logits of +-1000 do not overflow."""
     F = _F()
