@@ -803,7 +803,7 @@ int pratchya_linear_cross_entropy_bwd(const void* x, int64_t ldx, const void* w,
  * itself).  starts: pratchya_linear_attention_starts_floats of f32, 16-byte aligned
  * (null where that is 0): the states before the segments that a long sequence is cut
  * into, which the backward pass reads.  train: whether one follows (it takes fewer
- * segments).  A decay of 0 (log_decay -inf) forgets all. */
+ * segments, and reads starts of a call that said so).  A decay of 0 (log_decay -inf) forgets all. */
 int64_t pratchya_linear_attention_starts_floats(int64_t batch, int64_t length, int64_t heads, int64_t dk, int64_t dv,
                                                 int dtype, int train);
 int pratchya_linear_attention(const void* q, const void* k, const void* v, int dtype, const void* log_decay, int g_dtype,

@@ -27,12 +27,18 @@
 // (each below the rounding of the output itself).  The decays' gradient is f32, and what
 // it sums is not rounded: see k_mix_back.
 //
-// A sequence is cut into segments where heads alone leave the chip idle: their states
-// from 0 first (k_mix without outputs), joined from the first to the last, then all
-// segments at once.  Bound: neither HBM (8 x 4096 tokens of 32 heads of 64 in bf16, both
-// passes: 1.08 GB, 220 us at a copy's rate; 692 us) nor the MFMAs (a sixth of the time)
-// but vector instructions (two fifths) and LDS reads (a third), which overlap in part:
-// two or three workgroups fit a compute unit.
+// A sequence is cut into segments where heads alone leave the chip idle: the states that
+// their parts add first (k_mix without outputs), joined from the first to the last, then
+// all segments at once.
+//
+// Measured, 8 x 4096 tokens of 32 heads of 64 in bf16, both passes 650 us: states 36 us for
+// each of S and R, joins 7, o 136, dq 184, k_mix_back 301.  HBM at a copy's rate would take 220
+// (1.08 GB).  The MFMAs are busy a sixth of the time, the vector units two fifths (planes,
+// weights, masks), LDS a third, and two or three workgroups a compute unit overlap these in
+// part.  With dk and dv as walks of their own, as dq, whose scores then need three planes
+// each for the decays' sums, both passes took 991; with the states of whole segments, a
+// workgroup each, 693.  Without gradients (8192 tokens of 64 heads, 105 us) the walk
+// runs at 4.2 TB/s.
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 

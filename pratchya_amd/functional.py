@@ -1,6 +1,7 @@
-"""What stands between the quantized Linears of a model: layer norm,
-activations, and the log probabilities of tokens over the head's logits, each
-with its gradients, on the gfx950 kernels.
+"""What stands around and between the quantized Linears of a model: embedding, layer
+norm, activations, linear attention, the log probabilities of tokens over the head's
+logits, and the head's cross entropy without logits, each with its gradients, on the
+gfx950 kernels.
 
 ``layer_norm`` and ``activation`` can keep their input for the backward pass in
 8 bits (``tgrid=(1, b)``): the forward pass quantizes it as
@@ -13,6 +14,14 @@ to the backward pass, as the quantized Linear holds its own input.
     u = (QArrayImpl(h, (1, 128)) @ up).astype(h.dtype)
     x = x + (QArrayImpl(functional.activation(u, "relu2", tgrid=(1, 128)), (1, 128)) @ down).astype(x.dtype)
     loss = -functional.token_logprobs(logits, tokens).logprobs.mean()
+
+A language model with tied weights and linear attention begins, mixes and ends with
+
+    x = functional.embedding(table, tokens, scale=C ** 0.5)
+    r = functional.linear_attention(q, k, v, log_decay, lengths=lengths, scale=D ** -0.5)
+    loss = functional.linear_cross_entropy(x, table.t(), targets)
+
+and generates with ``linear_attention_step`` from ``r.state`` on.
 
 Arrays are bf16 or f32 on the GPU; rows may be a stride apart (slices of a wider
 array).  Arithmetic is f32, with one rounding to a result's type.  Gradients are
