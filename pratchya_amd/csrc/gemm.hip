@@ -1551,10 +1551,13 @@ __device__ __forceinline__ void store_tile_head(const v16f (&acc)[2][4], uint8_t
 __device__ __forceinline__ void head_rows(v16f (&acc)[2][4], const HeadArgs& p, int lane, int row0, int col0,
                                           int col_lo, int half) {
   const int l32 = lane & 31, lhi = lane >> 5;
+  int64_t targets[2];
+#pragma unroll
+  for (int mi = 0; mi < 2; ++mi) targets[mi] = p.targets[min(row0 + mi * 32 + l32, p.rows - 1)];
 #pragma unroll
   for (int mi = 0; mi < 2; ++mi) {
     const int row = row0 + mi * 32 + l32;
-    const int64_t target = p.targets[min(row, p.rows - 1)];
+    const int64_t target = targets[mi];
     // columns of the 128 that count, and the target's place among them (or none)
     const int lo = max(col_lo - col0, 0), hi = min(p.cols - col0, 128);
     const int64_t rel = target < 0 ? -1 : target - p.v0 - col0;
@@ -1599,7 +1602,7 @@ __device__ __forceinline__ void head_rows(v16f (&acc)[2][4], const HeadArgs& p, 
       for (int v = 0; v < 16; ++v) s += __expf(acc[mi][ni][v] - m);
     s += __shfl_xor(s, 32, 64);
     if (lhi == 0 && row < p.rows) {
-      const int64_t at = (int64_t)row * p.ld_part + half;
+      const int64_t at = half * p.ld_part + row;
       p.hpart[at] = make_float2(m, s);
       if (p.part_sum) p.part_sum[at] = sum;
     }
@@ -1609,11 +1612,20 @@ __device__ __forceinline__ void head_rows(v16f (&acc)[2][4], const HeadArgs& p, 
 // The logits of this wave's 64 x 128 turned into the loss's gradient of them.
 __device__ __forceinline__ void head_grad(v16f (&acc)[2][4], const HeadArgs& p, int lane, int row0, int col0) {
   const int l32 = lane & 31, lhi = lane >> 5;
+  int64_t targets[2];
+  float2 stats[2];
+  float cots[2];
 #pragma unroll
   for (int mi = 0; mi < 2; ++mi) {
     const int row = min(row0 + mi * 32 + l32, p.rows - 1);
-    const int64_t target = p.targets[row], rel = target - p.v0 - col0;
-    const float m = p.stats[2 * row], logs = p.stats[2 * row + 1] * 1.44269504f, g = target < 0 ? 0.0f : p.cot[row];
+    targets[mi] = p.targets[row];
+    stats[mi] = *reinterpret_cast<const float2*>(p.stats + 2 * row);
+    cots[mi] = p.cot[row];
+  }
+#pragma unroll
+  for (int mi = 0; mi < 2; ++mi) {
+    const int64_t target = targets[mi], rel = target - p.v0 - col0;
+    const float m = stats[mi].x, logs = stats[mi].y * 1.44269504f, g = target < 0 ? 0.0f : cots[mi];
     const int tc = target >= 0 && rel >= 0 && rel < 128 ? (int)rel : -1, hi = p.cols - col0;
     const float ge = g * p.even, gt = g * p.keep;
 #pragma unroll

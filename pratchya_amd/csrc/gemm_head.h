@@ -34,7 +34,7 @@ struct HeadProduct {
   const int64_t* targets;
   int64_t v0, vocab;
   float smooth;
-  float2* part;                            // [rows][ld_part], of 128 columns each
+  float2* part;                            // [..][ld_part], of the rows' 128 columns each
   float* part_sum;                         // likewise, or null
   float* target_value;                     // [rows]
   int64_t ld_part;

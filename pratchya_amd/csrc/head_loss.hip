@@ -152,36 +152,57 @@ __global__ __launch_bounds__(kRowThreads) void k_head_rows(const float* __restri
   s = block_add<kRowThreads / 64>(s, lds);
   if (part_sum) sum = block_add<kRowThreads / 64>(sum, lds);
   if (threadIdx.x) return;
-  const int64_t at = row * ld_part + blockIdx.y;
+  const int64_t at = blockIdx.y * ld_part + row;
   part[at] = make_float2(m, s);
   if (part_sum) part_sum[at] = sum;
 }
 
-// The rows' losses from the statistics of their parts: one wave a row.
-__global__ __launch_bounds__(256) void k_head_join(const float2* __restrict__ part, const float* __restrict__ part_sum,
-                                                   int64_t ld, int64_t held, const float* __restrict__ target_value,
-                                                   int64_t n,
-                                                   const int64_t* __restrict__ targets, int64_t vocab, float smooth,
-                                                   float* __restrict__ loss, float* __restrict__ stats) {
-  const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-  const int lane = threadIdx.x & 63;
-  if (row >= n) return;
-  const float2* p = part + row * ld;
-  float m = kLowest;
-  for (int64_t i = lane; i < held; i += 64) m = fmaxf(m, p[i].x);
+// The rows' losses from the statistics of their parts, [held][ld]: 64 rows a workgroup, a
+// lane a row and a wave every kJoinWaves-th part.
+constexpr int kJoinWaves = 16;
+
+__global__ __launch_bounds__(64 * kJoinWaves) void k_head_join(const float2* __restrict__ part,
+                                                               const float* __restrict__ part_sum, int64_t ld, int held,
+                                                               const float* __restrict__ target_value, int64_t n,
+                                                               const int64_t* __restrict__ targets, int64_t vocab,
+                                                               float smooth, float* __restrict__ loss,
+                                                               float* __restrict__ stats) {
+  __shared__ float ms[kJoinWaves][64], ss[kJoinWaves][64], sums[kJoinWaves][64];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int64_t row = (int64_t)blockIdx.x * 64 + lane, r = row < n ? row : n - 1;
   Seen a;
-  a.m = wave_max(m);
-  for (int64_t i = lane; i < held; i += 64) {
-    const float2 v = p[i];
-    if (v.y != 0.0f) a.s += v.y * expf(fmaxf(v.x - a.m, kLowest));
-    if (part_sum) a.sum += part_sum[row * ld + i];
-  }
+  constexpr int AHEAD = 8;
+  for (int i = wave; i < held; i += AHEAD * kJoinWaves) {
+    float2 v[AHEAD];
+    float t[AHEAD], m = a.m;
 #pragma unroll
-  for (int k = 32; k; k >>= 1) {
-    a.s += __shfl_xor(a.s, k, 64);
-    a.sum += __shfl_xor(a.sum, k, 64);
+    for (int k = 0; k < AHEAD; ++k) {
+      const int at = i + k * kJoinWaves;
+      v[k] = at < held ? part[at * ld + r] : make_float2(kLowest, 0.0f);
+      t[k] = part_sum && at < held ? part_sum[at * ld + r] : 0.0f;
+    }
+#pragma unroll
+    for (int k = 0; k < AHEAD; ++k) m = fmaxf(m, v[k].x);
+    a.s = a.s == 0.0f ? 0.0f : a.s * expf(fmaxf(a.m - m, kLowest));
+    a.m = m;
+#pragma unroll
+    for (int k = 0; k < AHEAD; ++k) {
+      a.s += v[k].y == 0.0f ? 0.0f : v[k].y * expf(fmaxf(v[k].x - m, kLowest));
+      a.sum += t[k];
+    }
   }
-  if (lane) return;
+  ms[wave][lane] = a.m;
+  ss[wave][lane] = a.s;
+  sums[wave][lane] = a.sum;
+  __syncthreads();
+  if (wave || row >= n) return;
+  for (int w = 1; w < kJoinWaves; ++w) a.m = fmaxf(a.m, ms[w][lane]);
+  a.s = a.sum = 0.0f;
+  for (int w = 0; w < kJoinWaves; ++w) {
+    const float s = ss[w][lane];
+    a.s += s == 0.0f ? 0.0f : s * expf(fmaxf(ms[w][lane] - a.m, kLowest));
+    a.sum += sums[w][lane];
+  }
   const int64_t target = targets[row];
   if (target >= 0 && target < vocab) a.zt = target_value[row];
   finish_row(a, target, vocab, smooth, loss + row, stats ? stats + 2 * row : nullptr);
@@ -290,7 +311,7 @@ struct Head {
   // 4183 us of a step without, 4117 with)
   int64_t pad() const { return fused ? 64 : 0; }
   bool fused;                    // logits on 256-row tiles, what follows them in the product's epilogue
-  int64_t parts, ld_part;        // of a row of a piece, of the whole row: what statistics are taken of
+  int64_t parts, ld_part;        // what statistics are taken of: of a row of a piece; from one to the next (rows)
   int64_t parts_of(int64_t cols) const { return fused ? 2 * ((cols + 255) / 256) : (cols + kRowColumns - 1) / kRowColumns; }
   // workspace
   int64_t part, part_sum, zt;
@@ -379,9 +400,11 @@ int plan(const char* what, bool bwd, bool want_dx, bool want_dw, Head* h) {
   h->xp = take(planes * h->n64 * h->C64);
   h->wp = take(h->w_direct ? 0 : planes * h->C64 * h->piece);
   h->parts = h->parts_of(h->piece);
-  h->ld_part = (V64 + h->piece - 1) / h->piece * h->parts;
-  h->part = take(bwd ? 0 : 8 * h->n * h->ld_part);
-  h->part_sum = take(bwd ? 0 : 4 * h->n * h->ld_part);
+  h->ld_part = h->n64;
+  const int64_t parts = (V64 + h->piece - 1) / h->piece * h->parts;
+  if (parts > INT32_MAX) return pratchya_set_error(PRATCHYA_EUNSUPPORTED, "%s: too large", what);
+  h->part = take(bwd ? 0 : 8 * parts * h->ld_part);
+  h->part_sum = take(bwd ? 0 : 4 * parts * h->ld_part);
   h->zt = take(bwd ? 0 : 4 * h->n);
   h->z = take(h->fused ? 0 : 4 * h->n * h->piece);
   h->split_bytes = 0;
@@ -535,7 +558,7 @@ int forward(const Call& c, const int64_t* targets, float smooth, float* loss, fl
   for (int64_t v0 = 0; v0 < h.V && !rc; v0 += h.piece) {
     const int64_t cols = h.V - v0 < h.piece ? h.V - v0 : h.piece, Vp = up64(cols);
     if ((rc = operand_w(c, v0, cols, Vp, &o))) break;
-    const int64_t at = v0 / h.piece * h.parts;
+    const int64_t at = v0 / h.piece * h.parts * h.ld_part;
     float2* part = reinterpret_cast<float2*>(c.ws + h.part) + at;
     float* part_sum = smooth != 0.0f ? c.floats_at(h.part_sum) + at : nullptr;
     if (h.fused) {
@@ -556,9 +579,9 @@ int forward(const Call& c, const int64_t* targets, float smooth, float* loss, fl
   // the last piece may have fewer parts than the others
   const int64_t last = (h.V - 1) / h.piece, rest = h.V - last * h.piece;
   const int64_t held = last * h.parts + h.parts_of(h.fused ? up64(rest) : rest);
-  hipLaunchKernelGGL(k_head_join, dim3((unsigned)((h.n + 3) / 4)), dim3(256), 0, c.stream,
+  hipLaunchKernelGGL(k_head_join, dim3((unsigned)((h.n + 63) / 64)), dim3(64 * kJoinWaves), 0, c.stream,
                      reinterpret_cast<const float2*>(c.ws + h.part), smooth != 0.0f ? c.floats_at(h.part_sum) : nullptr,
-                     h.ld_part, held, c.floats_at(h.zt), h.n, targets, h.V, smooth, loss, stats);
+                     h.ld_part, (int)held, c.floats_at(h.zt), h.n, targets, h.V, smooth, loss, stats);
   return check_launch("linear_cross_entropy");
 }
 
