@@ -18,7 +18,7 @@
 // Bound: the MFMAs' rate on 256-row tiles, 1.1 PFLOP/s of four products (logits twice) where
 // a large product alone reaches 1.27 and the library's 1.5: [8192, 4096] . [4096, 65536] in
 // bf16, both passes, 16.0 ms (19.4 with the logits written and 128-row tiles); f32
-// [1000, 1027] . [1027, 50021] 3.2 ms, the tiles' last of four rounds nearly empty.
+// [1000, 1027] . [1027, 50021] 3.0 ms.
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
@@ -216,17 +216,18 @@ __global__ __launch_bounds__(256) void k_head_zero_rows(uint16_t* __restrict__ d
   *reinterpret_cast<u32x4_t*>(dst + blockIdx.y * plane + (rows + i / per) * ld + i % per * 8) = u32x4_t{};
 }
 
-// dz of a piece's logits as planes [P][rows_to][cols_to], zeros around [rows, cols].
+// dz of a piece's logits as planes [P][rows_to][cols_to], rows ld_dst apart, zeros around
+// [rows, cols].
 template <int P>
 __global__ __launch_bounds__(256) void k_head_grad(const float* __restrict__ z, int64_t ld, int64_t rows, int64_t cols,
                                                    int64_t rows_to, int64_t cols_to, const int64_t* __restrict__ targets,
                                                    int64_t v0, int64_t vocab, float smooth,
                                                    const float* __restrict__ stats, const float* __restrict__ g,
-                                                   uint16_t* __restrict__ dst) {
+                                                   uint16_t* __restrict__ dst, int64_t ld_dst) {
   const int64_t per = cols_to / 8, i = (int64_t)blockIdx.x * 256 + threadIdx.x;
   if (i >= rows_to * per) return;
   const int64_t r = i / per, c = (i - r * per) * 8;
-  uint16_t* to = dst + r * cols_to + c;
+  uint16_t* to = dst + r * ld_dst + c;
   float d[8] = {};
   if (r < rows && targets[r] >= 0) {
     const int64_t target = targets[r];
@@ -251,7 +252,7 @@ __global__ __launch_bounds__(256) void k_head_grad(const float* __restrict__ z, 
       o[k] = P == 1 || q == P - 1 ? d[k] : top_piece(d[k]);
       d[k] -= o[k];
     }
-    *reinterpret_cast<u32x4_t*>(to + q * rows_to * cols_to) = narrow(o);
+    *reinterpret_cast<u32x4_t*>(to + q * rows_to * ld_dst) = narrow(o);
   }
 }
 
@@ -312,7 +313,26 @@ struct Head {
   int64_t pad() const { return fused ? 64 : 0; }
   bool fused;                    // logits on 256-row tiles, what follows them in the product's epilogue
   int64_t parts, ld_part;        // what statistics are taken of: of a row of a piece; from one to the next (rows)
-  int64_t parts_of(int64_t cols) const { return fused ? 2 * ((cols + 255) / 256) : (cols + kRowColumns - 1) / kRowColumns; }
+  int64_t parts_of(int64_t cols) const {
+    const int64_t main = fused ? main_of(cols) : 0, rest = main < cols ? cols - main : 0;
+    return 2 * ((main + 255) / 256) + (rest + kRowColumns - 1) / kRowColumns;
+  }
+  // pieces before the last one are whole
+  int64_t all_parts() const {
+    const int64_t last = (V - 1) / piece;
+    return last * parts + parts_of(V - last * piece);
+  }
+  // Columns of a piece's logits on the 256-row tiles: all (a multiple of 64 behind the
+  // piece's end), or those of full rounds of tiles on the 256 compute units, where the last
+  // round would be a third full or less; the others are few enough for the way of few rows
+  // (f32 [1000, 1027] . [1027, 50021], 784 tiles: both passes 3.21 ms with a
+  // fourth round of 16 tiles, 3.02 without).
+  int64_t main_of(int64_t cols) const {
+    const int64_t all = (cols + 63) / 64 * 64, tm = (n + 255) / 256, tn = (all + 255) / 256, full = tm * tn / 256;
+    if (full < 1 || tm * tn % 256 == 0 || tm * tn % 256 > 85 || C64 / 64 * (P == 1 ? 1 : 6) < 48) return all;
+    const int64_t main = full * 256 / tm * 256;
+    return main >= 256 && main < all && (tn * 256 - main) / 256 * tm <= 85 ? main : all;
+  }
   // workspace
   int64_t part, part_sum, zt;
   int64_t xp, wp, z, dzp, dx_sum, dx_tmp, dw_tmp, split, split_bytes, bytes;
@@ -401,20 +421,27 @@ int plan(const char* what, bool bwd, bool want_dx, bool want_dw, Head* h) {
   h->wp = take(h->w_direct ? 0 : planes * h->C64 * h->piece);
   h->parts = h->parts_of(h->piece);
   h->ld_part = h->n64;
-  const int64_t parts = (V64 + h->piece - 1) / h->piece * h->parts;
+  const int64_t parts = h->all_parts();
   if (parts > INT32_MAX) return pratchya_set_error(PRATCHYA_EUNSUPPORTED, "%s: too large", what);
   h->part = take(bwd ? 0 : 8 * parts * h->ld_part);
   h->part_sum = take(bwd ? 0 : 4 * parts * h->ld_part);
   h->zt = take(bwd ? 0 : 4 * h->n);
-  h->z = take(h->fused ? 0 : 4 * h->n * h->piece);
+  const int64_t rest = V64 - (V64 - 1) / h->piece * h->piece;      // the last piece
+  int64_t by_rows = h->piece;                                      // columns of f32 logits
+  if (h->fused) {
+    by_rows = 0;
+    for (int64_t Vp : {h->piece, rest})
+      if (Vp - h->main_of(Vp) > by_rows) by_rows = Vp - h->main_of(Vp);
+  }
+  h->z = take(4 * h->n * by_rows);
   h->split_bytes = 0;
   auto split = [&](int64_t M, int64_t N, int64_t K) {
     const int64_t b = pratchya_gemm_t128_workspace_bytes(M, N, segs * (K / 64), 1);
     if (b > h->split_bytes) h->split_bytes = b;
   };
-  const int64_t rest = V64 - (V64 - 1) / h->piece * h->piece;      // the last piece
   for (int64_t Vp : {h->piece, rest}) {
-    if (!h->fused) split(h->n, Vp, h->C64);
+    const int64_t main = h->fused ? h->main_of(Vp) : 0;
+    if (main < Vp) split(h->n, Vp - main, h->C64);
     if (bwd && want_dx && !dx256(*h, Vp)) split(h->n, h->C64, Vp);
     if (bwd && want_dw && !dw256(*h, Vp)) {
       split(h->rows ? Vp : h->C64, h->rows ? h->C64 : Vp, h->n64);
@@ -531,19 +558,19 @@ int operand_w(const Call& c, int64_t v0, int64_t cols, int64_t Vp, Operands* o) 
                 : c.planes(src, h.ldw, h.C, cols, h.C64, Vp, nullptr, c.planes_at(h.wp));
 }
 
-// A piece's logits into the workspace.
-int logits(const Call& c, const Operands& o, int64_t Vp) {
+// A piece's logits from column `from` on into the workspace, [n, Vp - from].
+int logits(const Call& c, const Operands& o, int64_t from, int64_t Vp) {
   const Head& h = c.h;
-  return c.product(o.x, o.ldx, o.x_rows, 0, o.w, o.ldw, o.w_rows, h.rows ? 0 : 1, h.n, Vp, h.C64, c.floats_at(h.z), Vp,
-                   PRATCHYA_DT_F32);
+  return c.product(o.x, o.ldx, o.x_rows, 0, o.w + (h.rows ? from * o.ldw : from), o.ldw, o.w_rows, h.rows ? 0 : 1, h.n,
+                   Vp - from, h.C64, c.floats_at(h.z), Vp - from, PRATCHYA_DT_F32);
 }
 
-HeadProduct logits_product(const Call& c, const Operands& o, int64_t v0, int64_t cols, const int64_t* targets,
-                           float smooth) {
+HeadProduct logits_product(const Call& c, const Operands& o, int64_t v0, int64_t cols, int64_t main,
+                           const int64_t* targets, float smooth) {
   const Head& h = c.h;
-  HeadProduct p = c.product256(o.x, o.ldx, o.x_rows, false, o.w, o.ldw, o.w_rows, !h.rows, h.n, up64(cols), h.C64);
+  HeadProduct p = c.product256(o.x, o.ldx, o.x_rows, false, o.w, o.ldw, o.w_rows, !h.rows, h.n, main, h.C64);
   p.rows = h.n;
-  p.cols = cols;
+  p.cols = cols < main ? cols : main;
   p.targets = targets;
   p.v0 = v0;
   p.vocab = h.V;
@@ -561,27 +588,28 @@ int forward(const Call& c, const int64_t* targets, float smooth, float* loss, fl
     const int64_t at = v0 / h.piece * h.parts * h.ld_part;
     float2* part = reinterpret_cast<float2*>(c.ws + h.part) + at;
     float* part_sum = smooth != 0.0f ? c.floats_at(h.part_sum) + at : nullptr;
-    if (h.fused) {
-      HeadProduct p = logits_product(c, o, v0, cols, targets, smooth);
+    const int64_t main = h.fused ? h.main_of(cols) : 0;
+    if (main) {
+      HeadProduct p = logits_product(c, o, v0, cols, main, targets, smooth);
       p.epilogue = kHeadRows;
       p.part = part;
       p.part_sum = part_sum;
       p.target_value = c.floats_at(h.zt);
       p.ld_part = h.ld_part;
       rc = head_product(p, c.stream);
-    } else if (!(rc = logits(c, o, Vp))) {
-      hipLaunchKernelGGL(k_head_rows, dim3((unsigned)h.n, (unsigned)h.parts_of(cols)), dim3(kRowThreads), 0, c.stream,
-                         c.floats_at(h.z), Vp, cols, targets, v0, part, part_sum, h.ld_part, c.floats_at(h.zt));
+    }
+    if (!rc && main < cols && !(rc = logits(c, o, main, Vp))) {
+      const int64_t skip = main / 128 * h.ld_part;
+      hipLaunchKernelGGL(k_head_rows, dim3((unsigned)h.n, (unsigned)((cols - main + kRowColumns - 1) / kRowColumns)),
+                         dim3(kRowThreads), 0, c.stream, c.floats_at(h.z), Vp - main, cols - main, targets, v0 + main,
+                         part + skip, part_sum ? part_sum + skip : nullptr, h.ld_part, c.floats_at(h.zt));
       rc = check_launch("linear_cross_entropy");
     }
   }
   if (rc) return rc;
-  // the last piece may have fewer parts than the others
-  const int64_t last = (h.V - 1) / h.piece, rest = h.V - last * h.piece;
-  const int64_t held = last * h.parts + h.parts_of(h.fused ? up64(rest) : rest);
   hipLaunchKernelGGL(k_head_join, dim3((unsigned)((h.n + 63) / 64)), dim3(64 * kJoinWaves), 0, c.stream,
                      reinterpret_cast<const float2*>(c.ws + h.part), smooth != 0.0f ? c.floats_at(h.part_sum) : nullptr,
-                     h.ld_part, (int)held, c.floats_at(h.zt), h.n, targets, h.V, smooth, loss, stats);
+                     h.ld_part, (int)h.all_parts(), c.floats_at(h.zt), h.n, targets, h.V, smooth, loss, stats);
   return check_launch("linear_cross_entropy");
 }
 
@@ -597,8 +625,9 @@ int backward(const Call& c, const int64_t* targets, float smooth, const float* s
     if ((rc = operand_w(c, v0, cols, Vp, &o))) break;
     const int64_t ldz = Vp + h.pad();
     uint16_t* dz = c.planes_at(h.dzp);
-    if (h.fused) {
-      HeadProduct p = logits_product(c, o, v0, cols, targets, smooth);
+    const int64_t main = h.fused ? h.main_of(cols) : 0;
+    if (main) {
+      HeadProduct p = logits_product(c, o, v0, cols, main, targets, smooth);
       p.epilogue = kHeadGrad;
       p.c = dz;
       p.ldc = ldz;
@@ -611,13 +640,14 @@ int backward(const Call& c, const int64_t* targets, float smooth, const float* s
                            0, c.stream, dz, p.plane_c, ldz, h.n, h.n64);
         if ((rc = check_launch(what))) break;
       }
-    } else {
-      if ((rc = logits(c, o, Vp))) break;
-      const int64_t blocks = (h.n64 * (Vp / 8) + 255) / 256;
+    }
+    if (main < cols) {
+      if ((rc = logits(c, o, main, Vp))) break;
+      const int64_t blocks = (h.n64 * ((Vp - main) / 8) + 255) / 256;
       if (!fits_launch(blocks, 256)) return pratchya_set_error(PRATCHYA_EUNSUPPORTED, "%s: too large", what);
       auto grad = h.P == 1 ? k_head_grad<1> : k_head_grad<3>;
-      hipLaunchKernelGGL(grad, dim3((unsigned)blocks), dim3(256), 0, c.stream, c.floats_at(h.z), Vp, h.n, cols, h.n64, Vp,
-                         targets, v0, h.V, smooth, stats, g, dz);
+      hipLaunchKernelGGL(grad, dim3((unsigned)blocks), dim3(256), 0, c.stream, c.floats_at(h.z), Vp - main, h.n, cols - main,
+                         h.n64, Vp - main, targets, v0 + main, h.V, smooth, stats, g, dz + main, ldz);
       if ((rc = check_launch(what))) break;
     }
     const int slices = dx ? dx256(h, Vp) : 0;

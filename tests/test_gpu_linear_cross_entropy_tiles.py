@@ -141,3 +141,15 @@ def test_near_and_far():
     few = math.log1p((V - 2) * math.exp(-14.0))
     y = F.linear_cross_entropy(x.cuda(), w.cuda(), targets.cuda())[0].double()
     assert abs(float(y) - few) <= 64 * R.U * few
+
+
+@pytest.mark.parametrize("tied", [False, True])
+@pytest.mark.parametrize("n,V,C,dt,smooth", [(300, 33100, 640, "f32", 0.1), (1000, 17000, 1027, "f32", 0.0),
+                                             (260, 33024, 512, "f32", 0.0), (513, 22016, 3136, "bf16", 0.1)])
+def test_last_round_of_tiles(n, V, C, dt, smooth, tied):
+    """One or a few tiles more than the chip computes at once: the vocabulary's end goes another way."""
+    x, w = _normal((n, C), DT[dt], 1), _normal((C, V), DT[dt], 2, 2.0 / math.sqrt(C))
+    targets = _targets(n, V, 3)
+    main = 256 // -(-n // 256) * 256
+    targets[40:48] = torch.tensor([main - 257, main - 256, main - 1, main, main + 1, main + 63, V - 65, V - 64])
+    _check(x, w, targets, smooth, _normal((n,), torch.float32, 4), tied)
