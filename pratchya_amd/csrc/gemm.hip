@@ -1449,12 +1449,13 @@ struct HeadArgs : FqArgs {
   int64_t ld_sums;
   const int64_t* targets;
   int64_t v0;
-  float keep, even;                  // 1 - smoothing, smoothing / vocabulary
+  float keep, even, scale_p;         // 1 - smoothing, smoothing / vocabulary, 1; in units of head_part
   float2* hpart;
   float* part_sum;
   float* target_value;
   int64_t ld_part;
   const float *stats, *cot;
+  const float* unit;                 // FQ 7: what results are multiplied by; FQ 9: (it, 1 / max |g|), or null
 };
 
 __device__ __forceinline__ float head_top(float v) { return u2f(f2u(v) & 0xFFFF0000u); }
@@ -1467,7 +1468,7 @@ __device__ __forceinline__ float head_top(float v) { return u2f(f2u(v) & 0xFFFF0
 template <bool OUT_BF16, int PLANE, bool LAST>
 __device__ __forceinline__ void store_tile_head(const v16f (&acc)[2][4], uint8_t* stage, int wave, int lane, void* C,
                                                 int64_t ldc, const float* sums, int64_t ld_sums, int row0, int col0,
-                                                int row_lo, int col_lo, int rows, int cols) {
+                                                int row_lo, int col_lo, int rows, int cols, float unit) {
   typedef uint32_t u32x4_a2 __attribute__((ext_vector_type(4), aligned(2)));
   constexpr int ESZ = OUT_BF16 ? 2 : 4, PITCH = 128 * 4 + 16, RP = 16, PER = 16 / ESZ, CHUNKS = 128 / PER;
   const int l32 = lane & 31, lhi = lane >> 5;
@@ -1520,6 +1521,8 @@ __device__ __forceinline__ void store_tile_head(const v16f (&acc)[2][4], uint8_t
             v[i + 3] += w.w;
           }
         }
+#pragma unroll
+        for (int i = 0; i < PER; ++i) v[i] *= unit;
         u32x4_a2 o;
         if constexpr (OUT_BF16) {
 #pragma unroll
@@ -1612,6 +1615,7 @@ __device__ __forceinline__ void head_rows(v16f (&acc)[2][4], const HeadArgs& p, 
 // The logits of this wave's 64 x 128 turned into the loss's gradient of them.
 __device__ __forceinline__ void head_grad(v16f (&acc)[2][4], const HeadArgs& p, int lane, int row0, int col0) {
   const int l32 = lane & 31, lhi = lane >> 5;
+  const float to_unit = p.unit ? p.unit[1] : 1.0f;
   int64_t targets[2];
   float2 stats[2];
   float cots[2];
@@ -1620,20 +1624,20 @@ __device__ __forceinline__ void head_grad(v16f (&acc)[2][4], const HeadArgs& p, 
     const int row = min(row0 + mi * 32 + l32, p.rows - 1);
     targets[mi] = p.targets[row];
     stats[mi] = *reinterpret_cast<const float2*>(p.stats + 2 * row);
-    cots[mi] = p.cot[row];
+    cots[mi] = p.cot[row] * to_unit;
   }
 #pragma unroll
   for (int mi = 0; mi < 2; ++mi) {
     const int64_t target = targets[mi], rel = target - p.v0 - col0;
     const float m = stats[mi].x, logs = stats[mi].y * 1.44269504f, g = target < 0 ? 0.0f : cots[mi];
     const int tc = target >= 0 && rel >= 0 && rel < 128 ? (int)rel : -1, hi = p.cols - col0;
-    const float ge = g * p.even, gt = g * p.keep;
+    const float ge = g * p.even, gt = g * p.keep, gp = g * p.scale_p;
 #pragma unroll
     for (int ni = 0; ni < 4; ++ni)
 #pragma unroll
       for (int v = 0; v < 16; ++v) {
         const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(acc[mi][ni][v] - m, 1.44269504f, -logs));
-        acc[mi][ni][v] = __builtin_fmaf(g, e, -ge);
+        acc[mi][ni][v] = __builtin_fmaf(gp, e, -ge);
       }
     if (hi < 128 || __any(tc >= 0 || target < 0)) {
       const int end = target < 0 ? -8 : hi - 4 * lhi, at = tc < 0 ? -8 : tc - 4 * lhi;
@@ -2089,17 +2093,17 @@ __global__ __launch_bounds__(NTHREADS, 1) void k_gemm_bs_nt(
       if constexpr (FQ == 7) {
         uint8_t* c = static_cast<uint8_t*>(C) + t / T * fq.split_c * (OUT_BF16 ? 2 : 4);
         store_tile_head<OUT_BF16, 0, true>(acc, stage, wave, lane, c, ldc, fq.sums, fq.ld_sums, row0, col0, tm * BM, col_lo,
-                                           fq.rows, fq.cols);
+                                           fq.rows, fq.cols, fq.unit ? fq.unit[0] : 1.0f);
       } else if constexpr (FQ == 8) {
         head_rows(acc, fq, lane, row0, col0, col_lo, 2 * tn + wn);
       } else {
         head_grad(acc, fq, lane, row0, col0);
         uint16_t* c = static_cast<uint16_t*>(C);
         constexpr bool ONE = FQ == 9;
-        store_tile_head<true, 0, ONE>(acc, stage, wave, lane, c, ldc, nullptr, 0, row0, col0, 0, 0, fq.rows, N);
+        store_tile_head<true, 0, ONE>(acc, stage, wave, lane, c, ldc, nullptr, 0, row0, col0, 0, 0, fq.rows, N, 1.0f);
         if constexpr (!ONE) {
-          store_tile_head<true, 1, false>(acc, stage, wave, lane, c + fq.plane_c, ldc, nullptr, 0, row0, col0, 0, 0, fq.rows, N);
-          store_tile_head<true, 2, true>(acc, stage, wave, lane, c + 2 * fq.plane_c, ldc, nullptr, 0, row0, col0, 0, 0, fq.rows, N);
+          store_tile_head<true, 1, false>(acc, stage, wave, lane, c + fq.plane_c, ldc, nullptr, 0, row0, col0, 0, 0, fq.rows, N, 1.0f);
+          store_tile_head<true, 2, true>(acc, stage, wave, lane, c + 2 * fq.plane_c, ldc, nullptr, 0, row0, col0, 0, 0, fq.rows, N, 1.0f);
         }
       }
     } else if constexpr (FQ == 3) {
@@ -2815,14 +2819,17 @@ int head_product(const HeadProduct& p, hipStream_t stream) {
   h.ld_sums = p.ld_sums;
   h.targets = p.targets;
   h.v0 = p.v0;
-  h.keep = 1.0f - p.smooth;
-  h.even = p.smooth / (float)p.vocab;
+  const float part = p.unit && p.epilogue == kHeadGrad ? head_part(p.smooth) : 1.0f;
+  h.keep = (1.0f - p.smooth) / part;
+  h.even = p.smooth / (float)p.vocab / part;
+  h.scale_p = 1.0f / part;
   h.hpart = p.part;
   h.part_sum = p.part_sum;
   h.target_value = p.target_value;
   h.ld_part = p.ld_part;
   h.stats = p.stats;
   h.cot = p.g;
+  h.unit = p.unit;
   const int64_t held = p.segs > 1 ? 2 : 0;
   const int64_t ab = 2 * (held * p.a_plane + (p.a_kmajor ? (p.K - 1) * p.lda + p.M : (p.M - 1) * p.lda + p.K));
   const int64_t bb = 2 * (held * p.b_plane + (p.b_kmajor ? (p.K - 1) * p.ldb + p.N : (p.N - 1) * p.ldb + p.K));

@@ -38,8 +38,16 @@ struct HeadProduct {
   float* part_sum;                         // likewise, or null
   float* target_value;                     // [rows]
   int64_t ld_part;
+  // kHeadStore: null, or what the results are multiplied by.  kHeadGrad: null, or behind that
+  // 1 / max |g|: C is then dz over the first.
+  const float* unit;
   const float *stats, *g;                  // kHeadGrad: (maximum, log of the sum about it), the loss's cotangent
 };
+
+// The part of a loss's gradient that its target has: what a gradient is measured in where it is
+// held in bf16, so that the target's value, -g of it where its probability is small, has no
+// rounding of its own that all rows share.
+inline float head_part(float smooth) { return smooth < 0.5f ? 1.0f - smooth : 1.0f; }
 
 // Whether the operands suit (sizes, alignment, 32-bit offsets).
 bool head_product_fits(const HeadProduct& p);

@@ -208,6 +208,27 @@ __global__ __launch_bounds__(64 * kJoinWaves) void k_head_join(const float2* __r
   finish_row(a, target, vocab, smooth, loss + row, stats ? stats + 2 * row : nullptr);
 }
 
+// What gradients in bf16 are measured in: the largest |g| of rows with a target times their
+// targets' part (head_part), and 1 / that |g|; 1 and 1 if none is a normal number.  With 1 / n for g, as a
+// mean has it, and no unit, the rounding of -g itself, up to 2^-8, stood in all rows' gradients.
+__global__ __launch_bounds__(1024) void k_head_unit(const float* __restrict__ g, const int64_t* __restrict__ targets,
+                                                    int64_t n, float part, float* __restrict__ unit) {
+  __shared__ float lds[16];
+  float m = 0.0f;
+  for (int64_t i = threadIdx.x; i < n; i += 1024) {
+    const float v = __builtin_fabsf(g[i]);
+    if (targets[i] >= 0 && v < 3e38f) m = fmaxf(m, v);
+  }
+  m = wave_max(m);
+  if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = m;
+  __syncthreads();
+  if (threadIdx.x) return;
+  for (int w = 0; w < 16; ++w) m = fmaxf(m, lds[w]);
+  const bool usual = m > 1e-30f && m < 1e30f;
+  unit[0] = usual ? m * part : part;
+  unit[1] = usual ? 1.0f / m : 1.0f;
+}
+
 // Zeros in the planes' rows [rows, rows_to), which the product of the gradients reads.
 __global__ __launch_bounds__(256) void k_head_zero_rows(uint16_t* __restrict__ dst, int64_t plane, int64_t ld, int64_t rows,
                                                         int64_t rows_to) {
@@ -223,7 +244,8 @@ __global__ __launch_bounds__(256) void k_head_grad(const float* __restrict__ z, 
                                                    int64_t rows_to, int64_t cols_to, const int64_t* __restrict__ targets,
                                                    int64_t v0, int64_t vocab, float smooth,
                                                    const float* __restrict__ stats, const float* __restrict__ g,
-                                                   uint16_t* __restrict__ dst, int64_t ld_dst) {
+                                                   uint16_t* __restrict__ dst, int64_t ld_dst,
+                                                   const float* __restrict__ unit, float part) {
   const int64_t per = cols_to / 8, i = (int64_t)blockIdx.x * 256 + threadIdx.x;
   if (i >= rows_to * per) return;
   const int64_t r = i / per, c = (i - r * per) * 8;
@@ -231,7 +253,8 @@ __global__ __launch_bounds__(256) void k_head_grad(const float* __restrict__ z, 
   float d[8] = {};
   if (r < rows && targets[r] >= 0) {
     const int64_t target = targets[r];
-    const float m = stats[2 * r], logs = stats[2 * r + 1], gr = g[r], even = smooth / (float)vocab;
+    const float m = stats[2 * r], logs = stats[2 * r + 1], gr = unit ? g[r] * unit[1] : g[r],
+                even = smooth / (float)vocab / part, keep = (1.0f - smooth) / part, one = 1.0f / part;
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
       float v[4];
@@ -239,7 +262,7 @@ __global__ __launch_bounds__(256) void k_head_grad(const float* __restrict__ z, 
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
         const int64_t col = c + 4 * h + k;
-        const float p = expf((v[k] - m) - logs) - even - (v0 + col == target ? 1.0f - smooth : 0.0f);
+        const float p = expf((v[k] - m) - logs) * one - even - (v0 + col == target ? keep : 0.0f);
         d[4 * h + k] = col < cols ? gr * p : 0.0f;
       }
     }
@@ -262,7 +285,8 @@ __global__ __launch_bounds__(256) void k_head_grad(const float* __restrict__ z, 
 template <typename T>
 __global__ __launch_bounds__(256) void k_head_out(const float* __restrict__ src, int64_t ld_src, int64_t rows,
                                                   int64_t cols, float* __restrict__ sum, int add, int last,
-                                                  T* __restrict__ out, int64_t ld_out, int slices) {
+                                                  T* __restrict__ out, int64_t ld_out, int slices,
+                                                  const float* __restrict__ unit) {
   const int64_t per = (cols + 3) / 4, i = (int64_t)blockIdx.x * 256 + threadIdx.x;
   if (i >= rows * per) return;
   const int64_t r = i / per, c = (i - r * per) * 4;
@@ -283,6 +307,10 @@ __global__ __launch_bounds__(256) void k_head_out(const float* __restrict__ src,
   if (!last) {
     store_vec(sum + r * ld_src + c, v);
     return;
+  }
+  if (unit) {
+#pragma unroll
+    for (int k = 0; k < 4; ++k) v[k] *= unit[0];
   }
   store_some(out + r * ld_out + c, cols - c < 4 ? cols - c : 4, v);
 }
@@ -334,7 +362,7 @@ struct Head {
     return main >= 256 && main < all && (tn * 256 - main) / 256 * tm <= 85 ? main : all;
   }
   // workspace
-  int64_t part, part_sum, zt;
+  int64_t part, part_sum, zt, unit;
   int64_t xp, wp, z, dzp, dx_sum, dx_tmp, dw_tmp, split, split_bytes, bytes;
 };
 
@@ -426,6 +454,7 @@ int plan(const char* what, bool bwd, bool want_dx, bool want_dw, Head* h) {
   h->part = take(bwd ? 0 : 8 * parts * h->ld_part);
   h->part_sum = take(bwd ? 0 : 4 * parts * h->ld_part);
   h->zt = take(bwd ? 0 : 4 * h->n);
+  h->unit = take(bwd ? 8 : 0);
   const int64_t rest = V64 - (V64 - 1) / h->piece * h->piece;      // the last piece
   int64_t by_rows = h->piece;                                      // columns of f32 logits
   if (h->fused) {
@@ -620,6 +649,11 @@ int backward(const Call& c, const int64_t* targets, float smooth, const float* s
   constexpr int64_t chunk = 16 / sizeof(T);
   Operands o;
   int rc = operand_x(c, dw ? targets : nullptr, &o);
+  float* unit = h.P == 1 ? c.floats_at(h.unit) : nullptr;
+  if (unit && !rc) {
+    hipLaunchKernelGGL(k_head_unit, dim3(1), dim3(1024), 0, c.stream, g, targets, h.n, head_part(smooth), unit);
+    rc = check_launch(what);
+  }
   for (int64_t v0 = 0; v0 < h.V && !rc; v0 += h.piece) {
     const int64_t cols = h.V - v0 < h.piece ? h.V - v0 : h.piece, Vp = up64(cols);
     if ((rc = operand_w(c, v0, cols, Vp, &o))) break;
@@ -634,6 +668,7 @@ int backward(const Call& c, const int64_t* targets, float smooth, const float* s
       p.plane_c = h.n64 * ldz;
       p.stats = stats;
       p.g = g;
+      p.unit = unit;
       if ((rc = head_product(p, c.stream))) break;
       if (h.n64 > h.n) {
         hipLaunchKernelGGL(k_head_zero_rows, dim3((unsigned)(((h.n64 - h.n) * (ldz / 8) + 255) / 256), (unsigned)h.P), dim3(256),
@@ -647,7 +682,7 @@ int backward(const Call& c, const int64_t* targets, float smooth, const float* s
       if (!fits_launch(blocks, 256)) return pratchya_set_error(PRATCHYA_EUNSUPPORTED, "%s: too large", what);
       auto grad = h.P == 1 ? k_head_grad<1> : k_head_grad<3>;
       hipLaunchKernelGGL(grad, dim3((unsigned)blocks), dim3(256), 0, c.stream, c.floats_at(h.z), Vp - main, h.n, cols - main,
-                         h.n64, Vp - main, targets, v0 + main, h.V, smooth, stats, g, dz + main, ldz);
+                         h.n64, Vp - main, targets, v0 + main, h.V, smooth, stats, g, dz + main, ldz, unit, unit ? head_part(smooth) : 1.0f);
       if ((rc = check_launch(what))) break;
     }
     const int slices = dx ? dx256(h, Vp) : 0;
@@ -667,11 +702,12 @@ int backward(const Call& c, const int64_t* targets, float smooth, const float* s
         p.c_bf16 = last && h.P == 1;
         p.sums = first ? nullptr : c.floats_at(h.dx_sum);
         p.ld_sums = h.C64;
+        p.unit = last ? unit : nullptr;
       }
       if ((rc = head_product(p, c.stream))) break;
       if (slices > 1) {
         hipLaunchKernelGGL((k_head_out<T>), dim3((unsigned)((h.n * ((h.C + 3) / 4) + 255) / 256)), dim3(256), 0, c.stream,
-                           c.floats_at(h.dx_tmp), h.C64, h.n, h.C, c.floats_at(h.dx_sum), !first, last, dx, h.C, slices);
+                           c.floats_at(h.dx_tmp), h.C64, h.n, h.C, c.floats_at(h.dx_sum), !first, last, dx, h.C, slices, unit);
         if ((rc = check_launch(what))) break;
       }
     } else if (dx) {
@@ -679,7 +715,7 @@ int backward(const Call& c, const int64_t* targets, float smooth, const float* s
       rc = c.product(dz, ldz, h.n64, 0, o.w, o.ldw, o.w_rows, h.rows ? 1 : 0, h.n, h.C64, Vp, tmp, h.C64, PRATCHYA_DT_F32);
       if (rc) break;
       hipLaunchKernelGGL((k_head_out<T>), dim3((unsigned)((h.n * ((h.C + 3) / 4) + 255) / 256)), dim3(256), 0, c.stream,
-                         tmp, h.C64, h.n, h.C, c.floats_at(h.dx_sum), v0 > 0, v0 + h.piece >= h.V, dx, h.C, 1);
+                         tmp, h.C64, h.n, h.C, c.floats_at(h.dx_sum), v0 > 0, v0 + h.piece >= h.V, dx, h.C, 1, unit);
       if ((rc = check_launch(what))) break;
     }
     if (dw) {
@@ -695,10 +731,11 @@ int backward(const Call& c, const int64_t* targets, float smooth, const float* s
         p.c = to;
         p.ldc = ld;
         p.c_bf16 = h.P == 1;
+        p.unit = unit;
         if ((rc = head_product(p, c.stream))) break;
         continue;
       }
-      const bool direct = M > 32 && M % 8 == 0 && N % 8 == 0 && ld % chunk == 0 && aligned16(to);
+      const bool direct = !unit && M > 32 && M % 8 == 0 && N % 8 == 0 && ld % chunk == 0 && aligned16(to);
       const int64_t Mt = direct ? M : up64(M), Nt = direct ? N : up64(N);
       void* out = direct ? static_cast<void*>(to) : c.ws + h.dw_tmp;
       const int type = direct ? h.dtype : PRATCHYA_DT_F32;
@@ -708,7 +745,7 @@ int backward(const Call& c, const int64_t* targets, float smooth, const float* s
       if (rc) break;
       if (!direct) {
         hipLaunchKernelGGL((k_head_out<T>), dim3((unsigned)((M * ((N + 3) / 4) + 255) / 256)), dim3(256), 0, c.stream,
-                           c.floats_at(h.dw_tmp), Nt, M, N, nullptr, 0, 1, to, ld, 1);
+                           c.floats_at(h.dw_tmp), Nt, M, N, nullptr, 0, 1, to, ld, 1, unit);
         rc = check_launch(what);
       }
     }
