@@ -12,7 +12,8 @@
 // each row's maximum and sum of 128 columns, which k_head_join joins, or turns its tile
 // into dz (backward, from lse), of which a piece of the vocabulary is held at a time.
 // Below, a piece's f32 logits are computed, read by k_head_rows or k_head_grad and
-// overwritten by the next piece's.  In f32 every operand of a product is the sum of three
+// overwritten by the next piece's.  In bf16 dz is rounded once, in units of the largest
+// cotangent (k_head_unit).  In f32 every operand of a product is the sum of three
 // exact bf16 planes and a product six products of planes.
 //
 // Bound: the MFMAs' rate on 256-row tiles, 1.1 PFLOP/s of four products (logits twice) where
