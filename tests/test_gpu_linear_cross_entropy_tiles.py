@@ -153,3 +153,22 @@ def test_last_round_of_tiles(n, V, C, dt, smooth, tied):
     main = 256 // -(-n // 256) * 256
     targets[40:48] = torch.tensor([main - 257, main - 256, main - 1, main, main + 1, main + 63, V - 65, V - 64])
     _check(x, w, targets, smooth, _normal((n,), torch.float32, 4), tied)
+
+
+@pytest.mark.parametrize("n,V,C", [(100, 2000, 256), (600, 4096, 512)])
+@pytest.mark.parametrize("smooth", [0.0, 0.1])
+def test_one_cotangent_for_all(n, V, C, smooth):
+    """A mean's cotangent, the same for all rows and halfway between two bf16 values: its rounding must
+    not stand in every row.  What is left of a gradient's error is its own rounding, 2^-8 / sqrt(3) of
+    its norm at most (uniform in half a step), and the logits' gradients', which is random and mostly in
+    their small values: together below sqrt(2) of it; the cotangent's own would be 2^-8."""
+    from tests.test_gpu_linear_cross_entropy import reference
+    F = _F()
+    x, w = _normal((n, C), DT["bf16"], 1), _normal((C, V), DT["bf16"], 2, 1.0 / math.sqrt(C))
+    targets = torch.randint(0, V, (n,), generator=torch.Generator().manual_seed(3))
+    g = torch.full((n,), (1 + 2.0 ** -8) / (1 - smooth) / 512)
+    xd, wd = x.cuda().requires_grad_(True), w.cuda().requires_grad_(True)
+    got = torch.autograd.grad(F.linear_cross_entropy(xd, wd, targets.cuda(), label_smoothing=smooth), (xd, wd), g.cuda())
+    want, _ = reference(x, w, targets, smooth, g)
+    for a, b in zip(got, want[1:]):
+        assert float((a.double().cpu() - b).norm() / b.norm()) < 2.0 ** -8 * math.sqrt(2 / 3)
