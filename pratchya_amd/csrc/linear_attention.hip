@@ -23,16 +23,19 @@
 // Products run on bf16 MFMAs.  Exact bf16 inputs are one plane; f32 values (f32 inputs,
 // states, decayed values) are the sum of three, of which products of 2^-24 of the
 // largest or more are taken.  States are f32, and what enters them is never rounded to
-// less.  The scores and the states that outputs in bf16 read are rounded to bf16 once
-// (each below the rounding of the output itself).  The decays' gradient is f32, and what
-// it sums is not rounded: see k_mix_back.
+// less.  The scores and the states that outputs in bf16 read are two planes, 2^-16 of
+// themselves: with one, 2^-9, what the terms of a sum lose stands in outputs in which they
+// cancel (error of 0.0023 of the norm against 64 bits, 0.0017 now, the output's own rounding;
+// a training pass of the size below 690 us, 653 with one).  The decays' gradient is f32, and
+// what it sums is not rounded: see k_mix_back.
 //
 // A sequence is cut into segments where heads alone leave the chip idle: the states that
 // their parts add first (k_mix without outputs), joined from the first to the last, then
 // all segments at once.
 //
-// Measured, 8 x 4096 tokens of 32 heads of 64 in bf16, both passes 650 us: states 36 us for
-// each of S and R, joins 7, o 136, dq 184, k_mix_back 301.  HBM at a copy's rate would take 220
+// Measured, 8 x 4096 tokens of 32 heads of 64 in bf16, both passes 690 us; with one plane of
+// scores and read states 650: states 36 us for each of S and R, joins 7, o 136, dq 184,
+// k_mix_back 301.  HBM at a copy's rate would take 220
 // (1.08 GB).  The MFMAs are busy a sixth of the time, the vector units two fifths (planes,
 // weights, masks), LDS a third, and two or three workgroups a compute unit overlap these in
 // part.  With dk and dv as walks of their own, as dq, whose scores then need three planes
@@ -535,7 +538,7 @@ __device__ __forceinline__ void write_scores(uint16_t (&t)[NP][SIZE], int at, fl
 // scores of a chunk are shared: wave w computes those of its 16 queries, weights and
 // masks them, and all read them from LDS.
 template <typename T, int NP, int NS, int L, int DP, int EP, bool OUT, bool FULL>
-__global__ __launch_bounds__(kThreads, NS == 1 && DP + EP == 128 ? 3 : 2) void k_mix(MixArgs p) {
+__global__ __launch_bounds__(kThreads, NS <= 2 && DP + EP == 128 ? 3 : 2) void k_mix(MixArgs p) {
   constexpr int NPI = sizeof(T) == 2 ? 1 : 3, IT = L / 16, KS = L / 32, DT = DP / 16, ET = EP / 64;
   constexpr bool DOT = OUT && NS == 3;
   using M = Lds<NPI, NP, L, DP, EP, OUT>;
@@ -744,7 +747,7 @@ struct BackLds {
 
 template <typename T, int L, int DP, int EP, bool FULL, bool KEYS, typename M>
 __device__ __forceinline__ void mix_back(const BackArgs& p, M& m) {
-  constexpr int NPI = sizeof(T) == 2 ? 1 : 3, NP = NPI, IT = L / 16, KS = L / 32, THREADS = 2 * kThreads;
+  constexpr int NPI = sizeof(T) == 2 ? 1 : 3, NP = sizeof(T) == 2 ? 2 : 3, IT = L / 16, KS = L / 32, THREADS = 2 * kThreads;
   constexpr int TILES = IT * (IT + 1) / 2;
   // the role's products: outputs of EO values from states [DO, EO]
   constexpr int DO = KEYS ? EP : DP, EO = KEYS ? DP : EP, ET = EO / 64;
@@ -984,7 +987,7 @@ __device__ __forceinline__ void mix_back(const BackArgs& p, M& m) {
 template <typename T, int L, int DP, int EP, bool FULL>
 __global__ __launch_bounds__(2 * kThreads, DP + EP == 128 ? 4 : 2) void k_mix_back(BackArgs p) {
   constexpr int NPI = sizeof(T) == 2 ? 1 : 3;
-  using M = BackLds<NPI, NPI, L, DP, EP>;
+  using M = BackLds<NPI, sizeof(T) == 2 ? 2 : 3, L, DP, EP>;
   __shared__ M m;
   if (__builtin_amdgcn_readfirstlane(threadIdx.x >> 8)) mix_back<T, L, DP, EP, FULL, true>(p, m);
   else mix_back<T, L, DP, EP, FULL, false>(p, m);
@@ -1145,8 +1148,8 @@ int launch_mix(const Shape& s, const MixArgs& a, bool out, hipStream_t stream) {
   if (!blocks) return PRATCHYA_OK;
   if (s.dtype == PRATCHYA_DT_BF16) {
     if (!out) launch_mix_as<uint16_t, 1, 1, 64, false>(a, (unsigned)blocks, stream);
-    else if (a.dot) launch_mix_as<uint16_t, 1, 3, 64, true>(a, (unsigned)blocks, stream);
-    else launch_mix_as<uint16_t, 1, 1, 64, true>(a, (unsigned)blocks, stream);
+    else if (a.dot) launch_mix_as<uint16_t, 2, 3, 64, true>(a, (unsigned)blocks, stream);
+    else launch_mix_as<uint16_t, 2, 2, 64, true>(a, (unsigned)blocks, stream);
   } else {
     if (!out) launch_mix_as<float, 3, 3, 32, false>(a, (unsigned)blocks, stream);
     else launch_mix_as<float, 3, 3, 32, true>(a, (unsigned)blocks, stream);

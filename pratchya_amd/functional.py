@@ -133,7 +133,8 @@ def linear_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log_deca
 
     ``lengths`` [B] (int64 or int32): tokens from a sequence's length on are padding.
     They are not read, their outputs and gradients are 0, and the state is that behind
-    the last token before them.  States are f32 throughout.  Long sequences are cut into
+    the last token before them.  States are f32; where results in bf16 read them, and for
+    the scores of tokens with each other, 16 bits of their values count.  Long sequences are cut into
     segments, into more of them where no gradient is recorded: the results then differ in
     roundings."""
     return LinearAttention(*_ops.linear_attention(q, k, v, log_decay, state, lengths, scale))
