@@ -26,15 +26,15 @@
 // less.  The scores and the states that outputs in bf16 read are two planes, 2^-16 of
 // themselves: with one, 2^-9, what the terms of a sum lose stands in outputs in which they
 // cancel (error of 0.0023 of the norm against 64 bits, 0.0017 now, the output's own rounding;
-// a training pass of the size below 690 us, 653 with one).  The decays' gradient is f32, and
+// a training pass of the size 690 us at the size below, 653 with one).  The decays' gradient is f32, and
 // what it sums is not rounded: see k_mix_back.
 //
 // A sequence is cut into segments where heads alone leave the chip idle: the states that
 // their parts add first (k_mix without outputs), joined from the first to the last, then
 // all segments at once.
 //
-// Measured, 8 x 4096 tokens of 32 heads of 64 in bf16, both passes 690 us; with one plane of
-// scores and read states 650: states 36 us for each of S and R, joins 7, o 136, dq 184,
+// Measured, 8 x 4096 tokens of 32 heads of 64 in bf16, both passes 735 us; with one plane of
+// scores and read states, and NaN not looked for, 650: states 36 us for each of S and R, joins 7, o 136, dq 184,
 // k_mix_back 301.  HBM at a copy's rate would take 220
 // (1.08 GB).  The MFMAs are busy a sixth of the time, the vector units two fifths (planes,
 // weights, masks), LDS a third, and two or three workgroups a compute unit overlap these in
@@ -504,6 +504,74 @@ __device__ __forceinline__ void add_scores(const uint16_t (&t)[NP][SIZE], int pi
     }
 }
 
+// Values that are not finite.  A score that its mask makes 0 is multiplied all the same, and 0
+// times NaN or infinity is NaN: such values are 0 in the products (drop_odd, which tells
+// whether the wave has any) and reach the tokens that they count for in a walk of their own.
+// The test and the branch take 6% of the training pass below (690 -> 735 us); with a flag from
+// the threads that store the values, or without a branch, it took as much or more.
+template <int KS, int ET, int NPI>
+__device__ __forceinline__ bool drop_odd(bf16x8_t (&val)[KS][ET][NPI]) {
+  auto odd_of = [](uint32_t w) { return ((w & 0x7F807F80u) + 0x00800080u) & 0x80008000u; };      // exponents all ones
+  uint32_t any = 0;
+#pragma unroll
+  for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+    for (int et = 0; et < ET; ++et) {
+      const v4i w = __builtin_bit_cast(v4i, val[ks][et][0]);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) any |= odd_of((uint32_t)w[i]);
+    }
+  if (!__any(any != 0)) return false;
+#pragma unroll
+  for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+    for (int et = 0; et < ET; ++et) {
+      const v4i top = __builtin_bit_cast(v4i, val[ks][et][0]);
+#pragma unroll
+      for (int x = 0; x < NPI; ++x) {
+        v4i w = __builtin_bit_cast(v4i, val[ks][et][x]);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const uint32_t odd = odd_of((uint32_t)top[i]);
+          w[i] &= (int)~(odd | (odd - (odd >> 15)));
+        }
+        val[ks][et][x] = __builtin_bit_cast(bf16x8_t, w);
+      }
+    }
+  return true;
+}
+// acc += scores t [token][key] times the values v [key][value] that are not finite.
+template <bool REV, int L, int IT, int ET, int NP, int NPI, int TS, int VS>
+__device__ __forceinline__ void add_odd(const uint16_t (&t)[NP][TS], int pt, const uint16_t (&v)[NPI][VS], int pv, int wave,
+                                        int lane, v4f (&acc)[IT][ET]) {
+  const int l16 = lane & 15, g4 = lane >> 4;
+#pragma unroll 1
+  for (int j = 0; j < L; ++j) {
+#pragma unroll
+    for (int et = 0; et < ET; ++et) {
+      float x[4] = {};
+#pragma unroll
+      for (int c = NPI - 1; c >= 0; --c) {
+        float y[4];
+        widen4(*reinterpret_cast<const u32x2_t*>(v[c] + j * pv + (wave * ET + et) * 16 + g4 * 4), y);
+#pragma unroll
+        for (int r = 0; r < 4; ++r) x[r] += y[r];
+      }
+#pragma unroll
+      for (int it = 0; it < IT; ++it) {
+        const int i = it * 16 + l16;
+        if (REV ? j < i : j > i) continue;
+        float w = 0.0f;
+#pragma unroll
+        for (int c = NP - 1; c >= 0; --c) w += load_elem(t[c] + i * pt + j);
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+          if (!((f2u(x[r]) & 0x7F800000u) < 0x7F800000u)) acc[it][et][r] += w * x[r];
+      }
+    }
+  }
+}
+
 // 16 x 16 products of two arrays' rows; rows of the result are a's.
 template <int DK, int NPI, int SIZE>
 __device__ __forceinline__ v4f row_products(const uint16_t (&a)[NPI][SIZE], int ra, const uint16_t (&b)[NPI][SIZE], int rb,
@@ -667,7 +735,9 @@ __global__ __launch_bounds__(kThreads, NS <= 2 && DP + EP == 128 ? 3 : 2) void k
     S.update(m.k, M::PD, val, !OUT && p.rev ? m.gates.start[par] : m.gates.rest[par], p.kscale, m.gates.total[par], lane);
     __syncthreads();                    // scores are whole
     if constexpr (OUT) {
+      const bool odd = drop_odd(val);
       add_scores<false>(m.t, M::PT, val, lane, acc);
+      if (odd) add_odd<false, L>(m.t, M::PT, m.v, M::PE, wave, lane, acc);
       const int end = (int)min(length - t0, (int64_t)L);
       // acc[it][et][r]: token 16 it + l16, value 16 (wave ET + et) + 4 g4 + r
 #pragma unroll
@@ -925,7 +995,12 @@ __device__ __forceinline__ void mix_back(const BackArgs& p, M& m) {
       R.update(m.q, M::PD, val, m.gates.start[par], p.scale, m.gates.total[par], lane);
     }
     __syncthreads();                    // scores are whole
+    const bool odd = drop_odd(val);
     add_scores<true>(KEYS ? m.tb : m.ta, M::PT, val, lane, acc);
+    if (odd) {
+      if constexpr (KEYS) add_odd<true, L>(m.tb, M::PT, m.q, M::PD, wave, lane, acc);
+      else add_odd<true, L>(m.ta, M::PT, m.g, M::PE, wave, lane, acc);
+    }
     const int end = (int)min(length - t0, (int64_t)L);
 #pragma unroll
     for (int it = 0; it < IT; ++it) {

@@ -133,7 +133,9 @@ def linear_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log_deca
 
     ``lengths`` [B] (int64 or int32): tokens from a sequence's length on are padding.
     They are not read, their outputs and gradients are 0, and the state is that behind
-    the last token before them.  States are f32; where results in bf16 read them, and for
+    the last token before them.  A NaN or an infinity reaches the results that the
+    recurrence takes it to, there as one or the other; in gradients of log_decay, sums
+    over later tokens, it reaches earlier tokens too.  States are f32; where results in bf16 read them, and for
     the scores of tokens with each other, 16 bits of their values count.  Long sequences are cut into
     segments, into more of them where no gradient is recorded: the results then differ in
     roundings."""
