@@ -38,7 +38,7 @@ struct HeadProduct {
   float* part_sum;                         // likewise, or null
   float* target_value;                     // [rows]
   int64_t ld_part;
-  // kHeadStore: null, or what the results are multiplied by.  kHeadGrad: null, or behind that
+  // kHeadStore, 128-row tiles: null, or what the results are multiplied by.  kHeadGrad: null, or behind that
   // 1 / max |g|: C is then dz over the first.
   const float* unit;
   const float *stats, *g;                  // kHeadGrad: (maximum, log of the sum about it), the loss's cotangent
@@ -48,6 +48,11 @@ struct HeadProduct {
 // held in bf16, so that the target's value, -g of it where its probability is small, has no
 // rounding of its own that all rows share.
 inline float head_part(float smooth) { return smooth < 0.5f ? 1.0f - smooth : 1.0f; }
+
+// C [M, N], f32 (or bf16 times *unit), on the 128-row tiles of gemm_t128.hip, for any M and N of
+// at least a row that pratchya_gemm_bf16_planes takes: a, b, their planes and segs, M, N, K, c,
+// ldc, c_bf16 and unit count.  ws: its workspace.
+int head_product128(const HeadProduct& p, void* ws, int64_t ws_bytes, hipStream_t stream);
 
 // Whether the operands suit (sizes, alignment, 32-bit offsets).
 bool head_product_fits(const HeadProduct& p);

@@ -29,6 +29,7 @@
 #include <numeric>
 #include <type_traits>
 
+#include "gemm_head.h"
 #include "pratchya_fp8.h"
 #include "quant_device.h"
 
@@ -71,6 +72,7 @@ struct T128Args {
   float* part;                           // splits > 1: f32 partials [splits][M][N]
   const uint16_t* X;                     // OUT 2
   const uint32_t* flags;                 // bf16 planes, may be null: see k_gemm_t128
+  const float* unit;                     // OUT 1, may be null: what results are multiplied by before they are rounded
   int64_t ldc, ldx;
   int M, N, spp, segs, segs_short, span, splits, tiles_m, tiles_n;
   // independent products of one shape: bytes (A, B) and elements (C, X) from
@@ -622,8 +624,14 @@ __global__ __launch_bounds__(256, 2) void k_gemm_t128(T128Args p) {
 #pragma unroll
       for (int it = 0; it < WN / 16; ++it) {
         const int q = it * 64 + lane, r = q / (WN / 8), c = (q % (WN / 8)) * 8;
-        const v4f v = *reinterpret_cast<const v4f*>(stg + r * PITCH + c * 4);
-        const v4f x = *reinterpret_cast<const v4f*>(stg + r * PITCH + c * 4 + 16);
+        v4f v = *reinterpret_cast<const v4f*>(stg + r * PITCH + c * 4);
+        v4f x = *reinterpret_cast<const v4f*>(stg + r * PITCH + c * 4 + 16);
+        if constexpr (OUT == 1) {
+          if (p.unit) {
+            v *= *p.unit;
+            x *= *p.unit;
+          }
+        }
         v4i o = {(int)pack_bf16x2(v.x, v.y), (int)pack_bf16x2(v.z, v.w), (int)pack_bf16x2(x.x, x.y),
                  (int)pack_bf16x2(x.z, x.w)};
         if (row0 + r < p.M && col0 + c < p.N) {
@@ -646,7 +654,7 @@ template <int OUT>
 __global__ __launch_bounds__(256) void k_reduce_slices(const float* part, int splits, int M, int N,
                                                        void* C, int64_t ldc,
                                                        const uint16_t* X, int64_t ldx, int64_t c_bs,
-                                                       int64_t x_bs) {
+                                                       int64_t x_bs, const float* unit) {
   part += (int64_t)blockIdx.y * splits * M * N;
   C = static_cast<uint8_t*>(C) + (int64_t)blockIdx.y * c_bs * (OUT == 0 ? 4 : 2);
   if constexpr (OUT == 2) X += (int64_t)blockIdx.y * x_bs;
@@ -667,6 +675,12 @@ __global__ __launch_bounds__(256) void k_reduce_slices(const float* part, int sp
     if constexpr (OUT == 0) {
       *reinterpret_cast<v4f*>(static_cast<float*>(C) + r * ldc + c) = v[0];
     } else {
+      if constexpr (OUT == 1) {
+        if (unit) {
+          v[0] *= *unit;
+          v[1] *= *unit;
+        }
+      }
       v4i o = {(int)pack_bf16x2(v[0].x, v[0].y), (int)pack_bf16x2(v[0].z, v[0].w), (int)pack_bf16x2(v[1].x, v[1].y),
                (int)pack_bf16x2(v[1].z, v[1].w)};
       if constexpr (OUT == 2) {
@@ -722,7 +736,7 @@ void t128_launch(const T128Args& p, hipStream_t stream, bool reduce = true) {
     const int64_t n = (int64_t)p.M * (p.N / (OUT == 0 ? 4 : 8));
     const int64_t blocks = (n + 255) / 256;
     hipLaunchKernelGGL((k_reduce_slices<OUT>), dim3((unsigned)(blocks < 2048 ? blocks : 2048), (unsigned)p.batch),
-                       dim3(256), 0, stream, p.part, p.splits, p.M, p.N, p.C, p.ldc, p.X, p.ldx, p.c_bs, p.x_bs);
+                       dim3(256), 0, stream, p.part, p.splits, p.M, p.N, p.C, p.ldc, p.X, p.ldx, p.c_bs, p.x_bs, p.unit);
   }
 }
 
@@ -882,14 +896,14 @@ extern "C" int pratchya_gemm_bs_t128_fq(const uint8_t* A, int64_t lda, const uin
                                           y_dtype == PRATCHYA_DT_BF16, fix_nan != 0, sc_fp8, sc_fp32, stream);
 }
 
-extern "C" int pratchya_gemm_bf16_planes(const void* A, int64_t lda, int64_t a_stride, int a_kmajor, int a_held,
-                                         uint32_t a_planes, const void* B, int64_t ldb, int64_t b_stride, int b_kmajor,
-                                         int b_held, uint32_t b_planes, uint32_t b_planes_alt, int64_t M, int64_t N,
-                                         int64_t K, int segs, int segs_short, const uint32_t* flags,
-                                         const float* b_sc32, int64_t b_brow, int64_t b_bcol, int64_t b_kg, void* C,
-                                         int64_t ldc, int c_dtype, const void* X, int64_t ldx, int64_t batch,
-                                         int64_t a_batch, int64_t b_batch, int64_t c_batch, int64_t x_batch, void* ws,
-                                         int64_t ws_bytes, hipStream_t stream) {
+namespace {
+
+int planes_product(const void* A, int64_t lda, int64_t a_stride, int a_kmajor, int a_held, uint32_t a_planes,
+                   const void* B, int64_t ldb, int64_t b_stride, int b_kmajor, int b_held, uint32_t b_planes,
+                   uint32_t b_planes_alt, int64_t M, int64_t N, int64_t K, int segs, int segs_short,
+                   const uint32_t* flags, const float* b_sc32, int64_t b_brow, int64_t b_bcol, int64_t b_kg, void* C,
+                   int64_t ldc, int c_dtype, const void* X, int64_t ldx, int64_t batch, int64_t a_batch, int64_t b_batch,
+                   int64_t c_batch, int64_t x_batch, void* ws, int64_t ws_bytes, const float* unit, hipStream_t stream) {
   const char* who = "gemm_bf16_planes";
   if (M <= 0 || N <= 0 || K <= 0 || batch <= 0) {
     if (M < 0 || N < 0 || K < 0 || batch < 0) return pratchya_set_error(PRATCHYA_EINVAL, "%s: negative size", who);
@@ -940,6 +954,7 @@ extern "C" int pratchya_gemm_bf16_planes(const void* A, int64_t lda, int64_t a_s
   p.X = static_cast<const uint16_t*>(X);
   p.ldx = ldx;
   p.flags = flags;
+  p.unit = unit;
   p.spp = (int)(K / 64);
   p.segs = segs;
   p.segs_short = segs_short;
@@ -996,6 +1011,28 @@ extern "C" int pratchya_gemm_bf16_planes(const void* A, int64_t lda, int64_t a_s
     else t128_launch<true, 128, false, false, 0, 0>(p, stream);
   }
   return t128_status(who);
+}
+
+}  // namespace
+
+extern "C" int pratchya_gemm_bf16_planes(const void* A, int64_t lda, int64_t a_stride, int a_kmajor, int a_held,
+                                         uint32_t a_planes, const void* B, int64_t ldb, int64_t b_stride, int b_kmajor,
+                                         int b_held, uint32_t b_planes, uint32_t b_planes_alt, int64_t M, int64_t N,
+                                         int64_t K, int segs, int segs_short, const uint32_t* flags,
+                                         const float* b_sc32, int64_t b_brow, int64_t b_bcol, int64_t b_kg, void* C,
+                                         int64_t ldc, int c_dtype, const void* X, int64_t ldx, int64_t batch,
+                                         int64_t a_batch, int64_t b_batch, int64_t c_batch, int64_t x_batch, void* ws,
+                                         int64_t ws_bytes, hipStream_t stream) {
+  return planes_product(A, lda, a_stride, a_kmajor, a_held, a_planes, B, ldb, b_stride, b_kmajor, b_held, b_planes,
+                        b_planes_alt, M, N, K, segs, segs_short, flags, b_sc32, b_brow, b_bcol, b_kg, C, ldc, c_dtype, X,
+                        ldx, batch, a_batch, b_batch, c_batch, x_batch, ws, ws_bytes, nullptr, stream);
+}
+
+int head_product128(const HeadProduct& p, void* ws, int64_t ws_bytes, hipStream_t stream) {
+  return planes_product(p.a, p.lda, p.a_plane, p.a_kmajor, p.planes, p.a_planes, p.b, p.ldb, p.b_plane, p.b_kmajor,
+                        p.planes, p.b_planes, p.b_planes, p.M, p.N, p.K, p.segs, p.segs, nullptr, nullptr, 0, 0, 0, p.c,
+                        p.ldc, p.c_bf16 ? PRATCHYA_DT_BF16 : PRATCHYA_DT_F32, nullptr, 0, 1, 0, 0, 0, 0, ws, ws_bytes,
+                        p.c_bf16 ? p.unit : nullptr, stream);
 }
 
 extern "C" int pratchya_gemm_fine(const void* A, int64_t lda, const float* a_sc32, const void* B, int64_t ldb,

@@ -362,6 +362,14 @@ struct Head {
     const int64_t main = full * 256 / tm * 256;
     return main >= 256 && main < all && (tn * 256 - main) / 256 * tm <= 85 ? main : all;
   }
+  // Whether the 128-row tiles store the weight's gradient of a piece's columns themselves, at
+  // a 16-byte aligned address; else it goes through f32 sums, of dw_cols columns at a time.
+  // ([128, 4096] . [4096, 65536] in bf16, both passes: 653 us, all of it through f32 1014.)
+  bool dw_plain(int64_t cols) const {
+    const int64_t M = rows ? cols : C, N = rows ? C : cols, ld = rows ? C : V;
+    return M > 32 && M % 8 == 0 && N % 8 == 0 && ld % (P == 1 ? 8 : 4) == 0;
+  }
+  int64_t dw_cols;
   // workspace
   int64_t part, part_sum, zt, unit;
   int64_t xp, wp, z, dzp, dx_sum, dx_tmp, dw_tmp, split, split_bytes, bytes;
@@ -464,6 +472,11 @@ int plan(const char* what, bool bwd, bool want_dx, bool want_dw, Head* h) {
       if (Vp - h->main_of(Vp) > by_rows) by_rows = Vp - h->main_of(Vp);
   }
   h->z = take(4 * h->n * by_rows);
+  const int64_t last = h->V - (h->V - 1) / h->piece * h->piece;
+  const int64_t tmp = h->dw_plain(last) && (last == h->V || h->dw_plain(h->piece)) ? kPieceBytes / 8 : kPieceBytes;
+  h->dw_cols = tmp / 4 / h->C64 / 64 * 64;
+  if (h->dw_cols < 64) h->dw_cols = 64;
+  if (h->dw_cols > h->piece) h->dw_cols = h->piece;
   h->split_bytes = 0;
   auto split = [&](int64_t M, int64_t N, int64_t K) {
     const int64_t b = pratchya_gemm_t128_workspace_bytes(M, N, segs * (K / 64), 1);
@@ -474,8 +487,9 @@ int plan(const char* what, bool bwd, bool want_dx, bool want_dw, Head* h) {
     if (main < Vp) split(h->n, Vp - main, h->C64);
     if (bwd && want_dx && !dx256(*h, Vp)) split(h->n, h->C64, Vp);
     if (bwd && want_dw && !dw256(*h, Vp)) {
-      split(h->rows ? Vp : h->C64, h->rows ? h->C64 : Vp, h->n64);
       split(h->rows ? Vp : h->C, h->rows ? h->C : Vp, h->n64);
+      for (int64_t wide : {Vp < h->dw_cols ? Vp : h->dw_cols, Vp % h->dw_cols})
+        if (wide) split(h->rows ? wide : h->C64, h->rows ? h->C64 : wide, h->n64);
     }
   }
   h->dzp = h->dx_sum = h->dx_tmp = h->dw_tmp = 0;
@@ -491,7 +505,7 @@ int plan(const char* what, bool bwd, bool want_dx, bool want_dw, Head* h) {
       h->dx_tmp = take(4 * slices * h->n * h->C64);
       h->dx_sum = take(h->piece < h->V ? 4 * h->n * h->C64 : 0);
     }
-    if (want_dw && !(dw256(*h, h->piece) && dw256(*h, rest))) h->dw_tmp = take(4 * h->C64 * h->piece);
+    if (want_dw && !(dw256(*h, h->piece) && dw256(*h, rest))) h->dw_tmp = take(4 * h->C64 * h->dw_cols);
   }
   h->split = take(h->split_bytes);
   h->bytes = at;
@@ -518,8 +532,9 @@ struct Call {
                          static_cast<const float*>(src), ld, rows, cols, rows_to, cols_to, targets, dst);
     return check_launch("linear_cross_entropy");
   }
-  // The same on 256-row tiles.
-  HeadProduct product256(const uint16_t* A, int64_t lda, int64_t a_rows, bool a_kmajor, const uint16_t* B, int64_t ldb,
+  // C [M, N] = A . B over K; a plane's rows lie lda / ldb apart, planes a_rows * lda: what both
+  // kinds of tiles take.
+  HeadProduct operands(const uint16_t* A, int64_t lda, int64_t a_rows, bool a_kmajor, const uint16_t* B, int64_t ldb,
                          int64_t b_rows, bool b_kmajor, int64_t M, int64_t N, int64_t K) const {
     HeadProduct p{};
     p.a = A;
@@ -542,14 +557,13 @@ struct Call {
     p.cols = N;
     return p;
   }
-  // C [M, N] = A . B over K; a plane's rows lie lda / ldb apart, planes a_rows * lda.
-  int product(const uint16_t* A, int64_t lda, int64_t a_rows, int a_kmajor, const uint16_t* B, int64_t ldb,
-              int64_t b_rows, int b_kmajor, int64_t M, int64_t N, int64_t K, void* C, int64_t ldc, int dtype) const {
-    const int segs = h.P == 1 ? 1 : 6;
-    return pratchya_gemm_bf16_planes(A, lda, a_rows * lda, a_kmajor, h.P, h.P == 1 ? 0 : kPairsA, B, ldb, b_rows * ldb,
-                                     b_kmajor, h.P, h.P == 1 ? 0 : kPairsB, h.P == 1 ? 0 : kPairsB, M, N, K, segs, segs,
-                                     nullptr, nullptr, 0, 0, 0, C, ldc, dtype, nullptr, 0, 1, 0, 0, 0, 0,
-                                     ws + h.split, h.split_bytes, stream);
+  // On 128-row tiles, to C in dtype, in bf16 times *unit.
+  int product(HeadProduct p, void* C, int64_t ldc, int dtype, const float* unit = nullptr) const {
+    p.c = C;
+    p.ldc = ldc;
+    p.c_bf16 = dtype == PRATCHYA_DT_BF16;
+    p.unit = unit;
+    return head_product128(p, ws + h.split, h.split_bytes, stream);
   }
 };
 
@@ -591,14 +605,14 @@ int operand_w(const Call& c, int64_t v0, int64_t cols, int64_t Vp, Operands* o) 
 // A piece's logits from column `from` on into the workspace, [n, Vp - from].
 int logits(const Call& c, const Operands& o, int64_t from, int64_t Vp) {
   const Head& h = c.h;
-  return c.product(o.x, o.ldx, o.x_rows, 0, o.w + (h.rows ? from * o.ldw : from), o.ldw, o.w_rows, h.rows ? 0 : 1, h.n,
-                   Vp - from, h.C64, c.floats_at(h.z), Vp - from, PRATCHYA_DT_F32);
+  return c.product(c.operands(o.x, o.ldx, o.x_rows, false, o.w + (h.rows ? from * o.ldw : from), o.ldw, o.w_rows, !h.rows, h.n,
+                              Vp - from, h.C64), c.floats_at(h.z), Vp - from, PRATCHYA_DT_F32);
 }
 
 HeadProduct logits_product(const Call& c, const Operands& o, int64_t v0, int64_t cols, int64_t main,
                            const int64_t* targets, float smooth) {
   const Head& h = c.h;
-  HeadProduct p = c.product256(o.x, o.ldx, o.x_rows, false, o.w, o.ldw, o.w_rows, !h.rows, h.n, main, h.C64);
+  HeadProduct p = c.operands(o.x, o.ldx, o.x_rows, false, o.w, o.ldw, o.w_rows, !h.rows, h.n, main, h.C64);
   p.rows = h.n;
   p.cols = cols < main ? cols : main;
   p.targets = targets;
@@ -689,7 +703,7 @@ int backward(const Call& c, const int64_t* targets, float smooth, const float* s
     const int slices = dx ? dx256(h, Vp) : 0;
     if (slices) {
       const bool first = v0 == 0, last = v0 + h.piece >= h.V;
-      HeadProduct p = c.product256(dz, ldz, h.n64, false, o.w, o.ldw, o.w_rows, h.rows, h.n, h.C64, Vp);
+      HeadProduct p = c.operands(dz, ldz, h.n64, false, o.w, o.ldw, o.w_rows, h.rows, h.n, h.C64, Vp);
       p.epilogue = kHeadStore;
       if (slices > 1) {
         p.splits = slices;
@@ -713,7 +727,8 @@ int backward(const Call& c, const int64_t* targets, float smooth, const float* s
       }
     } else if (dx) {
       float* tmp = c.floats_at(h.dx_tmp);
-      rc = c.product(dz, ldz, h.n64, 0, o.w, o.ldw, o.w_rows, h.rows ? 1 : 0, h.n, h.C64, Vp, tmp, h.C64, PRATCHYA_DT_F32);
+      rc = c.product(c.operands(dz, ldz, h.n64, false, o.w, o.ldw, o.w_rows, h.rows, h.n, h.C64, Vp), tmp, h.C64,
+                     PRATCHYA_DT_F32);
       if (rc) break;
       hipLaunchKernelGGL((k_head_out<T>), dim3((unsigned)((h.n * ((h.C + 3) / 4) + 255) / 256)), dim3(256), 0, c.stream,
                          tmp, h.C64, h.n, h.C, c.floats_at(h.dx_sum), v0 > 0, v0 + h.piece >= h.V, dx, h.C, 1, unit);
@@ -724,8 +739,8 @@ int backward(const Call& c, const int64_t* targets, float smooth, const float* s
       const int64_t M = h.rows ? cols : h.C, N = h.rows ? h.C : cols, ld = h.rows ? h.C : h.V;
       T* to = dw + (h.rows ? v0 * h.C : v0);
       if (dw256(h, Vp)) {
-        HeadProduct p = h.rows ? c.product256(dz, ldz, h.n64, true, o.x, o.ldx, o.x_rows, true, Vp, h.C64, h.n64)
-                               : c.product256(o.x, o.ldx, o.x_rows, true, dz, ldz, h.n64, true, h.C64, Vp, h.n64);
+        HeadProduct p = h.rows ? c.operands(dz, ldz, h.n64, true, o.x, o.ldx, o.x_rows, true, Vp, h.C64, h.n64)
+                               : c.operands(o.x, o.ldx, o.x_rows, true, dz, ldz, h.n64, true, h.C64, Vp, h.n64);
         p.epilogue = kHeadStore;
         p.rows = M;
         p.cols = N;
@@ -736,17 +751,21 @@ int backward(const Call& c, const int64_t* targets, float smooth, const float* s
         if ((rc = head_product(p, c.stream))) break;
         continue;
       }
-      const bool direct = !unit && M > 32 && M % 8 == 0 && N % 8 == 0 && ld % chunk == 0 && aligned16(to);
-      const int64_t Mt = direct ? M : up64(M), Nt = direct ? N : up64(N);
-      void* out = direct ? static_cast<void*>(to) : c.ws + h.dw_tmp;
-      const int type = direct ? h.dtype : PRATCHYA_DT_F32;
-      const int64_t ldo = direct ? ld : Nt;
-      rc = h.rows ? c.product(dz, ldz, h.n64, 1, o.x, o.ldx, o.x_rows, 1, Mt, Nt, h.n64, out, ldo, type)
-                  : c.product(o.x, o.ldx, o.x_rows, 1, dz, ldz, h.n64, 1, Mt, Nt, h.n64, out, ldo, type);
-      if (rc) break;
-      if (!direct) {
-        hipLaunchKernelGGL((k_head_out<T>), dim3((unsigned)((M * ((N + 3) / 4) + 255) / 256)), dim3(256), 0, c.stream,
-                           c.floats_at(h.dw_tmp), Nt, M, N, nullptr, 0, 1, to, ld, 1, unit);
+      // columns [b, b + wide) of the piece
+      auto dw_of = [&](int64_t b, int64_t Mt, int64_t Nt) {
+        return h.rows ? c.operands(dz + b, ldz, h.n64, true, o.x, o.ldx, o.x_rows, true, Mt, Nt, h.n64)
+                      : c.operands(o.x, o.ldx, o.x_rows, true, dz + b, ldz, h.n64, true, Mt, Nt, h.n64);
+      };
+      if (h.dw_plain(cols) && aligned16(to)) {
+        if ((rc = c.product(dw_of(0, M, N), to, ld, h.dtype, unit))) break;
+        continue;
+      }
+      for (int64_t b = 0; b < cols && !rc; b += h.dw_cols) {
+        const int64_t wide = Vp - b < h.dw_cols ? Vp - b : h.dw_cols, some = cols - b < wide ? cols - b : wide;
+        const int64_t Nt = h.rows ? h.C64 : wide, Mb = h.rows ? some : M, Nb = h.rows ? N : some;
+        if ((rc = c.product(dw_of(b, h.rows ? wide : h.C64, Nt), c.ws + h.dw_tmp, Nt, PRATCHYA_DT_F32))) break;
+        hipLaunchKernelGGL((k_head_out<T>), dim3((unsigned)((Mb * ((Nb + 3) / 4) + 255) / 256)), dim3(256), 0, c.stream,
+                           c.floats_at(h.dw_tmp), Nt, Mb, Nb, nullptr, 0, 1, to + (h.rows ? b * h.C : b), ld, 1, unit);
         rc = check_launch(what);
       }
     }

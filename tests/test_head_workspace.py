@@ -1,0 +1,27 @@
+"""What linear_cross_entropy asks of memory below 256 rows, by the library's size query: pieces of
+planes and sums, no f32 copy of the weight's gradient."""
+import pytest
+
+FAKE = 1 << 20
+MB = 1 << 20
+
+
+@pytest.mark.parametrize("dtype", [0, 1])
+@pytest.mark.parametrize("rows", [0, 1])
+@pytest.mark.parametrize("n,C,V", [(128, 4096, 65536), (255, 8192, 128256), (64, 4096, 262144), (1, 2048, 50257), (40, 4100, 20003)])
+def test_few_rows(n, C, V, rows, dtype):
+    from pratchya_amd import _lib
+    size = _lib.load().pratchya_linear_cross_entropy_workspace_bytes
+    n64, planes = (n + 63) // 64 * 64, 2 if dtype else 6
+    for back in ((0, 0), (1, 0), (0, 1), (1, 1)):
+        got = size(FAKE, C, FAKE, C if rows else V, dtype, rows, n, C, V, *back)
+        # logits and their gradient, x's planes, partial sums of x's gradient, what products hold of slices
+        bound = (4 + planes) * n64 * (V + 64) + planes * n64 * (C + 64) + 140 * n * (C + 64) + 64 * MB
+        if not (dtype == 1 and C % 64 == 0 and V % 64 == 0):
+            bound += 512 * MB      # a piece of the weight's planes
+        plain = C % 8 == 0 and V % 8 == 0
+        if back[1]:
+            bound += (32 if plain else 256) * MB
+        assert 0 < got < bound, (back, got / MB, bound / MB)
+    if (n, dtype) == (128, 1):
+        assert size(FAKE, C, FAKE, C if rows else V, 1, rows, n, C, V, 1, 1) < 150 * MB
