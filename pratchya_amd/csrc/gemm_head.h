@@ -52,6 +52,7 @@ inline float head_part(float smooth) { return smooth < 0.5f ? 1.0f - smooth : 1.
 // C [M, N], f32 (or bf16 times *unit), on the 128-row tiles of gemm_t128.hip, for any M and N of
 // at least a row that pratchya_gemm_bf16_planes takes: a, b, their planes and segs, M, N, K, c,
 // ldc, c_bf16 and unit count.  ws: its workspace.
+bool head_product128_fits(const HeadProduct& p);      // sizes only
 int head_product128(const HeadProduct& p, void* ws, int64_t ws_bytes, hipStream_t stream);
 
 // Whether the operands suit (sizes, alignment, 32-bit offsets).

@@ -898,6 +898,15 @@ extern "C" int pratchya_gemm_bs_t128_fq(const uint8_t* A, int64_t lda, const uin
 
 namespace {
 
+// Whether a product's operands, the last planes of which begin pa and pb elements behind the
+// first, lie within the offsets and counters of the kernels.
+bool planes_fit(int64_t pa, int64_t lda, bool a_kmajor, int64_t pb, int64_t ldb, bool b_kmajor, int64_t M, int64_t N,
+                int64_t K, int64_t segs) {
+  const int64_t Mr = (M + 127) / 128 * 128, Nr = (N + 127) / 128 * 128;
+  return 2 * (pa + (a_kmajor ? K + 1 : Mr) * lda + Mr) <= kMaxOffset && 2 * (pb + (b_kmajor ? K + 1 : Nr) * ldb + Nr) <= kMaxOffset &&
+         M <= INT32_MAX / 2 && N <= INT32_MAX / 2 && segs * (K / 64) <= (1 << 24);
+}
+
 int planes_product(const void* A, int64_t lda, int64_t a_stride, int a_kmajor, int a_held, uint32_t a_planes,
                    const void* B, int64_t ldb, int64_t b_stride, int b_kmajor, int b_held, uint32_t b_planes,
                    uint32_t b_planes_alt, int64_t M, int64_t N, int64_t K, int segs, int segs_short,
@@ -931,10 +940,9 @@ int planes_product(const void* A, int64_t lda, int64_t a_stride, int a_kmajor, i
       (reinterpret_cast<uintptr_t>(A) | reinterpret_cast<uintptr_t>(B) | reinterpret_cast<uintptr_t>(C)) % 16 ||
       (X && (c_dtype != PRATCHYA_DT_BF16 || ldx < N || ldx % 8 || reinterpret_cast<uintptr_t>(X) % 16)))
     return pratchya_set_error(PRATCHYA_EINVAL, "%s: leading dimensions / alignment not supported", who);
-  const int64_t Mr = (M + 127) / 128 * 128, Nr = (N + 127) / 128 * 128;
+  const int64_t Nr = (N + 127) / 128 * 128;
   const int64_t pa = a_held > 1 ? (a_held - 1) * a_stride : 0, pb = b_held > 1 ? (b_held - 1) * b_stride : 0;
-  if (2 * (pa + (a_kmajor ? K + 1 : Mr) * lda + Mr) > kMaxOffset || 2 * (pb + (b_kmajor ? K + 1 : Nr) * ldb + Nr) > kMaxOffset ||
-      M > INT32_MAX / 2 || N > INT32_MAX / 2 || segs * (K / 64) > (1 << 24))
+  if (!planes_fit(pa, lda, a_kmajor, pb, ldb, b_kmajor, M, N, K, segs))
     return pratchya_set_error(PRATCHYA_EUNSUPPORTED, "%s: operands beyond 32-bit offsets", who);
   T128Args p{};
   p.a.p = static_cast<const uint8_t*>(A);
@@ -1026,6 +1034,11 @@ extern "C" int pratchya_gemm_bf16_planes(const void* A, int64_t lda, int64_t a_s
   return planes_product(A, lda, a_stride, a_kmajor, a_held, a_planes, B, ldb, b_stride, b_kmajor, b_held, b_planes,
                         b_planes_alt, M, N, K, segs, segs_short, flags, b_sc32, b_brow, b_bcol, b_kg, C, ldc, c_dtype, X,
                         ldx, batch, a_batch, b_batch, c_batch, x_batch, ws, ws_bytes, nullptr, stream);
+}
+
+bool head_product128_fits(const HeadProduct& p) {
+  return planes_fit((p.planes - 1) * p.a_plane, p.lda, p.a_kmajor, (p.planes - 1) * p.b_plane, p.ldb, p.b_kmajor, p.M, p.N, p.K,
+                    p.segs);
 }
 
 int head_product128(const HeadProduct& p, void* ws, int64_t ws_bytes, hipStream_t stream) {

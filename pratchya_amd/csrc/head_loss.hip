@@ -320,6 +320,7 @@ __global__ __launch_bounds__(256) void k_head_out(const float* __restrict__ src,
 // host
 // --------------------------------------------------------------------------
 int64_t up64(int64_t v) { return (v + 63) / 64 * 64; }
+int64_t up128(int64_t v) { return (v + 127) / 128 * 128; }
 int64_t round256(int64_t v) { return (v + 255) / 256 * 256; }
 
 // Largest f32 logits of a piece, and the planes of its weight.
@@ -406,6 +407,62 @@ bool dw256(const Head& h, int64_t Vp) {
   return on256(h, h.rows ? Vp : h.C64, h.rows ? h.C64 : Vp, 1, 1) != 0;
 }
 
+// C [M, N] = A . B over K; a plane's rows lie lda / ldb apart, planes a_rows * lda: what both
+// kinds of tiles take.
+HeadProduct operands(const Head& h, const uint16_t* A, int64_t lda, int64_t a_rows, bool a_kmajor, const uint16_t* B, int64_t ldb,
+                     int64_t b_rows, bool b_kmajor, int64_t M, int64_t N, int64_t K) {
+  HeadProduct p{};
+  p.a = A;
+  p.b = B;
+  p.lda = lda;
+  p.ldb = ldb;
+  p.a_plane = h.P == 1 ? 0 : a_rows * lda;
+  p.b_plane = h.P == 1 ? 0 : b_rows * ldb;
+  p.a_kmajor = a_kmajor;
+  p.b_kmajor = b_kmajor;
+  p.a_planes = h.P == 1 ? 0 : kPairsA;
+  p.b_planes = h.P == 1 ? 0 : kPairsB;
+  p.segs = h.P == 1 ? 1 : 6;
+  p.splits = 1;
+  p.planes = h.P;
+  p.M = M;
+  p.N = N;
+  p.K = K;
+  p.rows = M;
+  p.cols = N;
+  return p;
+}
+
+// The operands x and a piece of w, as they are or as planes.
+struct Operands {
+  const uint16_t *x, *w;
+  int64_t ldx, ldw, x_rows, w_rows;
+};
+
+// How they lie, of a piece of Vp columns.
+Operands layout_of(const Head& h, int64_t Vp) {
+  return {nullptr, nullptr, h.x_direct ? h.ldx : h.C64, h.w_direct ? h.ldw : h.rows ? h.C64 : Vp, h.n64, h.rows ? Vp : h.C64};
+}
+
+// Whether the tiles take all products of a piece of Vp columns.
+bool products_fit(const Head& h, bool bwd, bool want_dx, bool want_dw, int64_t Vp) {
+  const Operands o = layout_of(h, Vp);
+  const int64_t main = h.fused ? h.main_of(Vp) : 0, ldz = Vp + h.pad(), n64 = h.n64;
+  auto logits = [&](int64_t N) { return operands(h, nullptr, o.ldx, o.x_rows, false, nullptr, o.ldw, o.w_rows, !h.rows, h.n, N, h.C64); };
+  if (main && !head_product_fits(logits(main))) return false;
+  if (main < Vp && !head_product128_fits(logits(Vp - main))) return false;
+  if (bwd && want_dx) {
+    const HeadProduct p = operands(h, nullptr, ldz, n64, false, nullptr, o.ldw, o.w_rows, h.rows, h.n, h.C64, Vp);
+    if (!(dx256(h, Vp) ? head_product_fits(p) : head_product128_fits(p))) return false;
+  }
+  if (bwd && want_dw) {
+    const HeadProduct p = h.rows ? operands(h, nullptr, ldz, n64, true, nullptr, o.ldx, o.x_rows, true, Vp, h.C64, n64)
+                                 : operands(h, nullptr, o.ldx, o.x_rows, true, nullptr, ldz, n64, true, h.C64, Vp, n64);
+    if (!(dw256(h, Vp) ? head_product_fits(p) : head_product128_fits(p))) return false;
+  }
+  return true;
+}
+
 // Sizes and workspace of a call; direct: whether x and w themselves are operands.
 int plan(const char* what, bool bwd, bool want_dx, bool want_dw, Head* h) {
   if (!is_float_dtype(h->dtype)) return pratchya_set_error(PRATCHYA_EINVAL, "%s: unsupported dtype %d", what, h->dtype);
@@ -426,7 +483,7 @@ int plan(const char* what, bool bwd, bool want_dx, bool want_dw, Head* h) {
   h->x_direct = bf && !(bwd && want_dw) && h->n % 64 == 0 && h->C % 64 == 0 && h->ldx % 8 == 0 && h->ldx >= h->C && aligned16(h->x) &&
                 2 * (h->n + 128) * h->ldx <= kMaxOffset;
   h->w_direct = bf && h->C % 64 == 0 && h->V % 64 == 0 && h->ldw % 8 == 0 && h->ldw >= (h->rows ? h->C : h->V) &&
-                aligned16(h->w) && 2 * ((h->rows ? 1152 : h->C + 1) * h->ldw + 128) <= kMaxOffset;
+                aligned16(h->w) && (h->rows ? 2 * (1152 * (h->ldw + 1)) : 2 * (up128(h->C) + 1) * (h->ldw + 1) + 256) <= kMaxOffset;
   // on 256-row tiles, whose operands' offsets have 31 bits
   const int64_t planes = 2 * h->P, segs = h->P == 1 ? 1 : 6, wide = h->n64 > h->C64 ? h->n64 : h->C64;
   h->fused = h->n >= 256 && h->C64 >= 256 && V64 >= 256 && planes * wide * 2560 <= INT32_MAX &&
@@ -439,7 +496,7 @@ int plan(const char* what, bool bwd, bool want_dx, bool want_dw, Head* h) {
   auto bound = [&](int64_t by) { piece = by < piece ? by : piece; };
   if (!h->w_direct) bound(2 * kPieceBytes / planes / h->C64);
   if (!h->fused) bound(kMaxOffset / planes / (wide + 128));
-  else if (h->w_direct && h->rows) bound(INT32_MAX / 4 / h->ldw);
+  if (h->w_direct && h->rows) bound(h->fused ? INT32_MAX / 4 / h->ldw : kMaxOffset / 2 / (h->ldw + 1) - 256);
   if (piece < V64) piece = piece / unit * unit;
   if (piece < 1024) piece = 1024;
   // pieces of one size
@@ -448,6 +505,9 @@ int plan(const char* what, bool bwd, bool want_dx, bool want_dw, Head* h) {
   if (h->fused)
     while (h->piece < V64 && (V64 - 1) % h->piece + 1 < 256) h->piece += 256;      // the last one: a tile or more
   if (h->piece > V64) h->piece = V64;
+  const int64_t rest = V64 - (V64 - 1) / h->piece * h->piece;      // the last piece
+  if (h->n && !(products_fit(*h, bwd, want_dx, want_dw, h->piece) && products_fit(*h, bwd, want_dx, want_dw, rest)))
+    return pratchya_set_error(PRATCHYA_EUNSUPPORTED, "%s: operands beyond 32-bit offsets", what);
   int64_t at = 0;
   auto take = [&](int64_t bytes) {
     const int64_t p = at;
@@ -464,7 +524,6 @@ int plan(const char* what, bool bwd, bool want_dx, bool want_dw, Head* h) {
   h->part_sum = take(bwd ? 0 : 4 * parts * h->ld_part);
   h->zt = take(bwd ? 0 : 4 * h->n);
   h->unit = take(bwd ? 8 : 0);
-  const int64_t rest = V64 - (V64 - 1) / h->piece * h->piece;      // the last piece
   int64_t by_rows = h->piece;                                      // columns of f32 logits
   if (h->fused) {
     by_rows = 0;
@@ -532,31 +591,6 @@ struct Call {
                          static_cast<const float*>(src), ld, rows, cols, rows_to, cols_to, targets, dst);
     return check_launch("linear_cross_entropy");
   }
-  // C [M, N] = A . B over K; a plane's rows lie lda / ldb apart, planes a_rows * lda: what both
-  // kinds of tiles take.
-  HeadProduct operands(const uint16_t* A, int64_t lda, int64_t a_rows, bool a_kmajor, const uint16_t* B, int64_t ldb,
-                         int64_t b_rows, bool b_kmajor, int64_t M, int64_t N, int64_t K) const {
-    HeadProduct p{};
-    p.a = A;
-    p.b = B;
-    p.lda = lda;
-    p.ldb = ldb;
-    p.a_plane = h.P == 1 ? 0 : a_rows * lda;
-    p.b_plane = h.P == 1 ? 0 : b_rows * ldb;
-    p.a_kmajor = a_kmajor;
-    p.b_kmajor = b_kmajor;
-    p.a_planes = h.P == 1 ? 0 : kPairsA;
-    p.b_planes = h.P == 1 ? 0 : kPairsB;
-    p.segs = h.P == 1 ? 1 : 6;
-    p.splits = 1;
-    p.planes = h.P;
-    p.M = M;
-    p.N = N;
-    p.K = K;
-    p.rows = M;
-    p.cols = N;
-    return p;
-  }
   // On 128-row tiles, to C in dtype, in bf16 times *unit.
   int product(HeadProduct p, void* C, int64_t ldc, int dtype, const float* unit = nullptr) const {
     p.c = C;
@@ -565,12 +599,6 @@ struct Call {
     p.unit = unit;
     return head_product128(p, ws + h.split, h.split_bytes, stream);
   }
-};
-
-// The operands x and a piece of w, as they are or as planes.
-struct Operands {
-  const uint16_t *x, *w;
-  int64_t ldx, ldw, x_rows, w_rows;
 };
 
 int operand_x(const Call& c, const int64_t* targets, Operands* o) {
@@ -605,14 +633,14 @@ int operand_w(const Call& c, int64_t v0, int64_t cols, int64_t Vp, Operands* o) 
 // A piece's logits from column `from` on into the workspace, [n, Vp - from].
 int logits(const Call& c, const Operands& o, int64_t from, int64_t Vp) {
   const Head& h = c.h;
-  return c.product(c.operands(o.x, o.ldx, o.x_rows, false, o.w + (h.rows ? from * o.ldw : from), o.ldw, o.w_rows, !h.rows, h.n,
+  return c.product(operands(c.h, o.x, o.ldx, o.x_rows, false, o.w + (h.rows ? from * o.ldw : from), o.ldw, o.w_rows, !h.rows, h.n,
                               Vp - from, h.C64), c.floats_at(h.z), Vp - from, PRATCHYA_DT_F32);
 }
 
 HeadProduct logits_product(const Call& c, const Operands& o, int64_t v0, int64_t cols, int64_t main,
                            const int64_t* targets, float smooth) {
   const Head& h = c.h;
-  HeadProduct p = c.operands(o.x, o.ldx, o.x_rows, false, o.w, o.ldw, o.w_rows, !h.rows, h.n, main, h.C64);
+  HeadProduct p = operands(c.h, o.x, o.ldx, o.x_rows, false, o.w, o.ldw, o.w_rows, !h.rows, h.n, main, h.C64);
   p.rows = h.n;
   p.cols = cols < main ? cols : main;
   p.targets = targets;
@@ -703,7 +731,7 @@ int backward(const Call& c, const int64_t* targets, float smooth, const float* s
     const int slices = dx ? dx256(h, Vp) : 0;
     if (slices) {
       const bool first = v0 == 0, last = v0 + h.piece >= h.V;
-      HeadProduct p = c.operands(dz, ldz, h.n64, false, o.w, o.ldw, o.w_rows, h.rows, h.n, h.C64, Vp);
+      HeadProduct p = operands(c.h, dz, ldz, h.n64, false, o.w, o.ldw, o.w_rows, h.rows, h.n, h.C64, Vp);
       p.epilogue = kHeadStore;
       if (slices > 1) {
         p.splits = slices;
@@ -727,7 +755,7 @@ int backward(const Call& c, const int64_t* targets, float smooth, const float* s
       }
     } else if (dx) {
       float* tmp = c.floats_at(h.dx_tmp);
-      rc = c.product(c.operands(dz, ldz, h.n64, false, o.w, o.ldw, o.w_rows, h.rows, h.n, h.C64, Vp), tmp, h.C64,
+      rc = c.product(operands(c.h, dz, ldz, h.n64, false, o.w, o.ldw, o.w_rows, h.rows, h.n, h.C64, Vp), tmp, h.C64,
                      PRATCHYA_DT_F32);
       if (rc) break;
       hipLaunchKernelGGL((k_head_out<T>), dim3((unsigned)((h.n * ((h.C + 3) / 4) + 255) / 256)), dim3(256), 0, c.stream,
@@ -739,8 +767,8 @@ int backward(const Call& c, const int64_t* targets, float smooth, const float* s
       const int64_t M = h.rows ? cols : h.C, N = h.rows ? h.C : cols, ld = h.rows ? h.C : h.V;
       T* to = dw + (h.rows ? v0 * h.C : v0);
       if (dw256(h, Vp)) {
-        HeadProduct p = h.rows ? c.operands(dz, ldz, h.n64, true, o.x, o.ldx, o.x_rows, true, Vp, h.C64, h.n64)
-                               : c.operands(o.x, o.ldx, o.x_rows, true, dz, ldz, h.n64, true, h.C64, Vp, h.n64);
+        HeadProduct p = h.rows ? operands(c.h, dz, ldz, h.n64, true, o.x, o.ldx, o.x_rows, true, Vp, h.C64, h.n64)
+                               : operands(c.h, o.x, o.ldx, o.x_rows, true, dz, ldz, h.n64, true, h.C64, Vp, h.n64);
         p.epilogue = kHeadStore;
         p.rows = M;
         p.cols = N;
@@ -753,8 +781,8 @@ int backward(const Call& c, const int64_t* targets, float smooth, const float* s
       }
       // columns [b, b + wide) of the piece
       auto dw_of = [&](int64_t b, int64_t Mt, int64_t Nt) {
-        return h.rows ? c.operands(dz + b, ldz, h.n64, true, o.x, o.ldx, o.x_rows, true, Mt, Nt, h.n64)
-                      : c.operands(o.x, o.ldx, o.x_rows, true, dz + b, ldz, h.n64, true, Mt, Nt, h.n64);
+        return h.rows ? operands(c.h, dz + b, ldz, h.n64, true, o.x, o.ldx, o.x_rows, true, Mt, Nt, h.n64)
+                      : operands(c.h, o.x, o.ldx, o.x_rows, true, dz + b, ldz, h.n64, true, Mt, Nt, h.n64);
       };
       if (h.dw_plain(cols) && aligned16(to)) {
         if ((rc = c.product(dw_of(0, M, N), to, ld, h.dtype, unit))) break;

@@ -53,3 +53,22 @@ def test_gradient_at_any_address(offset, rows):
     dw = out[offset:offset + C * V].view(wd.shape)
     R.close(dw.t() if rows else dw, want[2], bound[2], "dw")
     assert bool((out[:offset] == 7).all()) and bool((out[offset + C * V:] == 7).all())
+
+
+@pytest.mark.parametrize("n,V,C,ld,tied", [(64, 20032, 64, 131072, True), (40, 1024, 64, 30000000, False)])
+def test_weight_inside_a_wider_array(n, V, C, ld, tied):
+    """Rows so far apart that a whole piece of them lies beyond 32-bit offsets."""
+    from pratchya_amd import functional as F
+    x, w = _normal((n, C), torch.bfloat16, 1), _normal((C, V), torch.bfloat16, 2, 0.2)
+    t, g = torch.arange(n) * 17 % V, _normal((n,), torch.float32, 3)
+    wide = torch.empty((V if tied else C, ld), dtype=torch.bfloat16, device="cuda")
+    view = wide[:, :C if tied else V]
+    view.copy_(w.t() if tied else w)
+    view = view.detach().requires_grad_(True)
+    xd = x.cuda().requires_grad_(True)
+    y = F.linear_cross_entropy(xd, view.t() if tied else view, t.cuda())
+    dx, dw = torch.autograd.grad(y, (xd, view), g.cuda())
+    want, bound = reference(x, w, t, 0.0, g)
+    R.close(y, want[0], bound[0], "loss")
+    R.close(dx, want[1], bound[1], "dx")
+    R.close(dw.t() if tied else dw, want[2], bound[2], "dw")

@@ -25,3 +25,19 @@ def test_few_rows(n, C, V, rows, dtype):
         assert 0 < got < bound, (back, got / MB, bound / MB)
     if (n, dtype) == (128, 1):
         assert size(FAKE, C, FAKE, C if rows else V, 1, rows, n, C, V, 1, 1) < 150 * MB
+
+
+@pytest.mark.parametrize("rows", [0, 1])
+def test_weights_inside_wider_arrays(rows):
+    """A table of rows far apart, or [C, V] columns of a wide array: pieces that the products take."""
+    from pratchya_amd import _lib
+    lib = _lib.load()
+    size = lib.pratchya_linear_cross_entropy_workspace_bytes
+    for n, C, V, ld in ((64, 4096, 262144, 8192), (64, 64, 20032, 131072), (1, 4096, 65536, 1 << 16), (200, 2048, 128256, 40000),
+                        (300, 256, 40000, 100000), (64, 64, 1024, 30000000), (255, 192, 100096, 200000)):
+        if not rows and ld < V:
+            continue
+        for back in ((0, 0), (1, 0), (0, 1), (1, 1)):
+            got = size(FAKE, C, FAKE, ld, 1, rows, n, C, V, *back)
+            # at most as a copy of the weight's pieces would need
+            assert 0 < got < size(FAKE, C, FAKE, ld + 1, 1, rows, n, C, V, *back) + 4 * n * V, (n, C, V, ld, back)
