@@ -8,12 +8,15 @@
 // A negative target stands for none: l = 0 and dz = 0.  A target of V or more has no
 // logit: l is NaN and dz the formula's without its second term.
 //
-// From 256 rows on, logits are not written: the product's epilogue (head_product) takes
-// each row's maximum and sum of 128 columns, which k_head_join joins, or turns its tile
-// into dz (backward, from lse), of which a piece of the vocabulary is held at a time.
-// Below, a piece's f32 logits are computed, read by k_head_rows or k_head_grad and
-// overwritten by the next piece's.  In bf16 dz is rounded once, in units of the largest
-// cotangent (k_head_unit).  In f32 every operand of a product is the sum of three
+// From 256 rows, columns and a vocabulary of 256 on, where x's planes lie within 2^31 bytes,
+// logits are not written: the product's epilogue (head_product) takes each row's maximum and
+// sum of 128 columns, which k_head_join joins, or turns its tile into dz (backward, from lse),
+// of which a piece of the vocabulary is held at a time.  Elsewhere, and for the vocabulary's
+// end that main_of leaves out, a piece's f32 logits are computed, read by k_head_rows or
+// k_head_grad and overwritten by the next piece's.  In bf16 dz is rounded once, in units of the
+// largest cotangent (k_head_unit): half a step of its own, 2^-9, stands in both gradients before
+// their own rounding, and where dz is alike in all rows (probabilities far below a smoothed
+// label's share) it stands in all alike.  In f32 every operand of a product is the sum of three
 // exact bf16 planes and a product six products of planes.
 //
 // Bound: the MFMAs' rate on 256-row tiles, 1.1 PFLOP/s of four products (logits twice) where
@@ -484,11 +487,16 @@ int plan(const char* what, bool bwd, bool want_dx, bool want_dw, Head* h) {
                 2 * (h->n + 128) * h->ldx <= kMaxOffset;
   h->w_direct = bf && h->C % 64 == 0 && h->V % 64 == 0 && h->ldw % 8 == 0 && h->ldw >= (h->rows ? h->C : h->V) &&
                 aligned16(h->w) && (h->rows ? 2 * (1152 * (h->ldw + 1)) : 2 * (up128(h->C) + 1) * (h->ldw + 1) + 256) <= kMaxOffset;
-  // on 256-row tiles, whose operands' offsets have 31 bits
+  // on 256-row tiles, whose operands' offsets have 31 bits: x and w themselves, or copies as planes
+  // where they are larger ([8192, 8192] . [8192, 131072] in bf16, both passes: 67 ms, 77 on the
+  // 128-row tiles with w in place)
   const int64_t planes = 2 * h->P, segs = h->P == 1 ? 1 : 6, wide = h->n64 > h->C64 ? h->n64 : h->C64;
   h->fused = h->n >= 256 && h->C64 >= 256 && V64 >= 256 && planes * wide * 2560 <= INT32_MAX &&
-             planes * h->n64 * h->C64 <= INT32_MAX && (!h->x_direct || 2 * h->n * h->ldx <= INT32_MAX) &&
-             (!h->w_direct || 2 * (h->rows ? 2560 : h->C) * h->ldw <= INT32_MAX);
+             planes * h->n64 * h->C64 <= INT32_MAX;
+  if (h->fused) {
+    h->x_direct = h->x_direct && 2 * h->n * h->ldx <= INT32_MAX;
+    h->w_direct = h->w_direct && 2 * (h->rows ? 2560 : h->C) * h->ldw <= INT32_MAX;
+  }
   const int64_t unit = h->fused ? 256 : 64;
   // what of a piece is kept: f32 logits, or only the planes of their gradient; the planes
   // of its weight: 512 MB

@@ -72,3 +72,24 @@ def test_weight_inside_a_wider_array(n, V, C, ld, tied):
     R.close(y, want[0], bound[0], "loss")
     R.close(dx, want[1], bound[1], "dx")
     R.close(dw.t() if tied else dw, want[2], bound[2], "dw")
+
+
+def test_rows_beyond_31_bits():
+    """From 256 rows on, of a table and of x so far apart that the tiles take copies of them."""
+    from pratchya_amd import functional as F
+    n, V, C = 300, 512, 256
+    x, w = _normal((n, C), torch.bfloat16, 1), _normal((C, V), torch.bfloat16, 2, 0.2)
+    t, g = torch.arange(n) * 17 % V, _normal((n,), torch.float32, 3)
+    want, bound = reference(x, w, t, 0.0, g)
+    for wide_x in (False, True):
+        apart = torch.empty((n if wide_x else V, 1 << 22), dtype=torch.bfloat16, device="cuda")
+        view = apart[:, :C]
+        view.copy_(x if wide_x else w.t())
+        view = view.detach().requires_grad_(True)
+        other = (w.t().contiguous() if wide_x else x).cuda().requires_grad_(True)
+        xd, table = (view, other) if wide_x else (other, view)
+        y = F.linear_cross_entropy(xd, table.t(), t.cuda())
+        dx, dw = torch.autograd.grad(y, (xd, table), g.cuda())
+        R.close(y, want[0], bound[0], "loss")
+        R.close(dx, want[1], bound[1], "dx")
+        R.close(dw.t(), want[2], bound[2], "dw")

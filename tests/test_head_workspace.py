@@ -41,3 +41,28 @@ def test_weights_inside_wider_arrays(rows):
             got = size(FAKE, C, FAKE, ld, 1, rows, n, C, V, *back)
             # at most as a copy of the weight's pieces would need
             assert 0 < got < size(FAKE, C, FAKE, ld + 1, 1, rows, n, C, V, *back) + 4 * n * V, (n, C, V, ld, back)
+
+
+def _by_tiles(n, C, V, ldx, ldw, rows):
+    """Whether the loss takes each row's statistics from the products' tiles, of 128 columns each and
+    12 bytes, with no logits written: what it holds for 2 n rows more than for n."""
+    from pratchya_amd import _lib
+    size = _lib.load().pratchya_linear_cross_entropy_workspace_bytes
+    one, two = (size(FAKE, ldx, FAKE, ldw, 1, rows, m, C, V, 0, 0) for m in (n, 2 * n))
+    assert 0 < one and 0 < two
+    more, statistics = two - one - 2 * n * C, 12 * n * (V // 128)      # but for x's planes
+    return 0.4 * statistics < more < 1.6 * statistics      # the vocabulary's end may go by written logits, in one or both
+
+
+@pytest.mark.parametrize("rows", [0, 1])
+@pytest.mark.parametrize("C,V", [(4096, 65536), (8192, 131072), (8192, 152064), (4096, 262144 + 4096)])
+def test_large_heads_keep_no_logits(C, V, rows):
+    """Also where the weight's size exceeds 31 bits."""
+    assert _by_tiles(8192, C, V, C, C if rows else V, rows)
+
+
+def test_rows_far_apart_keep_no_logits():
+    """Rows of x and of a table that lie beyond 31 bits in place."""
+    assert _by_tiles(8192, 4096, 65536, 1 << 18, 4096, 1)
+    assert _by_tiles(8192, 4096, 65536, 4096, 1 << 19, 1)
+    assert not _by_tiles(64, 4096, 65536, 4096, 4096, 1)
