@@ -8,8 +8,8 @@
 // A negative target stands for none: l = 0 and dz = 0.  A target of V or more has no
 // logit: l is NaN and dz the formula's without its second term.
 //
-// From 256 rows, columns and a vocabulary of 256 on, where x's planes lie within 2^31 bytes,
-// logits are not written: the product's epilogue (head_product) takes each row's maximum and
+// From 256 rows on, of more than 192 columns and words of a vocabulary, where x's planes lie
+// within 2^31 bytes, logits are not written: the product's epilogue (head_product) takes each row's maximum and
 // sum of 128 columns, which k_head_join joins, or turns its tile into dz (backward, from lse),
 // of which a piece of the vocabulary is held at a time.  Elsewhere, and for the vocabulary's
 // end that main_of leaves out, a piece's f32 logits are computed, read by k_head_rows or
@@ -38,8 +38,6 @@ constexpr float kLowest = -3.4028234663852886e38f;
 // --------------------------------------------------------------------------
 // operands
 // --------------------------------------------------------------------------
-__device__ __forceinline__ float top_piece(float v) { return u2f(f2u(v) & 0xFFFF0000u); }
-
 // Planes [P][rows_to][cols_to] of src [rows, cols] (rows ld elements apart, at any
 // element's address), zeros around it: bf16 as it is (P 1) or an f32 value's three
 // pieces (P 3), 8 columns a thread.  Rows whose target (targets, if not null) is negative
@@ -357,9 +355,11 @@ struct Head {
   }
   // Columns of a piece's logits on the 256-row tiles: all (a multiple of 64 behind the
   // piece's end), or those of full rounds of tiles on the 256 compute units, where the last
-  // round would be a third full or less; the others are few enough for the way of few rows
-  // (f32 [1000, 1027] . [1027, 50021], 784 tiles: both passes 3.21 ms with a
-  // fourth round of 16 tiles, 3.02 without).
+  // round would be a third full or less and a tile has 48 steps of K or more; the others go the
+  // way of few rows, in four launches more.  Loss alone of [1000, C] . [C, 50176], 784 tiles, and
+  // [4096, C] . [C, 33792], 2112, in bf16, all on tiles and the end apart, us:
+  //   C 1024   164 150   332 352      C 2048   272 248   582 604      C 4096   522 450   1115 1098
+  // f32 [1000, 1024] . [1024, 50176], 96 steps, both passes 2926 and 2686.
   int64_t main_of(int64_t cols) const {
     const int64_t all = (cols + 63) / 64 * 64, tm = (n + 255) / 256, tn = (all + 255) / 256, full = tm * tn / 256;
     if (full < 1 || tm * tn % 256 == 0 || tm * tn % 256 > 85 || C64 / 64 * (P == 1 ? 1 : 6) < 48) return all;

@@ -115,7 +115,6 @@ __device__ __forceinline__ bf16x8_t read_columns(const uint16_t* p, int pitch, i
   return frag(__builtin_bit_cast(v2i, a), __builtin_bit_cast(v2i, b));
 }
 
-__device__ __forceinline__ float top_piece(float v) { return u2f(f2u(v) & 0xFFFF0000u); }
 // Values as NP planes of pairs: one rounded plane, or the three exact pieces.
 template <int NP, int N>
 __device__ __forceinline__ void split(float (&v)[N], uint32_t (&o)[NP][N / 2]) {
@@ -163,7 +162,9 @@ struct Gates {
 
 template <int NPI, int NP, int L, int DP, int EP, bool OUT>
 struct Lds {
-  static constexpr int PD = DP + 8, PE = EP + 8, PT = L + 8;   // row pitches: no two rows of a read on one bank
+  // row pitches: 4 words more than whole turns of the 64 banks, or of half of them (a third of the
+  // cycles that the LDS is busy are conflicts still; other pitches took as long)
+  static constexpr int PD = DP + 8, PE = EP + 8, PT = L + 8;
   alignas(16) uint16_t q[OUT ? NPI : 1][OUT ? L * PD : 8];
   alignas(16) uint16_t k[NPI][L * PD];
   alignas(16) uint16_t v[NPI][L * PE];

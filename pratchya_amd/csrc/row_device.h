@@ -72,6 +72,9 @@ __device__ __forceinline__ void store_some(T* p, int64_t n, const float (&v)[N])
     if (i < n) store_elem(p + i, v[i]);
 }
 
+// The first bf16 piece of an f32 value: its upper half, exactly.
+__device__ __forceinline__ float top_piece(float v) { return u2f(f2u(v) & 0xFFFF0000u); }
+
 // Sum over aligned groups of BL lanes, for every lane of the group (the
 // exchanges of lane_group_max; every lane adds the same pairs, so all get the
 // same bits).
