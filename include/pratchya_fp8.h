@@ -802,14 +802,25 @@ int pratchya_linear_cross_entropy_bwd(const void* x, int64_t ldx, const void* w,
  * heads, dv] of dtype; state_out: S behind the last token, f32 as state (not state
  * itself).  starts: pratchya_linear_attention_starts_floats of f32, 16-byte aligned
  * (null where that is 0): the states before the segments that a long sequence is cut
- * into, which the backward pass reads.  train: whether one follows (it takes fewer
- * segments, and reads starts of a call that said so).  A decay of 0 (log_decay -inf) forgets all. */
+ * into, which the backward pass reads, and behind them (from
+ * pratchya_linear_attention_states_floats on) those of the segments' parts, which this
+ * call alone reads.  train: whether a backward pass follows (it takes fewer
+ * segments, and reads starts of a call that said so).  A decay of 0 (log_decay -inf)
+ * forgets all but what is not finite.  pratchya_linear_attention_parts: the same with
+ * the parts' floats at an address of their own, to be given up behind the call. */
 int64_t pratchya_linear_attention_starts_floats(int64_t batch, int64_t length, int64_t heads, int64_t dk, int64_t dv,
                                                 int dtype, int train);
 int pratchya_linear_attention(const void* q, const void* k, const void* v, int dtype, const void* log_decay, int g_dtype,
                               const int64_t* strides, const int64_t* lengths, const float* state, int64_t batch,
                               int64_t length, int64_t heads, int64_t dk, int64_t dv, float scale, int train,
                               void* out, float* state_out, float* starts, hipStream_t stream);
+int64_t pratchya_linear_attention_states_floats(int64_t batch, int64_t length, int64_t heads, int64_t dk, int64_t dv,
+                                                int dtype, int train);
+int pratchya_linear_attention_parts(const void* q, const void* k, const void* v, int dtype, const void* log_decay,
+                                    int g_dtype, const int64_t* strides, const int64_t* lengths, const float* state,
+                                    int64_t batch, int64_t length, int64_t heads, int64_t dk, int64_t dv, float scale,
+                                    int train, void* out, float* state_out, float* starts, float* parts,
+                                    hipStream_t stream);
 
 /* Its gradients from the cotangents dout (of dtype, strides[12 .. 14], last axis
  * contiguous) and dstate_out (f32 as state, or null for 0), with the forward pass's

@@ -156,6 +156,10 @@ SIGNATURES = {
     "pratchya_linear_attention_starts_floats": (_c_i64, [_c_i64] * 5 + [_c_int] * 2),
     "pratchya_linear_attention": (_c_int, [_c_p, _c_p, _c_p, _c_int, _c_p, _c_int, _c_p, _c_p, _c_p, _c_i64, _c_i64,
                                            _c_i64, _c_i64, _c_i64, ctypes.c_float, _c_int, _c_p, _c_p, _c_p, _c_p]),
+    "pratchya_linear_attention_states_floats": (_c_i64, [_c_i64] * 5 + [_c_int] * 2),
+    "pratchya_linear_attention_parts": (_c_int, [_c_p, _c_p, _c_p, _c_int, _c_p, _c_int, _c_p, _c_p, _c_p, _c_i64,
+                                                 _c_i64, _c_i64, _c_i64, _c_i64, ctypes.c_float, _c_int, _c_p, _c_p,
+                                                 _c_p, _c_p, _c_p]),
     "pratchya_linear_attention_bwd_workspace_bytes": (_c_i64, [_c_i64] * 5 + [_c_int]),
     "pratchya_linear_attention_bwd": (_c_int, [_c_p, _c_p, _c_p, _c_int, _c_p, _c_int, _c_p, _c_p, _c_p, _c_p, _c_p,
                                                _c_p, _c_p, _c_i64, _c_i64, _c_i64, _c_i64, _c_i64, ctypes.c_float, _c_p,

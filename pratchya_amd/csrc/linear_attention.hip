@@ -1168,11 +1168,9 @@ struct Shape {
     return n < 1 ? 1 : n;
   }
   // states before the segments; of their parts, with their decays
-  int64_t states_floats() const { return B * H * segments() * state(); }
-  int64_t starts_floats() const {
-    const int64_t n = segments();
-    return n > 1 ? states_floats() + B * H * (n - 1) * parts() * (state() + 1) : 0;
-  }
+  int64_t states_floats() const { return segments() > 1 ? B * H * segments() * state() : 0; }
+  int64_t parts_floats() const { return B * H * (segments() - 1) * parts() * (state() + 1); }
+  int64_t starts_floats() const { return states_floats() + parts_floats(); }
 };
 
 int check_shape(const char* what, const Shape& s, int g_dtype) {
@@ -1270,12 +1268,12 @@ Array packed(const Shape& s, const void* p, int64_t d) {
 }
 
 // The states before the segments (rev: behind them), where there are several.
-int segment_states(const Shape& s, MixArgs a, float* starts, const float* init, hipStream_t stream) {
+int segment_states(const Shape& s, MixArgs a, float* starts, float* parts, const float* init, hipStream_t stream) {
   if (a.nseg < 2) return PRATCHYA_OK;
   const int64_t size = s.state(), n = s.B * s.H * (a.nseg - 1) * s.parts();
   a.parts = (int)s.parts();
   a.per_part = (a.per + a.parts - 1) / a.parts;
-  a.last = starts + s.states_floats();
+  a.last = parts;
   a.last_seg = size;
   a.last_r = a.dv;
   a.last_c = 1;
@@ -1307,17 +1305,23 @@ extern "C" int64_t pratchya_linear_attention_starts_floats(int64_t batch, int64_
   return check_shape("linear_attention", s, PRATCHYA_DT_F32) ? 0 : s.starts_floats();
 }
 
-extern "C" int pratchya_linear_attention(const void* q, const void* k, const void* v, int dtype, const void* log_decay,
-                                         int g_dtype, const int64_t* strides, const int64_t* lengths, const float* state,
-                                         int64_t batch, int64_t length, int64_t heads, int64_t dk, int64_t dv,
-                                         float scale, int train, void* out, float* state_out, float* starts,
-                                         hipStream_t stream) {
+extern "C" int64_t pratchya_linear_attention_states_floats(int64_t batch, int64_t length, int64_t heads, int64_t dk,
+                                                           int64_t dv, int dtype, int train) {
+  const Shape s = {batch, length, heads, dk, dv, dtype, train != 0};
+  return check_shape("linear_attention", s, PRATCHYA_DT_F32) ? 0 : s.states_floats();
+}
+
+extern "C" int pratchya_linear_attention_parts(const void* q, const void* k, const void* v, int dtype, const void* log_decay,
+                                               int g_dtype, const int64_t* strides, const int64_t* lengths,
+                                               const float* state, int64_t batch, int64_t length, int64_t heads, int64_t dk,
+                                               int64_t dv, float scale, int train, void* out, float* state_out,
+                                               float* starts, float* parts, hipStream_t stream) {
   const char* what = "linear_attention";
   const Shape s = {batch, length, heads, dk, dv, dtype, train != 0};
   const int rc = check_shape(what, s, g_dtype);
   if (rc) return rc;
   if (batch == 0) return pratchya_set_error(PRATCHYA_OK, "");
-  if (!strides || (length && (!q || !k || !v || !log_decay || !out)) || !state_out || (s.starts_floats() && !starts))
+  if (!strides || (length && (!q || !k || !v || !log_decay || !out)) || !state_out || (s.starts_floats() && !(starts && parts)))
     return pratchya_set_error(PRATCHYA_EINVAL, "%s: null buffer", what);
   MixArgs a = base_args(s, log_decay, g_dtype, strides + 9, lengths);
   a.q = array(q, strides);
@@ -1328,8 +1332,19 @@ extern "C" int pratchya_linear_attention(const void* q, const void* k, const voi
   a.dv = (int)dv;
   a.scale = scale;
   a.kscale = 1.0f;
-  const int rc2 = segment_states(s, a, starts, state, stream);
+  const int rc2 = segment_states(s, a, starts, parts, state, stream);
   return rc2 ? rc2 : outputs(s, a, starts, state, false, state_out, stream);
+}
+
+extern "C" int pratchya_linear_attention(const void* q, const void* k, const void* v, int dtype, const void* log_decay,
+                                         int g_dtype, const int64_t* strides, const int64_t* lengths, const float* state,
+                                         int64_t batch, int64_t length, int64_t heads, int64_t dk, int64_t dv,
+                                         float scale, int train, void* out, float* state_out, float* starts,
+                                         hipStream_t stream) {
+  // the parts' states behind those that a backward pass reads
+  float* parts = starts ? starts + pratchya_linear_attention_states_floats(batch, length, heads, dk, dv, dtype, train) : nullptr;
+  return pratchya_linear_attention_parts(q, k, v, dtype, log_decay, g_dtype, strides, lengths, state, batch, length, heads, dk,
+                                         dv, scale, train, out, state_out, starts, parts, stream);
 }
 
 extern "C" int64_t pratchya_linear_attention_bwd_workspace_bytes(int64_t batch, int64_t length, int64_t heads, int64_t dk,
@@ -1385,7 +1400,7 @@ extern "C" int pratchya_linear_attention_bwd(const void* q, const void* k, const
   a.dq = (int)dk;
   a.dv = (int)dv;
   a.kscale = scale;
-  if ((rc = segment_states(s, a, rstarts, dstate_out, stream))) return rc;
+  if ((rc = segment_states(s, a, rstarts, rstarts + s.states_floats(), dstate_out, stream))) return rc;
   BackArgs g = {};
   g.q = Q;
   g.k = K;

@@ -583,12 +583,19 @@ Mixed linear_attention_fwd(const Mix& m, double scale, bool train) {
   Mixed r;
   r.out = new_empty({m.B, m.T, m.H, m.dv}, m.q.scalar_type(), m.q);
   r.state = new_empty({m.B, m.H, m.dk, m.dv}, at::kFloat, m.q);
-  const int64_t floats = pratchya_linear_attention_starts_floats(m.B, m.T, m.H, m.dk, m.dv, m.code, train);
-  if (floats) r.starts = new_empty({floats}, at::kFloat, m.q);
-  check(pratchya_linear_attention(m.q.data_ptr(), m.k.data_ptr(), m.v.data_ptr(), m.code, m.decay.data_ptr(), m.g_code,
-                                  m.strides.data(), m.length_ptr(), m.state_ptr(), m.B, m.T, m.H, m.dk, m.dv,
-                                  (float)scale, train, r.out.data_ptr(), static_cast<float*>(r.state.data_ptr()),
-                                  static_cast<float*>(address(r.starts)), stream_of(m.q)),
+  // what a backward pass reads, and what this call alone does
+  const int64_t floats = pratchya_linear_attention_starts_floats(m.B, m.T, m.H, m.dk, m.dv, m.code, train),
+                kept = pratchya_linear_attention_states_floats(m.B, m.T, m.H, m.dk, m.dv, m.code, train);
+  Tensor parts;
+  if (floats) {
+    r.starts = new_empty({kept}, at::kFloat, m.q);
+    parts = new_empty({floats - kept}, at::kFloat, m.q);
+  }
+  check(pratchya_linear_attention_parts(
+            m.q.data_ptr(), m.k.data_ptr(), m.v.data_ptr(), m.code, m.decay.data_ptr(), m.g_code, m.strides.data(),
+            m.length_ptr(), m.state_ptr(), m.B, m.T, m.H, m.dk, m.dv, (float)scale, train, r.out.data_ptr(),
+            static_cast<float*>(r.state.data_ptr()), static_cast<float*>(address(r.starts)),
+            static_cast<float*>(address(parts)), stream_of(m.q)),
         "linear_attention");
   return r;
 }
