@@ -770,10 +770,17 @@ int pratchya_embedding_bwd(const void* dy, int64_t ldy, int dtype, const int64_t
  * target's term.  stats, if not null, [n][2] f32 for the backward pass.  workspace:
  * pratchya_linear_cross_entropy_workspace_bytes of the same arguments (backward_dx and
  * backward_dw 0 for the forward pass, else whether that gradient is wanted), 256-byte
- * aligned: the f32 logits of a piece of the vocabulary (256 MB at most, but for 64 Ki
- * rows or more), and copies of operands whose sizes are no multiples of 64 or that are
- * f32 (three bf16 planes).  Rows and one piece's planes lie within 2^32 bytes
- * (PRATCHYA_EUNSUPPORTED otherwise). */
+ * aligned.  It holds, with 2 bytes a value in bf16 and 6 (three planes) in f32: x; a
+ * piece of W (512 MB) where it is not bf16 of sizes, a row distance and an address of
+ * whole vectors; forward, 12 bytes a row and 128 columns of the vocabulary (whether
+ * smoothing needs all of them or not; 4096 columns where logits are written);
+ * backward, a piece of the logits' gradient (512 MB), the f32 sums of dx, of as many
+ * slices of K as few tiles take (16), and f32 sums of columns of dw (256 MB, 32 where its
+ * sizes are whole vectors).  With fewer than 256 rows, with 192 columns or words or fewer,
+ * or where x takes over 2^31 bytes, also the f32 logits of a piece (256 MB; elsewhere of
+ * the vocabulary's end at most, 22 MB); and partial sums of products (34 MB).  A piece
+ * has 1024 columns at least, however large that makes it.  Calls whose operands lie beyond
+ * 2^32 bytes are refused before any launch (PRATCHYA_EUNSUPPORTED). */
 int64_t pratchya_linear_cross_entropy_workspace_bytes(const void* x, int64_t ldx, const void* w, int64_t ldw, int dtype,
                                                       int w_rows, int64_t n, int64_t width, int64_t vocab,
                                                       int backward_dx, int backward_dw);

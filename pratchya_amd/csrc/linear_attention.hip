@@ -26,22 +26,21 @@
 // less.  The scores and the states that outputs in bf16 read are two planes, 2^-16 of
 // themselves: with one, 2^-9, what the terms of a sum lose stands in outputs in which they
 // cancel (error of 0.0023 of the norm against 64 bits, 0.0017 now, the output's own rounding;
-// a training pass of the size 690 us at the size below, 653 with one).  The decays' gradient is f32, and
-// what it sums is not rounded: see k_mix_back.
+// both passes of the size below 690 us, 653 with one).  The decays' gradient is f32, and what
+// it sums is not rounded: see k_mix_back.
 //
 // A sequence is cut into segments where heads alone leave the chip idle: the states that
 // their parts add first (k_mix without outputs), joined from the first to the last, then
 // all segments at once.
 //
-// Measured, 8 x 4096 tokens of 32 heads of 64 in bf16, both passes 735 us; with one plane of
-// scores and read states, and NaN not looked for, 650: states 36 us for each of S and R, joins 7, o 136, dq 184,
-// k_mix_back 301.  HBM at a copy's rate would take 220
+// Measured, 8 x 4096 tokens of 32 heads of 64 in bf16, both passes 735 us: states 36 us for
+// each of S and R, joins 7, o 158, dq 196, k_mix_back 337.  HBM at a copy's rate would take 220
 // (1.08 GB).  The MFMAs are busy a sixth of the time, the vector units two fifths (planes,
 // weights, masks), LDS a third, and two or three workgroups a compute unit overlap these in
-// part.  With dk and dv as walks of their own, as dq, whose scores then need three planes
-// each for the decays' sums, both passes took 991; with the states of whole segments, a
-// workgroup each, 693.  Without gradients (8192 tokens of 64 heads, 105 us) the walk
-// runs at 4.2 TB/s.
+// part.  Without gradients (8192 tokens of 64 heads, 113 us) the walk runs at 3.7 TB/s.  With
+// one plane of scores and read states, and values that are not finite not looked for (650),
+// dk and dv as walks of their own, as dq, whose scores then need three planes each for the
+// decays' sums, took both passes to 991; states of whole segments, a workgroup each, to 693.
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 

@@ -24,8 +24,8 @@ A language model with tied weights and linear attention begins, mixes and ends w
 and generates with ``linear_attention_step`` from ``r.state`` on.
 
 Arrays are bf16 or f32 on the GPU; rows may be a stride apart (slices of a wider
-array).  Arithmetic is f32, with one rounding to a result's type.  Gradients are
-reverse-mode and of first order: inputs with a forward-mode tangent are refused, and
+array).  Arithmetic is f32, with one rounding to a result's type; where values between
+have fewer bits, the operator says so.  Gradients are reverse-mode and of first order: inputs with a forward-mode tangent are refused, and
 so is the gradient of a gradient.
 """
 from __future__ import annotations
@@ -101,13 +101,18 @@ def linear_cross_entropy(x: torch.Tensor, weight: torch.Tensor, targets: torch.T
     weight [C, V] of x's dtype and targets [...] (int64 or int32): f32 [...],
     ``(1 - a) (lse - z_t) + a (lse - mean z)`` with a the label smoothing,
     differentiable in x and weight.  The logits are not kept: both passes compute them,
-    in f32; their gradient, of a piece of the vocabulary at a time, is rounded to x's dtype
-    before the products that give the gradients of x and weight.  An embedding table [V, C] serves as weight
-    through its transposed view ``table.t()``, which is read as it lies.
+    in f32, by tiles or a piece of the vocabulary at a time; their gradient, likewise, is
+    rounded to x's dtype before the products that give the gradients of x and weight.  In
+    bf16 the gradients' error is then that of their own rounding (0.0017 of the norm) with
+    thousands of rows, and up to 1.4 times that with few rows and a small vocabulary.  An
+    embedding table [V, C] serves as weight through its transposed view ``table.t()``,
+    which is read as it lies.
 
     A negative target stands for none: its loss is 0 and has no gradient.  A target of V
     or more gives NaN, as no logit stands for it; its gradient is that of the other
-    terms."""
+    terms.  A row of x that holds a NaN or an infinity has a loss and a gradient that are
+    not finite, and so is the weight's gradient unless the row has no target; the other
+    rows' are not touched."""
     return _ops.linear_cross_entropy(x, weight, targets, label_smoothing)
 
 
